@@ -17,12 +17,40 @@ PP = ctypes.POINTER(c_void_p)
 PI = ctypes.POINTER(c_int)
 
 ACT_NONE, ACT_RELU, ACT_SWISH, ACT_LEAKY = 0, 1, 2, 3
+F16, BF16 = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_RAMP, ROPE_TURNS = 0, 1, 2, 3
 
 
 class ConvDesc(ctypes.Structure):
     _fields_ = [(n, c_int) for n in ("batch", "in_c", "in_d", "in_h", "in_w", "out_c", "kd", "kh", "kw", "sd", "sh",
                                      "sw", "pd", "ph", "pw", "act")] + [("slope", c_float), ("two_step", c_int)]
 
+
+class Heads(ctypes.Structure):
+    """aig_heads: a tensor [tokens][heads][head_dim]."""
+    _fields_ = [("data", c_void_p), ("heads", c_int), ("token_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong)]
+
+
+class SeqHeads(ctypes.Structure):
+    """aig_seq_heads: a tensor [batch][tokens][heads][head_dim]."""
+    _fields_ = [("data", c_void_p)] + [(n, ctypes.c_longlong) for n in ("batch_stride", "token_stride", "head_stride")]
+
+
+class RopeDesc(ctypes.Structure):
+    _fields_ = [("head_dim", c_int), ("rot_dim", c_int), ("interleaved", c_int), ("scaling", c_int), ("base", c_float), ("factor", c_float),
+                ("original_len", c_int), ("low", c_float), ("high", c_float), ("magnitude", c_float)]
+
+
+class KvCacheDesc(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p)] + [(n, c_int) for n in ("dtype", "kv_heads", "head_dim", "page_size", "num_pages")] + [
+        (n, ctypes.c_longlong) for n in ("page_stride", "token_stride", "head_stride")]
+
+
+class WindowDesc(ctypes.Structure):
+    _fields_ = [(n, c_int) for n in ("dtype", "batch", "q_len", "kv_len", "heads", "kv_heads", "head_dim", "window", "sinks")] + [("scale", c_float)]
+
+
+PH, PS = ctypes.POINTER(Heads), ctypes.POINTER(SeqHeads)
 
 # name -> argtypes (restype is int unless listed in _RESTYPES)
 SIGNATURES = {
@@ -124,6 +152,28 @@ SIGNATURES = {
     "aig_resdown_plan_set_output_padded": [P, c_int],
     "aig_conv_plan_set_input_padded": [P, c_int],
     "aig_actions_from_outputs": [P, P, c_int, c_int, c_int],
+    "aig_rope_frequencies": [ctypes.POINTER(RopeDesc), P, c_int],
+    "aig_rope_plan_create": [P, ctypes.POINTER(RopeDesc), PP],
+    "aig_rope_plan_destroy": [P],
+    "aig_rope_forward": [P, c_int, P, ctypes.c_longlong, PH, PH, PH, PH],
+    "aig_rope_backward": [P, c_int, P, ctypes.c_longlong, PH, PH, PH, PH],
+    "aig_kv_append": [P, ctypes.POINTER(KvCacheDesc), P, PH, PH, PH, PH, P, P, ctypes.c_longlong, P, c_int, c_int],
+    "aig_kv_copy_pages": [P, ctypes.POINTER(KvCacheDesc), P, P, c_int],
+    "aig_paged_attention": [P, ctypes.POINTER(KvCacheDesc), PH, PH, P, c_int, P, c_int, c_int, c_float, c_int, c_int],
+    "aig_page_pool_create": [c_int, c_int, PP],
+    "aig_page_pool_destroy": [P],
+    "aig_page_pool_open": [P, PI],
+    "aig_page_pool_grow": [P, c_int, c_int, PI, PI],
+    "aig_page_pool_fork": [P, c_int, PI],
+    "aig_page_pool_trim": [P, c_int, c_int, c_int],
+    "aig_page_pool_close": [P, c_int],
+    "aig_page_pool_compact": [P, P, P, c_int, PI],
+    "aig_page_pool_table": [P, c_int, P, c_int],
+    "aig_page_pool_length": [P, c_int],
+    "aig_page_pool_free_pages": [P],
+    "aig_page_pool_shared": [P, c_int],
+    "aig_window_attention_forward": [P, ctypes.POINTER(WindowDesc), PS, PS, PS, PS, P, P],
+    "aig_window_attention_backward": [P, ctypes.POINTER(WindowDesc), PS, PS, PS, PS, P, PS, PS, PS, PS, P, P],
     # include/aig_compat.h: the reference's launcher names (no context argument; most return void)
     "InitCUDA": [],
     "ConvertAndNormalize": [P, P, c_size_t],
@@ -651,6 +701,234 @@ class MhaPlan(_Plan):
 
     def reset(self):
         self.check(lib().aig_mha_reset(self.handle))
+
+
+def _dtype_of(*tensors):
+    import torch
+
+    kinds = {t.dtype for t in tensors if t is not None}
+    code = {torch.float16: F16, torch.bfloat16: BF16}.get(next(iter(kinds))) if len(kinds) == 1 else None
+    if code is None:
+        raise ValueError("tensors of one type, fp16 or bf16: got %s" % sorted(map(str, kinds)))
+    return code
+
+
+def _rows(t, what, dims, dtype=None):
+    """Checks that a tensor has `dims` dimensions, or the shape `dims`, with consecutive values in the last one; returns it."""
+    shape = tuple(t.shape)
+    if (len(shape) != dims) if isinstance(dims, int) else (shape != tuple(dims)):
+        raise ValueError("%s: shape %s where %s is wanted" % (what, shape, "%d dimensions" % dims if isinstance(dims, int) else tuple(dims)))
+    if shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError("%s: the last dimension has to be dense" % what)
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError("%s: %s where %s is wanted" % (what, t.dtype, dtype))
+    return t
+
+
+def _device_ints(t, what, shape):
+    """A dense int32 tensor of this shape on the device."""
+    import torch
+
+    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or not t.is_cuda:
+        raise ValueError("%s: a dense int32 device tensor of shape %s is wanted, got %s %s" % (what, tuple(shape), t.dtype, tuple(t.shape)))
+    return t.data_ptr()
+
+
+def _heads(t):
+    s = t.stride()
+    return ctypes.byref(Heads(t.data_ptr(), t.shape[1], s[0], s[1]))
+
+
+class RopePlan(_Plan):
+    """aig_rope_plan: rotary positions, by position tensors int32 [tokens] and head tensors [tokens][heads][head_dim]."""
+    _destroy = "aig_rope_plan_destroy"
+
+    def __init__(self, ctx, head_dim, rot_dim=0, interleaved=False, base=10000.0, scaling=ROPE_PLAIN, factor=1.0, original_len=0, low=1.0,
+                 high=32.0, magnitude=1.0):
+        super().__init__(ctx)
+        self.desc = RopeDesc(head_dim, rot_dim or head_dim, 1 if interleaved else 0, scaling, base, factor, original_len, low, high, magnitude)
+        self.check(lib().aig_rope_plan_create(ctx.handle, ctypes.byref(self.desc), ctypes.byref(self.handle)))
+
+    def frequencies(self):
+        """Radians per position of each pair."""
+        n = self.desc.rot_dim // 2
+        out = (ctypes.c_double * n)()
+        self.check(lib().aig_rope_frequencies(ctypes.byref(self.desc), ctypes.cast(out, P), n))
+        return list(out)
+
+    def _apply(self, fn, positions, q, q_out, k, k_out):
+        n, d = q.shape[0], self.desc.head_dim
+        _rows(q, "q", (n, q.shape[1], d))
+        _rows(q_out, "q_out", q.shape)
+        if k is not None:
+            _rows(k, "k", (n, k.shape[1], d))
+            _rows(k_out, "k_out", k.shape)
+        self.check(fn(self.handle, _dtype_of(q, q_out, k, k_out), _device_ints(positions, "positions", (n,)), n, _heads(q), _heads(q_out),
+                      None if k is None else _heads(k), None if k is None else _heads(k_out)))
+
+    def forward(self, positions, q, q_out, k=None, k_out=None):
+        self._apply(lib().aig_rope_forward, positions, q, q_out, k, k_out)
+
+    def backward(self, positions, dq, dq_out, dk=None, dk_out=None):
+        """Gradients of the turned tensors -> gradients of the tensors before."""
+        self._apply(lib().aig_rope_backward, positions, dq, dq_out, dk, dk_out)
+
+
+class PagedCache:
+    """aig_kv_cache over two tensors [pages][page_size][kv_heads][head_dim] (other orders as strided views)."""
+
+    def __init__(self, ctx, k_pages, v_pages):
+        _rows(k_pages, "k_pages", 4)
+        _rows(v_pages, "v_pages", k_pages.shape)
+        if k_pages.stride() != v_pages.stride():
+            raise ValueError("keys and values have the same strides")
+        self.ctx, self._keep = ctx, (k_pages, v_pages)
+        pages, size, heads, dim = k_pages.shape
+        s = k_pages.stride()
+        self.dtype = k_pages.dtype
+        self.desc = KvCacheDesc(k_pages.data_ptr(), v_pages.data_ptr(), _dtype_of(k_pages, v_pages), heads, dim, size, pages, s[0], s[1], s[2])
+        self._ref = ctypes.byref(self.desc)
+
+    def append(self, k, v, positions, table, seqs=None, rope=None, q=None, q_out=None):
+        """New tokens' k, v [tokens][kv_heads][head_dim] to positions[i] of sequence seqs[i] (None: i); with a rope plan turned on
+        the way, q [tokens][heads][head_dim] into q_out too."""
+        n, d = k.shape[0], self.desc.head_dim
+        _rows(k, "k", (n, self.desc.kv_heads, d), self.dtype)
+        _rows(v, "v", k.shape, self.dtype)
+        if q is not None:
+            _rows(q, "q", (n, q.shape[1], d), self.dtype)
+            _rows(q_out, "q_out", q.shape, self.dtype)
+        batch, width = table.shape
+        self.ctx.check(lib().aig_kv_append(self.ctx.handle, self._ref, None if rope is None else rope.handle, _heads(k), _heads(v),
+                                           None if q is None else _heads(q), None if q is None else _heads(q_out),
+                                           None if seqs is None else _device_ints(seqs, "seqs", (n,)), _device_ints(positions, "positions", (n,)), n,
+                                           _device_ints(table, "table", (batch, width)), batch, width))
+
+    def copy_pages(self, src, dst):
+        """Pages src[i] -> dst[i], host numbers."""
+        n = len(src)
+        if len(dst) != n:
+            raise ValueError("as many sources as destinations")
+        ints = c_int * max(n, 1)
+        self.ctx.check(lib().aig_kv_copy_pages(self.ctx.handle, self._ref, ints(*src), ints(*dst), n))
+
+    def attend(self, q, out, table, lengths, max_length, scale=None, window=0, sinks=0):
+        """One new token of each sequence, q and out [batch][heads][head_dim], over lengths[b] cached positions (its own the last)."""
+        batch, heads, d = q.shape
+        _rows(q, "q", (batch, heads, self.desc.head_dim), self.dtype)
+        _rows(out, "out", q.shape, self.dtype)
+        width = table.shape[1]
+        self.ctx.check(lib().aig_paged_attention(self.ctx.handle, self._ref, _heads(q), _heads(out), _device_ints(table, "table", (batch, width)), width,
+                                                 _device_ints(lengths, "lengths", (batch,)), batch, max_length, d ** -0.5 if scale is None else scale,
+                                                 window, sinks))
+        return out
+
+
+class PagePool:
+    """aig_page_pool: which sequence has which pages (host bookkeeping; copies are made by PagedCache.copy_pages)."""
+
+    def __init__(self, num_pages, page_size):
+        self.handle = c_void_p()
+        self._call("aig_page_pool_create", num_pages, page_size, ctypes.byref(self.handle), bare=True)
+
+    def _call(self, name, *args, bare=False):
+        rc = getattr(lib(), name)(*(args if bare else (self.handle,) + args))
+        if rc < 0:
+            raise AigError(rc, "%s: %s" % (name, "too few free pages" if rc == -6 else "bad argument"))
+        return rc
+
+    def open(self):
+        seq = c_int()
+        self._call("aig_page_pool_open", ctypes.byref(seq))
+        return seq.value
+
+    def grow(self, seq, tokens):
+        """Room for `tokens` more; the copy to make first as (source, destination), or None."""
+        src, dst = c_int(), c_int()
+        self._call("aig_page_pool_grow", seq, tokens, ctypes.byref(src), ctypes.byref(dst))
+        return None if dst.value < 0 else (src.value, dst.value)
+
+    def fork(self, seq):
+        new = c_int()
+        self._call("aig_page_pool_fork", seq, ctypes.byref(new))
+        return new.value
+
+    def trim(self, seq, window, sinks=0):
+        self._call("aig_page_pool_trim", seq, window, sinks)
+
+    def close_sequence(self, seq):
+        self._call("aig_page_pool_close", seq)
+
+    def compact(self, capacity):
+        """(sources, destinations) of the copies to make."""
+        src, dst, n = (c_int * max(capacity, 1))(), (c_int * max(capacity, 1))(), c_int()
+        self._call("aig_page_pool_compact", ctypes.cast(src, P), ctypes.cast(dst, P), capacity, ctypes.byref(n))
+        return list(src[:n.value]), list(dst[:n.value])
+
+    def table(self, seq, width):
+        out = (c_int * max(width, 1))()
+        self._call("aig_page_pool_table", seq, ctypes.cast(out, P), width)
+        return list(out[:width])
+
+    def length(self, seq):
+        return self._call("aig_page_pool_length", seq)
+
+    def shared(self, page):
+        return self._call("aig_page_pool_shared", page)
+
+    @property
+    def free_pages(self):
+        return self._call("aig_page_pool_free_pages")
+
+    def close(self):
+        if self.handle:
+            lib().aig_page_pool_destroy(self.handle)
+            self.handle = c_void_p()
+
+
+def _seq_heads(t):
+    s = t.stride()
+    return ctypes.byref(SeqHeads(t.data_ptr(), s[0], s[1], s[2]))
+
+
+class WindowAttention:
+    """aig_window_attention_*: causal attention over whole sequences with a sliding window and sinks, and its gradients.
+    q, out [batch][q_len][heads][head_dim], k, v [batch][kv_len][kv_heads][head_dim], lse fp32 [batch][heads][q_len]."""
+
+    def __init__(self, ctx, window=0, sinks=0, scale=None):
+        self.ctx, self.window, self.sinks, self.scale = ctx, window, sinks, scale
+
+    def _desc(self, q, k, lse, like_q, like_k, lengths):
+        import torch
+
+        batch, q_len, heads, dim = _rows(q, "q", 4).shape
+        kv_len, kv_heads = _rows(k, "k", 4).shape[1:3]
+        _rows(k, "k", (batch, kv_len, kv_heads, dim))
+        for t in like_q:
+            _rows(t, "a tensor of q's shape", q.shape)
+        for t in like_k:
+            _rows(t, "a tensor of k's shape", k.shape)
+        for t in lse:
+            if not t.is_contiguous():
+                raise ValueError("lse and delta are dense")
+            _rows(t, "lse or delta", (batch, heads, q_len), torch.float32)
+        return (ctypes.byref(WindowDesc(_dtype_of(q, k, *like_q, *like_k), batch, q_len, kv_len, heads, kv_heads, dim, self.window, self.sinks,
+                                        dim ** -0.5 if self.scale is None else self.scale)),
+                None if lengths is None else _device_ints(lengths, "lengths", (batch,)))
+
+    def forward(self, q, k, v, out, lse, lengths=None):
+        desc, n = self._desc(q, k, (lse,), (out,), (v,), lengths)
+        self.ctx.check(lib().aig_window_attention_forward(self.ctx.handle, desc, _seq_heads(q), _seq_heads(k), _seq_heads(v), _seq_heads(out),
+                                                          lse.data_ptr(), n))
+        return out
+
+    def backward(self, q, k, v, out, lse, dout, dq, dk, dv, delta, lengths=None):
+        """`delta`: scratch of lse's shape."""
+        desc, n = self._desc(q, k, (lse, delta), (out, dout, dq), (v, dk, dv), lengths)
+        self.ctx.check(lib().aig_window_attention_backward(self.ctx.handle, desc, _seq_heads(q), _seq_heads(k), _seq_heads(v), _seq_heads(out),
+                                                           lse.data_ptr(), _seq_heads(dout), _seq_heads(dq), _seq_heads(dk), _seq_heads(dv),
+                                                           delta.data_ptr(), n))
+        return dq, dk, dv
 
 
 class Recording:

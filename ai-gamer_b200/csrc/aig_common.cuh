@@ -29,6 +29,9 @@ struct aig_graph {
 
 int aig_fail(aig_ctx* ctx, int code, const char* fmt, ...);
 
+// Codes of the device error word that are no expired wait: what a kernel of the paged cache found and left out
+constexpr int kErrBadPage = 1001, kErrBadPlace = 1002;
+
 // FC plans whose weight operand is produced inside the library (igemm_tcgen05.cu): the K-major buffer
 // [out_c][in_c] to write in place, the epilogue's fp32 shift [out_c] (the bias), and the identity epilogue folded once.
 struct aig_conv_plan;

@@ -106,6 +106,8 @@ int aig_ctx_sync(aig_ctx* ctx) {
   if (code != 0) {
     cudaMemsetAsync(ctx->d_err, 0, sizeof(int), ctx->stream);
     cudaStreamSynchronize(ctx->stream);
+    if (code == kErrBadPage) return aig_fail(ctx, AIG_ERR_INVALID, "a paged cache: a table entry that a call needed names no page of the pool");
+    if (code == kErrBadPlace) return aig_fail(ctx, AIG_ERR_INVALID, "a paged cache: a position or length beyond the page table, or a sequence number beyond the batch");
     return aig_fail(ctx, AIG_ERR_TIMEOUT, "a bounded device-side wait expired (kernel site code %d)", code);
   }
   return AIG_OK;

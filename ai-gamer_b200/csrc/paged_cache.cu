@@ -1,0 +1,502 @@
+// paged_cache.cu -- copies of a cache's pages, and attention of one new token of each sequence over its pages.
+#include <cooperative_groups.h>
+#include <string.h>
+
+#include <new>
+#include <type_traits>
+#include <vector>
+
+#include "long_context.h"
+
+namespace cg = cooperative_groups;
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------
+// Page copies.  The pairs travel as kernel parameters: nothing to upload, nothing that a later call could overwrite while
+// an earlier one (or a captured graph) still reads it.
+constexpr int kPairs = 1000;  // per launch
+constexpr int kCopyThreads = 256, kCopyUnroll = 4;
+
+struct CopyParams {
+  uint4 *k, *v;
+  long long page, place, head;  // strides in 16-byte units
+  int run, heads;               // consecutive 16-byte units of a run; runs: places x heads (1 x 1 where a page is one run)
+  int units, blocks;            // of a page, and blocks that copy it
+  int32_t src[kPairs], dst[kPairs];
+};
+
+__global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyParams p) {
+  const int pair = blockIdx.x / p.blocks;
+  const int first = (blockIdx.x - pair * p.blocks) * kCopyThreads * kCopyUnroll + threadIdx.x;
+  uint4* const base = blockIdx.y ? p.v : p.k;
+  const uint4* const src = base + p.src[pair] * p.page;
+  uint4* const dst = base + p.dst[pair] * p.page;
+  uint4 got[kCopyUnroll];
+  long long at[kCopyUnroll];
+#pragma unroll
+  for (int i = 0; i < kCopyUnroll; ++i) {
+    const int u = first + i * kCopyThreads;
+    const int run = u / p.run, place = run / p.heads;
+    at[i] = place * p.place + (run - place * p.heads) * p.head + (u - run * p.run);
+    if (u < p.units) got[i] = __ldcs(src + at[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kCopyUnroll; ++i)
+    if (first + i * kCopyThreads < p.units) dst[at[i]] = got[i];
+}
+
+// ---------------------------------------------------------------------------------------------
+// Attention of one new token.  For each (sequence, cached head) the visible positions are split over the CTAs of a cluster
+// and over their warps; a warp takes tiles of 16 positions through a ring of shared memory filled by cp.async, and holds the
+// query heads of the group as the 16 rows of mma.sync products (the tensor cores' only use here is that 16 query heads
+// cost no more instructions than one: the kernel is bound by reading the cache).  Softmax with a running maximum and sum
+// in fp32; the weights enter the second product as a sum of two 16-bit values each, so that their rounding does not add to
+// the result's.  Warps are joined in shared memory, CTAs over the cluster's distributed shared memory, in a fixed order: one
+// launch, no scratch in global memory, nothing that two calls or captured graphs could share.
+constexpr int kWarps = 4;
+constexpr int kTile = 16;      // positions
+constexpr int kRows = 16;      // query heads per CTA
+constexpr int kMaxCluster = 16;
+
+struct AttendParams {
+  const uint8_t *k, *v, *q;
+  uint8_t* out;
+  long long page, place, head;                 // cache strides in bytes
+  long long q_seq, q_head, out_seq, out_head;  // in bytes
+  const int32_t *table, *lengths;
+  int table_width, page_size, num_pages;
+  int kv_heads, group, row_blocks;             // query heads per cached one, in blocks of kRows
+  int splits;
+  int window, sinks;
+  float scale_log2;                            // scale * log2(e)
+  int* gerr;
+};
+
+template <int D>
+struct AttendShape {
+  static constexpr int kStages = D == 64 ? 4 : 3;
+  static constexpr int kRowBytes = D * 2;
+  static constexpr int kTileBytes = kTile * kRowBytes;              // of keys, and of values
+  static constexpr int kRing = kWarps * kStages * 2 * kTileBytes;   // 64 KB, 96 KB
+  static constexpr int kJoin = kWarps * kRows * (D + 2) * 4;        // the warps' sums take the ring's place
+  static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
+  static constexpr int kCtasPerSm = D == 64 ? 3 : 2;
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+  const int bytes = there ? 16 : 0;  // 0: the destination is filled with zeros, nothing is read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <class T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// a pair of weights as the sum of two pairs of 16-bit values
+template <class T>
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = pack2<T>(x, y);
+  const float2 h = unpack2<T>(hi);
+  lo = pack2<T>(x - h.x, y - h.y);
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(kWarps * 32, AttendShape<D>::kCtasPerSm) paged_attention_kernel(const __grid_constant__ AttendParams p) {
+  using S = AttendShape<D>;
+  constexpr int kChunks = D / 8;             // 16-byte pieces of a row
+  constexpr int kLoads = kTile * kChunks / 32;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float s_scale[kMaxCluster][kRows];
+  cg::cluster_group cluster = cg::this_cluster();
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = blockIdx.x % p.splits;
+  int item = blockIdx.x / p.splits;
+  const int row_block = item % p.row_blocks;
+  item /= p.row_blocks;
+  const int b = item / p.kv_heads, kvh = item - b * p.kv_heads;
+  const int rows = min(p.group - row_block * kRows, kRows);
+  const int q_head0 = kvh * p.group + row_block * kRows;
+
+  // visible positions: `front` of them from 0 on, the others from `back` on
+  int len = p.lengths[b];
+  const long long most = (long long)p.table_width * p.page_size;
+  if (len > most) {
+    if (threadIdx.x == 0) note_error(p.gerr, kErrBadPlace);
+    len = (int)most;
+  }
+  int front = 0, back = 0, visible = max(len, 0);
+  if (p.window > 0 && len > p.window) {
+    back = len - p.window;
+    front = min(p.sinks, back);
+    visible = front + p.window;
+  }
+  // this CTA's share, in whole tiles; its warps take the tiles in turn
+  const int tiles = (visible + kTile - 1) / kTile;
+  const int share = (tiles + p.splits - 1) / p.splits;
+  const int tile_end = min((split + 1) * share, tiles);
+  const int tile0 = split * share + warp;
+
+  // ---- queries as the A operand: rows are query heads
+  uint32_t qa[D / 16][4];
+  {
+    const int r0 = lane >> 2, c = (lane & 3) * 2;
+    const uint8_t* q = p.q + b * p.q_seq + c * 2;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = r0 + (e & 1) * 8, col = ks * 16 + (e >> 1) * 8;
+        qa[ks][e] = r < rows ? *reinterpret_cast<const uint32_t*>(q + (q_head0 + r) * p.q_head + col * 2) : 0u;
+      }
+  }
+
+  const uint32_t ring = smem_u32(smem) + warp * S::kStages * 2 * S::kTileBytes;
+  const uint8_t* const kbase = p.k + kvh * p.head;
+  const uint8_t* const vbase = p.v + kvh * p.head;
+  const int32_t* const pages = p.table + (long long)b * p.table_width;
+
+  // Row `lane` of a tile (lanes 0..15): its page (-1: none) and its place there, looked up one tile before it is loaded so
+  // that the table's latency is not in the way.
+  int row_page = -1, row_place = 0;
+  auto look_up = [&](int tile) {
+    const int i = tile * kTile + (lane & 15);
+    row_page = -1;
+    if (tile < tile_end && i < visible) {
+      const int t = i < front ? i : back + (i - front);
+      const int slot = t / p.page_size;
+      row_place = t - slot * p.page_size;
+      row_page = pages[slot];
+      if (row_page < 0 || row_page >= p.num_pages) {
+        note_error(p.gerr, kErrBadPage);
+        row_page = -1;
+      }
+    }
+  };
+  auto load = [&](int tile, int stage) {
+    if (tile < tile_end) {
+      const long long mine = row_page < 0 ? -1 : row_page * p.page + row_place * p.place;
+      const uint32_t kd = ring + stage * 2 * S::kTileBytes, vd = kd + S::kTileBytes;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int piece = i * 32 + lane, r = piece / kChunks, c = piece % kChunks;
+        const long long at = __shfl_sync(0xffffffffu, mine, r);
+        const uint32_t to = r * S::kRowBytes + ((c ^ (r & 7)) << 4);  // pieces of 8 rows fall into different banks
+        cp_async16(kd + to, kbase + (at < 0 ? 0 : at) + c * 16, at >= 0);
+        cp_async16(vd + to, vbase + (at < 0 ? 0 : at) + c * 16, at >= 0);
+      }
+    }
+    cp_async_commit();  // (an empty group where there is no tile: groups are counted)
+  };
+
+  float o[D / 8][4];
+#pragma unroll
+  for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+  float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};  // of rows lane/4 and lane/4 + 8, sums of this lane's columns
+
+  look_up(tile0);
+#pragma unroll
+  for (int s = 0; s < S::kStages - 1; ++s) {
+    load(tile0 + s * kWarps, s);
+    look_up(tile0 + (s + 1) * kWarps);
+  }
+  int stage = 0;
+  for (int tile = tile0; tile < tile_end; tile += kWarps) {
+    cp_async_wait<S::kStages - 2>();
+    __syncwarp();
+    {
+      const int next = tile + (S::kStages - 1) * kWarps;
+      load(next, stage == 0 ? S::kStages - 1 : stage - 1);
+      look_up(next + kWarps);
+    }
+    const uint32_t kd = ring + stage * 2 * S::kTileBytes, vd = kd + S::kTileBytes;
+    // ---- scores of 16 positions
+    float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    {
+      const int r = (lane & 7) + ((lane >> 4) << 3), c0 = (lane >> 3) & 1;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        uint32_t kb[4];
+        ldmatrix4(kd + r * S::kRowBytes + (((ks * 2 + c0) ^ (r & 7)) << 4), kb);
+        mma16816<T>(sc[0], qa[ks], kb[0], kb[1]);
+        mma16816<T>(sc[1], qa[ks], kb[2], kb[3]);
+      }
+    }
+    const int left = visible - tile * kTile;  // positions from here on
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int col = n * 8 + (lane & 3) * 2 + (e & 1);
+        sc[n][e] = col < left ? sc[n][e] * p.scale_log2 : -INFINITY;
+      }
+    float mx[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float m = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      mx[h] = fmaxf(m, top[h]);
+    }
+    if (__any_sync(0xffffffffu, mx[0] > top[0] || mx[1] > top[1])) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float f = exp2f(top[h] - mx[h]);  // (a tile has a visible position, so mx is finite if the scores are)
+        top[h] = mx[h];
+        sum[h] *= f;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+          o[n][2 * h] *= f;
+          o[n][2 * h + 1] *= f;
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sc[n][e] = exp2f(sc[n][e] - top[e >> 1]);
+        sum[e >> 1] += sc[n][e];
+      }
+    uint32_t hi[4], lo[4];
+    split2<T>(sc[0][0], sc[0][1], hi[0], lo[0]);
+    split2<T>(sc[0][2], sc[0][3], hi[1], lo[1]);
+    split2<T>(sc[1][0], sc[1][1], hi[2], lo[2]);
+    split2<T>(sc[1][2], sc[1][3], hi[3], lo[3]);
+    {
+      const int r = lane & 15, c0 = lane >> 4;
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) {
+        uint32_t vb[4];
+        ldmatrix4_trans(vd + r * S::kRowBytes + (((n * 2 + c0) ^ (r & 7)) << 4), vb);
+        mma16816<T>(o[2 * n], hi, vb[0], vb[1]);
+        mma16816<T>(o[2 * n + 1], hi, vb[2], vb[3]);
+        mma16816<T>(o[2 * n], lo, vb[0], vb[1]);
+        mma16816<T>(o[2 * n + 1], lo, vb[2], vb[3]);
+      }
+    }
+    __syncwarp();  // the stage is free for the load after next
+    stage = stage + 1 == S::kStages ? 0 : stage + 1;
+  }
+  cp_async_wait<0>();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+    sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+  }
+
+  // ---- join the warps: [warp][row][D] weighted sums, then [warp][row] maxima and sums, in the ring's place
+  __syncthreads();
+  float* const acc = reinterpret_cast<float*>(smem);
+  float* const tops = acc + kWarps * kRows * D;
+  float* const sums = tops + kWarps * kRows;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = (lane >> 2) + 8 * h;
+    if (r < rows) {
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+        *reinterpret_cast<float2*>(acc + (warp * kRows + r) * D + n * 8 + (lane & 3) * 2) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+    }
+    if ((lane & 3) == 0) {
+      tops[warp * kRows + r] = top[h];
+      sums[warp * kRows + r] = sum[h];
+    }
+  }
+  __syncthreads();
+  // each warp's factor, and the CTA's maximum and sum in the first warp's place
+  if (threadIdx.x < kRows) {
+    const int r = threadIdx.x;
+    float m = tops[r], f[kWarps], total = 0.f;
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) m = fmaxf(m, tops[w * kRows + r]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float mw = tops[w * kRows + r];
+      f[w] = mw == -INFINITY ? 0.f : exp2f(mw - m);  // a warp without a position has the weight 0
+      total += f[w] * sums[w * kRows + r];
+    }
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) s_scale[w][r] = f[w];
+    tops[r] = m;
+    sums[r] = total;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * D; i += kWarps * 32) {
+    const int r = i / D;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) v = fmaf(s_scale[w][r], acc[w * kRows * D + i], v);
+    acc[i] = v;
+  }
+  // ---- join the CTAs: each takes a share of the outputs
+  if (p.splits > 1) cluster.sync();
+  else __syncthreads();
+  if (threadIdx.x < kRows) {
+    const int r = threadIdx.x;
+    float m = -INFINITY, total = 0.f;
+    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, *cluster.map_shared_rank(tops + r, s));
+    for (int s = 0; s < p.splits; ++s) {
+      const float ms = *cluster.map_shared_rank(tops + r, s);
+      const float f = ms == -INFINITY ? 0.f : exp2f(ms - m);
+      s_scale[s][r] = f;
+      total += f * *cluster.map_shared_rank(sums + r, s);
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;  // nothing visible: zeros
+    for (int s = 0; s < p.splits; ++s) s_scale[s][r] *= inv;
+  }
+  __syncthreads();
+  const int pairs = rows * (D / 2);
+  for (int i = split * kWarps * 32 + threadIdx.x; i < pairs; i += p.splits * kWarps * 32) {
+    const int r = i / (D / 2);
+    float2 v = make_float2(0.f, 0.f);
+    for (int s = 0; s < p.splits; ++s) {
+      const float2 x = *cluster.map_shared_rank(reinterpret_cast<float2*>(acc) + i, s);
+      const float f = s_scale[s][r];
+      v.x = fmaf(f, x.x, v.x);
+      v.y = fmaf(f, x.y, v.y);
+    }
+    uint8_t* out = p.out + b * p.out_seq + (q_head0 + r) * p.out_head;
+    *reinterpret_cast<uint32_t*>(out + (i - r * (D / 2)) * 4) = pack2<T>(v.x, v.y);
+  }
+  if (p.splits > 1) cluster.sync();  // nobody leaves while its shared memory is read
+}
+
+template <class T, int D>
+int launch_attend(aig_ctx* ctx, const AttendParams& p, int items) {
+  using S = AttendShape<D>;
+  auto kernel = paged_attention_kernel<T, D>;
+  AIG_CUDA_OK(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+  if (p.splits > 8) AIG_CUDA_OK(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)items * p.splits);
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  AIG_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, kernel, p));
+  return AIG_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int aig_kv_copy_pages(aig_ctx* ctx, const aig_kv_cache* cache, const int32_t* src, const int32_t* dst, int pairs) {
+  if (!ctx) return AIG_ERR_INVALID;
+  DeviceGuard g(ctx->device);
+  const int rc = check_cache(ctx, cache, "kv copy pages");
+  if (rc != AIG_OK) return rc;
+  AIG_REQUIRE(ctx, pairs >= 0 && (pairs == 0 || (src && dst)), "kv copy pages: null list or negative number");
+  try {
+    std::vector<uint8_t> role(cache->num_pages, 0);  // 1: a source, 2: a destination
+    for (int i = 0; i < pairs; ++i) {
+      AIG_REQUIRE(ctx, src[i] >= 0 && src[i] < cache->num_pages && dst[i] >= 0 && dst[i] < cache->num_pages,
+                  "kv copy pages: pair %d (%d -> %d) names no page of the pool", i, src[i], dst[i]);
+      AIG_REQUIRE(ctx, role[dst[i]] == 0 && !(role[src[i]] & 2) && src[i] != dst[i],
+                  "kv copy pages: pair %d (%d -> %d): a page is a destination twice, or a source and a destination", i, src[i], dst[i]);
+      role[src[i]] |= 1;
+      role[dst[i]] |= 2;
+    }
+  } catch (const std::bad_alloc&) {
+    return aig_fail(ctx, AIG_ERR_CUDA, "kv copy pages: out of host memory");
+  }
+  CopyParams p;
+  p.k = (uint4*)cache->k;
+  p.v = (uint4*)cache->v;
+  p.page = cache->page_stride / 8;
+  p.place = cache->token_stride / 8;
+  p.head = cache->head_stride / 8;
+  const long long units = (long long)cache->page_size * cache->kv_heads * (cache->head_dim / 8);
+  if (units > (1ll << 30)) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "kv copy pages: pages above 16 GB");
+  p.units = (int)units;
+  const int row = cache->head_dim / 8;
+  const bool places_outside = (cache->kv_heads == 1 || p.head == row) && (cache->page_size == 1 || p.place == (long long)row * cache->kv_heads);
+  const bool heads_outside = (cache->page_size == 1 || p.place == row) && (cache->kv_heads == 1 || p.head == (long long)row * cache->page_size);
+  p.run = places_outside || heads_outside ? p.units : row;
+  p.heads = places_outside || heads_outside ? 1 : cache->kv_heads;
+  p.blocks = (int)ceil_div_ll(units, kCopyThreads * kCopyUnroll);
+  for (int done = 0; done < pairs; done += kPairs) {
+    const int n = pairs - done < kPairs ? pairs - done : kPairs;
+    memcpy(p.src, src + done, n * sizeof(int32_t));
+    memcpy(p.dst, dst + done, n * sizeof(int32_t));
+    if ((long long)n * p.blocks > 0x7fffffffll) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "kv copy pages: too much for one call");
+    copy_pages_kernel<<<dim3((unsigned)(n * p.blocks), 2), kCopyThreads, 0, ctx->stream>>>(p);
+    AIG_LAUNCH_OK(ctx);
+  }
+  return AIG_OK;
+}
+
+int aig_paged_attention(aig_ctx* ctx, const aig_kv_cache* cache, const aig_heads* q, const aig_heads* out, const int32_t* table, int table_width,
+                        const int32_t* lengths, int batch, int max_length, float scale, int window, int sinks) {
+  if (!ctx) return AIG_ERR_INVALID;
+  DeviceGuard g(ctx->device);
+  const int rc = check_cache(ctx, cache, "paged attention");
+  if (rc != AIG_OK) return rc;
+  if (cache->head_dim != 64 && cache->head_dim != 128)
+    return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "paged attention: head dimension must be 64 or 128 (got %d)", cache->head_dim);
+  AIG_REQUIRE(ctx, batch >= 0 && table_width > 0 && max_length >= 0 && sinks >= 0, "paged attention: bad extents");
+  AIG_REQUIRE(ctx, scale == scale && scale - scale == 0.f, "paged attention: the scale is not finite");
+  if (batch == 0) return AIG_OK;
+  AIG_REQUIRE(ctx, heads_sane(q) && heads_sane(out) && table && lengths, "paged attention: null tensor or negative stride");
+  AIG_REQUIRE(ctx, heads_vectorised(*q) && heads_vectorised(*out), "paged attention: q and out on 16-byte boundaries, strides multiples of 8");
+  AIG_REQUIRE(ctx, q->heads == out->heads && q->heads % cache->kv_heads == 0, "paged attention: %d query heads, %d in the output, %d cached", q->heads,
+              out->heads, cache->kv_heads);
+  AttendParams p{};
+  p.k = (const uint8_t*)cache->k;
+  p.v = (const uint8_t*)cache->v;
+  p.q = (const uint8_t*)q->data;
+  p.out = (uint8_t*)out->data;
+  p.page = cache->page_stride * 2;
+  p.place = cache->token_stride * 2;
+  p.head = cache->head_stride * 2;
+  p.q_seq = q->token_stride * 2;
+  p.q_head = q->head_stride * 2;
+  p.out_seq = out->token_stride * 2;
+  p.out_head = out->head_stride * 2;
+  p.table = table;
+  p.lengths = lengths;
+  p.table_width = table_width;
+  p.page_size = cache->page_size;
+  p.num_pages = cache->num_pages;
+  p.kv_heads = cache->kv_heads;
+  p.group = q->heads / cache->kv_heads;
+  p.row_blocks = ceil_div(p.group, kRows);
+  p.window = window;
+  p.sinks = sinks;
+  p.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  p.gerr = ctx->d_err;
+  const long long items = (long long)batch * cache->kv_heads * p.row_blocks;
+  if (items * kMaxCluster > 0x7fffffffll) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "paged attention: too many sequences and heads for one call");
+  // Splits: enough CTAs for every SM twice, each with a tile per warp at least.
+  long long visible = max_length;
+  if (window > 0 && visible > (long long)window + sinks) visible = (long long)window + sinks;
+  p.splits = 1;
+  while (p.splits < kMaxCluster && items * p.splits < 4ll * ctx->sm_count && visible > (long long)p.splits * kWarps * kTile) p.splits *= 2;
+  if (cache->dtype == AIG_F16)
+    return cache->head_dim == 64 ? launch_attend<__half, 64>(ctx, p, (int)items) : launch_attend<__half, 128>(ctx, p, (int)items);
+  return cache->head_dim == 64 ? launch_attend<__nv_bfloat16, 64>(ctx, p, (int)items) : launch_attend<__nv_bfloat16, 128>(ctx, p, (int)items);
+}
+
+}  // extern "C"

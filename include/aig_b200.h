@@ -26,7 +26,8 @@ enum {
   AIG_ERR_CUDA = -2,        /* a CUDA runtime/driver call failed */
   AIG_ERR_TIMEOUT = -3,     /* a bounded device-side wait expired (kernel returned early) */
   AIG_ERR_UNSUPPORTED = -4, /* shape outside what the sm_100a kernels cover */
-  AIG_ERR_IO = -5           /* checkpoint file problem */
+  AIG_ERR_IO = -5,          /* checkpoint file problem */
+  AIG_ERR_NO_PAGES = -6     /* a page pool has too few free pages; nothing was changed */
 };
 
 /* activation codes used by the fused epilogues */
@@ -45,7 +46,8 @@ int aig_ctx_destroy(aig_ctx* ctx);
 int aig_ctx_set_stream(aig_ctx* ctx, void* cuda_stream);
 void* aig_ctx_stream(aig_ctx* ctx);
 /* Synchronise the stream and report any deferred kernel error (including AIG_ERR_TIMEOUT raised by a
- * bounded device-side wait).  The device error word is cleared. */
+ * bounded device-side wait, and AIG_ERR_INVALID for a page table that a paged cache could not follow).  The device error
+ * word is cleared. */
 int aig_ctx_sync(aig_ctx* ctx);
 const char* aig_last_error(aig_ctx* ctx);
 /* Self-test of the time-out path every kernel of this library shares (no counterpart in the reference, whose
@@ -405,6 +407,139 @@ int aig_mha_forward(aig_mha_plan* plan, const aig_half* x, aig_half* y, int pos0
  * (absolute frame index; the cache holds the last `window` steps).  aig_mha_reset empties it. */
 int aig_mha_step(aig_mha_plan* plan, const aig_half* x, aig_half* y, int position);
 int aig_mha_reset(aig_mha_plan* plan);
+
+/* ---------------------------------------------------------------------------------------------
+ * Attention over long contexts.  None of this is in the reference, whose attention (MHALayer.cpp:128-146) sees one
+ * sequence of a fixed length; aig_mha_* above covers that and a ring of `window` slots which all sequences of a batch
+ * fill in step.  Here: rotary positions of every common form, a cache in pages for sequences of lengths of their own,
+ * attention of one new token over it, and attention over whole sequences, with gradients.
+ *
+ * Tensors hold fp16 or bf16 values (`dtype`), heads are rows of head_dim consecutive elements, all strides count elements
+ * and are at least 0.  Sums, softmax statistics and angles are held in 32 bits or more and results are rounded once.
+ * Nothing is kept between calls except in the objects that the caller makes, and no call allocates: all of them can be
+ * captured (aig_graph_begin), and captured graphs share nothing but the tensors they were given. */
+enum { AIG_F16 = 0, AIG_BF16 = 1 };
+
+/* A tensor [tokens][heads][head_dim]. */
+typedef struct aig_heads {
+  void* data;
+  int heads;
+  long long token_stride, head_stride;
+} aig_heads;
+
+/* Rotary positions.  The first rot_dim elements of each head are turned in pairs, (2j, 2j+1) if interleaved, else
+ * (j, j + rot_dim/2); pair j of a token at position p by the angle p * f[j], and scaled by `magnitude`; the rest is copied.
+ * f[j] = base^(-2j/rot_dim), and for contexts beyond the original length L = original_len
+ *   AIG_ROPE_LINEAR  f / factor
+ *   AIG_ROPE_RAMP    between f (share 0) and f / factor (share 1), the share rising linearly with the pair's index from
+ *                    floor(j(high)) to ceil(j(low)), where j(t) = rot_dim * ln(L / (2 pi t)) / (2 ln base) is the pair that
+ *                    makes t turns over L; the ends are held within 0 .. rot_dim - 1
+ *   AIG_ROPE_TURNS   the share falls linearly with the turns L * f / (2 pi) from 1 at `low` to 0 at `high`
+ * Angles are exact for every 32-bit position, negative ones too: a frequency is kept as a 64-bit fraction of a turn.
+ * backward applies the transpose, which takes gradients of turned tensors to gradients of the tensors before.
+ * Outputs may be the inputs themselves (same data and strides); other overlaps are not allowed.  k and k_out may both be
+ * null.  head_dim even and at most 1024, rot_dim even. */
+enum { AIG_ROPE_PLAIN = 0, AIG_ROPE_LINEAR = 1, AIG_ROPE_RAMP = 2, AIG_ROPE_TURNS = 3 };
+typedef struct aig_rope_desc {
+  int head_dim, rot_dim;
+  int interleaved;
+  int scaling; /* AIG_ROPE_* */
+  float base, factor;
+  int original_len;
+  float low, high; /* turns over the original length; RAMP and TURNS */
+  float magnitude;
+} aig_rope_desc;
+typedef struct aig_rope_plan aig_rope_plan;
+/* The frequencies in radians per position as the plan uses them, computed on the host; n = rot_dim / 2 values. */
+int aig_rope_frequencies(const aig_rope_desc* desc, double* out, int n);
+int aig_rope_plan_create(aig_ctx* ctx, const aig_rope_desc* desc, aig_rope_plan** out);
+int aig_rope_plan_destroy(aig_rope_plan* plan);
+/* positions: int32 [tokens] on the device. */
+int aig_rope_forward(aig_rope_plan* plan, int dtype, const int32_t* positions, long long tokens, const aig_heads* q, const aig_heads* q_out,
+                     const aig_heads* k, const aig_heads* k_out);
+int aig_rope_backward(aig_rope_plan* plan, int dtype, const int32_t* positions, long long tokens, const aig_heads* dq, const aig_heads* dq_out,
+                      const aig_heads* dk, const aig_heads* dk_out);
+
+/* Keys and values in pages: element (page, place, head, i) of both tensors lies at page * page_stride + place *
+ * token_stride + head * head_stride + i.  A sequence's position p lies at place p % page_size of the page that its row of
+ * the page table (int32, device) names at p / page_size.  head_dim and the strides are multiples of 8, data on 16-byte
+ * boundaries.  A table entry that a call needs and that names no page of the pool, or a position beyond the table's
+ * width, faults nothing: the access is left out and the next aig_ctx_sync returns AIG_ERR_INVALID. */
+typedef struct aig_kv_cache {
+  void *k, *v;
+  int dtype, kv_heads, head_dim, page_size, num_pages;
+  long long page_stride, token_stride, head_stride;
+} aig_kv_cache;
+/* Writes new keys and values to their places: token i belongs to sequence seqs[i] (null: sequence i) at positions[i]; one
+ * with a negative position is padding and left out (its q_out too).  With a rope plan (null: none) keys are turned by
+ * their positions on the way, and queries too: q -> q_out (both may be null).  No two tokens of a call may have the same place.
+ * table [batch][table_width]. */
+int aig_kv_append(aig_ctx* ctx, const aig_kv_cache* cache, aig_rope_plan* rope, const aig_heads* k, const aig_heads* v, const aig_heads* q,
+                  const aig_heads* q_out, const int32_t* seqs, const int32_t* positions, long long tokens, const int32_t* table, int batch,
+                  int table_width);
+/* Copies whole pages, keys and values: src[i] -> dst[i], host arrays.  No page may be a destination twice, or a source
+ * and a destination. */
+int aig_kv_copy_pages(aig_ctx* ctx, const aig_kv_cache* cache, const int32_t* src, const int32_t* dst, int pairs);
+/* Attention of one new token of each sequence over its pages: q, out [batch][q_heads][head_dim] (token_stride from
+ * sequence to sequence), lengths int32 [batch] on the device: positions 0 .. lengths[b]-1 are in the cache, the new token
+ * is the last of them.  Query head h reads cached head h / (q_heads / kv_heads); out = softmax(scale * q.k) v over the
+ * visible positions: the last `window` (<= 0: all) and the first `sinks` (with a window).  Pages without a visible position are
+ * not read and their table entries may be anything; a length of 0 or less gives zeros.  max_length is the host's bound of
+ * the lengths: work is split by it, and lengths above it are as right, only slower.  head_dim 64 or 128. */
+int aig_paged_attention(aig_ctx* ctx, const aig_kv_cache* cache, const aig_heads* q, const aig_heads* out, const int32_t* table, int table_width,
+                        const int32_t* lengths, int batch, int max_length, float scale, int window, int sinks);
+
+/* Host bookkeeping of a cache's pages (no device needed).  A sequence is a number from aig_page_pool_open; pages are
+ * shared by forked sequences and counted.  Calls from several threads at once are the caller's to order.
+ *   grow     makes room for `tokens` more.  Where the page that it writes to next is shared, the sequence gets a page of
+ *            its own, and the copy that aig_kv_copy_pages has to make is handed out (copy_src, copy_dst: -1 for none).
+ *            AIG_ERR_NO_PAGES, and nothing changed, where pages are lacking.
+ *   fork     a new sequence with the same contents; no page is copied
+ *   trim     gives up pages that a window and sinks leave without a visible position now and later (table entries become -1)
+ *   close    gives up the sequence and the pages that nobody else has
+ *   compact  moves the pages in use to the lowest numbers and hands out the copies to make (at most `capacity`, a call
+ *            that would need more moves that many); *pairs of them
+ *   table    writes the page numbers of a sequence, -1 behind the last; returns the pages that its length needs
+ *   length, free_pages, shared (sequences that have this page) return numbers, or a negative status */
+typedef struct aig_page_pool aig_page_pool;
+int aig_page_pool_create(int num_pages, int page_size, aig_page_pool** out);
+int aig_page_pool_destroy(aig_page_pool* pool);
+int aig_page_pool_open(aig_page_pool* pool, int* seq);
+int aig_page_pool_grow(aig_page_pool* pool, int seq, int tokens, int32_t* copy_src, int32_t* copy_dst);
+int aig_page_pool_fork(aig_page_pool* pool, int seq, int* new_seq);
+int aig_page_pool_trim(aig_page_pool* pool, int seq, int window, int sinks);
+int aig_page_pool_close(aig_page_pool* pool, int seq);
+int aig_page_pool_compact(aig_page_pool* pool, int32_t* copy_src, int32_t* copy_dst, int capacity, int* pairs);
+int aig_page_pool_table(const aig_page_pool* pool, int seq, int32_t* out, int width);
+int aig_page_pool_length(const aig_page_pool* pool, int seq);
+int aig_page_pool_free_pages(const aig_page_pool* pool);
+int aig_page_pool_shared(const aig_page_pool* pool, int page);
+
+/* Attention over whole sequences: q, out [batch][q_len][heads][head_dim], k, v [batch][kv_len][kv_heads][head_dim], lse
+ * fp32 [batch][heads][q_len].  Query row i stands at position i + kv_len - q_len (q_len <= kv_len: a prompt's last part
+ * against all of it) and sees the keys at positions up to its own: the last `window` of them (<= 0: all) and the first
+ * `sinks`.  Query head h reads head h / (heads / kv_heads).  out = softmax(scale * q.k) v; lse = ln sum exp(scale * q.k).
+ * lengths (int32 [batch] on the device, or null) ends each sequence: rows of q at or behind it are neither read for others
+ * nor written, rows of k and v behind it are not read for others, whatever they hold.  Values of rows that are there have
+ * to be finite: a product with the weight 0 of a key in the same tile of 128 that the mask hides is computed.
+ * backward: from the forward's inputs, out, lse and the gradient dout, writes dq, dk, dv (each rounded once; dk and dv
+ * summed over the query heads that read them, in a fixed order); rows at or behind a sequence's length are left as they
+ * were.  delta: fp32 scratch of lse's shape, the caller's.
+ * head_dim 64 or 128; data on 16-byte boundaries, strides multiples of 8. */
+typedef struct aig_seq_heads {
+  void* data;
+  long long batch_stride, token_stride, head_stride;
+} aig_seq_heads;
+typedef struct aig_window_desc {
+  int dtype, batch, q_len, kv_len, heads, kv_heads, head_dim;
+  int window, sinks;
+  float scale;
+} aig_window_desc;
+int aig_window_attention_forward(aig_ctx* ctx, const aig_window_desc* desc, const aig_seq_heads* q, const aig_seq_heads* k,
+                                 const aig_seq_heads* v, const aig_seq_heads* out, float* lse, const int32_t* lengths);
+int aig_window_attention_backward(aig_ctx* ctx, const aig_window_desc* desc, const aig_seq_heads* q, const aig_seq_heads* k,
+                                  const aig_seq_heads* v, const aig_seq_heads* out, const float* lse, const aig_seq_heads* dout,
+                                  const aig_seq_heads* dq, const aig_seq_heads* dk, const aig_seq_heads* dv, float* delta, const int32_t* lengths);
 
 /* Output decisions of Infer::ProcessOutput (Infer.cpp:8-57) as a pure function on host values:
  * actions[i] = p[i] > 0.5 for i < n_buttons, (int)(p[i]*256.0f) otherwise. */
