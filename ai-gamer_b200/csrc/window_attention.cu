@@ -4,12 +4,20 @@
 //   S = scale * Q K^T,  P = softmax(S) over the keys j <= p that are within `window` of p or below `sinks`,  O = P V
 //   dV = P^T dO,  dP = dO V^T,  D = rowsum(dO o O),  dS = scale * P o (dP - D),  dQ = dS K,  dK = dS^T Q
 //
-// A row per warp, a value of the head per lane and register; softmax with a running maximum and sum in fp32.
+// Forward: tiles of 128 queries x 128 keys on tcgen05.  A CTA has one or two tiles of queries, each with 128 threads that
+// own a row of scores; one warp fetches tiles by TMA, one issues the products.  Scores and outputs stay in TMEM; the
+// weights go back to TMEM as 16-bit values over the scores and are the second product's A operand from there, V its B
+// operand as it lies in memory (MN-major).  Tiles that the window, the sinks and the causal order leave empty are not
+// visited; only tiles that they cut are masked.
+#include <type_traits>
+
 #include "long_context.h"
 
 namespace {
 
 constexpr int kWarps = 4;
+constexpr int kTile = 128;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct View {
   uint8_t* data;
@@ -23,7 +31,96 @@ struct WinParams {
   int batch, q_len, kv_len, heads, kv_heads;
   int window, sinks;
   float scale;
+  int blocks;  // of query rows per head
+  int* gerr;
 };
+
+// ---- PTX that the other kernels have no use for
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* desc, uint32_t bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(desc)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+      "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 2^x on the special-function unit (relative error 2^-22; -inf gives 0)
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Shared-memory descriptor of an operand whose rows (of 128 bytes, swizzled) run along the product's K dimension: 64
+// elements of M or N per row, the next 64 `block` bytes on, groups of eight rows 1024 bytes apart.
+__device__ __forceinline__ uint64_t umma_smem_desc_mn(uint32_t saddr, uint32_t block) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(block >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+template <class T>
+__host__ __device__ constexpr uint32_t idesc_for(int m, int n, bool b_mn_major) {
+  return umma_idesc_f16(m, n) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7 | 1u << 10) : 0u) | (b_mn_major ? 1u << 16 : 0u);
+}
+
+// A tile of 128 rows of D elements as D/64 blocks of [128 rows][64 elements], 128-byte swizzled
+template <int D>
+constexpr uint32_t kTileBytes = kTile * D * 2;
+template <int D>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int head, int row, int b) {
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) tma_load_4d(dst + c * kTile * 128, map, bar, c * 64, head, row, b);
+}
+// K-major operand, K step `ks` of 16 elements
+__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int ks) { return umma_smem_desc(tile + (ks >> 2) * kTile * 128 + (ks & 3) * 32, 128); }
+// the same tile with its rows as the K dimension, K step of 16 rows
+__device__ __forceinline__ uint64_t desc_rows(uint32_t tile, int ks) { return umma_smem_desc_mn(tile + ks * 16 * 128, kTile * 128); }
+// Rows from `from` on become zeros (a product with the weight 0 would keep a NaN); by one warp, before the product reads them
+template <int D>
+__device__ __forceinline__ void clear_rows(uint8_t* tile, int from, int lane) {
+  const int pieces = (kTile - from) * 8;
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c)
+    for (int i = lane; i < pieces; i += 32) *reinterpret_cast<uint4*>(tile + c * kTile * 128 + from * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// Key tiles that a tile of queries at positions first .. last visits: [0, sink_end) and [begin, end)
+struct KeyTiles {
+  int sink_end, begin, end;
+  __device__ __forceinline__ bool has(int t) const { return t < sink_end || (t >= begin && t < end); }
+};
+__device__ __forceinline__ KeyTiles key_tiles(int first, int last, int window, int sinks) {
+  KeyTiles k;
+  k.begin = window > 0 ? max(0, first - window + 1) / kTile : 0;
+  k.end = last < first ? k.begin : last / kTile + 1;
+  k.sink_end = window > 0 && last >= first ? min((sinks + kTile - 1) / kTile, k.begin) : 0;
+  return k;
+}
 
 template <class T>
 __device__ __forceinline__ T* row_of(const View& v, int b, int t, int h) {
@@ -56,31 +153,263 @@ __device__ __forceinline__ void keys_of(const WinParams& p, int pos, int& front,
   front = min(p.sinks, back);
 }
 
-template <class T, int D>
-__global__ void __launch_bounds__(kWarps * 32) forward_rows_kernel(const __grid_constant__ WinParams p) {
-  constexpr int N = D / 32;
-  const int lane = threadIdx.x & 31, i = blockIdx.x * kWarps + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z;
-  const int pos = i + p.kv_len - p.q_len;
-  if (i >= p.q_len || pos >= length_of(p, b)) return;
+// ---------------------------------------------------------------------------------------------
+// Forward
+template <int D, int NT>  // NT tiles of queries
+struct FwdShape {
+  static constexpr int kStages = NT == 2 ? (D == 64 ? 4 : 2) : 2;
+  static constexpr int kThreads = 128 + 128 * NT;
+  static constexpr int kCtasPerSm = NT == 2 ? 1 : (D == 64 ? 2 : 1);
+  static constexpr int kTmemCols = NT == 2 ? 512 : 256;  // scores 128 columns a tile, then outputs D columns a tile
+  static constexpr uint32_t kQ = NT * kTileBytes<D>;
+  static constexpr size_t kSmem = kQ + 2 * kStages * kTileBytes<D> + 1024 + 256;
+};
+constexpr float kLazy = 8.f;  // a row's maximum may grow by 2^8 before its sums are rescaled: weights stay below 2^8
+
+template <class T, int D, int NT>
+__global__ void __launch_bounds__(FwdShape<D, NT>::kThreads, FwdShape<D, NT>::kCtasPerSm)
+window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
+                      const __grid_constant__ WinParams p) {
+  using S = FwdShape<D, NT>;
+  constexpr int NS = S::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* const sm = smem_raw + (base - raw);
+  const uint32_t sQ = base, sK = sQ + S::kQ, sV = sK + NS * kTileBytes<D>;
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(sm + S::kQ + 2 * NS * kTileBytes<D>);
+  const uint32_t bar0 = smem_u32(bars);
+  const uint32_t q_full = bar0, s_full = bar0 + 8, p_full = s_full + 8 * NT, o_full = p_full + 8 * NT, k_full = o_full + 8 * NT,
+                 k_free = k_full + 8 * NS, v_full = k_free + 8 * NS, v_free = v_full + 8 * NS;
+  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bars + 1 + 3 * NT + 4 * NS);
+  volatile int* const s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+
+  // the blocks of the last queries, which see the most keys, come first
+  int item = blockIdx.x;
+  const int b = item % p.batch;
+  item /= p.batch;
+  const int h = item % p.heads, block = p.blocks - 1 - item / p.heads;
   const int kvh = h / (p.heads / p.kv_heads);
-  float q[N], o[N] = {}, x[N];
-  load_row<T>(q, row_of<T>(p.q, b, i, h), lane);
-  float top = -INFINITY, sum = 0.f;
-  int front, back;
-  keys_of(p, pos, front, back);
-  for (int j = front > 0 ? 0 : back; j <= pos; j = j + 1 == front ? back : j + 1) {
-    load_row<T>(x, row_of<T>(p.k, b, j, kvh), lane);
-    const float s = dot(q, x) * p.scale, m = fmaxf(top, s), f = expf(top - m), w = expf(s - m);
-    load_row<T>(x, row_of<T>(p.v, b, j, kvh), lane);
-    sum = sum * f + w;
-    top = m;
+  const int len = p.lengths ? min(max(p.lengths[b], 0), p.kv_len) : p.kv_len;
+  const int off = p.kv_len - p.q_len;  // position of query row 0
+  const int rows_end = min(p.q_len, len - off);
+  KeyTiles kt[NT];
+  int sink_end = 0, begin = 0x7fffffff, end = 0;
 #pragma unroll
-    for (int n = 0; n < N; ++n) o[n] = fmaf(o[n], f, w * x[n]);
+  for (int w = 0; w < NT; ++w) {
+    const int r0 = (block * NT + w) * kTile;
+    kt[w] = key_tiles(off + r0, off + min(r0 + kTile, rows_end) - 1, p.window, p.sinks);
+    if (kt[w].end > kt[w].begin) {
+      sink_end = max(sink_end, kt[w].sink_end);
+      begin = min(begin, kt[w].begin);
+      end = max(end, kt[w].end);
+    }
   }
-  T* out = row_of<T>(p.o, b, i, h);
+  if (end == 0) return;  // no query row within the sequence
+  begin = max(begin, sink_end);
+  const int tiles = sink_end + end - begin;
+  auto tile_at = [&](int it) { return it < sink_end ? it : begin + (it - sink_end); };
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int w = 0; w < NT; ++w) {
+      mbar_init(s_full + 8 * w, 1);
+      mbar_init(p_full + 8 * w, 128);
+      mbar_init(o_full + 8 * w, 1);
+    }
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(k_full + 8 * s, 1);
+      mbar_init(k_free + 8 * s, 1);
+      mbar_init(v_full + 8 * s, 1);
+      mbar_init(v_free + 8 * s, 1);
+    }
+    *s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(s_tmem), S::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  const uint32_t tS = tmem, tO = tmem + 128 * NT;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      mbar_expect_tx(q_full, S::kQ);
 #pragma unroll
-  for (int n = 0; n < N; ++n) out[n * 32 + lane] = from_f32<T>(o[n] / sum);
-  if (lane == 0) p.lse[((long long)b * p.heads + h) * p.q_len + i] = top + logf(sum);
+      for (int w = 0; w < NT; ++w) load_tile<D>(sQ + w * kTileBytes<D>, &mapQ, q_full, h, (block * NT + w) * kTile, b);
+      for (int it = 0; it < tiles; ++it) {
+        const int s = it % NS, row = tile_at(it) * kTile;
+        const uint32_t ph = (uint32_t)(it / NS + 1) & 1u;  // (the first round finds the stages free)
+        if (it >= NS && !mbar_wait_bounded(k_free + 8 * s, ph, s_abort, p.gerr, 1101)) break;
+        mbar_expect_tx(k_full + 8 * s, kTileBytes<D>);
+        load_tile<D>(sK + s * kTileBytes<D>, &mapK, k_full + 8 * s, kvh, row, b);
+        if (it >= NS && !mbar_wait_bounded(v_free + 8 * s, ph, s_abort, p.gerr, 1102)) break;
+        mbar_expect_tx(v_full + 8 * s, kTileBytes<D>);
+        load_tile<D>(sV + s * kTileBytes<D>, &mapV, v_full + 8 * s, kvh, row, b);
+      }
+    }
+  } else if (warp == 1) {
+    constexpr uint32_t idesc_s = idesc_for<T>(kTile, kTile, false), idesc_o = idesc_for<T>(kTile, D, true);
+    const bool leader = elect_one();
+    int done[NT];  // tiles whose second product has been issued
+#pragma unroll
+    for (int w = 0; w < NT; ++w) done[w] = 0;
+    auto scores = [&](int w, int it) {
+      const uint32_t k = sK + (it % NS) * kTileBytes<D>;
+      if (leader) {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) umma_f16_ss(tS + 128 * w, desc_k(sQ + w * kTileBytes<D>, ks), desc_k(k, ks), idesc_s, ks != 0);
+        umma_commit(s_full + 8 * w);
+      }
+    };
+    bool ok = mbar_wait_bounded(q_full, 0, s_abort, p.gerr, 1103) && mbar_wait_bounded(k_full, 0, s_abort, p.gerr, 1104);
+    if (ok) {
+      tc_fence_after();
+#pragma unroll
+      for (int w = 0; w < NT; ++w)
+        if (kt[w].has(tile_at(0))) scores(w, 0);
+      if (leader) umma_commit(k_free);
+      for (int it = 0; it < tiles && ok; ++it) {
+        const int t = tile_at(it), s = it % NS, next = it + 1, ns = next % NS;
+        if (next < tiles && !mbar_wait_bounded(k_full + 8 * ns, (uint32_t)(next / NS) & 1u, s_abort, p.gerr, 1105)) break;
+        if (!mbar_wait_bounded(v_full + 8 * s, (uint32_t)(it / NS) & 1u, s_abort, p.gerr, 1106)) break;
+        if (t * kTile + kTile > len) clear_rows<D>(sm + (sV - base) + s * kTileBytes<D>, len - t * kTile, lane);
+#pragma unroll
+        for (int w = 0; w < NT; ++w) {
+          if (kt[w].has(t)) {
+            if (!(ok = mbar_wait_bounded(p_full + 8 * w, (uint32_t)done[w] & 1u, s_abort, p.gerr, 1107))) break;
+            tc_fence_after();
+            if (leader) {
+#pragma unroll
+              for (int ks = 0; ks < kTile / 16; ++ks)
+                umma_f16_ts(tO + D * w, tS + 128 * w + ks * 8, desc_rows(sV + s * kTileBytes<D>, ks), idesc_o, done[w] != 0 || ks != 0);
+            }
+            ++done[w];
+            if (t + 1 == kt[w].end && leader) umma_commit(o_full + 8 * w);
+          }
+          if (next < tiles && kt[w].has(tile_at(next))) scores(w, next);
+        }
+        if (leader) {
+          umma_commit(v_free + 8 * s);
+          if (next < tiles) umma_commit(k_free + 8 * ns);
+        }
+      }
+    }
+  } else if (warp >= 4) {
+    const int w = (warp - 4) >> 2, q = warp & 3;
+    const int row = (block * NT + w) * kTile + q * 32 + lane, pos = off + row;
+    const int first = off + (block * NT + w) * kTile;  // position of the tile's first row
+    KeyTiles mine = kt[0];
+    if (NT == 2 && w == 1) mine = kt[NT - 1];
+    const uint32_t lanes = (uint32_t)(q * 32) << 16;
+    const uint32_t tSw = tS + 128 * w + lanes, tOw = tO + D * w + lanes;
+    const float c = p.scale * kLog2e;
+    float top = -INFINITY, sum = 0.f;  // top: in units of log2, what the weights are relative to
+    int n = 0;
+    bool ok = true;
+    for (int it = 0; it < tiles; ++it) {
+      const int t = tile_at(it);
+      if (!mine.has(t)) continue;
+      if (!(ok = mbar_wait_bounded(s_full + 8 * w, (uint32_t)n & 1u, s_abort, p.gerr, 1108))) break;
+      tc_fence_after();
+      const int j0 = t * kTile;
+      const bool cut = j0 + kTile - 1 > first || (p.window > 0 && j0 <= first + kTile - 1 - p.window && j0 + kTile > p.sinks);
+      const int lo = p.window > 0 ? pos - p.window + 1 - j0 : -1, hi = pos - j0, sinks = p.sinks - j0;  // columns
+      auto shown = [&](int j) { return j <= hi && (j >= lo || j < sinks); };
+      float m = -INFINITY;
+#pragma unroll
+      for (int c0 = 0; c0 < kTile; c0 += 32) {
+        uint32_t v[32];
+        tmem_ld_32x32(tSw + c0, v);
+        tmem_ld_wait();
+        if (cut) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) m = fmaxf(m, shown(c0 + e) ? __uint_as_float(v[e]) * c : -INFINITY);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) m = fmaxf(m, __uint_as_float(v[e]) * c);
+        }
+      }
+      const bool grew = m > top + kLazy;  // (from -inf any finite value)
+      if (__any_sync(0xffffffffu, grew)) {
+        const float f = grew ? ex2(top - m) : 1.f;
+        if (grew) {
+          top = m;
+          sum *= f;
+        }
+        if (n > 0) {  // the products that went into the output have completed: the scores were issued behind them
+#pragma unroll
+          for (int c0 = 0; c0 < D; c0 += 32) {
+            uint32_t v[32];
+            tmem_ld_32x32(tOw + c0, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+            tmem_st_32x32(tOw + c0, v);
+          }
+        }
+      }
+      const float ref = top == -INFINITY ? 0.f : top;  // a row that has seen no key yet
+#pragma unroll
+      for (int c0 = 0; c0 < kTile; c0 += 32) {
+        uint32_t v[32], o[16];
+        tmem_ld_32x32(tSw + c0, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          float x = ex2(fmaf(__uint_as_float(v[e]), c, -ref)), y = ex2(fmaf(__uint_as_float(v[e + 1]), c, -ref));
+          if (cut) {
+            x = shown(c0 + e) ? x : 0.f;
+            y = shown(c0 + e + 1) ? y : 0.f;
+          }
+          sum += x + y;
+          o[e / 2] = pack2<T>(x, y);
+        }
+        tmem_st_32x16(tSw + c0 / 2, o);  // over scores that have been read
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(p_full + 8 * w);
+      ++n;
+    }
+    if (ok && n > 0 && mbar_wait_bounded(o_full + 8 * w, 0, s_abort, p.gerr, 1109)) {
+      tc_fence_after();
+      const float inv = 1.f / sum;
+      T* const out = reinterpret_cast<T*>(p.o.data) + b * p.o.batch + row * p.o.token + h * p.o.head;
+#pragma unroll
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t v[32];
+        tmem_ld_32x32(tOw + c0, v);
+        tmem_ld_wait();
+        if (row < rows_end) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint4 x;
+            x.x = pack2<T>(__uint_as_float(v[e]) * inv, __uint_as_float(v[e + 1]) * inv);
+            x.y = pack2<T>(__uint_as_float(v[e + 2]) * inv, __uint_as_float(v[e + 3]) * inv);
+            x.z = pack2<T>(__uint_as_float(v[e + 4]) * inv, __uint_as_float(v[e + 5]) * inv);
+            x.w = pack2<T>(__uint_as_float(v[e + 6]) * inv, __uint_as_float(v[e + 7]) * inv);
+            *reinterpret_cast<uint4*>(out + c0 + e) = x;
+          }
+        }
+      }
+      if (row < rows_end) p.lse[((long long)b * p.heads + h) * p.q_len + row] = fmaf(top, kLn2, logf(sum));
+    }
+  }
+
+  if (*s_abort) {
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // copies in flight land
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, S::kTmemCols);
+  }
 }
 
 template <class T, int D>
@@ -169,20 +498,64 @@ WinParams params_of(const aig_window_desc* d) {
   p.kv_len = d->kv_len;
   p.heads = d->heads;
   p.kv_heads = d->kv_heads;
-  p.window = d->window;
-  p.sinks = d->sinks;
+  p.window = d->window > 0 && d->window < d->kv_len ? d->window : 0;  // (one that hides nothing is none)
+  p.sinks = d->sinks < d->kv_len ? d->sinks : d->kv_len;
   p.scale = d->scale;
   return p;
 }
 
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+  static const EncodeTiledFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) == cudaSuccess && found == cudaDriverEntryPointSuccess;
+    return ok ? reinterpret_cast<EncodeTiledFn>(f) : nullptr;
+  }();
+  return fn;
+}
+
+// A tensor [batch][tokens][heads][D] in boxes of 128 tokens x 64 elements of one head; tokens behind the last read as zeros.
 template <class T, int D>
-int forward(aig_ctx* ctx, const WinParams& p) {
-  forward_rows_kernel<T, D><<<dim3(ceil_div(p.q_len, kWarps), p.heads, p.batch), kWarps * 32, 0, ctx->stream>>>(p);
+int encode(aig_ctx* ctx, CUtensorMap* m, const View& v, int batch, int tokens, int heads) {
+  const EncodeTiledFn enc = encode_fn();
+  if (!enc) return aig_fail(ctx, AIG_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available");
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)batch};
+  // (the stride of a dimension of one has no meaning, but has to be a possible one)
+  const cuuint64_t strides[3] = {(cuuint64_t)(heads > 1 ? v.head : D) * 2, (cuuint64_t)(tokens > 1 ? v.token : D) * 2, (cuuint64_t)(batch > 1 ? v.batch : D) * 2};
+  const cuuint32_t box[4] = {64, 1, kTile, 1}, step[4] = {1, 1, 1, 1};
+  const CUresult r = enc(m, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, v.data, dims, strides,
+                         box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return aig_fail(ctx, AIG_ERR_CUDA, "cuTensorMapEncodeTiled failed: %d", (int)r);
+  return AIG_OK;
+}
+
+template <class T, int D, int NT>
+int launch_forward(aig_ctx* ctx, WinParams& p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv) {
+  using S = FwdShape<D, NT>;
+  p.blocks = ceil_div(p.q_len, kTile * NT);
+  const long long grid = (long long)p.blocks * p.heads * p.batch;
+  if (grid > 0x7fffffffll) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "window attention: too many rows for one call");
+  AIG_CUDA_OK(ctx, cudaFuncSetAttribute(window_forward_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
+  window_forward_kernel<T, D, NT><<<(unsigned)grid, S::kThreads, S::kSmem, ctx->stream>>>(mq, mk, mv, p);
   AIG_LAUNCH_OK(ctx);
   return AIG_OK;
 }
+
 template <class T, int D>
-int backward(aig_ctx* ctx, const WinParams& p) {
+int forward(aig_ctx* ctx, WinParams& p) {
+  p.gerr = ctx->d_err;
+  CUtensorMap mq, mk, mv;
+  int rc = encode<T, D>(ctx, &mq, p.q, p.batch, p.q_len, p.heads);
+  if (rc == AIG_OK) rc = encode<T, D>(ctx, &mk, p.k, p.batch, p.kv_len, p.kv_heads);
+  if (rc == AIG_OK) rc = encode<T, D>(ctx, &mv, p.v, p.batch, p.kv_len, p.kv_heads);
+  if (rc != AIG_OK) return rc;
+  return p.q_len <= kTile ? launch_forward<T, D, 1>(ctx, p, mq, mk, mv) : launch_forward<T, D, 2>(ctx, p, mq, mk, mv);
+}
+template <class T, int D>
+int backward(aig_ctx* ctx, WinParams& p) {
   backward_q_kernel<T, D><<<dim3(ceil_div(p.q_len, kWarps), p.heads, p.batch), kWarps * 32, 0, ctx->stream>>>(p);
   AIG_LAUNCH_OK(ctx);
   backward_kv_kernel<T, D><<<dim3(ceil_div(p.kv_len, kWarps), p.kv_heads, p.batch), kWarps * 32, 0, ctx->stream>>>(p);
