@@ -15,7 +15,6 @@
 
 namespace {
 
-constexpr int kWarps = 4;
 constexpr int kTile = 128;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -76,6 +75,10 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// A bounded wait whose answer all lanes of the warp share
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* gerr, int code) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, gerr, code));
+}
 // Shared-memory descriptor of an operand whose rows (of 128 bytes, swizzled) run along the product's K dimension: 64
 // elements of M or N per row, the next 64 `block` bytes on, groups of eight rows 1024 bytes apart.
 __device__ __forceinline__ uint64_t umma_smem_desc_mn(uint32_t saddr, uint32_t block) {
@@ -109,6 +112,42 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, int from, int lane) {
   __syncwarp();
 }
 
+// N values of a row in TMEM, times f, to memory (every lane takes part in the reads)
+template <class T, int N>
+__device__ __forceinline__ void store_row(uint32_t taddr, T* out, float f, bool there) {
+#pragma unroll
+  for (int c0 = 0; c0 < N; c0 += 32) {
+    uint32_t v[32];
+    tmem_ld_32x32(taddr + c0, v);
+    tmem_ld_wait();
+    if (there) {
+#pragma unroll
+      for (int e = 0; e < 32; e += 8) {
+        uint4 x;
+        x.x = pack2<T>(__uint_as_float(v[e]) * f, __uint_as_float(v[e + 1]) * f);
+        x.y = pack2<T>(__uint_as_float(v[e + 2]) * f, __uint_as_float(v[e + 3]) * f);
+        x.z = pack2<T>(__uint_as_float(v[e + 4]) * f, __uint_as_float(v[e + 5]) * f);
+        x.w = pack2<T>(__uint_as_float(v[e + 6]) * f, __uint_as_float(v[e + 7]) * f);
+        *reinterpret_cast<uint4*>(out + c0 + e) = x;
+      }
+    }
+  }
+}
+
+// N sums of a row in TMEM, times f
+template <int N>
+__device__ __forceinline__ void scale_row(uint32_t taddr, float f) {
+#pragma unroll 1
+  for (int c0 = 0; c0 < N; c0 += 16) {
+    uint32_t v[16];
+    tmem_ld_32x16(taddr + c0, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+    tmem_st_32x16(taddr + c0, v);
+  }
+}
+
 // Key tiles that a tile of queries at positions first .. last visits: [0, sink_end) and [begin, end)
 struct KeyTiles {
   int sink_end, begin, end;
@@ -120,37 +159,6 @@ __device__ __forceinline__ KeyTiles key_tiles(int first, int last, int window, i
   k.end = last < first ? k.begin : last / kTile + 1;
   k.sink_end = window > 0 && last >= first ? min((sinks + kTile - 1) / kTile, k.begin) : 0;
   return k;
-}
-
-template <class T>
-__device__ __forceinline__ T* row_of(const View& v, int b, int t, int h) {
-  return reinterpret_cast<T*>(v.data) + b * v.batch + t * v.token + h * v.head;
-}
-__device__ __forceinline__ float warp_sum(float x) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  return x;
-}
-__device__ __forceinline__ int length_of(const WinParams& p, int b) {
-  return p.lengths ? min(max(p.lengths[b], 0), p.kv_len) : p.kv_len;
-}
-template <class T, int N>
-__device__ __forceinline__ void load_row(float (&x)[N], const T* p, int lane) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = to_f32(p[i * 32 + lane]);
-}
-template <int N>
-__device__ __forceinline__ float dot(const float (&a)[N], const float (&b)[N]) {
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) s = fmaf(a[i], b[i], s);
-  return warp_sum(s);
-}
-
-// keys of a query at position pos: [0, front) and [back, pos]
-__device__ __forceinline__ void keys_of(const WinParams& p, int pos, int& front, int& back) {
-  back = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-  front = min(p.sinks, back);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -266,7 +274,7 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
         umma_commit(s_full + 8 * w);
       }
     };
-    bool ok = mbar_wait_bounded(q_full, 0, s_abort, p.gerr, 1103) && mbar_wait_bounded(k_full, 0, s_abort, p.gerr, 1104);
+    bool ok = warp_wait(q_full, 0, s_abort, p.gerr, 1103) && warp_wait(k_full, 0, s_abort, p.gerr, 1104);
     if (ok) {
       tc_fence_after();
 #pragma unroll
@@ -275,13 +283,13 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
       if (leader) umma_commit(k_free);
       for (int it = 0; it < tiles && ok; ++it) {
         const int t = tile_at(it), s = it % NS, next = it + 1, ns = next % NS;
-        if (next < tiles && !mbar_wait_bounded(k_full + 8 * ns, (uint32_t)(next / NS) & 1u, s_abort, p.gerr, 1105)) break;
-        if (!mbar_wait_bounded(v_full + 8 * s, (uint32_t)(it / NS) & 1u, s_abort, p.gerr, 1106)) break;
+        if (next < tiles && !warp_wait(k_full + 8 * ns, (uint32_t)(next / NS) & 1u, s_abort, p.gerr, 1105)) break;
+        if (!warp_wait(v_full + 8 * s, (uint32_t)(it / NS) & 1u, s_abort, p.gerr, 1106)) break;
         if (t * kTile + kTile > len) clear_rows<D>(sm + (sV - base) + s * kTileBytes<D>, len - t * kTile, lane);
 #pragma unroll
         for (int w = 0; w < NT; ++w) {
           if (kt[w].has(t)) {
-            if (!(ok = mbar_wait_bounded(p_full + 8 * w, (uint32_t)done[w] & 1u, s_abort, p.gerr, 1107))) break;
+            if (!(ok = warp_wait(p_full + 8 * w, (uint32_t)done[w] & 1u, s_abort, p.gerr, 1107))) break;
             tc_fence_after();
             if (leader) {
 #pragma unroll
@@ -314,7 +322,7 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
     for (int it = 0; it < tiles; ++it) {
       const int t = tile_at(it);
       if (!mine.has(t)) continue;
-      if (!(ok = mbar_wait_bounded(s_full + 8 * w, (uint32_t)n & 1u, s_abort, p.gerr, 1108))) break;
+      if (!(ok = warp_wait(s_full + 8 * w, (uint32_t)n & 1u, s_abort, p.gerr, 1108))) break;
       tc_fence_after();
       const int j0 = t * kTile;
       const bool cut = j0 + kTile - 1 > first || (p.window > 0 && j0 <= first + kTile - 1 - p.window && j0 + kTile > p.sinks);
@@ -341,17 +349,7 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
           top = m;
           sum *= f;
         }
-        if (n > 0) {  // the products that went into the output have completed: the scores were issued behind them
-#pragma unroll
-          for (int c0 = 0; c0 < D; c0 += 32) {
-            uint32_t v[32];
-            tmem_ld_32x32(tOw + c0, v);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-            tmem_st_32x32(tOw + c0, v);
-          }
-        }
+        if (n > 0) scale_row<D>(tOw, f);  // the products that went into the output have completed: the scores were issued behind them
       }
       const float ref = top == -INFINITY ? 0.f : top;  // a row that has seen no key yet
 #pragma unroll
@@ -376,27 +374,11 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
       mbar_arrive(p_full + 8 * w);
       ++n;
     }
-    if (ok && n > 0 && mbar_wait_bounded(o_full + 8 * w, 0, s_abort, p.gerr, 1109)) {
+    if (ok && n > 0 && warp_wait(o_full + 8 * w, 0, s_abort, p.gerr, 1109)) {
       tc_fence_after();
       const float inv = 1.f / sum;
       T* const out = reinterpret_cast<T*>(p.o.data) + b * p.o.batch + row * p.o.token + h * p.o.head;
-#pragma unroll
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        uint32_t v[32];
-        tmem_ld_32x32(tOw + c0, v);
-        tmem_ld_wait();
-        if (row < rows_end) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint4 x;
-            x.x = pack2<T>(__uint_as_float(v[e]) * inv, __uint_as_float(v[e + 1]) * inv);
-            x.y = pack2<T>(__uint_as_float(v[e + 2]) * inv, __uint_as_float(v[e + 3]) * inv);
-            x.z = pack2<T>(__uint_as_float(v[e + 4]) * inv, __uint_as_float(v[e + 5]) * inv);
-            x.w = pack2<T>(__uint_as_float(v[e + 6]) * inv, __uint_as_float(v[e + 7]) * inv);
-            *reinterpret_cast<uint4*>(out + c0 + e) = x;
-          }
-        }
-      }
+      store_row<T, D>(tOw, out, inv, row < rows_end);
       if (row < rows_end) p.lse[((long long)b * p.heads + h) * p.q_len + row] = fmaf(top, kLn2, logf(sum));
     }
   }
@@ -412,66 +394,572 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
   }
 }
 
-template <class T, int D>
-__global__ void __launch_bounds__(kWarps * 32) backward_q_kernel(const __grid_constant__ WinParams p) {
-  constexpr int N = D / 32;
-  const int lane = threadIdx.x & 31, i = blockIdx.x * kWarps + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z;
-  const int pos = i + p.kv_len - p.q_len;
-  if (i >= p.q_len || pos >= length_of(p, b)) return;
-  const int kvh = h / (p.heads / p.kv_heads);
-  float q[N], g[N], x[N], dq[N] = {};
-  load_row<T>(q, row_of<T>(p.q, b, i, h), lane);
-  load_row<T>(g, row_of<T>(p.dout, b, i, h), lane);
-  load_row<T>(x, row_of<T>(p.o, b, i, h), lane);
-  const float delta = dot(g, x);
-  const long long stat = ((long long)b * p.heads + h) * p.q_len + i;
-  const float lse = p.lse[stat];
-  if (lane == 0) p.delta[stat] = delta;
-  int front, back;
-  keys_of(p, pos, front, back);
-  for (int j = front > 0 ? 0 : back; j <= pos; j = j + 1 == front ? back : j + 1) {
-    load_row<T>(x, row_of<T>(p.v, b, j, kvh), lane);
-    const float dp = dot(g, x);
-    load_row<T>(x, row_of<T>(p.k, b, j, kvh), lane);
-    const float ds = expf(dot(q, x) * p.scale - lse) * (dp - delta) * p.scale;
+// ---------------------------------------------------------------------------------------------
+// Backward: one kernel for dQ (a tile of queries stays, keys pass by), one for dK and dV (a tile of keys stays, the queries of
+// the group's heads pass by).  Each computes the weights again from lse: two more products than one kernel that adds dQ
+// into memory with atomics would need, but every sum has a fixed order.  256 threads share a tile of scores, 64 columns
+// each.
+//
+// fp16 has few small numbers: weights of a row over thousands of keys, and dS of small gradients, would be rounded to
+// multiples of 2^-24.  So the weights are multiplied by 2^8, and dS by a power of two 2^k that follows the largest
+// |dO| * |V| seen so far: |dS| stays below 2^15.5 whatever the values, and typical ones around 1.  Where a tile asks for a
+// smaller power the sums so far are scaled (rare: it keeps two bits in hand).
+constexpr int kBwdThreads = 384;
+template <class T>
+constexpr int kWeightBits = std::is_same<T, __half>::value ? 8 : 0;
+constexpr int kMostBits = 11, kAimBits = 9;  // of 2^k * |dO| * |V| * sqrt(D)
+
+__device__ __forceinline__ float pow2(int k) { return __int_as_float((k + 127) << 23); }  // -126 .. 127
+
+// Exponent e with max |x| < 2^e over rows [0, rows) of a tile in shared memory, by 64 threads (x finite; -126 at least)
+template <int D>
+__device__ __forceinline__ int tile_exponent(const uint8_t* tile, int rows, int tid, int* s_pair) {
+  __half2 m = __half2half2(__ushort_as_half(0));
 #pragma unroll
-    for (int n = 0; n < N; ++n) dq[n] = fmaf(ds, x[n], dq[n]);
-  }
-  T* out = row_of<T>(p.dq, b, i, h);
+  for (int c = 0; c < D / 64; ++c)
+    for (int i = tid; i < rows * 8; i += 64) {
+      const uint4 v = *reinterpret_cast<const uint4*>(tile + c * kTile * 128 + i * 16);
+      const __half2* h = reinterpret_cast<const __half2*>(&v);
+      m = __hmax2(m, __hmax2(__hmax2(__habs2(h[0]), __habs2(h[1])), __hmax2(__habs2(h[2]), __habs2(h[3]))));
+    }
+  float x = fmaxf(__low2float(m), __high2float(m));
 #pragma unroll
-  for (int n = 0; n < N; ++n) out[n * 32 + lane] = from_f32<T>(dq[n]);
+  for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  const int e = min((int)(__float_as_uint(x) >> 23) - 126, 20);
+  if ((tid & 31) == 0) s_pair[tid >> 5] = e;
+  named_bar_sync(1, 64);
+  const int both = max(s_pair[0], s_pair[1]);
+  named_bar_sync(1, 64);
+  return both;
+}
+// the power for a tile whose bound has the exponent e, given the one so far
+__device__ __forceinline__ int next_power(int k, int e) {
+  return e + k > kMostBits ? max(kAimBits - e, -100) : k;
 }
 
+template <int D>
+struct DqShape {
+  static constexpr int kStages = D == 64 ? 3 : 2;
+  static constexpr size_t kSmem = 2 * kTileBytes<D> + 2 * kStages * kTileBytes<D> + 1024 + 2048;
+};
+
 template <class T, int D>
-__global__ void __launch_bounds__(kWarps * 32) backward_kv_kernel(const __grid_constant__ WinParams p) {
-  constexpr int N = D / 32;
-  const int lane = threadIdx.x & 31, j = blockIdx.x * kWarps + (threadIdx.x >> 5), kvh = blockIdx.y, b = blockIdx.z;
-  const int len = length_of(p, b), first = p.kv_len - p.q_len, group = p.heads / p.kv_heads;
-  if (j >= len) return;
-  float k[N], v[N], x[N], g[N], dk[N] = {}, dv[N] = {};
-  load_row<T>(k, row_of<T>(p.k, b, j, kvh), lane);
-  load_row<T>(v, row_of<T>(p.v, b, j, kvh), lane);
-  // queries that see key j: positions j .. last
-  const int last = p.window > 0 && j >= p.sinks ? (int)min((long long)len - 1, (long long)j + p.window - 1) : len - 1;
-  for (int h = kvh * group; h < (kvh + 1) * group; ++h)
-    for (int pos = max(j, first); pos <= last; ++pos) {
-      const int i = pos - first;
-      const long long stat = ((long long)b * p.heads + h) * p.q_len + i;
-      load_row<T>(x, row_of<T>(p.q, b, i, h), lane);
-      load_row<T>(g, row_of<T>(p.dout, b, i, h), lane);
-      const float w = expf(dot(k, x) * p.scale - p.lse[stat]);
-      const float ds = w * (dot(v, g) - p.delta[stat]) * p.scale;
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        dk[n] = fmaf(ds, x[n], dk[n]);
-        dv[n] = fmaf(w, g[n], dv[n]);
+__global__ void __launch_bounds__(kBwdThreads, 1)
+window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
+                 const __grid_constant__ CUtensorMap mapG, const __grid_constant__ WinParams p) {
+  constexpr int NS = DqShape<D>::kStages;
+  constexpr bool kScaled = std::is_same<T, __half>::value;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* const sm = smem_raw + (base - raw);
+  const uint32_t sQ = base, sG = sQ + kTileBytes<D>, sK = sG + kTileBytes<D>, sV = sK + NS * kTileBytes<D>;
+  float* const s_sum = reinterpret_cast<float*>(sm + (2 + 2 * NS) * kTileBytes<D>);  // [2][128]
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(s_sum + 256);
+  const uint32_t bar0 = smem_u32(bars);
+  const uint32_t q_full = bar0, sd_full = bar0 + 8, sd_free = bar0 + 16, ds_full = bar0 + 24, ds_free = bar0 + 32, dq_full = bar0 + 40,
+                 k_full = bar0 + 48, k_free = k_full + 8 * NS, v_full = k_free + 8 * NS, v_free = v_full + 8 * NS, st_full = v_free + 8 * NS;
+  int* const s_power = reinterpret_cast<int*>(bars + 6 + 5 * NS);  // [NS]
+  int* const s_pair = s_power + NS;                                // [2]
+  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(s_pair + 2);
+  volatile int* const s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+
+  int item = blockIdx.x;
+  const int b = item % p.batch;
+  item /= p.batch;
+  const int h = item % p.heads, block = p.blocks - 1 - item / p.heads;
+  const int kvh = h / (p.heads / p.kv_heads);
+  const int len = p.lengths ? min(max(p.lengths[b], 0), p.kv_len) : p.kv_len;
+  const int off = p.kv_len - p.q_len, r0 = block * kTile;
+  const int rows_end = min(p.q_len, len - off);
+  if (r0 >= rows_end) return;
+  const KeyTiles kt = key_tiles(off + r0, off + min(r0 + kTile, rows_end) - 1, p.window, p.sinks);
+  const int tiles = kt.sink_end + kt.end - kt.begin;
+  auto tile_at = [&](int it) { return it < kt.sink_end ? it : kt.begin + (it - kt.sink_end); };
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(sd_full, 1);
+    mbar_init(sd_free, 256);
+    mbar_init(ds_full, 256);
+    mbar_init(ds_free, 1);
+    mbar_init(dq_full, 1);
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(k_full + 8 * s, 1);
+      mbar_init(k_free + 8 * s, 1);
+      mbar_init(v_full + 8 * s, 1);
+      mbar_init(v_free + 8 * s, kScaled ? 9 : 1);  // the products are done with it, and each of 8 warps has its power
+      mbar_init(st_full + 8 * s, 64);
+    }
+    *s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(s_tmem), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem, tS = tmem, tdP = tmem + 128, tdS = tmem + 256, tdQ = tmem + 320;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      mbar_expect_tx(q_full, 2 * kTileBytes<D>);
+      load_tile<D>(sQ, &mapQ, q_full, h, r0, b);
+      load_tile<D>(sG, &mapG, q_full, h, r0, b);
+      for (int it = 0; it < tiles; ++it) {
+        const int s = it % NS, row = tile_at(it) * kTile;
+        const uint32_t ph = (uint32_t)(it / NS + 1) & 1u;
+        if (it >= NS && !mbar_wait_bounded(k_free + 8 * s, ph, s_abort, p.gerr, 1121)) break;
+        mbar_expect_tx(k_full + 8 * s, kTileBytes<D>);
+        load_tile<D>(sK + s * kTileBytes<D>, &mapK, k_full + 8 * s, kvh, row, b);
+        if (it >= NS && !mbar_wait_bounded(v_free + 8 * s, ph, s_abort, p.gerr, 1122)) break;
+        mbar_expect_tx(v_full + 8 * s, kTileBytes<D>);
+        load_tile<D>(sV + s * kTileBytes<D>, &mapV, v_full + 8 * s, kvh, row, b);
       }
     }
-  T *out_k = row_of<T>(p.dk, b, j, kvh), *out_v = row_of<T>(p.dv, b, j, kvh);
+  } else if (warp == 1) {
+    constexpr uint32_t idesc_s = idesc_for<T>(kTile, kTile, false), idesc_q = idesc_for<T>(kTile, D, true);
+    const bool leader = elect_one();
+    // the scores and dP of tile `it`; the stages' tiles are there when it returns true
+    auto scores = [&](int it) {
+      const int s = it % NS, t = tile_at(it);
+      const uint32_t ph = (uint32_t)(it / NS) & 1u;
+      if (!warp_wait(k_full + 8 * s, ph, s_abort, p.gerr, 1123) || !warp_wait(v_full + 8 * s, ph, s_abort, p.gerr, 1124)) return false;
+      if (t * kTile + kTile > len) clear_rows<D>(sm + (sK - base) + s * kTileBytes<D>, len - t * kTile, lane);
+      tc_fence_after();
+      if (leader) {
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-    out_k[n * 32 + lane] = from_f32<T>(dk[n]);
-    out_v[n * 32 + lane] = from_f32<T>(dv[n]);
+        for (int ks = 0; ks < D / 16; ++ks) umma_f16_ss(tS, desc_k(sQ, ks), desc_k(sK + s * kTileBytes<D>, ks), idesc_s, ks != 0);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) umma_f16_ss(tdP, desc_k(sG, ks), desc_k(sV + s * kTileBytes<D>, ks), idesc_s, ks != 0);
+        umma_commit(sd_full);
+        umma_commit(v_free + 8 * s);
+      }
+      return true;
+    };
+    if (warp_wait(q_full, 0, s_abort, p.gerr, 1125) && scores(0)) {
+      for (int it = 0; it < tiles; ++it) {
+        const uint32_t ph = (uint32_t)it & 1u;
+        if (it + 1 < tiles) {
+          if (!warp_wait(sd_free, ph, s_abort, p.gerr, 1126)) break;
+          if (!scores(it + 1)) break;
+        }
+        if (!warp_wait(ds_full, ph, s_abort, p.gerr, 1127)) break;
+        tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int ks = 0; ks < kTile / 16; ++ks)
+            umma_f16_ts(tdQ, tdS + ks * 8, desc_rows(sK + (it % NS) * kTileBytes<D>, ks), idesc_q, it != 0 || ks != 0);
+          umma_commit(ds_free);
+          umma_commit(k_free + 8 * (it % NS));
+          if (it + 1 == tiles) umma_commit(dq_full);
+        }
+      }
+    }
+  } else if (warp < 4) {
+    if (kScaled) {
+      const int tid = threadIdx.x - 64;
+      if (named_bar_and(1, 64, warp_wait(q_full, 0, s_abort, p.gerr, 1128))) {
+        const int eg = tile_exponent<D>(sm + (sG - base), min(kTile, rows_end - r0), tid, s_pair) + (D == 64 ? 3 : 4);
+        int k = 100;
+        for (int it = 0; it < tiles; ++it) {
+          const int s = it % NS;
+          if (!named_bar_and(1, 64, warp_wait(v_full + 8 * s, (uint32_t)(it / NS) & 1u, s_abort, p.gerr, 1129))) break;
+          k = next_power(k, eg + tile_exponent<D>(sm + (sV - base) + s * kTileBytes<D>, min(kTile, len - tile_at(it) * kTile), tid, s_pair));
+          if (tid == 0) s_power[s] = k;
+          mbar_arrive(st_full + 8 * s);
+        }
+      }
+    }
+  } else {
+    const int half = (warp - 4) >> 2, q = warp & 3, in_tile = q * 32 + lane;
+    const int row = r0 + in_tile, pos = off + row;
+    const bool there = row < rows_end;
+    const uint32_t lanes = (uint32_t)(q * 32) << 16;
+    const float c = p.scale * kLog2e;
+    const long long stat = ((long long)b * p.heads + h) * p.q_len + row;
+    const float lse2 = there ? p.lse[stat] * kLog2e : INFINITY;  // (weights of 0)
+    // a query that sees one key has the weight 1 whatever its score: no gradient through it
+    const bool single = pos == 0 || (p.window == 1 && p.sinks == 0);
+    float delta = 0.f;
+    if (tiles > 1) {
+      // (dO . O has the output's rounding in it: with a tile's keys or fewer, where that is large against dP, the sum over
+      // the weights is taken instead, below)
+      float d = 0.f;
+      if (there) {
+        const T* g = reinterpret_cast<const T*>(p.dout.data) + b * p.dout.batch + row * p.dout.token + h * p.dout.head + half * (D / 2);
+        const T* o = reinterpret_cast<const T*>(p.o.data) + b * p.o.batch + row * p.o.token + h * p.o.head + half * (D / 2);
+#pragma unroll
+        for (int i = 0; i < D / 2; i += 8) {
+          const uint4 x = *reinterpret_cast<const uint4*>(g + i), y = *reinterpret_cast<const uint4*>(o + i);
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 u = unpack2<T>(xs[e]), v = unpack2<T>(ys[e]);
+            d = fmaf(u.x, v.x, fmaf(u.y, v.y, d));
+          }
+        }
+      }
+      s_sum[half * 128 + in_tile] = d;
+      named_bar_sync(2, 256);
+      delta = s_sum[in_tile] + s_sum[128 + in_tile];
+    }
+    int k = 0;
+    bool ok = true;
+    for (int it = 0; it < tiles; ++it) {
+      const int s = it % NS, j0 = tile_at(it) * kTile;
+      const uint32_t ph = (uint32_t)it & 1u;
+      if (!(ok = warp_wait(sd_full, ph, s_abort, p.gerr, 1130))) {
+        if (tiles == 1) named_bar_sync(2, 256);  // (the others may be waiting below)
+        break;
+      }
+      tc_fence_after();
+      uint32_t sc[2][32], dp[2][32];
+      tmem_ld_32x32(tS + lanes + half * 64, sc[0]);
+      tmem_ld_32x32(tS + lanes + half * 64 + 32, sc[1]);
+      tmem_ld_32x32(tdP + lanes + half * 64, dp[0]);
+      tmem_ld_32x32(tdP + lanes + half * 64 + 32, dp[1]);
+      tmem_ld_wait();
+      tc_fence_before();
+      mbar_arrive(sd_free);
+      float r = 1.f;
+      int k_new = 0;
+      if (kScaled) {
+        if (!(ok = warp_wait(st_full + 8 * s, (uint32_t)(it / NS) & 1u, s_abort, p.gerr, 1131))) {
+          if (tiles == 1) named_bar_sync(2, 256);
+          break;
+        }
+        k_new = s_power[s];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_free + 8 * s);
+        r = pow2(k_new);
+      }
+      if (single) r = 0.f;
+      const bool cut = j0 + kTile - 1 > off + r0 || (p.window > 0 && j0 <= off + r0 + kTile - 1 - p.window && j0 + kTile > p.sinks);
+      const int c_0 = half * 64;
+      const int lo = p.window > 0 ? pos - p.window + 1 - j0 - c_0 : -1, hi = pos - j0 - c_0, sinks = p.sinks - j0 - c_0;
+      float own = 0.f;
+#pragma unroll
+      for (int e = 0; e < 64; ++e) {
+        float w = ex2(fmaf(__uint_as_float(sc[e >> 5][e & 31]), c, -lse2));
+        float d = __uint_as_float(dp[e >> 5][e & 31]);
+        if (cut) {
+          const bool shown = e <= hi && (e >= lo || e < sinks);
+          w = shown ? w : 0.f;
+          d = shown ? d : 0.f;
+        }
+        sc[e >> 5][e & 31] = __float_as_uint(w);
+        dp[e >> 5][e & 31] = __float_as_uint(d);
+        if (tiles == 1) own = fmaf(w, d, own);
+      }
+      if (tiles == 1) {
+        s_sum[half * 128 + in_tile] = own;
+        named_bar_sync(2, 256);
+        delta = s_sum[in_tile] + s_sum[128 + in_tile];
+      }
+      if (it > 0) {
+        if (!(ok = warp_wait(ds_free, ph ^ 1u, s_abort, p.gerr, 1132))) break;
+        if (kScaled && k_new != k) {
+          tc_fence_after();
+          scale_row<D / 2>(tdQ + lanes + half * (D / 2), pow2(max(k_new - k, -126)));
+        }
+      }
+      k = k_new;
+#pragma unroll
+      for (int c0 = 0; c0 < 2; ++c0) {
+        uint32_t o[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2)
+          o[e / 2] = pack2<T>(__uint_as_float(sc[c0][e]) * r * (__uint_as_float(dp[c0][e]) - delta),
+                              __uint_as_float(sc[c0][e + 1]) * r * (__uint_as_float(dp[c0][e + 1]) - delta));
+        tmem_st_32x16(tdS + lanes + half * 32 + c0 * 16, o);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(ds_full);
+    }
+    if (ok && warp_wait(dq_full, 0, s_abort, p.gerr, 1133)) {
+      tc_fence_after();
+      if (there && half == 0) p.delta[stat] = delta;
+      const float f = p.scale * pow2(-k);
+      T* const out = reinterpret_cast<T*>(p.dq.data) + b * p.dq.batch + row * p.dq.token + h * p.dq.head + half * (D / 2);
+      store_row<T, D / 2>(tdQ + lanes + half * (D / 2), out, f, there);
+    }
+  }
+
+  if (*s_abort) {
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int D>
+struct DkvShape {
+  static constexpr int kStages = D == 64 ? 3 : 2;
+  static constexpr size_t kSmem = 2 * kTileBytes<D> + 2 * kStages * kTileBytes<D> + 1024 + 4096;
+};
+
+template <class T, int D>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
+                  const __grid_constant__ CUtensorMap mapG, const __grid_constant__ WinParams p) {
+  constexpr int NS = DkvShape<D>::kStages;
+  constexpr bool kScaled = std::is_same<T, __half>::value;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* const sm = smem_raw + (base - raw);
+  const uint32_t sK = base, sV = sK + kTileBytes<D>, sQ = sV + kTileBytes<D>, sG = sQ + NS * kTileBytes<D>;
+  float* const s_lse = reinterpret_cast<float*>(sm + (2 + 2 * NS) * kTileBytes<D>);  // [NS][128], in log2, less the weights' power
+  float* const s_delta = s_lse + NS * 128;                                            // [NS][128]
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(s_delta + NS * 128);
+  const uint32_t bar0 = smem_u32(bars);
+  const uint32_t kv_full = bar0, s_full = bar0 + 8, p_full = bar0 + 16, dp_full = bar0 + 24, ds_full = bar0 + 32, all_done = bar0 + 40,
+                 q_full = bar0 + 48, q_free = q_full + 8 * NS, st_full = q_free + 8 * NS;
+  int* const s_power = reinterpret_cast<int*>(bars + 6 + 3 * NS);  // [NS]
+  int* const s_pair = s_power + NS;                                // [2]
+  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(s_pair + 2);
+  volatile int* const s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+
+  int item = blockIdx.x;
+  const int b = item % p.batch;
+  item /= p.batch;
+  const int kvh = item % p.kv_heads, j0 = item / p.kv_heads * kTile;
+  const int group = p.heads / p.kv_heads;
+  const int len = p.lengths ? min(max(p.lengths[b], 0), p.kv_len) : p.kv_len;
+  const int off = p.kv_len - p.q_len;
+  const int rows_end = min(p.q_len, len - off);
+  if (j0 >= len) return;
+  // tiles of queries that see a key of this one: rows from the first key's position on, as far as the window of the last key
+  // reaches, or all where a key is a sink
+  const int j1 = min(j0 + kTile, len) - 1;
+  const int row_first = max(0, j0 - off);
+  const int row_last = p.window > 0 && j0 >= p.sinks ? min(rows_end - 1, j1 + p.window - 1 - off) : rows_end - 1;
+  const int t_first = row_first / kTile, per_head = row_last < row_first ? 0 : row_last / kTile - t_first + 1;
+  const int tiles = per_head * group;
+
+  if (tiles == 0) {  // no query sees these keys
+    for (int i = threadIdx.x; i < (j1 - j0 + 1) * (D / 8); i += kBwdThreads) {
+      const int j = j0 + i / (D / 8), c = i % (D / 8) * 8;
+      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.dk.data) + b * p.dk.batch + j * p.dk.token + kvh * p.dk.head + c) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.dv.data) + b * p.dv.batch + j * p.dv.token + kvh * p.dv.head + c) = make_uint4(0, 0, 0, 0);
+    }
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1);
+    mbar_init(s_full, 1);
+    mbar_init(p_full, 256);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_full, 256);
+    mbar_init(all_done, 1);
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(q_full + 8 * s, 1);
+      mbar_init(q_free + 8 * s, 1);
+      mbar_init(st_full + 8 * s, 64);
+    }
+    *s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(s_tmem), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // weights over the scores, dS over dP, each half of the columns where its own scores were
+  const uint32_t tmem = *s_tmem, tS = tmem, tdP = tmem + 128, tdV = tmem + 256, tdK = tmem + 256 + D;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      mbar_expect_tx(kv_full, 2 * kTileBytes<D>);
+      load_tile<D>(sK, &mapK, kv_full, kvh, j0, b);
+      load_tile<D>(sV, &mapV, kv_full, kvh, j0, b);
+      for (int it = 0; it < tiles; ++it) {
+        const int s = it % NS, h = kvh * group + it / per_head, row = (t_first + it % per_head) * kTile;
+        if (it >= NS && !mbar_wait_bounded(q_free + 8 * s, (uint32_t)(it / NS + 1) & 1u, s_abort, p.gerr, 1141)) break;
+        mbar_expect_tx(q_full + 8 * s, 2 * kTileBytes<D>);
+        load_tile<D>(sQ + s * kTileBytes<D>, &mapQ, q_full + 8 * s, h, row, b);
+        load_tile<D>(sG + s * kTileBytes<D>, &mapG, q_full + 8 * s, h, row, b);
+      }
+    }
+  } else if (warp == 1) {
+    constexpr uint32_t idesc_s = idesc_for<T>(kTile, kTile, false), idesc_g = idesc_for<T>(kTile, D, true);
+    const bool leader = elect_one();
+    auto arrived = [&](int it) {
+      const int s = it % NS, row = (t_first + it % per_head) * kTile;
+      if (!warp_wait(q_full + 8 * s, (uint32_t)(it / NS) & 1u, s_abort, p.gerr, 1142)) return false;
+      if (row + kTile > rows_end) {  // rows behind the sequence's end are summed over too
+        clear_rows<D>(sm + (sQ - base) + s * kTileBytes<D>, rows_end - row, lane);
+        clear_rows<D>(sm + (sG - base) + s * kTileBytes<D>, rows_end - row, lane);
+      }
+      return true;
+    };
+    auto scores = [&](int it) {
+      if (leader) {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) umma_f16_ss(tS, desc_k(sK, ks), desc_k(sQ + (it % NS) * kTileBytes<D>, ks), idesc_s, ks != 0);
+        umma_commit(s_full);
+      }
+    };
+    auto dps = [&](int it) {
+      if (leader) {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) umma_f16_ss(tdP, desc_k(sV, ks), desc_k(sG + (it % NS) * kTileBytes<D>, ks), idesc_s, ks != 0);
+        umma_commit(dp_full);
+      }
+    };
+    if (warp_wait(kv_full, 0, s_abort, p.gerr, 1143) && arrived(0)) {
+      tc_fence_after();
+      scores(0);
+      dps(0);
+      for (int it = 0; it < tiles; ++it) {
+        const int s = it % NS;
+        const uint32_t ph = (uint32_t)it & 1u;
+        if (!warp_wait(p_full, ph, s_abort, p.gerr, 1144)) break;
+        tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int ks = 0; ks < kTile / 16; ++ks)
+            umma_f16_ts(tdV, tS + (ks >> 2) * 64 + (ks & 3) * 8, desc_rows(sG + s * kTileBytes<D>, ks), idesc_g, it != 0 || ks != 0);
+        }
+        if (it + 1 < tiles) {
+          if (!arrived(it + 1)) break;
+          scores(it + 1);
+        }
+        if (!warp_wait(ds_full, ph, s_abort, p.gerr, 1145)) break;
+        tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int ks = 0; ks < kTile / 16; ++ks)
+            umma_f16_ts(tdK, tdP + (ks >> 2) * 64 + (ks & 3) * 8, desc_rows(sQ + s * kTileBytes<D>, ks), idesc_g, it != 0 || ks != 0);
+          umma_commit(q_free + 8 * s);
+          if (it + 1 == tiles) umma_commit(all_done);
+        }
+        if (it + 1 < tiles) dps(it + 1);
+      }
+    }
+  } else if (warp < 4) {
+    // statistics of the queries, and the power for dS
+    const int tid = threadIdx.x - 64;
+    int k = 100, ev = 0;
+    bool ok = true;
+    if (kScaled) {
+      ok = named_bar_and(1, 64, warp_wait(kv_full, 0, s_abort, p.gerr, 1146));
+      if (ok) ev = tile_exponent<D>(sm + (sV - base), min(kTile, len - j0), tid, s_pair) + (D == 64 ? 3 : 4);
+    }
+    for (int it = 0; it < tiles && ok; ++it) {
+      const int s = it % NS, h = kvh * group + it / per_head, row = (t_first + it % per_head) * kTile;
+      ok = it < NS || warp_wait(q_free + 8 * s, (uint32_t)(it / NS + 1) & 1u, s_abort, p.gerr, 1147);
+      if (kScaled) ok = named_bar_and(1, 64, ok && warp_wait(q_full + 8 * s, (uint32_t)(it / NS) & 1u, s_abort, p.gerr, 1148));
+      if (!ok) break;
+      const long long stat = ((long long)b * p.heads + h) * p.q_len;
+#pragma unroll
+      for (int i = tid; i < kTile; i += 64) {
+        const bool there = row + i < rows_end;
+        s_lse[s * 128 + i] = there ? fmaf(p.lse[stat + row + i], kLog2e, -(float)kWeightBits<T>) : INFINITY;  // (a weight of 0)
+        s_delta[s * 128 + i] = there ? p.delta[stat + row + i] : 0.f;
+      }
+      if (kScaled) {
+        k = next_power(k, ev + tile_exponent<D>(sm + (sG - base) + s * kTileBytes<D>, min(kTile, rows_end - row), tid, s_pair));
+        if (tid == 0) s_power[s] = k;
+      }
+      mbar_arrive(st_full + 8 * s);
+    }
+  } else {
+    const int half = (warp - 4) >> 2, q = warp & 3, in_tile = q * 32 + lane;
+    const int key = j0 + in_tile;
+    const uint32_t lanes = (uint32_t)(q * 32) << 16;
+    const float c = p.scale * kLog2e;
+    const bool sink = key < p.sinks, no_ds = p.window == 1 && p.sinks == 0;
+    int k = 0;
+    bool ok = true;
+    for (int it = 0; it < tiles; ++it) {
+      const int s = it % NS, first = off + (t_first + it % per_head) * kTile;  // position of the tile's first query
+      const uint32_t ph = (uint32_t)it & 1u;
+      const float *lse2 = s_lse + s * 128 + half * 64, *delta = s_delta + s * 128 + half * 64;
+      const bool cut = j0 + kTile - 1 > first || (p.window > 0 && j0 <= first + kTile - 1 - p.window && j0 + kTile > p.sinks);
+      // columns whose queries see this thread's key: from `from` on, and before `to` unless it is a sink
+      const int from = key - first - half * 64, to = p.window > 0 && !sink ? from + p.window : 0x7fffffff;
+      if (!(ok = warp_wait(st_full + 8 * s, (uint32_t)(it / NS) & 1u, s_abort, p.gerr, 1149))) break;
+      if (!(ok = warp_wait(s_full, ph, s_abort, p.gerr, 1150))) break;
+      tc_fence_after();
+      float w[64];
+#pragma unroll
+      for (int c0 = 0; c0 < 64; c0 += 32) {
+        uint32_t v[32], o[16];
+        tmem_ld_32x32(tS + lanes + half * 64 + c0, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          float x = ex2(fmaf(__uint_as_float(v[e]), c, -lse2[c0 + e]));
+          if (cut) x = c0 + e >= from && c0 + e < to ? x : 0.f;
+          w[c0 + e] = x;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) o[e / 2] = pack2<T>(w[c0 + e], w[c0 + e + 1]);
+        tmem_st_32x16(tS + lanes + half * 64 + c0 / 2, o);  // over scores that have been read
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(p_full);
+      float r = no_ds ? 0.f : 1.f;
+      if (!(ok = warp_wait(dp_full, ph, s_abort, p.gerr, 1151))) break;
+      tc_fence_after();
+      if (kScaled) {
+        const int k_new = s_power[s];
+        if (it > 0 && k_new != k)  // dP was issued behind the product that added to dK
+          scale_row<D / 2>(tdK + lanes + half * (D / 2), pow2(max(k_new - k, -126)));
+        k = k_new;
+        r *= pow2(k - kWeightBits<T>);
+      }
+      const int alone = -first - half * 64;  // the column of the query at position 0, which sees one key: no gradient through it
+#pragma unroll
+      for (int c0 = 0; c0 < 64; c0 += 32) {
+        uint32_t v[32], o[16];
+        tmem_ld_32x32(tdP + lanes + half * 64 + c0, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          float x = w[c0 + e] * r * (__uint_as_float(v[e]) - delta[c0 + e]), y = w[c0 + e + 1] * r * (__uint_as_float(v[e + 1]) - delta[c0 + e + 1]);
+          if (cut) {
+            x = c0 + e >= from && c0 + e < to && c0 + e != alone ? x : 0.f;
+            y = c0 + e + 1 >= from && c0 + e + 1 < to && c0 + e + 1 != alone ? y : 0.f;
+          }
+          o[e / 2] = pack2<T>(x, y);
+        }
+        tmem_st_32x16(tdP + lanes + half * 64 + c0 / 2, o);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(ds_full);
+    }
+    if (ok && warp_wait(all_done, 0, s_abort, p.gerr, 1152)) {
+      tc_fence_after();
+      T* const dk = reinterpret_cast<T*>(p.dk.data) + b * p.dk.batch + key * p.dk.token + kvh * p.dk.head + half * (D / 2);
+      T* const dv = reinterpret_cast<T*>(p.dv.data) + b * p.dv.batch + key * p.dv.token + kvh * p.dv.head + half * (D / 2);
+      store_row<T, D / 2>(tdV + lanes + half * (D / 2), dv, pow2(-kWeightBits<T>), key < len);
+      store_row<T, D / 2>(tdK + lanes + half * (D / 2), dk, p.scale * pow2(-k), key < len);
+    }
+  }
+
+  if (*s_abort) {
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -556,9 +1044,21 @@ int forward(aig_ctx* ctx, WinParams& p) {
 }
 template <class T, int D>
 int backward(aig_ctx* ctx, WinParams& p) {
-  backward_q_kernel<T, D><<<dim3(ceil_div(p.q_len, kWarps), p.heads, p.batch), kWarps * 32, 0, ctx->stream>>>(p);
+  p.gerr = ctx->d_err;
+  CUtensorMap mq{}, mk, mv, mg{};
+  int rc = encode<T, D>(ctx, &mk, p.k, p.batch, p.kv_len, p.kv_heads);
+  if (rc == AIG_OK) rc = encode<T, D>(ctx, &mv, p.v, p.batch, p.kv_len, p.kv_heads);
+  if (rc == AIG_OK) rc = encode<T, D>(ctx, &mq, p.q, p.batch, p.q_len, p.heads);
+  if (rc == AIG_OK) rc = encode<T, D>(ctx, &mg, p.dout, p.batch, p.q_len, p.heads);
+  if (rc != AIG_OK) return rc;
+  p.blocks = ceil_div(p.q_len, kTile);
+  const long long grid = (long long)p.blocks * p.heads * p.batch, grid_kv = (long long)ceil_div(p.kv_len, kTile) * p.kv_heads * p.batch;
+  if (grid > 0x7fffffffll || grid_kv > 0x7fffffffll) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "window attention backward: too many rows for one call");
+  AIG_CUDA_OK(ctx, cudaFuncSetAttribute(window_dq_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DqShape<D>::kSmem));
+  AIG_CUDA_OK(ctx, cudaFuncSetAttribute(window_dkv_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DkvShape<D>::kSmem));
+  window_dq_kernel<T, D><<<(unsigned)grid, kBwdThreads, DqShape<D>::kSmem, ctx->stream>>>(mq, mk, mv, mg, p);
   AIG_LAUNCH_OK(ctx);
-  backward_kv_kernel<T, D><<<dim3(ceil_div(p.kv_len, kWarps), p.kv_heads, p.batch), kWarps * 32, 0, ctx->stream>>>(p);
+  window_dkv_kernel<T, D><<<(unsigned)grid_kv, kBwdThreads, DkvShape<D>::kSmem, ctx->stream>>>(mq, mk, mv, mg, p);
   AIG_LAUNCH_OK(ctx);
   return AIG_OK;
 }
