@@ -457,7 +457,7 @@ int aig_paged_attention(aig_ctx* ctx, const aig_kv_cache* cache, const aig_heads
   if (cache->head_dim != 64 && cache->head_dim != 128)
     return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "paged attention: head dimension must be 64 or 128 (got %d)", cache->head_dim);
   AIG_REQUIRE(ctx, batch >= 0 && table_width > 0 && max_length >= 0 && sinks >= 0, "paged attention: bad extents");
-  AIG_REQUIRE(ctx, scale == scale && scale - scale == 0.f, "paged attention: the scale is not finite");
+  AIG_REQUIRE(ctx, scale > 0.f && scale - scale == 0.f, "paged attention: the scale has to be positive and finite");
   if (batch == 0) return AIG_OK;
   AIG_REQUIRE(ctx, heads_sane(q) && heads_sane(out) && table && lengths, "paged attention: null tensor or negative stride");
   AIG_REQUIRE(ctx, heads_vectorised(*q) && heads_vectorised(*out), "paged attention: q and out on 16-byte boundaries, strides multiples of 8");

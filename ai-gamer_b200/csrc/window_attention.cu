@@ -75,6 +75,38 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// two operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 pair_of(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
+// bits 0 .. n-1
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+constexpr uint32_t kMinusInf = 0xff800000u;
 // A bounded wait whose answer all lanes of the warp share
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* gerr, int code) {
   return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, gerr, code));
@@ -167,7 +199,7 @@ template <int D, int NT>  // NT tiles of queries
 struct FwdShape {
   static constexpr int kStages = NT == 2 ? (D == 64 ? 4 : 2) : 2;
   static constexpr int kThreads = 128 + 128 * NT;
-  static constexpr int kCtasPerSm = NT == 2 ? 1 : (D == 64 ? 2 : 1);
+  static constexpr int kCtasPerSm = 1;
   static constexpr int kTmemCols = NT == 2 ? 512 : 256;  // scores 128 columns a tile, then outputs D columns a tile
   static constexpr uint32_t kQ = NT * kTileBytes<D>;
   static constexpr size_t kSmem = kQ + 2 * kStages * kTileBytes<D> + 1024 + 256;
@@ -327,21 +359,27 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
       const int j0 = t * kTile;
       const bool cut = j0 + kTile - 1 > first || (p.window > 0 && j0 <= first + kTile - 1 - p.window && j0 + kTile > p.sinks);
       const int lo = p.window > 0 ? pos - p.window + 1 - j0 : -1, hi = pos - j0, sinks = p.sinks - j0;  // columns
-      auto shown = [&](int j) { return j <= hi && (j >= lo || j < sinks); };
-      float m = -INFINITY;
+      uint32_t v[4][32];
 #pragma unroll
-      for (int c0 = 0; c0 < kTile; c0 += 32) {
-        uint32_t v[32];
-        tmem_ld_32x32(tSw + c0, v);
-        tmem_ld_wait();
-        if (cut) {
+      for (int i = 0; i < 4; ++i) tmem_ld_32x32(tSw + 32 * i, v[i]);
+      tmem_ld_wait();
+      if (cut) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) m = fmaxf(m, shown(c0 + e) ? __uint_as_float(v[e]) * c : -INFINITY);
-        } else {
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t shown = bits_below(hi + 1 - 32 * i) & (~bits_below(lo - 32 * i) | bits_below(sinks - 32 * i));
 #pragma unroll
-          for (int e = 0; e < 32; ++e) m = fmaxf(m, __uint_as_float(v[e]) * c);
+          for (int e = 0; e < 32; ++e) v[i][e] = shown >> e & 1 ? v[i][e] : kMinusInf;
         }
       }
+      float part[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        part[i] = __uint_as_float(v[i][0]);
+#pragma unroll
+        for (int e = 1; e < 31; e += 2) part[i] = fmaxf(fmaxf(part[i], __uint_as_float(v[i][e])), __uint_as_float(v[i][e + 1]));
+        part[i] = fmaxf(part[i], __uint_as_float(v[i][31]));
+      }
+      const float m = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * c;
       const bool grew = m > top + kLazy;  // (from -inf any finite value)
       if (__any_sync(0xffffffffu, grew)) {
         const float f = grew ? ex2(top - m) : 1.f;
@@ -352,23 +390,21 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
         if (n > 0) scale_row<D>(tOw, f);  // the products that went into the output have completed: the scores were issued behind them
       }
       const float ref = top == -INFINITY ? 0.f : top;  // a row that has seen no key yet
+      float2 sums[4];
 #pragma unroll
-      for (int c0 = 0; c0 < kTile; c0 += 32) {
-        uint32_t v[32], o[16];
-        tmem_ld_32x32(tSw + c0, v);
-        tmem_ld_wait();
+      for (int i = 0; i < 4; ++i) {
+        uint32_t o[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          float x = ex2(fmaf(__uint_as_float(v[e]), c, -ref)), y = ex2(fmaf(__uint_as_float(v[e + 1]), c, -ref));
-          if (cut) {
-            x = shown(c0 + e) ? x : 0.f;
-            y = shown(c0 + e + 1) ? y : 0.f;
-          }
-          sum += x + y;
-          o[e / 2] = pack2<T>(x, y);
+          const float2 x = fma2(pair_of(v[i][e], v[i][e + 1]), make_float2(c, c), make_float2(-ref, -ref));
+          const float2 y = make_float2(ex2(x.x), ex2(x.y));
+          sums[(e >> 1) & 3] = i == 0 && e < 8 ? y : add2(sums[(e >> 1) & 3], y);
+          o[e / 2] = pack2<T>(y.x, y.y);
         }
-        tmem_st_32x16(tSw + c0 / 2, o);  // over scores that have been read
+        tmem_st_32x16(tSw + 16 * i, o);  // over scores that have been read
       }
+      sums[0] = add2(add2(sums[0], sums[1]), add2(sums[2], sums[3]));
+      sum += sums[0].x + sums[0].y;
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(p_full + 8 * w);
@@ -973,7 +1009,7 @@ int check_desc(aig_ctx* ctx, const aig_window_desc* d, const char* who) {
   AIG_REQUIRE(ctx, d && dtype_known(d->dtype), "%s: null description or unknown element type", who);
   AIG_REQUIRE(ctx, d->batch >= 0 && d->q_len >= 0 && d->kv_len >= d->q_len && d->heads > 0 && d->kv_heads > 0 && d->heads % d->kv_heads == 0 && d->sinks >= 0,
               "%s: bad extents (q_len at most kv_len, heads a multiple of kv_heads)", who);
-  AIG_REQUIRE(ctx, d->scale == d->scale && d->scale - d->scale == 0.f, "%s: the scale is not finite", who);
+  AIG_REQUIRE(ctx, d->scale > 0.f && d->scale - d->scale == 0.f, "%s: the scale has to be positive and finite", who);
   if (d->head_dim != 64 && d->head_dim != 128)
     return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "%s: head dimension must be 64 or 128 (got %d)", who, d->head_dim);
   if (d->batch > 65535 || d->heads > 65535) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "%s: more than 65535 sequences or heads", who);
