@@ -676,22 +676,30 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
       const bool cut = j0 + kTile - 1 > off + r0 || (p.window > 0 && j0 <= off + r0 + kTile - 1 - p.window && j0 + kTile > p.sinks);
       const int c_0 = half * 64;
       const int lo = p.window > 0 ? pos - p.window + 1 - j0 - c_0 : -1, hi = pos - j0 - c_0, sinks = p.sinks - j0 - c_0;
-      float own = 0.f;
+      if (cut) {
 #pragma unroll
-      for (int e = 0; e < 64; ++e) {
-        float w = ex2(fmaf(__uint_as_float(sc[e >> 5][e & 31]), c, -lse2));
-        float d = __uint_as_float(dp[e >> 5][e & 31]);
-        if (cut) {
-          const bool shown = e <= hi && (e >= lo || e < sinks);
-          w = shown ? w : 0.f;
-          d = shown ? d : 0.f;
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t shown = bits_below(hi + 1 - 32 * i) & (~bits_below(lo - 32 * i) | bits_below(sinks - 32 * i));
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            sc[i][e] = shown >> e & 1 ? sc[i][e] : kMinusInf;
+            dp[i][e] = shown >> e & 1 ? dp[i][e] : 0u;
+          }
         }
-        sc[e >> 5][e & 31] = __float_as_uint(w);
-        dp[e >> 5][e & 31] = __float_as_uint(d);
-        if (tiles == 1) own = fmaf(w, d, own);
       }
+      float2 own = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float2 x = fma2(pair_of(sc[i][e], sc[i][e + 1]), make_float2(c, c), make_float2(-lse2, -lse2));
+          const float2 w = make_float2(ex2(x.x), ex2(x.y));
+          sc[i][e] = __float_as_uint(w.x);
+          sc[i][e + 1] = __float_as_uint(w.y);
+          if (tiles == 1) own = fma2(w, pair_of(dp[i][e], dp[i][e + 1]), own);
+        }
       if (tiles == 1) {
-        s_sum[half * 128 + in_tile] = own;
+        s_sum[half * 128 + in_tile] = own.x + own.y;
         named_bar_sync(2, 256);
         delta = s_sum[in_tile] + s_sum[128 + in_tile];
       }
@@ -707,9 +715,10 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
       for (int c0 = 0; c0 < 2; ++c0) {
         uint32_t o[16];
 #pragma unroll
-        for (int e = 0; e < 32; e += 2)
-          o[e / 2] = pack2<T>(__uint_as_float(sc[c0][e]) * r * (__uint_as_float(dp[c0][e]) - delta),
-                              __uint_as_float(sc[c0][e + 1]) * r * (__uint_as_float(dp[c0][e + 1]) - delta));
+        for (int e = 0; e < 32; e += 2) {
+          const float2 x = mul2(mul2(pair_of(sc[c0][e], sc[c0][e + 1]), make_float2(r, r)), add2(pair_of(dp[c0][e], dp[c0][e + 1]), make_float2(-delta, -delta)));
+          o[e / 2] = pack2<T>(x.x, x.y);
+        }
         tmem_st_32x16(tdS + lanes + half * 32 + c0 * 16, o);
       }
       tmem_st_wait();
@@ -752,8 +761,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* const sm = smem_raw + (base - raw);
   const uint32_t sK = base, sV = sK + kTileBytes<D>, sQ = sV + kTileBytes<D>, sG = sQ + NS * kTileBytes<D>;
-  float* const s_lse = reinterpret_cast<float*>(sm + (2 + 2 * NS) * kTileBytes<D>);  // [NS][128], in log2, less the weights' power
-  float* const s_delta = s_lse + NS * 128;                                            // [NS][128]
+  float* const s_lse = reinterpret_cast<float*>(sm + (2 + 2 * NS) * kTileBytes<D>);  // [NS][128]: -lse in log2, plus the weights' power
+  float* const s_delta = s_lse + NS * 128;                                            // [NS][128]: -delta
   uint64_t* const bars = reinterpret_cast<uint64_t*>(s_delta + NS * 128);
   const uint32_t bar0 = smem_u32(bars);
   const uint32_t kv_full = bar0, s_full = bar0 + 8, p_full = bar0 + 16, dp_full = bar0 + 24, ds_full = bar0 + 32, all_done = bar0 + 40,
@@ -902,8 +911,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
 #pragma unroll
       for (int i = tid; i < kTile; i += 64) {
         const bool there = row + i < rows_end;
-        s_lse[s * 128 + i] = there ? fmaf(p.lse[stat + row + i], kLog2e, -(float)kWeightBits<T>) : INFINITY;  // (a weight of 0)
-        s_delta[s * 128 + i] = there ? p.delta[stat + row + i] : 0.f;
+        s_lse[s * 128 + i] = there ? fmaf(p.lse[stat + row + i], -kLog2e, (float)kWeightBits<T>) : -INFINITY;  // (a weight of 0)
+        s_delta[s * 128 + i] = there ? -p.delta[stat + row + i] : 0.f;
       }
       if (kScaled) {
         k = next_power(k, ev + tile_exponent<D>(sm + (sG - base) + s * kTileBytes<D>, min(kTile, rows_end - row), tid, s_pair));
@@ -922,28 +931,42 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
     for (int it = 0; it < tiles; ++it) {
       const int s = it % NS, first = off + (t_first + it % per_head) * kTile;  // position of the tile's first query
       const uint32_t ph = (uint32_t)it & 1u;
-      const float *lse2 = s_lse + s * 128 + half * 64, *delta = s_delta + s * 128 + half * 64;
+      const float4 *lse2 = reinterpret_cast<const float4*>(s_lse + s * 128 + half * 64), *delta = reinterpret_cast<const float4*>(s_delta + s * 128 + half * 64);
       const bool cut = j0 + kTile - 1 > first || (p.window > 0 && j0 <= first + kTile - 1 - p.window && j0 + kTile > p.sinks);
       // columns whose queries see this thread's key: from `from` on, and before `to` unless it is a sink
       const int from = key - first - half * 64, to = p.window > 0 && !sink ? from + p.window : 0x7fffffff;
       if (!(ok = warp_wait(st_full + 8 * s, (uint32_t)(it / NS) & 1u, s_abort, p.gerr, 1149))) break;
       if (!(ok = warp_wait(s_full, ph, s_abort, p.gerr, 1150))) break;
       tc_fence_after();
-      float w[64];
+      uint32_t w[2][32];
+      tmem_ld_32x32(tS + lanes + half * 64, w[0]);
+      tmem_ld_32x32(tS + lanes + half * 64 + 32, w[1]);
+      tmem_ld_wait();
+      if (cut) {
 #pragma unroll
-      for (int c0 = 0; c0 < 64; c0 += 32) {
-        uint32_t v[32], o[16];
-        tmem_ld_32x32(tS + lanes + half * 64 + c0, v);
-        tmem_ld_wait();
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t shown = ~bits_below(from - 32 * i) & bits_below(to - 32 * i);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          float x = ex2(fmaf(__uint_as_float(v[e]), c, -lse2[c0 + e]));
-          if (cut) x = c0 + e >= from && c0 + e < to ? x : 0.f;
-          w[c0 + e] = x;
+          for (int e = 0; e < 32; ++e) w[i][e] = shown >> e & 1 ? w[i][e] : kMinusInf;
         }
+      }
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) o[e / 2] = pack2<T>(w[c0 + e], w[c0 + e + 1]);
-        tmem_st_32x16(tS + lanes + half * 64 + c0 / 2, o);  // over scores that have been read
+      for (int i = 0; i < 2; ++i) {
+        uint32_t o[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 l = lse2[8 * i + e / 4];
+          const float2 x = fma2(pair_of(w[i][e], w[i][e + 1]), make_float2(c, c), make_float2(l.x, l.y));
+          const float2 y = fma2(pair_of(w[i][e + 2], w[i][e + 3]), make_float2(c, c), make_float2(l.z, l.w));
+          const float4 z = make_float4(ex2(x.x), ex2(x.y), ex2(y.x), ex2(y.y));
+          w[i][e] = __float_as_uint(z.x);
+          w[i][e + 1] = __float_as_uint(z.y);
+          w[i][e + 2] = __float_as_uint(z.z);
+          w[i][e + 3] = __float_as_uint(z.w);
+          o[e / 2] = pack2<T>(z.x, z.y);
+          o[e / 2 + 1] = pack2<T>(z.z, z.w);
+        }
+        tmem_st_32x16(tS + lanes + half * 64 + 16 * i, o);  // over scores that have been read
       }
       tmem_st_wait();
       tc_fence_before();
@@ -958,22 +981,35 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
         k = k_new;
         r *= pow2(k - kWeightBits<T>);
       }
-      const int alone = -first - half * 64;  // the column of the query at position 0, which sees one key: no gradient through it
+      uint32_t d[2][32];
+      tmem_ld_32x32(tdP + lanes + half * 64, d[0]);
+      tmem_ld_32x32(tdP + lanes + half * 64 + 32, d[1]);
+      tmem_ld_wait();
+      if (cut) {
+        // hidden values may be of rows that are not there; the query at position 0 sees one key: no gradient through it
 #pragma unroll
-      for (int c0 = 0; c0 < 64; c0 += 32) {
-        uint32_t v[32], o[16];
-        tmem_ld_32x32(tdP + lanes + half * 64 + c0, v);
-        tmem_ld_wait();
+        for (int i = 0; i < 2; ++i) {
+          const int alone = -first - half * 64 - 32 * i;
+          const uint32_t shown = ~bits_below(from - 32 * i) & bits_below(to - 32 * i) & ~(bits_below(alone + 1) & ~bits_below(alone));
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          float x = w[c0 + e] * r * (__uint_as_float(v[e]) - delta[c0 + e]), y = w[c0 + e + 1] * r * (__uint_as_float(v[e + 1]) - delta[c0 + e + 1]);
-          if (cut) {
-            x = c0 + e >= from && c0 + e < to && c0 + e != alone ? x : 0.f;
-            y = c0 + e + 1 >= from && c0 + e + 1 < to && c0 + e + 1 != alone ? y : 0.f;
+          for (int e = 0; e < 32; ++e) {
+            d[i][e] = shown >> e & 1 ? d[i][e] : 0u;
+            w[i][e] = shown >> e & 1 ? w[i][e] : 0u;
           }
-          o[e / 2] = pack2<T>(x, y);
         }
-        tmem_st_32x16(tdP + lanes + half * 64 + c0 / 2, o);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t o[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 l = delta[8 * i + e / 4];
+          const float2 x = mul2(mul2(pair_of(w[i][e], w[i][e + 1]), make_float2(r, r)), add2(pair_of(d[i][e], d[i][e + 1]), make_float2(l.x, l.y)));
+          const float2 y = mul2(mul2(pair_of(w[i][e + 2], w[i][e + 3]), make_float2(r, r)), add2(pair_of(d[i][e + 2], d[i][e + 3]), make_float2(l.z, l.w)));
+          o[e / 2] = pack2<T>(x.x, x.y);
+          o[e / 2 + 1] = pack2<T>(y.x, y.y);
+        }
+        tmem_st_32x16(tdP + lanes + half * 64 + 16 * i, o);
       }
       tmem_st_wait();
       tc_fence_before();
