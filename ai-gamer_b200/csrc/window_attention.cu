@@ -41,13 +41,35 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* desc, uint
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(desc)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
-// D[tmem] (+)= A[tmem] * B[smem]
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// tcgen05.mma and commit by the lane whose `issue` is set.  The predicate is inside: the whole warp runs the code around it
+// with the same values, so that descriptors are advanced in uniform registers.  (In a branch that one lane takes, every
+// operand is moved from a vector register: four products and two commits took 365 clocks to issue.)  Descriptors are given by
+// their low words; the high word is the same for all tiles here.
+constexpr uint32_t kDescHi = umma_desc_hi(128);
+// D[tmem] (+)= A[smem] * B[smem]
+__device__ __forceinline__ void mma_ss(uint32_t issue, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p, l;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %4};\n\tmov.b64 db, {%2, %4};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 l, %6, 0;\n\t"
+      "@l tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(kDescHi), "r"(accumulate), "r"(issue)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void mma_ts(uint32_t issue, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, l;\n\t.reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %4};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 l, %6, 0;\n\t"
+      "@l tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(kDescHi), "r"(accumulate), "r"(issue)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t issue, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred l;\n\tsetp.ne.b32 l, %1, 0;\n\t"
+      "@l tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(issue)
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -111,35 +133,36 @@ constexpr uint32_t kMinusInf = 0xff800000u;
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* gerr, int code) {
   return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, gerr, code));
 }
-// Shared-memory descriptor of an operand whose rows (of 128 bytes, swizzled) run along the product's K dimension: 64
-// elements of M or N per row, the next 64 `block` bytes on, groups of eight rows 1024 bytes apart.
-__device__ __forceinline__ uint64_t umma_smem_desc_mn(uint32_t saddr, uint32_t block) {
-  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(block >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
 template <class T>
 __host__ __device__ constexpr uint32_t idesc_for(int m, int n, bool b_mn_major) {
   return umma_idesc_f16(m, n) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7 | 1u << 10) : 0u) | (b_mn_major ? 1u << 16 : 0u);
 }
 
-// A tile of 128 rows of D elements as D/64 blocks of [128 rows][64 elements], 128-byte swizzled
-template <int D>
-constexpr uint32_t kTileBytes = kTile * D * 2;
-template <int D>
+// A tile of R rows of D elements as D/64 blocks of [R rows][64 elements], 128-byte swizzled
+template <int D, int R>
+constexpr uint32_t kTileBytes = R * D * 2;
+// by boxes of B rows
+template <int D, int R, int B>
 __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int head, int row, int b) {
 #pragma unroll
-  for (int c = 0; c < D / 64; ++c) tma_load_4d(dst + c * kTile * 128, map, bar, c * 64, head, row, b);
+  for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+    for (int r = 0; r < R; r += B) tma_load_4d(dst + (c * R + r) * 128, map, bar, c * 64, head, row + r, b);
 }
-// K-major operand, K step `ks` of 16 elements
-__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int ks) { return umma_smem_desc(tile + (ks >> 2) * kTile * 128 + (ks & 3) * 32, 128); }
-// the same tile with its rows as the K dimension, K step of 16 rows
-__device__ __forceinline__ uint64_t desc_rows(uint32_t tile, int ks) { return umma_smem_desc_mn(tile + ks * 16 * 128, kTile * 128); }
+// Low descriptor words of a tile as a K-major operand, K step `ks` of 16 elements of its rows (128-byte swizzled, groups of
+// eight rows 1024 bytes apart) ...
+template <int R>
+__device__ __forceinline__ uint32_t desc_k(uint32_t tile, int ks) { return umma_desc_lo(tile) + (((ks >> 2) * R * 128 + (ks & 3) * 32) >> 4); }
+// ... and with its rows as the K dimension, K step of 16 rows (64 elements of N per row, the next 64 a block further on)
+template <int R>
+__device__ __forceinline__ uint32_t desc_rows(uint32_t tile, int ks) { return ((tile & 0x3FFFFu) >> 4 | (uint32_t)(R * 128 / 16) << 16) + ks * (16 * 128 / 16); }
 // Rows from `from` on become zeros (a product with the weight 0 would keep a NaN); by one warp, before the product reads them
-template <int D>
+template <int D, int R>
 __device__ __forceinline__ void clear_rows(uint8_t* tile, int from, int lane) {
-  const int pieces = (kTile - from) * 8;
+  const int pieces = (R - from) * 8;
 #pragma unroll
   for (int c = 0; c < D / 64; ++c)
-    for (int i = lane; i < pieces; i += 32) *reinterpret_cast<uint4*>(tile + c * kTile * 128 + from * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+    for (int i = lane; i < pieces; i += 32) *reinterpret_cast<uint4*>(tile + c * R * 128 + from * 128 + i * 16) = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
   __syncwarp();
 }
@@ -180,16 +203,17 @@ __device__ __forceinline__ void scale_row(uint32_t taddr, float f) {
   }
 }
 
-// Key tiles that a tile of queries at positions first .. last visits: [0, sink_end) and [begin, end)
+// Tiles of R keys that queries at positions first .. last visit: [0, sink_end) and [begin, end)
 struct KeyTiles {
   int sink_end, begin, end;
   __device__ __forceinline__ bool has(int t) const { return t < sink_end || (t >= begin && t < end); }
 };
+template <int R>
 __device__ __forceinline__ KeyTiles key_tiles(int first, int last, int window, int sinks) {
   KeyTiles k;
-  k.begin = window > 0 ? max(0, first - window + 1) / kTile : 0;
-  k.end = last < first ? k.begin : last / kTile + 1;
-  k.sink_end = window > 0 && last >= first ? min((sinks + kTile - 1) / kTile, k.begin) : 0;
+  k.begin = window > 0 ? max(0, first - window + 1) / R : 0;
+  k.end = last < first ? k.begin : last / R + 1;
+  k.sink_end = window > 0 && last >= first ? min((sinks + R - 1) / R, k.begin) : 0;
   return k;
 }
 
@@ -201,8 +225,8 @@ struct FwdShape {
   static constexpr int kThreads = 128 + 128 * NT;
   static constexpr int kCtasPerSm = 1;
   static constexpr int kTmemCols = NT == 2 ? 512 : 256;  // scores 128 columns a tile, then outputs D columns a tile
-  static constexpr uint32_t kQ = NT * kTileBytes<D>;
-  static constexpr size_t kSmem = kQ + 2 * kStages * kTileBytes<D> + 1024 + 256;
+  static constexpr uint32_t kQ = NT * kTileBytes<D, kTile>;
+  static constexpr size_t kSmem = kQ + 2 * kStages * kTileBytes<D, kTile> + 1024 + 256;
 };
 constexpr float kLazy = 8.f;  // a row's maximum may grow by 2^8 before its sums are rescaled: weights stay below 2^8
 
@@ -215,8 +239,8 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* const sm = smem_raw + (base - raw);
-  const uint32_t sQ = base, sK = sQ + S::kQ, sV = sK + NS * kTileBytes<D>;
-  uint64_t* const bars = reinterpret_cast<uint64_t*>(sm + S::kQ + 2 * NS * kTileBytes<D>);
+  const uint32_t sQ = base, sK = sQ + S::kQ, sV = sK + NS * kTileBytes<D, kTile>;
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(sm + S::kQ + 2 * NS * kTileBytes<D, kTile>);
   const uint32_t bar0 = smem_u32(bars);
   const uint32_t q_full = bar0, s_full = bar0 + 8, p_full = s_full + 8 * NT, o_full = p_full + 8 * NT, k_full = o_full + 8 * NT,
                  k_free = k_full + 8 * NS, v_full = k_free + 8 * NS, v_free = v_full + 8 * NS;
@@ -238,7 +262,7 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
 #pragma unroll
   for (int w = 0; w < NT; ++w) {
     const int r0 = (block * NT + w) * kTile;
-    kt[w] = key_tiles(off + r0, off + min(r0 + kTile, rows_end) - 1, p.window, p.sinks);
+    kt[w] = key_tiles<kTile>(off + r0, off + min(r0 + kTile, rows_end) - 1, p.window, p.sinks);
     if (kt[w].end > kt[w].begin) {
       sink_end = max(sink_end, kt[w].sink_end);
       begin = min(begin, kt[w].begin);
@@ -280,30 +304,30 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
     if (lane == 0) {
       mbar_expect_tx(q_full, S::kQ);
 #pragma unroll
-      for (int w = 0; w < NT; ++w) load_tile<D>(sQ + w * kTileBytes<D>, &mapQ, q_full, h, (block * NT + w) * kTile, b);
+      for (int w = 0; w < NT; ++w) load_tile<D, kTile, kTile>(sQ + w * kTileBytes<D, kTile>, &mapQ, q_full, h, (block * NT + w) * kTile, b);
       for (int it = 0; it < tiles; ++it) {
         const int s = it % NS, row = tile_at(it) * kTile;
         const uint32_t ph = (uint32_t)(it / NS + 1) & 1u;  // (the first round finds the stages free)
         if (it >= NS && !mbar_wait_bounded(k_free + 8 * s, ph, s_abort, p.gerr, 1101)) break;
-        mbar_expect_tx(k_full + 8 * s, kTileBytes<D>);
-        load_tile<D>(sK + s * kTileBytes<D>, &mapK, k_full + 8 * s, kvh, row, b);
+        mbar_expect_tx(k_full + 8 * s, kTileBytes<D, kTile>);
+        load_tile<D, kTile, kTile>(sK + s * kTileBytes<D, kTile>, &mapK, k_full + 8 * s, kvh, row, b);
         if (it >= NS && !mbar_wait_bounded(v_free + 8 * s, ph, s_abort, p.gerr, 1102)) break;
-        mbar_expect_tx(v_full + 8 * s, kTileBytes<D>);
-        load_tile<D>(sV + s * kTileBytes<D>, &mapV, v_full + 8 * s, kvh, row, b);
+        mbar_expect_tx(v_full + 8 * s, kTileBytes<D, kTile>);
+        load_tile<D, kTile, kTile>(sV + s * kTileBytes<D, kTile>, &mapV, v_full + 8 * s, kvh, row, b);
       }
     }
   } else if (warp == 1) {
     constexpr uint32_t idesc_s = idesc_for<T>(kTile, kTile, false), idesc_o = idesc_for<T>(kTile, D, true);
-    const bool leader = elect_one();
+    const uint32_t leader = elect_one() ? 1u : 0u;
     int done[NT];  // tiles whose second product has been issued
 #pragma unroll
     for (int w = 0; w < NT; ++w) done[w] = 0;
     auto scores = [&](int w, int it) {
-      const uint32_t k = sK + (it % NS) * kTileBytes<D>;
-      if (leader) {
+      const uint32_t k = sK + (it % NS) * kTileBytes<D, kTile>;
+      {
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) umma_f16_ss(tS + 128 * w, desc_k(sQ + w * kTileBytes<D>, ks), desc_k(k, ks), idesc_s, ks != 0);
-        umma_commit(s_full + 8 * w);
+        for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, tS + 128 * w, desc_k<kTile>(sQ + w * kTileBytes<D, kTile>, ks), desc_k<kTile>(k, ks), idesc_s, ks != 0);
+        commit(leader, s_full + 8 * w);
       }
     };
     bool ok = warp_wait(q_full, 0, s_abort, p.gerr, 1103) && warp_wait(k_full, 0, s_abort, p.gerr, 1104);
@@ -312,30 +336,30 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
 #pragma unroll
       for (int w = 0; w < NT; ++w)
         if (kt[w].has(tile_at(0))) scores(w, 0);
-      if (leader) umma_commit(k_free);
+      commit(leader, k_free);
       for (int it = 0; it < tiles && ok; ++it) {
         const int t = tile_at(it), s = it % NS, next = it + 1, ns = next % NS;
         if (next < tiles && !warp_wait(k_full + 8 * ns, (uint32_t)(next / NS) & 1u, s_abort, p.gerr, 1105)) break;
         if (!warp_wait(v_full + 8 * s, (uint32_t)(it / NS) & 1u, s_abort, p.gerr, 1106)) break;
-        if (t * kTile + kTile > len) clear_rows<D>(sm + (sV - base) + s * kTileBytes<D>, len - t * kTile, lane);
+        if (t * kTile + kTile > len) clear_rows<D, kTile>(sm + (sV - base) + s * kTileBytes<D, kTile>, len - t * kTile, lane);
 #pragma unroll
         for (int w = 0; w < NT; ++w) {
           if (kt[w].has(t)) {
             if (!(ok = warp_wait(p_full + 8 * w, (uint32_t)done[w] & 1u, s_abort, p.gerr, 1107))) break;
             tc_fence_after();
-            if (leader) {
+            {
 #pragma unroll
               for (int ks = 0; ks < kTile / 16; ++ks)
-                umma_f16_ts(tO + D * w, tS + 128 * w + ks * 8, desc_rows(sV + s * kTileBytes<D>, ks), idesc_o, done[w] != 0 || ks != 0);
+                mma_ts(leader, tO + D * w, tS + 128 * w + ks * 8, desc_rows<kTile>(sV + s * kTileBytes<D, kTile>, ks), idesc_o, done[w] != 0 || ks != 0);
             }
             ++done[w];
-            if (t + 1 == kt[w].end && leader) umma_commit(o_full + 8 * w);
+            if (t + 1 == kt[w].end) commit(leader, o_full + 8 * w);
           }
           if (next < tiles && kt[w].has(tile_at(next))) scores(w, next);
         }
-        if (leader) {
-          umma_commit(v_free + 8 * s);
-          if (next < tiles) umma_commit(k_free + 8 * ns);
+        {
+          commit(leader, v_free + 8 * s);
+          if (next < tiles) commit(leader, k_free + 8 * ns);
         }
       }
     }
@@ -431,72 +455,88 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
 }
 
 // ---------------------------------------------------------------------------------------------
-// Backward: one kernel for dQ (a tile of queries stays, keys pass by), one for dK and dV (a tile of keys stays, the queries of
-// the group's heads pass by).  Each computes the weights again from lse: two more products than one kernel that adds dQ
-// into memory with atomics would need, but every sum has a fixed order.  256 threads share a tile of scores, 64 columns
-// each.
+// Backward: one kernel for dQ (a tile of 128 queries stays, keys pass by), one for dK and dV (a tile of 128 keys stays, the
+// queries of the group's heads pass by).  Each computes the weights again from lse: two more products than one kernel that
+// adds dQ into memory with atomics would need, but every sum has a fixed order.  What passes by comes in tiles of 64 rows
+// for two groups of 128 threads in turn, so that one group's exponentials (the special-function unit's share is the
+// longest) run beside the other's waits, loads and products; a thread owns a row of scores.  (One tile of 128 at a
+// time for both groups, whose products are faster by a third per row, took 257 us where this takes XXX: 2 x 4099, 16 heads of 64.)
 //
 // fp16 has few small numbers: weights of a row over thousands of keys, and dS of small gradients, would be rounded to
 // multiples of 2^-24.  So the weights are multiplied by 2^8, and dS by a power of two 2^k that follows the largest
 // |dO| * |V| seen so far: |dS| stays below 2^15.5 whatever the values, and typical ones around 1.  Where a tile asks for a
 // smaller power the sums so far are scaled (rare: it keeps two bits in hand).
 constexpr int kBwdThreads = 384;
+constexpr int kSub = 64;
 template <class T>
 constexpr int kWeightBits = std::is_same<T, __half>::value ? 8 : 0;
 constexpr int kMostBits = 11, kAimBits = 9;  // of 2^k * |dO| * |V| * sqrt(D)
 
 __device__ __forceinline__ float pow2(int k) { return __int_as_float((k + 127) << 23); }  // -126 .. 127
 
-// Exponent e with max |x| < 2^e over rows [0, rows) of a tile in shared memory, by 64 threads (x finite; -126 at least)
-template <int D>
-__device__ __forceinline__ int tile_exponent(const uint8_t* tile, int rows, int tid, int* s_pair) {
-  __half2 m = __half2half2(__ushort_as_half(0));
+// Exponent e with max |x| < 2^e over rows [0, rows) of a tile in shared memory, by one warp (x finite; -126 at least)
+template <int D, int R>
+__device__ __forceinline__ int tile_exponent(const uint8_t* tile, int rows, int lane) {
+  __half2 m[2] = {__half2half2(__ushort_as_half(0)), __half2half2(__ushort_as_half(0))};
 #pragma unroll
   for (int c = 0; c < D / 64; ++c)
-    for (int i = tid; i < rows * 8; i += 64) {
-      const uint4 v = *reinterpret_cast<const uint4*>(tile + c * kTile * 128 + i * 16);
+#pragma unroll 4
+    for (int i = lane; i < rows * 8; i += 32) {
+      const uint4 v = *reinterpret_cast<const uint4*>(tile + c * R * 128 + i * 16);
       const __half2* h = reinterpret_cast<const __half2*>(&v);
-      m = __hmax2(m, __hmax2(__hmax2(__habs2(h[0]), __habs2(h[1])), __hmax2(__habs2(h[2]), __habs2(h[3]))));
+      m[0] = __hmax2(m[0], __hmax2(__habs2(h[0]), __habs2(h[1])));
+      m[1] = __hmax2(m[1], __hmax2(__habs2(h[2]), __habs2(h[3])));
     }
-  float x = fmaxf(__low2float(m), __high2float(m));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-  const int e = min((int)(__float_as_uint(x) >> 23) - 126, 20);
-  if ((tid & 31) == 0) s_pair[tid >> 5] = e;
-  named_bar_sync(1, 64);
-  const int both = max(s_pair[0], s_pair[1]);
-  named_bar_sync(1, 64);
-  return both;
+  const __half2 both = __hmax2(m[0], m[1]);
+  const uint32_t x = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(__low2float(both), __high2float(both))));  // (not negative: as integers)
+  return min((int)(x >> 23) - 126, 20);
 }
 // the power for a tile whose bound has the exponent e, given the one so far
 __device__ __forceinline__ int next_power(int k, int e) {
   return e + k > kMostBits ? max(kAimBits - e, -100) : k;
 }
+constexpr int kFirstPower = 100;
 
+// Shared memory is handed out to the last kilobytes at D = 128 (a tile has to be fetched two before it is needed): dynamic
+// shared memory starts on a 1024-byte boundary, which the tiles' swizzling needs.
 template <int D>
 struct DqShape {
-  static constexpr int kStages = D == 64 ? 3 : 2;
-  static constexpr size_t kSmem = 2 * kTileBytes<D> + 2 * kStages * kTileBytes<D> + 1024 + 2048;
+  static constexpr int kKeys = D == 64 ? 8 : 6, kValues = D == 64 ? 6 : 4;  // stages: keys are needed for longer
+  static constexpr uint32_t kFixed = 2 * kTileBytes<D, kTile>, kStage = kTileBytes<D, kSub>;
+  static constexpr uint32_t kTiles = kFixed + (kKeys + kValues) * kStage;
+  static constexpr size_t kSmem = kTiles + 1024 + 512;
+};
+template <int D>
+struct DkvShape {
+  static constexpr int kStages = D == 64 ? 7 : 5;
+  static constexpr uint32_t kFixed = 2 * kTileBytes<D, kTile>, kStage = 2 * kTileBytes<D, kSub>;
+  static constexpr uint32_t kTiles = kFixed + kStages * kStage;
+  static constexpr size_t kSmem = kTiles + kStages * kSub * 8 + 384;
 };
 
 template <class T, int D>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
                  const __grid_constant__ CUtensorMap mapG, const __grid_constant__ WinParams p) {
-  constexpr int NS = DqShape<D>::kStages;
+  using S = DqShape<D>;
+  constexpr int NK = S::kKeys, NV = S::kValues;
   constexpr bool kScaled = std::is_same<T, __half>::value;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-  uint8_t* const sm = smem_raw + (base - raw);
-  const uint32_t sQ = base, sG = sQ + kTileBytes<D>, sK = sG + kTileBytes<D>, sV = sK + NS * kTileBytes<D>;
-  float* const s_sum = reinterpret_cast<float*>(sm + (2 + 2 * NS) * kTileBytes<D>);  // [2][128]
+  extern __shared__ __align__(1024) uint8_t sm[];
+  const uint32_t base = smem_u32(sm);
+  if (base & 1023u) {  // (never seen; tiles could not be fetched)
+    if (threadIdx.x == 0) note_error(p.gerr, 1100);
+    return;
+  }
+  const uint32_t sQ = base, sG = sQ + kTileBytes<D, kTile>, sK = base + S::kFixed, sV = sK + NK * S::kStage;
+  float* const s_sum = reinterpret_cast<float*>(sm + S::kTiles);  // [2][128]
   uint64_t* const bars = reinterpret_cast<uint64_t*>(s_sum + 256);
   const uint32_t bar0 = smem_u32(bars);
-  const uint32_t q_full = bar0, sd_full = bar0 + 8, sd_free = bar0 + 16, ds_full = bar0 + 24, ds_free = bar0 + 32, dq_full = bar0 + 40,
-                 k_full = bar0 + 48, k_free = k_full + 8 * NS, v_full = k_free + 8 * NS, v_free = v_full + 8 * NS, st_full = v_free + 8 * NS;
-  int* const s_power = reinterpret_cast<int*>(bars + 6 + 5 * NS);  // [NS]
-  int* const s_pair = s_power + NS;                                // [2]
-  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(s_pair + 2);
+  // of each group: scores and dP are there, they have been read; of each of four buffers: dS is there, it has been used
+  const uint32_t q_full = bar0, dq_full = bar0 + 8, sd_full = bar0 + 16, sd_free = sd_full + 16, ds_full = sd_free + 16, ds_free = ds_full + 32,
+                 k_full = ds_free + 32, k_free = k_full + 8 * NK, v_full = k_free + 8 * NK, v_free = v_full + 8 * NV, st_full = v_free + 8 * NV;
+  int* const s_power = reinterpret_cast<int*>(bars + 14 + 3 * NK + 2 * NV);  // [NK]
+  int* const s_step = s_power + NK;                                          // [NK]: its change against the tile before
+  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(s_step + NK);
   volatile int* const s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
@@ -509,23 +549,29 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   const int off = p.kv_len - p.q_len, r0 = block * kTile;
   const int rows_end = min(p.q_len, len - off);
   if (r0 >= rows_end) return;
-  const KeyTiles kt = key_tiles(off + r0, off + min(r0 + kTile, rows_end) - 1, p.window, p.sinks);
+  const KeyTiles kt = key_tiles<kSub>(off + r0, off + min(r0 + kTile, rows_end) - 1, p.window, p.sinks);
   const int tiles = kt.sink_end + kt.end - kt.begin;
-  auto tile_at = [&](int it) { return it < kt.sink_end ? it : kt.begin + (it - kt.sink_end); };
+  auto first_key = [&](int u) { return (u < kt.sink_end ? u : kt.begin + (u - kt.sink_end)) * kSub; };
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    mbar_init(sd_full, 1);
-    mbar_init(sd_free, 256);
-    mbar_init(ds_full, 256);
-    mbar_init(ds_free, 1);
     mbar_init(dq_full, 1);
-    for (int s = 0; s < NS; ++s) {
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(sd_full + 8 * w, 1);
+      mbar_init(sd_free + 8 * w, 128);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(ds_full + 8 * i, 128);
+      mbar_init(ds_free + 8 * i, 1);
+    }
+    for (int s = 0; s < NK; ++s) {
       mbar_init(k_full + 8 * s, 1);
       mbar_init(k_free + 8 * s, 1);
+      mbar_init(st_full + 8 * s, 1);
+    }
+    for (int s = 0; s < NV; ++s) {
       mbar_init(v_full + 8 * s, 1);
-      mbar_init(v_free + 8 * s, kScaled ? 9 : 1);  // the products are done with it, and each of 8 warps has its power
-      mbar_init(st_full + 8 * s, 64);
+      mbar_init(v_free + 8 * s, kScaled ? 2 : 1);  // the products are done with it, and so is the search for its largest value
     }
     *s_abort = 0;
     fence_mbar_init();
@@ -537,80 +583,82 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *s_tmem, tS = tmem, tdP = tmem + 128, tdS = tmem + 256, tdQ = tmem + 320;
+  // of each group: 64 columns of scores, 64 of dP; then four buffers of 32 for dS; then dQ
+  const uint32_t tmem = *s_tmem, tdS = tmem + 256, tdQ = tmem + 384;
 
   if (warp == 0) {
     if (lane == 0) {
-      mbar_expect_tx(q_full, 2 * kTileBytes<D>);
-      load_tile<D>(sQ, &mapQ, q_full, h, r0, b);
-      load_tile<D>(sG, &mapG, q_full, h, r0, b);
-      for (int it = 0; it < tiles; ++it) {
-        const int s = it % NS, row = tile_at(it) * kTile;
-        const uint32_t ph = (uint32_t)(it / NS + 1) & 1u;
-        if (it >= NS && !mbar_wait_bounded(k_free + 8 * s, ph, s_abort, p.gerr, 1121)) break;
-        mbar_expect_tx(k_full + 8 * s, kTileBytes<D>);
-        load_tile<D>(sK + s * kTileBytes<D>, &mapK, k_full + 8 * s, kvh, row, b);
-        if (it >= NS && !mbar_wait_bounded(v_free + 8 * s, ph, s_abort, p.gerr, 1122)) break;
-        mbar_expect_tx(v_full + 8 * s, kTileBytes<D>);
-        load_tile<D>(sV + s * kTileBytes<D>, &mapV, v_full + 8 * s, kvh, row, b);
+      mbar_expect_tx(q_full, S::kFixed);
+      load_tile<D, kTile, kSub>(sQ, &mapQ, q_full, h, r0, b);
+      load_tile<D, kTile, kSub>(sG, &mapG, q_full, h, r0, b);
+      for (int u = 0; u < tiles; ++u) {
+        const int sk = u % NK, sv = u % NV;
+        if (u >= NK && !mbar_wait_bounded(k_free + 8 * sk, (uint32_t)(u / NK + 1) & 1u, s_abort, p.gerr, 1121)) break;
+        mbar_expect_tx(k_full + 8 * sk, S::kStage);
+        load_tile<D, kSub, kSub>(sK + sk * S::kStage, &mapK, k_full + 8 * sk, kvh, first_key(u), b);
+        if (u >= NV && !mbar_wait_bounded(v_free + 8 * sv, (uint32_t)(u / NV + 1) & 1u, s_abort, p.gerr, 1133)) break;
+        mbar_expect_tx(v_full + 8 * sv, S::kStage);
+        load_tile<D, kSub, kSub>(sV + sv * S::kStage, &mapV, v_full + 8 * sv, kvh, first_key(u), b);
       }
     }
   } else if (warp == 1) {
-    constexpr uint32_t idesc_s = idesc_for<T>(kTile, kTile, false), idesc_q = idesc_for<T>(kTile, D, true);
-    const bool leader = elect_one();
-    // the scores and dP of tile `it`; the stages' tiles are there when it returns true
-    auto scores = [&](int it) {
-      const int s = it % NS, t = tile_at(it);
-      const uint32_t ph = (uint32_t)(it / NS) & 1u;
-      if (!warp_wait(k_full + 8 * s, ph, s_abort, p.gerr, 1123) || !warp_wait(v_full + 8 * s, ph, s_abort, p.gerr, 1124)) return false;
-      if (t * kTile + kTile > len) clear_rows<D>(sm + (sK - base) + s * kTileBytes<D>, len - t * kTile, lane);
+    constexpr uint32_t idesc_s = idesc_for<T>(kTile, kSub, false), idesc_q = idesc_for<T>(kTile, D, true);
+    const uint32_t leader = elect_one() ? 1u : 0u;
+    auto scores = [&](int u) {
+      const uint32_t k = sK + (u % NK) * S::kStage, v = sV + (u % NV) * S::kStage, t = tmem + 128 * (u & 1);
+      if (!warp_wait(k_full + 8 * (u % NK), (uint32_t)(u / NK) & 1u, s_abort, p.gerr, 1122)) return false;
+      if (first_key(u) + kSub > len) clear_rows<D, kSub>(sm + (k - base), len - first_key(u), lane);
+      if (!warp_wait(v_full + 8 * (u % NV), (uint32_t)(u / NV) & 1u, s_abort, p.gerr, 1134)) return false;
       tc_fence_after();
-      if (leader) {
+      {
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) umma_f16_ss(tS, desc_k(sQ, ks), desc_k(sK + s * kTileBytes<D>, ks), idesc_s, ks != 0);
+        for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, t, desc_k<kTile>(sQ, ks), desc_k<kSub>(k, ks), idesc_s, ks != 0);
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) umma_f16_ss(tdP, desc_k(sG, ks), desc_k(sV + s * kTileBytes<D>, ks), idesc_s, ks != 0);
-        umma_commit(sd_full);
-        umma_commit(v_free + 8 * s);
+        for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, t + 64, desc_k<kTile>(sG, ks), desc_k<kSub>(v, ks), idesc_s, ks != 0);
+        commit(leader, sd_full + 8 * (u & 1));
+        commit(leader, v_free + 8 * (u % NV));
       }
       return true;
     };
-    if (warp_wait(q_full, 0, s_abort, p.gerr, 1125) && scores(0)) {
-      for (int it = 0; it < tiles; ++it) {
-        const uint32_t ph = (uint32_t)it & 1u;
-        if (it + 1 < tiles) {
-          if (!warp_wait(sd_free, ph, s_abort, p.gerr, 1126)) break;
-          if (!scores(it + 1)) break;
+    if (warp_wait(q_full, 0, s_abort, p.gerr, 1123) && scores(0) && (tiles < 2 || scores(1))) {
+      for (int u = 0; u < tiles + 2; ++u) {
+        if (u + 2 < tiles) {
+          if (!warp_wait(sd_free + 8 * (u & 1), (uint32_t)(u >> 1) & 1u, s_abort, p.gerr, 1124)) break;
+          if (!scores(u + 2)) break;
         }
-        if (!warp_wait(ds_full, ph, s_abort, p.gerr, 1127)) break;
+        if (u < 2 || u - 2 >= tiles) continue;
+        const int x = u - 2;  // the tile that this group had before: its dS is there
+        if (!warp_wait(ds_full + 8 * (x & 3), (uint32_t)(x >> 2) & 1u, s_abort, p.gerr, 1125)) break;
         tc_fence_after();
-        if (leader) {
+        {
 #pragma unroll
-          for (int ks = 0; ks < kTile / 16; ++ks)
-            umma_f16_ts(tdQ, tdS + ks * 8, desc_rows(sK + (it % NS) * kTileBytes<D>, ks), idesc_q, it != 0 || ks != 0);
-          umma_commit(ds_free);
-          umma_commit(k_free + 8 * (it % NS));
-          if (it + 1 == tiles) umma_commit(dq_full);
+          for (int ks = 0; ks < kSub / 16; ++ks)
+            mma_ts(leader, tdQ, tdS + 32 * (x & 3) + ks * 8, desc_rows<kSub>(sK + (x % NK) * S::kStage, ks), idesc_q, x != 0 || ks != 0);
+          commit(leader, ds_free + 8 * (x & 3));
+          commit(leader, k_free + 8 * (x % NK));
+          if (x + 1 == tiles) commit(leader, dq_full);
         }
       }
     }
-  } else if (warp < 4) {
-    if (kScaled) {
-      const int tid = threadIdx.x - 64;
-      if (named_bar_and(1, 64, warp_wait(q_full, 0, s_abort, p.gerr, 1128))) {
-        const int eg = tile_exponent<D>(sm + (sG - base), min(kTile, rows_end - r0), tid, s_pair) + (D == 64 ? 3 : 4);
-        int k = 100;
-        for (int it = 0; it < tiles; ++it) {
-          const int s = it % NS;
-          if (!named_bar_and(1, 64, warp_wait(v_full + 8 * s, (uint32_t)(it / NS) & 1u, s_abort, p.gerr, 1129))) break;
-          k = next_power(k, eg + tile_exponent<D>(sm + (sV - base) + s * kTileBytes<D>, min(kTile, len - tile_at(it) * kTile), tid, s_pair));
-          if (tid == 0) s_power[s] = k;
-          mbar_arrive(st_full + 8 * s);
+  } else if (warp == 2) {
+    if (kScaled && warp_wait(q_full, 0, s_abort, p.gerr, 1126)) {
+      const int eg = tile_exponent<D, kTile>(sm + (sG - base), min(kTile, rows_end - r0), lane) + (D == 64 ? 3 : 4);
+      int k = kFirstPower;
+      for (int u = 0; u < tiles; ++u) {
+        if (!warp_wait(v_full + 8 * (u % NV), (uint32_t)(u / NV) & 1u, s_abort, p.gerr, 1127)) break;
+        const int k_new = next_power(k, eg + tile_exponent<D, kSub>(sm + (sV - base) + (u % NV) * S::kStage, min(kSub, len - first_key(u)), lane));
+        __syncwarp();
+        if (lane == 0) {
+          s_power[u % NK] = k_new;
+          s_step[u % NK] = u == 0 ? 0 : k_new - k;
+          mbar_arrive(st_full + 8 * (u % NK));
+          mbar_arrive(v_free + 8 * (u % NV));
         }
+        k = k_new;
       }
     }
-  } else {
-    const int half = (warp - 4) >> 2, q = warp & 3, in_tile = q * 32 + lane;
+  } else if (warp >= 4) {
+    const int w = (warp - 4) >> 2, q = warp & 3, in_tile = q * 32 + lane;
     const int row = r0 + in_tile, pos = off + row;
     const bool there = row < rows_end;
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
@@ -620,63 +668,60 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
     // a query that sees one key has the weight 1 whatever its score: no gradient through it
     const bool single = pos == 0 || (p.window == 1 && p.sinks == 0);
     float delta = 0.f;
-    if (tiles > 1) {
-      // (dO . O has the output's rounding in it: with a tile's keys or fewer, where that is large against dP, the sum over
+    if (tiles > 2) {
+      // (dO . O has the output's rounding in it; with two tiles' keys or fewer, where that is large against dP, the sum over
       // the weights is taken instead, below)
       float d = 0.f;
       if (there) {
-        const T* g = reinterpret_cast<const T*>(p.dout.data) + b * p.dout.batch + row * p.dout.token + h * p.dout.head + half * (D / 2);
-        const T* o = reinterpret_cast<const T*>(p.o.data) + b * p.o.batch + row * p.o.token + h * p.o.head + half * (D / 2);
+        const T* g = reinterpret_cast<const T*>(p.dout.data) + b * p.dout.batch + row * p.dout.token + h * p.dout.head + w * (D / 2);
+        const T* o = reinterpret_cast<const T*>(p.o.data) + b * p.o.batch + row * p.o.token + h * p.o.head + w * (D / 2);
 #pragma unroll
         for (int i = 0; i < D / 2; i += 8) {
           const uint4 x = *reinterpret_cast<const uint4*>(g + i), y = *reinterpret_cast<const uint4*>(o + i);
           const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float2 u = unpack2<T>(xs[e]), v = unpack2<T>(ys[e]);
-            d = fmaf(u.x, v.x, fmaf(u.y, v.y, d));
+            const float2 a = unpack2<T>(xs[e]), z = unpack2<T>(ys[e]);
+            d = fmaf(a.x, z.x, fmaf(a.y, z.y, d));
           }
         }
       }
-      s_sum[half * 128 + in_tile] = d;
+      s_sum[w * 128 + in_tile] = d;
       named_bar_sync(2, 256);
       delta = s_sum[in_tile] + s_sum[128 + in_tile];
+    } else if (w >= tiles) {
+      s_sum[w * 128 + in_tile] = 0.f;
+      named_bar_sync(2, 256);
     }
-    int k = 0;
     bool ok = true;
-    for (int it = 0; it < tiles; ++it) {
-      const int s = it % NS, j0 = tile_at(it) * kTile;
-      const uint32_t ph = (uint32_t)it & 1u;
-      if (!(ok = warp_wait(sd_full, ph, s_abort, p.gerr, 1130))) {
-        if (tiles == 1) named_bar_sync(2, 256);  // (the others may be waiting below)
+    for (int u = w, n = 0; u < tiles; u += 2, ++n) {
+      const int s = u % NK, j0 = first_key(u);
+      const uint32_t t = tmem + 128 * w + lanes;
+      float r = 1.f;
+      int step = 0;
+      ok = warp_wait(sd_full + 8 * w, (uint32_t)n & 1u, s_abort, p.gerr, 1128);
+      if (kScaled && ok) {
+        ok = warp_wait(st_full + 8 * s, (uint32_t)(u / NK) & 1u, s_abort, p.gerr, 1129);
+        r = pow2(s_power[s]);
+        step = s_step[s];
+      }
+      if (!ok) {
+        if (tiles <= 2) named_bar_sync(2, 256);  // (the other group may be waiting below)
         break;
       }
       tc_fence_after();
       uint32_t sc[2][32], dp[2][32];
-      tmem_ld_32x32(tS + lanes + half * 64, sc[0]);
-      tmem_ld_32x32(tS + lanes + half * 64 + 32, sc[1]);
-      tmem_ld_32x32(tdP + lanes + half * 64, dp[0]);
-      tmem_ld_32x32(tdP + lanes + half * 64 + 32, dp[1]);
+      tmem_ld_32x32(t, sc[0]);
+      tmem_ld_32x32(t + 32, sc[1]);
+      tmem_ld_32x32(t + 64, dp[0]);
+      tmem_ld_32x32(t + 96, dp[1]);
       tmem_ld_wait();
       tc_fence_before();
-      mbar_arrive(sd_free);
-      float r = 1.f;
-      int k_new = 0;
-      if (kScaled) {
-        if (!(ok = warp_wait(st_full + 8 * s, (uint32_t)(it / NS) & 1u, s_abort, p.gerr, 1131))) {
-          if (tiles == 1) named_bar_sync(2, 256);
-          break;
-        }
-        k_new = s_power[s];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(v_free + 8 * s);
-        r = pow2(k_new);
-      }
+      mbar_arrive(sd_free + 8 * w);
       if (single) r = 0.f;
-      const bool cut = j0 + kTile - 1 > off + r0 || (p.window > 0 && j0 <= off + r0 + kTile - 1 - p.window && j0 + kTile > p.sinks);
-      const int c_0 = half * 64;
-      const int lo = p.window > 0 ? pos - p.window + 1 - j0 - c_0 : -1, hi = pos - j0 - c_0, sinks = p.sinks - j0 - c_0;
+      const bool cut = j0 + kSub - 1 > off + r0 || (p.window > 0 && j0 <= off + r0 + kTile - 1 - p.window && j0 + kSub > p.sinks);
       if (cut) {
+        const int lo = p.window > 0 ? pos - p.window + 1 - j0 : -1, hi = pos - j0, sinks = p.sinks - j0;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint32_t shown = bits_below(hi + 1 - 32 * i) & (~bits_below(lo - 32 * i) | bits_below(sinks - 32 * i));
@@ -693,44 +738,43 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           const float2 x = fma2(pair_of(sc[i][e], sc[i][e + 1]), make_float2(c, c), make_float2(-lse2, -lse2));
-          const float2 w = make_float2(ex2(x.x), ex2(x.y));
-          sc[i][e] = __float_as_uint(w.x);
-          sc[i][e + 1] = __float_as_uint(w.y);
-          if (tiles == 1) own = fma2(w, pair_of(dp[i][e], dp[i][e + 1]), own);
+          const float2 y = make_float2(ex2(x.x), ex2(x.y));
+          sc[i][e] = __float_as_uint(y.x);
+          sc[i][e + 1] = __float_as_uint(y.y);
+          if (tiles <= 2) own = fma2(y, pair_of(dp[i][e], dp[i][e + 1]), own);
         }
-      if (tiles == 1) {
-        s_sum[half * 128 + in_tile] = own.x + own.y;
+      if (tiles <= 2) {
+        s_sum[w * 128 + in_tile] = own.x + own.y;
         named_bar_sync(2, 256);
         delta = s_sum[in_tile] + s_sum[128 + in_tile];
       }
-      if (it > 0) {
-        if (!(ok = warp_wait(ds_free, ph ^ 1u, s_abort, p.gerr, 1132))) break;
-        if (kScaled && k_new != k) {
-          tc_fence_after();
-          scale_row<D / 2>(tdQ + lanes + half * (D / 2), pow2(max(k_new - k, -126)));
-        }
+      if (u >= 4 && !(ok = warp_wait(ds_free + 8 * (u & 3), (uint32_t)(u / 4 - 1) & 1u, s_abort, p.gerr, 1130))) break;
+      if (kScaled && step != 0) {  // what has been summed so far, the other group's last tile included, follows
+        if (!(ok = warp_wait(ds_free + 8 * ((u - 1) & 3), (uint32_t)((u - 1) >> 2) & 1u, s_abort, p.gerr, 1131))) break;
+        tc_fence_after();
+        scale_row<D>(tdQ + lanes, pow2(max(step, -126)));
       }
-      k = k_new;
 #pragma unroll
-      for (int c0 = 0; c0 < 2; ++c0) {
+      for (int i = 0; i < 2; ++i) {
         uint32_t o[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          const float2 x = mul2(mul2(pair_of(sc[c0][e], sc[c0][e + 1]), make_float2(r, r)), add2(pair_of(dp[c0][e], dp[c0][e + 1]), make_float2(-delta, -delta)));
+          const float2 x = mul2(mul2(pair_of(sc[i][e], sc[i][e + 1]), make_float2(r, r)), add2(pair_of(dp[i][e], dp[i][e + 1]), make_float2(-delta, -delta)));
           o[e / 2] = pack2<T>(x.x, x.y);
         }
-        tmem_st_32x16(tdS + lanes + half * 32 + c0 * 16, o);
+        tmem_st_32x16(tdS + 32 * (u & 3) + lanes + 16 * i, o);
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(ds_full);
+      mbar_arrive(ds_full + 8 * (u & 3));
     }
-    if (ok && warp_wait(dq_full, 0, s_abort, p.gerr, 1133)) {
+    if (ok && warp_wait(dq_full, 0, s_abort, p.gerr, 1132)) {
       tc_fence_after();
-      if (there && half == 0) p.delta[stat] = delta;
-      const float f = p.scale * pow2(-k);
-      T* const out = reinterpret_cast<T*>(p.dq.data) + b * p.dq.batch + row * p.dq.token + h * p.dq.head + half * (D / 2);
-      store_row<T, D / 2>(tdQ + lanes + half * (D / 2), out, f, there);
+      if (there && w == 0) p.delta[stat] = delta;
+      float f = p.scale;
+      if (kScaled) f *= pow2(-s_power[(tiles - 1) % NK]);
+      T* const out = reinterpret_cast<T*>(p.dq.data) + b * p.dq.batch + row * p.dq.token + h * p.dq.head + w * (D / 2);
+      store_row<T, D / 2>(tdQ + lanes + w * (D / 2), out, f, there);
     }
   }
 
@@ -745,31 +789,30 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   }
 }
 
-template <int D>
-struct DkvShape {
-  static constexpr int kStages = D == 64 ? 3 : 2;
-  static constexpr size_t kSmem = 2 * kTileBytes<D> + 2 * kStages * kTileBytes<D> + 1024 + 4096;
-};
-
 template <class T, int D>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
                   const __grid_constant__ CUtensorMap mapG, const __grid_constant__ WinParams p) {
-  constexpr int NS = DkvShape<D>::kStages;
+  using S = DkvShape<D>;
+  constexpr int NS = S::kStages;
   constexpr bool kScaled = std::is_same<T, __half>::value;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-  uint8_t* const sm = smem_raw + (base - raw);
-  const uint32_t sK = base, sV = sK + kTileBytes<D>, sQ = sV + kTileBytes<D>, sG = sQ + NS * kTileBytes<D>;
-  float* const s_lse = reinterpret_cast<float*>(sm + (2 + 2 * NS) * kTileBytes<D>);  // [NS][128]: -lse in log2, plus the weights' power
-  float* const s_delta = s_lse + NS * 128;                                            // [NS][128]: -delta
-  uint64_t* const bars = reinterpret_cast<uint64_t*>(s_delta + NS * 128);
+  extern __shared__ __align__(1024) uint8_t sm[];
+  const uint32_t base = smem_u32(sm);
+  if (base & 1023u) {  // (never seen; tiles could not be fetched)
+    if (threadIdx.x == 0) note_error(p.gerr, 1100);
+    return;
+  }
+  const uint32_t sK = base, sV = sK + kTileBytes<D, kTile>, ring = base + S::kFixed;  // a stage: queries, gradients of outputs
+  float* const s_lse = reinterpret_cast<float*>(sm + S::kTiles);  // [NS][64]: -lse in log2, plus the weights' power
+  float* const s_delta = s_lse + NS * kSub;                       // [NS][64]: -delta
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(s_delta + NS * kSub);
   const uint32_t bar0 = smem_u32(bars);
-  const uint32_t kv_full = bar0, s_full = bar0 + 8, p_full = bar0 + 16, dp_full = bar0 + 24, ds_full = bar0 + 32, all_done = bar0 + 40,
-                 q_full = bar0 + 48, q_free = q_full + 8 * NS, st_full = q_free + 8 * NS;
-  int* const s_power = reinterpret_cast<int*>(bars + 6 + 3 * NS);  // [NS]
-  int* const s_pair = s_power + NS;                                // [2]
-  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(s_pair + 2);
+  // of each group: scores are there, weights are there, dP is there, dS is there
+  const uint32_t kv_full = bar0, all_done = bar0 + 8, s_full = bar0 + 16, p_full = s_full + 16, dp_full = p_full + 16, ds_full = dp_full + 16,
+                 q_full = ds_full + 16, q_free = q_full + 8 * NS, st_full = q_free + 8 * NS;
+  int* const s_power = reinterpret_cast<int*>(bars + 10 + 3 * NS);  // [NS]
+  int* const s_step = s_power + NS;                                 // [NS]
+  uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(s_step + NS);
   volatile int* const s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
@@ -787,8 +830,9 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
   const int j1 = min(j0 + kTile, len) - 1;
   const int row_first = max(0, j0 - off);
   const int row_last = p.window > 0 && j0 >= p.sinks ? min(rows_end - 1, j1 + p.window - 1 - off) : rows_end - 1;
-  const int t_first = row_first / kTile, per_head = row_last < row_first ? 0 : row_last / kTile - t_first + 1;
+  const int t_first = row_first / kSub, per_head = row_last < row_first ? 0 : row_last / kSub - t_first + 1;
   const int tiles = per_head * group;
+  auto first_row = [&](int u) { return (t_first + u % per_head) * kSub; };
 
   if (tiles == 0) {  // no query sees these keys
     for (int i = threadIdx.x; i < (j1 - j0 + 1) * (D / 8); i += kBwdThreads) {
@@ -801,15 +845,17 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
 
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
-    mbar_init(s_full, 1);
-    mbar_init(p_full, 256);
-    mbar_init(dp_full, 1);
-    mbar_init(ds_full, 256);
     mbar_init(all_done, 1);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(s_full + 8 * w, 1);
+      mbar_init(p_full + 8 * w, 128);
+      mbar_init(dp_full + 8 * w, 1);
+      mbar_init(ds_full + 8 * w, 128);
+    }
     for (int s = 0; s < NS; ++s) {
       mbar_init(q_full + 8 * s, 1);
       mbar_init(q_free + 8 * s, 1);
-      mbar_init(st_full + 8 * s, 64);
+      mbar_init(st_full + 8 * s, kScaled ? 2 : 1);
     }
     *s_abort = 0;
     fence_mbar_init();
@@ -821,133 +867,148 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // weights over the scores, dS over dP, each half of the columns where its own scores were
-  const uint32_t tmem = *s_tmem, tS = tmem, tdP = tmem + 128, tdV = tmem + 256, tdK = tmem + 256 + D;
+  // of each group: 64 columns of scores, then weights, 64 of dP, then dS; then dV and dK
+  const uint32_t tmem = *s_tmem, tdV = tmem + 256, tdK = tmem + 256 + D;
 
   if (warp == 0) {
     if (lane == 0) {
-      mbar_expect_tx(kv_full, 2 * kTileBytes<D>);
-      load_tile<D>(sK, &mapK, kv_full, kvh, j0, b);
-      load_tile<D>(sV, &mapV, kv_full, kvh, j0, b);
-      for (int it = 0; it < tiles; ++it) {
-        const int s = it % NS, h = kvh * group + it / per_head, row = (t_first + it % per_head) * kTile;
-        if (it >= NS && !mbar_wait_bounded(q_free + 8 * s, (uint32_t)(it / NS + 1) & 1u, s_abort, p.gerr, 1141)) break;
-        mbar_expect_tx(q_full + 8 * s, 2 * kTileBytes<D>);
-        load_tile<D>(sQ + s * kTileBytes<D>, &mapQ, q_full + 8 * s, h, row, b);
-        load_tile<D>(sG + s * kTileBytes<D>, &mapG, q_full + 8 * s, h, row, b);
+      mbar_expect_tx(kv_full, S::kFixed);
+      load_tile<D, kTile, kSub>(sK, &mapK, kv_full, kvh, j0, b);
+      load_tile<D, kTile, kSub>(sV, &mapV, kv_full, kvh, j0, b);
+      for (int u = 0; u < tiles; ++u) {
+        const int s = u % NS, h = kvh * group + u / per_head;
+        if (u >= NS && !mbar_wait_bounded(q_free + 8 * s, (uint32_t)(u / NS + 1) & 1u, s_abort, p.gerr, 1141)) break;
+        mbar_expect_tx(q_full + 8 * s, S::kStage);
+        load_tile<D, kSub, kSub>(ring + s * S::kStage, &mapQ, q_full + 8 * s, h, first_row(u), b);
+        load_tile<D, kSub, kSub>(ring + s * S::kStage + kTileBytes<D, kSub>, &mapG, q_full + 8 * s, h, first_row(u), b);
       }
     }
   } else if (warp == 1) {
-    constexpr uint32_t idesc_s = idesc_for<T>(kTile, kTile, false), idesc_g = idesc_for<T>(kTile, D, true);
-    const bool leader = elect_one();
-    auto arrived = [&](int it) {
-      const int s = it % NS, row = (t_first + it % per_head) * kTile;
-      if (!warp_wait(q_full + 8 * s, (uint32_t)(it / NS) & 1u, s_abort, p.gerr, 1142)) return false;
-      if (row + kTile > rows_end) {  // rows behind the sequence's end are summed over too
-        clear_rows<D>(sm + (sQ - base) + s * kTileBytes<D>, rows_end - row, lane);
-        clear_rows<D>(sm + (sG - base) + s * kTileBytes<D>, rows_end - row, lane);
+    constexpr uint32_t idesc_s = idesc_for<T>(kTile, kSub, false), idesc_g = idesc_for<T>(kTile, D, true);
+    const uint32_t leader = elect_one() ? 1u : 0u;
+    auto scores = [&](int u) {
+      const int s = u % NS, row = first_row(u);
+      const uint32_t at = ring + s * S::kStage;
+      if (!warp_wait(q_full + 8 * s, (uint32_t)(u / NS) & 1u, s_abort, p.gerr, 1142)) return false;
+      if (row + kSub > rows_end) {  // rows behind the sequence's end are summed over too
+        clear_rows<D, kSub>(sm + (at - base), rows_end - row, lane);
+        clear_rows<D, kSub>(sm + (at - base) + kTileBytes<D, kSub>, rows_end - row, lane);
+      }
+      tc_fence_after();
+      {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, tmem + 128 * (u & 1), desc_k<kTile>(sK, ks), desc_k<kSub>(at, ks), idesc_s, ks != 0);
+        commit(leader, s_full + 8 * (u & 1));
       }
       return true;
     };
-    auto scores = [&](int it) {
-      if (leader) {
+    auto dps = [&](int u) {
+      {
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) umma_f16_ss(tS, desc_k(sK, ks), desc_k(sQ + (it % NS) * kTileBytes<D>, ks), idesc_s, ks != 0);
-        umma_commit(s_full);
+        for (int ks = 0; ks < D / 16; ++ks)
+          mma_ss(leader, tmem + 128 * (u & 1) + 64, desc_k<kTile>(sV, ks), desc_k<kSub>(ring + (u % NS) * S::kStage + kTileBytes<D, kSub>, ks), idesc_s, ks != 0);
+        commit(leader, dp_full + 8 * (u & 1));
       }
     };
-    auto dps = [&](int it) {
-      if (leader) {
+    bool ok = warp_wait(kv_full, 0, s_abort, p.gerr, 1143);
+    for (int u = 0; u < 2 && u < tiles && ok; ++u) {
+      ok = scores(u);
+      if (ok) dps(u);
+    }
+    for (int u = 0; u <= tiles && ok; ++u) {
+      if (u < tiles) {
+        if (!warp_wait(p_full + 8 * (u & 1), (uint32_t)(u >> 1) & 1u, s_abort, p.gerr, 1144)) break;
+        tc_fence_after();
+        {
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) umma_f16_ss(tdP, desc_k(sV, ks), desc_k(sG + (it % NS) * kTileBytes<D>, ks), idesc_s, ks != 0);
-        umma_commit(dp_full);
+          for (int ks = 0; ks < kSub / 16; ++ks)
+            mma_ts(leader, tdV, tmem + 128 * (u & 1) + ks * 8, desc_rows<kSub>(ring + (u % NS) * S::kStage + kTileBytes<D, kSub>, ks), idesc_g, u != 0 || ks != 0);
+        }
+        if (u + 2 < tiles && !scores(u + 2)) break;
       }
-    };
-    if (warp_wait(kv_full, 0, s_abort, p.gerr, 1143) && arrived(0)) {
+      if (u == 0) continue;
+      const int x = u - 1;  // the other group's tile
+      if (!warp_wait(ds_full + 8 * (x & 1), (uint32_t)(x >> 1) & 1u, s_abort, p.gerr, 1145)) break;
       tc_fence_after();
-      scores(0);
-      dps(0);
-      for (int it = 0; it < tiles; ++it) {
-        const int s = it % NS;
-        const uint32_t ph = (uint32_t)it & 1u;
-        if (!warp_wait(p_full, ph, s_abort, p.gerr, 1144)) break;
-        tc_fence_after();
-        if (leader) {
+      {
 #pragma unroll
-          for (int ks = 0; ks < kTile / 16; ++ks)
-            umma_f16_ts(tdV, tS + (ks >> 2) * 64 + (ks & 3) * 8, desc_rows(sG + s * kTileBytes<D>, ks), idesc_g, it != 0 || ks != 0);
-        }
-        if (it + 1 < tiles) {
-          if (!arrived(it + 1)) break;
-          scores(it + 1);
-        }
-        if (!warp_wait(ds_full, ph, s_abort, p.gerr, 1145)) break;
-        tc_fence_after();
-        if (leader) {
-#pragma unroll
-          for (int ks = 0; ks < kTile / 16; ++ks)
-            umma_f16_ts(tdK, tdP + (ks >> 2) * 64 + (ks & 3) * 8, desc_rows(sQ + s * kTileBytes<D>, ks), idesc_g, it != 0 || ks != 0);
-          umma_commit(q_free + 8 * s);
-          if (it + 1 == tiles) umma_commit(all_done);
-        }
-        if (it + 1 < tiles) dps(it + 1);
+        for (int ks = 0; ks < kSub / 16; ++ks)
+          mma_ts(leader, tdK, tmem + 128 * (x & 1) + 64 + ks * 8, desc_rows<kSub>(ring + (x % NS) * S::kStage, ks), idesc_g, x != 0 || ks != 0);
+        commit(leader, q_free + 8 * (x % NS));
+        if (u == tiles) commit(leader, all_done);
       }
+      if (x + 2 < tiles) dps(x + 2);
     }
-  } else if (warp < 4) {
-    // statistics of the queries, and the power for dS
-    const int tid = threadIdx.x - 64;
-    int k = 100, ev = 0;
-    bool ok = true;
-    if (kScaled) {
-      ok = named_bar_and(1, 64, warp_wait(kv_full, 0, s_abort, p.gerr, 1146));
-      if (ok) ev = tile_exponent<D>(sm + (sV - base), min(kTile, len - j0), tid, s_pair) + (D == 64 ? 3 : 4);
-    }
-    for (int it = 0; it < tiles && ok; ++it) {
-      const int s = it % NS, h = kvh * group + it / per_head, row = (t_first + it % per_head) * kTile;
-      ok = it < NS || warp_wait(q_free + 8 * s, (uint32_t)(it / NS + 1) & 1u, s_abort, p.gerr, 1147);
-      if (kScaled) ok = named_bar_and(1, 64, ok && warp_wait(q_full + 8 * s, (uint32_t)(it / NS) & 1u, s_abort, p.gerr, 1148));
-      if (!ok) break;
-      const long long stat = ((long long)b * p.heads + h) * p.q_len;
+  } else if (warp == 2) {
+    // statistics of the queries, the next tile's on their way while the stage is awaited
+    auto fetch = [&](int u, float2 (&x)[2]) {
+      const int h = kvh * group + u / per_head, row = first_row(u);
+      const long long stat = ((long long)b * p.heads + h) * p.q_len + row;
 #pragma unroll
-      for (int i = tid; i < kTile; i += 64) {
-        const bool there = row + i < rows_end;
-        s_lse[s * 128 + i] = there ? fmaf(p.lse[stat + row + i], -kLog2e, (float)kWeightBits<T>) : -INFINITY;  // (a weight of 0)
-        s_delta[s * 128 + i] = there ? -p.delta[stat + row + i] : 0.f;
+      for (int i = 0; i < 2; ++i) {
+        const int r = lane + 32 * i;
+        const bool there = u < tiles && row + r < rows_end;
+        x[i].x = there ? p.lse[stat + r] : INFINITY;  // (a weight of 0)
+        x[i].y = there ? p.delta[stat + r] : 0.f;
       }
-      if (kScaled) {
-        k = next_power(k, ev + tile_exponent<D>(sm + (sG - base) + s * kTileBytes<D>, min(kTile, rows_end - row), tid, s_pair));
-        if (tid == 0) s_power[s] = k;
+    };
+    float2 x[2];
+    fetch(0, x);
+    for (int u = 0; u < tiles; ++u) {
+      const int s = u % NS;
+      if (u >= NS && !warp_wait(q_free + 8 * s, (uint32_t)(u / NS + 1) & 1u, s_abort, p.gerr, 1147)) break;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        s_lse[s * kSub + lane + 32 * i] = fmaf(x[i].x, -kLog2e, (float)kWeightBits<T>);
+        s_delta[s * kSub + lane + 32 * i] = -x[i].y;
       }
-      mbar_arrive(st_full + 8 * s);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(st_full + 8 * s);
+      fetch(u + 1, x);
+    }
+  } else if (warp == 3) {
+    // the power for dS
+    if (kScaled && warp_wait(kv_full, 0, s_abort, p.gerr, 1146)) {
+      const int ev = tile_exponent<D, kTile>(sm + (sV - base), min(kTile, len - j0), lane) + (D == 64 ? 3 : 4);
+      int k = kFirstPower;
+      for (int u = 0; u < tiles; ++u) {
+        const int s = u % NS;
+        if (!warp_wait(q_full + 8 * s, (uint32_t)(u / NS) & 1u, s_abort, p.gerr, 1148)) break;
+        const int k_new = next_power(k, ev + tile_exponent<D, kSub>(sm + S::kFixed + s * S::kStage + kTileBytes<D, kSub>, min(kSub, rows_end - first_row(u)), lane));
+        if (lane == 0) {
+          s_power[s] = k_new;
+          s_step[s] = u == 0 ? 0 : k_new - k;
+          mbar_arrive(st_full + 8 * s);
+        }
+        k = k_new;
+      }
     }
   } else {
-    const int half = (warp - 4) >> 2, q = warp & 3, in_tile = q * 32 + lane;
+    const int w = (warp - 4) >> 2, q = warp & 3, in_tile = q * 32 + lane;
     const int key = j0 + in_tile;
-    const uint32_t lanes = (uint32_t)(q * 32) << 16;
+    const uint32_t lanes = (uint32_t)(q * 32) << 16, t = tmem + 128 * w + lanes;
     const float c = p.scale * kLog2e;
     const bool sink = key < p.sinks, no_ds = p.window == 1 && p.sinks == 0;
-    int k = 0;
     bool ok = true;
-    for (int it = 0; it < tiles; ++it) {
-      const int s = it % NS, first = off + (t_first + it % per_head) * kTile;  // position of the tile's first query
-      const uint32_t ph = (uint32_t)it & 1u;
-      const float4 *lse2 = reinterpret_cast<const float4*>(s_lse + s * 128 + half * 64), *delta = reinterpret_cast<const float4*>(s_delta + s * 128 + half * 64);
-      const bool cut = j0 + kTile - 1 > first || (p.window > 0 && j0 <= first + kTile - 1 - p.window && j0 + kTile > p.sinks);
+    for (int u = w, n = 0; u < tiles; u += 2, ++n) {
+      const int s = u % NS, first = off + first_row(u);  // position of the tile's first query
+      const float4 *lse2 = reinterpret_cast<const float4*>(s_lse + s * kSub), *delta = reinterpret_cast<const float4*>(s_delta + s * kSub);
+      const bool cut = j0 + kTile - 1 > first || (p.window > 0 && j0 <= first + kSub - 1 - p.window && j0 + kTile > p.sinks);
       // columns whose queries see this thread's key: from `from` on, and before `to` unless it is a sink
-      const int from = key - first - half * 64, to = p.window > 0 && !sink ? from + p.window : 0x7fffffff;
-      if (!(ok = warp_wait(st_full + 8 * s, (uint32_t)(it / NS) & 1u, s_abort, p.gerr, 1149))) break;
-      if (!(ok = warp_wait(s_full, ph, s_abort, p.gerr, 1150))) break;
+      const int from = key - first, to = p.window > 0 && !sink ? from + p.window : 0x7fffffff;
+      if (!(ok = warp_wait(st_full + 8 * s, (uint32_t)(u / NS) & 1u, s_abort, p.gerr, 1149))) break;
+      if (!(ok = warp_wait(s_full + 8 * w, (uint32_t)n & 1u, s_abort, p.gerr, 1150))) break;
       tc_fence_after();
-      uint32_t w[2][32];
-      tmem_ld_32x32(tS + lanes + half * 64, w[0]);
-      tmem_ld_32x32(tS + lanes + half * 64 + 32, w[1]);
+      uint32_t wt[2][32];
+      tmem_ld_32x32(t, wt[0]);
+      tmem_ld_32x32(t + 32, wt[1]);
       tmem_ld_wait();
       if (cut) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint32_t shown = ~bits_below(from - 32 * i) & bits_below(to - 32 * i);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) w[i][e] = shown >> e & 1 ? w[i][e] : kMinusInf;
+          for (int e = 0; e < 32; ++e) wt[i][e] = shown >> e & 1 ? wt[i][e] : kMinusInf;
         }
       }
 #pragma unroll
@@ -956,45 +1017,47 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
           const float4 l = lse2[8 * i + e / 4];
-          const float2 x = fma2(pair_of(w[i][e], w[i][e + 1]), make_float2(c, c), make_float2(l.x, l.y));
-          const float2 y = fma2(pair_of(w[i][e + 2], w[i][e + 3]), make_float2(c, c), make_float2(l.z, l.w));
+          const float2 x = fma2(pair_of(wt[i][e], wt[i][e + 1]), make_float2(c, c), make_float2(l.x, l.y));
+          const float2 y = fma2(pair_of(wt[i][e + 2], wt[i][e + 3]), make_float2(c, c), make_float2(l.z, l.w));
           const float4 z = make_float4(ex2(x.x), ex2(x.y), ex2(y.x), ex2(y.y));
-          w[i][e] = __float_as_uint(z.x);
-          w[i][e + 1] = __float_as_uint(z.y);
-          w[i][e + 2] = __float_as_uint(z.z);
-          w[i][e + 3] = __float_as_uint(z.w);
+          wt[i][e] = __float_as_uint(z.x);
+          wt[i][e + 1] = __float_as_uint(z.y);
+          wt[i][e + 2] = __float_as_uint(z.z);
+          wt[i][e + 3] = __float_as_uint(z.w);
           o[e / 2] = pack2<T>(z.x, z.y);
           o[e / 2 + 1] = pack2<T>(z.z, z.w);
         }
-        tmem_st_32x16(tS + lanes + half * 64 + 16 * i, o);  // over scores that have been read
+        tmem_st_32x16(t + 16 * i, o);  // over scores that have been read
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(p_full);
+      mbar_arrive(p_full + 8 * w);
       float r = no_ds ? 0.f : 1.f;
-      if (!(ok = warp_wait(dp_full, ph, s_abort, p.gerr, 1151))) break;
+      if (!(ok = warp_wait(dp_full + 8 * w, (uint32_t)n & 1u, s_abort, p.gerr, 1151))) break;
       tc_fence_after();
       if (kScaled) {
-        const int k_new = s_power[s];
-        if (it > 0 && k_new != k)  // dP was issued behind the product that added to dK
-          scale_row<D / 2>(tdK + lanes + half * (D / 2), pow2(max(k_new - k, -126)));
-        k = k_new;
-        r *= pow2(k - kWeightBits<T>);
+        const int step = s_step[s];
+        if (step != 0) {  // what has been summed so far, the other group's last tile included, follows
+          if (!(ok = warp_wait(q_free + 8 * ((u - 1) % NS), (uint32_t)((u - 1) / NS) & 1u, s_abort, p.gerr, 1152))) break;
+          tc_fence_after();
+          scale_row<D>(tdK + lanes, pow2(max(step, -126)));
+        }
+        r *= pow2(s_power[s] - kWeightBits<T>);
       }
       uint32_t d[2][32];
-      tmem_ld_32x32(tdP + lanes + half * 64, d[0]);
-      tmem_ld_32x32(tdP + lanes + half * 64 + 32, d[1]);
+      tmem_ld_32x32(t + 64, d[0]);
+      tmem_ld_32x32(t + 96, d[1]);
       tmem_ld_wait();
       if (cut) {
         // hidden values may be of rows that are not there; the query at position 0 sees one key: no gradient through it
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int alone = -first - half * 64 - 32 * i;
+          const int alone = -first - 32 * i;
           const uint32_t shown = ~bits_below(from - 32 * i) & bits_below(to - 32 * i) & ~(bits_below(alone + 1) & ~bits_below(alone));
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             d[i][e] = shown >> e & 1 ? d[i][e] : 0u;
-            w[i][e] = shown >> e & 1 ? w[i][e] : 0u;
+            wt[i][e] = shown >> e & 1 ? wt[i][e] : 0u;
           }
         }
       }
@@ -1004,23 +1067,25 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
           const float4 l = delta[8 * i + e / 4];
-          const float2 x = mul2(mul2(pair_of(w[i][e], w[i][e + 1]), make_float2(r, r)), add2(pair_of(d[i][e], d[i][e + 1]), make_float2(l.x, l.y)));
-          const float2 y = mul2(mul2(pair_of(w[i][e + 2], w[i][e + 3]), make_float2(r, r)), add2(pair_of(d[i][e + 2], d[i][e + 3]), make_float2(l.z, l.w)));
+          const float2 x = mul2(mul2(pair_of(wt[i][e], wt[i][e + 1]), make_float2(r, r)), add2(pair_of(d[i][e], d[i][e + 1]), make_float2(l.x, l.y)));
+          const float2 y = mul2(mul2(pair_of(wt[i][e + 2], wt[i][e + 3]), make_float2(r, r)), add2(pair_of(d[i][e + 2], d[i][e + 3]), make_float2(l.z, l.w)));
           o[e / 2] = pack2<T>(x.x, x.y);
           o[e / 2 + 1] = pack2<T>(y.x, y.y);
         }
-        tmem_st_32x16(tdP + lanes + half * 64 + 16 * i, o);
+        tmem_st_32x16(t + 64 + 16 * i, o);
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(ds_full);
+      mbar_arrive(ds_full + 8 * w);
     }
-    if (ok && warp_wait(all_done, 0, s_abort, p.gerr, 1152)) {
+    if (ok && warp_wait(all_done, 0, s_abort, p.gerr, 1153)) {
       tc_fence_after();
-      T* const dk = reinterpret_cast<T*>(p.dk.data) + b * p.dk.batch + key * p.dk.token + kvh * p.dk.head + half * (D / 2);
-      T* const dv = reinterpret_cast<T*>(p.dv.data) + b * p.dv.batch + key * p.dv.token + kvh * p.dv.head + half * (D / 2);
-      store_row<T, D / 2>(tdV + lanes + half * (D / 2), dv, pow2(-kWeightBits<T>), key < len);
-      store_row<T, D / 2>(tdK + lanes + half * (D / 2), dk, p.scale * pow2(-k), key < len);
+      float f = p.scale;
+      if (kScaled) f *= pow2(-s_power[(tiles - 1) % NS]);
+      T* const dk = reinterpret_cast<T*>(p.dk.data) + b * p.dk.batch + key * p.dk.token + kvh * p.dk.head + w * (D / 2);
+      T* const dv = reinterpret_cast<T*>(p.dv.data) + b * p.dv.batch + key * p.dv.token + kvh * p.dv.head + w * (D / 2);
+      store_row<T, D / 2>(tdV + lanes + w * (D / 2), dv, pow2(-kWeightBits<T>), key < len);
+      store_row<T, D / 2>(tdK + lanes + w * (D / 2), dk, f, key < len);
     }
   }
 
@@ -1076,15 +1141,15 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// A tensor [batch][tokens][heads][D] in boxes of 128 tokens x 64 elements of one head; tokens behind the last read as zeros.
-template <class T, int D>
+// A tensor [batch][tokens][heads][D] in boxes of B tokens x 64 elements of one head; tokens behind the last read as zeros.
+template <class T, int D, int B>
 int encode(aig_ctx* ctx, CUtensorMap* m, const View& v, int batch, int tokens, int heads) {
   const EncodeTiledFn enc = encode_fn();
   if (!enc) return aig_fail(ctx, AIG_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available");
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)batch};
   // (the stride of a dimension of one has no meaning, but has to be a possible one)
   const cuuint64_t strides[3] = {(cuuint64_t)(heads > 1 ? v.head : D) * 2, (cuuint64_t)(tokens > 1 ? v.token : D) * 2, (cuuint64_t)(batch > 1 ? v.batch : D) * 2};
-  const cuuint32_t box[4] = {64, 1, kTile, 1}, step[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, 1, B, 1}, step[4] = {1, 1, 1, 1};
   const CUresult r = enc(m, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, v.data, dims, strides,
                          box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -1108,9 +1173,9 @@ template <class T, int D>
 int forward(aig_ctx* ctx, WinParams& p) {
   p.gerr = ctx->d_err;
   CUtensorMap mq, mk, mv;
-  int rc = encode<T, D>(ctx, &mq, p.q, p.batch, p.q_len, p.heads);
-  if (rc == AIG_OK) rc = encode<T, D>(ctx, &mk, p.k, p.batch, p.kv_len, p.kv_heads);
-  if (rc == AIG_OK) rc = encode<T, D>(ctx, &mv, p.v, p.batch, p.kv_len, p.kv_heads);
+  int rc = encode<T, D, kTile>(ctx, &mq, p.q, p.batch, p.q_len, p.heads);
+  if (rc == AIG_OK) rc = encode<T, D, kTile>(ctx, &mk, p.k, p.batch, p.kv_len, p.kv_heads);
+  if (rc == AIG_OK) rc = encode<T, D, kTile>(ctx, &mv, p.v, p.batch, p.kv_len, p.kv_heads);
   if (rc != AIG_OK) return rc;
   return p.q_len <= kTile ? launch_forward<T, D, 1>(ctx, p, mq, mk, mv) : launch_forward<T, D, 2>(ctx, p, mq, mk, mv);
 }
@@ -1118,10 +1183,10 @@ template <class T, int D>
 int backward(aig_ctx* ctx, WinParams& p) {
   p.gerr = ctx->d_err;
   CUtensorMap mq{}, mk, mv, mg{};
-  int rc = encode<T, D>(ctx, &mk, p.k, p.batch, p.kv_len, p.kv_heads);
-  if (rc == AIG_OK) rc = encode<T, D>(ctx, &mv, p.v, p.batch, p.kv_len, p.kv_heads);
-  if (rc == AIG_OK) rc = encode<T, D>(ctx, &mq, p.q, p.batch, p.q_len, p.heads);
-  if (rc == AIG_OK) rc = encode<T, D>(ctx, &mg, p.dout, p.batch, p.q_len, p.heads);
+  int rc = encode<T, D, kSub>(ctx, &mk, p.k, p.batch, p.kv_len, p.kv_heads);
+  if (rc == AIG_OK) rc = encode<T, D, kSub>(ctx, &mv, p.v, p.batch, p.kv_len, p.kv_heads);
+  if (rc == AIG_OK) rc = encode<T, D, kSub>(ctx, &mq, p.q, p.batch, p.q_len, p.heads);
+  if (rc == AIG_OK) rc = encode<T, D, kSub>(ctx, &mg, p.dout, p.batch, p.q_len, p.heads);
   if (rc != AIG_OK) return rc;
   p.blocks = ceil_div(p.q_len, kTile);
   const long long grid = (long long)p.blocks * p.heads * p.batch, grid_kv = (long long)ceil_div(p.kv_len, kTile) * p.kv_heads * p.batch;
