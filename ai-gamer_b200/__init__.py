@@ -5,8 +5,10 @@ only loads it with ctypes, declares every entry point's signature, and offers th
 torch CUDA tensors (torch is used for device memory and streams, nothing else).  There is no
 fallback: if the library is missing or a call fails, an exception is raised.
 """
+import array
 import ctypes
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libaig_b200.so")
@@ -26,16 +28,6 @@ class ConvDesc(ctypes.Structure):
                                      "sw", "pd", "ph", "pw", "act")] + [("slope", c_float), ("two_step", c_int)]
 
 
-class Heads(ctypes.Structure):
-    """aig_heads: a tensor [tokens][heads][head_dim]."""
-    _fields_ = [("data", c_void_p), ("heads", c_int), ("token_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong)]
-
-
-class SeqHeads(ctypes.Structure):
-    """aig_seq_heads: a tensor [batch][tokens][heads][head_dim]."""
-    _fields_ = [("data", c_void_p)] + [(n, ctypes.c_longlong) for n in ("batch_stride", "token_stride", "head_stride")]
-
-
 class RopeDesc(ctypes.Structure):
     _fields_ = [("head_dim", c_int), ("rot_dim", c_int), ("interleaved", c_int), ("scaling", c_int), ("base", c_float), ("factor", c_float),
                 ("original_len", c_int), ("low", c_float), ("high", c_float), ("magnitude", c_float)]
@@ -46,11 +38,10 @@ class KvCacheDesc(ctypes.Structure):
         (n, ctypes.c_longlong) for n in ("page_stride", "token_stride", "head_stride")]
 
 
-class WindowDesc(ctypes.Structure):
-    _fields_ = [(n, c_int) for n in ("dtype", "batch", "q_len", "kv_len", "heads", "kv_heads", "head_dim", "window", "sinks")] + [("scale", c_float)]
-
-
-PH, PS = ctypes.POINTER(Heads), ctypes.POINTER(SeqHeads)
+# Structures that a call makes anew each time are packed as bytes (a quarter of the time of a ctypes structure)
+_pack_heads = struct.Struct("Pi4xqq").pack
+_pack_seq_heads = struct.Struct("Pqqq").pack
+_pack_window = struct.Struct("9if").pack
 
 # name -> argtypes (restype is int unless listed in _RESTYPES)
 SIGNATURES = {
@@ -155,11 +146,11 @@ SIGNATURES = {
     "aig_rope_frequencies": [ctypes.POINTER(RopeDesc), P, c_int],
     "aig_rope_plan_create": [P, ctypes.POINTER(RopeDesc), PP],
     "aig_rope_plan_destroy": [P],
-    "aig_rope_forward": [P, c_int, P, ctypes.c_longlong, PH, PH, PH, PH],
-    "aig_rope_backward": [P, c_int, P, ctypes.c_longlong, PH, PH, PH, PH],
-    "aig_kv_append": [P, ctypes.POINTER(KvCacheDesc), P, PH, PH, PH, PH, P, P, ctypes.c_longlong, P, c_int, c_int],
-    "aig_kv_copy_pages": [P, ctypes.POINTER(KvCacheDesc), P, P, c_int],
-    "aig_paged_attention": [P, ctypes.POINTER(KvCacheDesc), PH, PH, P, c_int, P, c_int, c_int, c_float, c_int, c_int],
+    "aig_rope_forward": [P, c_int, P, ctypes.c_longlong, P, P, P, P],
+    "aig_rope_backward": [P, c_int, P, ctypes.c_longlong, P, P, P, P],
+    "aig_kv_append": [P, P, P, P, P, P, P, P, P, ctypes.c_longlong, P, c_int, c_int],
+    "aig_kv_copy_pages": [P, P, P, P, c_int],
+    "aig_paged_attention": [P, P, P, P, P, c_int, P, c_int, c_int, c_float, c_int, c_int],
     "aig_page_pool_create": [c_int, c_int, PP],
     "aig_page_pool_destroy": [P],
     "aig_page_pool_open": [P, PI],
@@ -172,8 +163,8 @@ SIGNATURES = {
     "aig_page_pool_length": [P, c_int],
     "aig_page_pool_free_pages": [P],
     "aig_page_pool_shared": [P, c_int],
-    "aig_window_attention_forward": [P, ctypes.POINTER(WindowDesc), PS, PS, PS, PS, P, P],
-    "aig_window_attention_backward": [P, ctypes.POINTER(WindowDesc), PS, PS, PS, PS, P, PS, PS, PS, PS, P, P],
+    "aig_window_attention_forward": [P, P, P, P, P, P, P, P],
+    "aig_window_attention_backward": [P, P, P, P, P, P, P, P, P, P, P, P, P],
     # include/aig_compat.h: the reference's launcher names (no context argument; most return void)
     "InitCUDA": [],
     "ConvertAndNormalize": [P, P, c_size_t],
@@ -703,40 +694,36 @@ class MhaPlan(_Plan):
         self.check(lib().aig_mha_reset(self.handle))
 
 
-def _dtype_of(*tensors):
-    import torch
-
-    kinds = {t.dtype for t in tensors if t is not None}
-    code = {torch.float16: F16, torch.bfloat16: BF16}.get(next(iter(kinds))) if len(kinds) == 1 else None
-    if code is None:
-        raise ValueError("tensors of one type, fp16 or bf16: got %s" % sorted(map(str, kinds)))
-    return code
+_types = {}  # torch's types of the values that the operators for long contexts take, filled on first use (torch is not imported with this module)
 
 
-def _rows(t, what, dims, dtype=None):
-    """Checks that a tensor has `dims` dimensions, or the shape `dims`, with consecutive values in the last one; returns it."""
-    shape = tuple(t.shape)
-    if (len(shape) != dims) if isinstance(dims, int) else (shape != tuple(dims)):
-        raise ValueError("%s: shape %s where %s is wanted" % (what, shape, "%d dimensions" % dims if isinstance(dims, int) else tuple(dims)))
-    if shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError("%s: the last dimension has to be dense" % what)
-    if dtype is not None and t.dtype != dtype:
-        raise ValueError("%s: %s where %s is wanted" % (what, t.dtype, dtype))
-    return t
+def _value_type(t):
+    if not _types:
+        import torch
+
+        _types.update({torch.float16: F16, torch.bfloat16: BF16, "i32": torch.int32, "f32": torch.float32})
+    if t.dtype not in _types:
+        raise ValueError("fp16 or bf16 tensors are wanted: got %s" % t.dtype)
+    return t.dtype
 
 
-def _device_ints(t, what, shape):
-    """A dense int32 tensor of this shape on the device."""
-    import torch
+def _check(t, shape, dtype, device, what):
+    """A tensor of this shape and type on the context's device whose last dimension is dense."""
+    if t.shape != shape or t.dtype != dtype or t.get_device() != device or (t.stride(-1) != 1 and shape[-1] > 1):
+        raise ValueError("%s: shape %s and type %s on device %d with a dense last dimension is wanted, got %s, %s, strides %s on %s" % (
+            what, tuple(shape), dtype, device, tuple(t.shape), t.dtype, t.stride(), t.device))
 
-    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or not t.is_cuda:
-        raise ValueError("%s: a dense int32 device tensor of shape %s is wanted, got %s %s" % (what, tuple(shape), t.dtype, tuple(t.shape)))
+
+def _ints(t, shape, device, what):
+    """The address of a dense int32 tensor on the context's device."""
+    if t.shape != shape or t.dtype != _types["i32"] or not t.is_contiguous() or t.get_device() != device:
+        raise ValueError("%s: dense int32 of shape %s on device %d is wanted, got %s of %s on %s" % (what, tuple(shape), device, t.dtype, tuple(t.shape), t.device))
     return t.data_ptr()
 
 
 def _heads(t):
     s = t.stride()
-    return ctypes.byref(Heads(t.data_ptr(), t.shape[1], s[0], s[1]))
+    return _pack_heads(t.data_ptr(), t.shape[1], s[0], s[1])
 
 
 class RopePlan(_Plan):
@@ -757,13 +744,18 @@ class RopePlan(_Plan):
         return list(out)
 
     def _apply(self, fn, positions, q, q_out, k, k_out):
-        n, d = q.shape[0], self.desc.head_dim
-        _rows(q, "q", (n, q.shape[1], d))
-        _rows(q_out, "q_out", q.shape)
+        dtype, shape = _value_type(q), q.shape
+        if len(shape) != 3 or shape[2] != self.desc.head_dim:
+            raise ValueError("q: [tokens][heads][%d] is wanted, got %s" % (self.desc.head_dim, tuple(shape)))
+        n, on = shape[0], self.ctx.device
+        _check(q, shape, dtype, on, "q")
+        _check(q_out, shape, dtype, on, "q_out")
+        if (k is None) != (k_out is None):
+            raise ValueError("k and k_out come together")
         if k is not None:
-            _rows(k, "k", (n, k.shape[1], d))
-            _rows(k_out, "k_out", k.shape)
-        self.check(fn(self.handle, _dtype_of(q, q_out, k, k_out), _device_ints(positions, "positions", (n,)), n, _heads(q), _heads(q_out),
+            _check(k, (n, k.shape[1], shape[2]), dtype, on, "k")
+            _check(k_out, k.shape, dtype, on, "k_out")
+        self.check(fn(self.handle, _types[dtype], _ints(positions, (n,), on, "positions"), n, _heads(q), _heads(q_out),
                       None if k is None else _heads(k), None if k is None else _heads(k_out)))
 
     def forward(self, positions, q, q_out, k=None, k_out=None):
@@ -778,49 +770,57 @@ class PagedCache:
     """aig_kv_cache over two tensors [pages][page_size][kv_heads][head_dim] (other orders as strided views)."""
 
     def __init__(self, ctx, k_pages, v_pages):
-        _rows(k_pages, "k_pages", 4)
-        _rows(v_pages, "v_pages", k_pages.shape)
-        if k_pages.stride() != v_pages.stride():
-            raise ValueError("keys and values have the same strides")
+        self.dtype = _value_type(k_pages)
+        if k_pages.dim() != 4 or k_pages.stride() != v_pages.stride():
+            raise ValueError("[pages][page_size][kv_heads][head_dim] twice, with the same strides, is wanted")
+        on = ctx.device
+        _check(k_pages, k_pages.shape, self.dtype, on, "k_pages")
+        _check(v_pages, k_pages.shape, self.dtype, on, "v_pages")
         self.ctx, self._keep = ctx, (k_pages, v_pages)
-        pages, size, heads, dim = k_pages.shape
+        pages, size, self.heads, self.dim = k_pages.shape
         s = k_pages.stride()
-        self.dtype = k_pages.dtype
-        self.desc = KvCacheDesc(k_pages.data_ptr(), v_pages.data_ptr(), _dtype_of(k_pages, v_pages), heads, dim, size, pages, s[0], s[1], s[2])
-        self._ref = ctypes.byref(self.desc)
+        self.desc = KvCacheDesc(k_pages.data_ptr(), v_pages.data_ptr(), _types[self.dtype], self.heads, self.dim, size, pages, s[0], s[1], s[2])
+        self._ref = c_void_p(ctypes.addressof(self.desc))
 
     def append(self, k, v, positions, table, seqs=None, rope=None, q=None, q_out=None):
         """New tokens' k, v [tokens][kv_heads][head_dim] to positions[i] of sequence seqs[i] (None: i); with a rope plan turned on
         the way, q [tokens][heads][head_dim] into q_out too."""
-        n, d = k.shape[0], self.desc.head_dim
-        _rows(k, "k", (n, self.desc.kv_heads, d), self.dtype)
-        _rows(v, "v", k.shape, self.dtype)
+        n, dtype, on = k.shape[0], self.dtype, self.ctx.device
+        shape = (n, self.heads, self.dim)
+        _check(k, shape, dtype, on, "k")
+        _check(v, shape, dtype, on, "v")
+        if (q is None) != (q_out is None):
+            raise ValueError("q and q_out come together")
         if q is not None:
-            _rows(q, "q", (n, q.shape[1], d), self.dtype)
-            _rows(q_out, "q_out", q.shape, self.dtype)
+            _check(q, (n, q.shape[1], self.dim), dtype, on, "q")
+            _check(q_out, q.shape, dtype, on, "q_out")
         batch, width = table.shape
-        self.ctx.check(lib().aig_kv_append(self.ctx.handle, self._ref, None if rope is None else rope.handle, _heads(k), _heads(v),
-                                           None if q is None else _heads(q), None if q is None else _heads(q_out),
-                                           None if seqs is None else _device_ints(seqs, "seqs", (n,)), _device_ints(positions, "positions", (n,)), n,
-                                           _device_ints(table, "table", (batch, width)), batch, width))
+        ctx = self.ctx
+        ctx.check(lib().aig_kv_append(ctx.handle, self._ref, None if rope is None else rope.handle, _heads(k), _heads(v),
+                                      None if q is None else _heads(q), None if q is None else _heads(q_out),
+                                      None if seqs is None else _ints(seqs, (n,), on, "seqs"), _ints(positions, (n,), on, "positions"), n,
+                                      _ints(table, (batch, width), on, "table"), batch, width))
 
     def copy_pages(self, src, dst):
         """Pages src[i] -> dst[i], host numbers."""
         n = len(src)
         if len(dst) != n:
             raise ValueError("as many sources as destinations")
-        ints = c_int * max(n, 1)
-        self.ctx.check(lib().aig_kv_copy_pages(self.ctx.handle, self._ref, ints(*src), ints(*dst), n))
+        src, dst = array.array("i", src), array.array("i", dst)
+        self.ctx.check(lib().aig_kv_copy_pages(self.ctx.handle, self._ref, src.buffer_info()[0], dst.buffer_info()[0], n))
 
     def attend(self, q, out, table, lengths, max_length, scale=None, window=0, sinks=0):
         """One new token of each sequence, q and out [batch][heads][head_dim], over lengths[b] cached positions (its own the last)."""
-        batch, heads, d = q.shape
-        _rows(q, "q", (batch, heads, self.desc.head_dim), self.dtype)
-        _rows(out, "out", q.shape, self.dtype)
+        batch, heads, dim = shape = q.shape
+        if dim != self.dim:
+            raise ValueError("q: heads of %d are wanted, got %d" % (self.dim, dim))
+        on = self.ctx.device
+        _check(q, shape, self.dtype, on, "q")
+        _check(out, shape, self.dtype, on, "out")
         width = table.shape[1]
-        self.ctx.check(lib().aig_paged_attention(self.ctx.handle, self._ref, _heads(q), _heads(out), _device_ints(table, "table", (batch, width)), width,
-                                                 _device_ints(lengths, "lengths", (batch,)), batch, max_length, d ** -0.5 if scale is None else scale,
-                                                 window, sinks))
+        ctx = self.ctx
+        ctx.check(lib().aig_paged_attention(ctx.handle, self._ref, _heads(q), _heads(out), _ints(table, (batch, width), on, "table"), width,
+                                            _ints(lengths, (batch,), on, "lengths"), batch, max_length, dim ** -0.5 if scale is None else scale, window, sinks))
         return out
 
 
@@ -887,8 +887,7 @@ class PagePool:
 
 
 def _seq_heads(t):
-    s = t.stride()
-    return ctypes.byref(SeqHeads(t.data_ptr(), s[0], s[1], s[2]))
+    return _pack_seq_heads(t.data_ptr(), *t.stride()[:3])
 
 
 class WindowAttention:
@@ -898,36 +897,38 @@ class WindowAttention:
     def __init__(self, ctx, window=0, sinks=0, scale=None):
         self.ctx, self.window, self.sinks, self.scale = ctx, window, sinks, scale
 
-    def _desc(self, q, k, lse, like_q, like_k, lengths):
-        import torch
-
-        batch, q_len, heads, dim = _rows(q, "q", 4).shape
-        kv_len, kv_heads = _rows(k, "k", 4).shape[1:3]
-        _rows(k, "k", (batch, kv_len, kv_heads, dim))
+    def _desc(self, q, k, stats, like_q, like_k):
+        dtype, on = _value_type(q), self.ctx.device
+        if q.dim() != 4 or k.dim() != 4:
+            raise ValueError("[batch][tokens][heads][head_dim] is wanted, got %s and %s" % (tuple(q.shape), tuple(k.shape)))
+        batch, q_len, heads, dim = q.shape
+        kv_len, kv_heads = k.shape[1], k.shape[2]
         for t in like_q:
-            _rows(t, "a tensor of q's shape", q.shape)
+            _check(t, q.shape, dtype, on, "a tensor of the queries' shape")
+        _check(k, (batch, kv_len, kv_heads, dim), dtype, on, "k")
         for t in like_k:
-            _rows(t, "a tensor of k's shape", k.shape)
-        for t in lse:
-            if not t.is_contiguous():
-                raise ValueError("lse and delta are dense")
-            _rows(t, "lse or delta", (batch, heads, q_len), torch.float32)
-        return (ctypes.byref(WindowDesc(_dtype_of(q, k, *like_q, *like_k), batch, q_len, kv_len, heads, kv_heads, dim, self.window, self.sinks,
-                                        dim ** -0.5 if self.scale is None else self.scale)),
-                None if lengths is None else _device_ints(lengths, "lengths", (batch,)))
+            _check(t, k.shape, dtype, on, "a tensor of the keys' shape")
+        for t in stats:
+            if t.shape != (batch, heads, q_len) or t.dtype != _types["f32"] or not t.is_contiguous() or t.get_device() != on:
+                raise ValueError("lse, delta: dense fp32 tensors of shape %s on device %d are wanted" % ((batch, heads, q_len), on))
+        return _pack_window(_types[dtype], batch, q_len, kv_len, heads, kv_heads, dim, self.window, self.sinks, dim ** -0.5 if self.scale is None else self.scale)
 
     def forward(self, q, k, v, out, lse, lengths=None):
-        desc, n = self._desc(q, k, (lse,), (out,), (v,), lengths)
-        self.ctx.check(lib().aig_window_attention_forward(self.ctx.handle, desc, _seq_heads(q), _seq_heads(k), _seq_heads(v), _seq_heads(out),
-                                                          lse.data_ptr(), n))
+        desc = self._desc(q, k, (lse,), (q, out), (v,))
+        ctx = self.ctx
+        on = ctx.device
+        ctx.check(lib().aig_window_attention_forward(ctx.handle, desc, _seq_heads(q), _seq_heads(k), _seq_heads(v), _seq_heads(out), lse.data_ptr(),
+                                                     None if lengths is None else _ints(lengths, (q.shape[0],), on, "lengths")))
         return out
 
     def backward(self, q, k, v, out, lse, dout, dq, dk, dv, delta, lengths=None):
         """`delta`: scratch of lse's shape."""
-        desc, n = self._desc(q, k, (lse, delta), (out, dout, dq), (v, dk, dv), lengths)
-        self.ctx.check(lib().aig_window_attention_backward(self.ctx.handle, desc, _seq_heads(q), _seq_heads(k), _seq_heads(v), _seq_heads(out),
-                                                           lse.data_ptr(), _seq_heads(dout), _seq_heads(dq), _seq_heads(dk), _seq_heads(dv),
-                                                           delta.data_ptr(), n))
+        desc = self._desc(q, k, (lse, delta), (q, out, dout, dq), (v, dk, dv))
+        ctx = self.ctx
+        on = ctx.device
+        ctx.check(lib().aig_window_attention_backward(ctx.handle, desc, _seq_heads(q), _seq_heads(k), _seq_heads(v), _seq_heads(out), lse.data_ptr(),
+                                                      _seq_heads(dout), _seq_heads(dq), _seq_heads(dk), _seq_heads(dv), delta.data_ptr(),
+                                                      None if lengths is None else _ints(lengths, (q.shape[0],), on, "lengths")))
         return dq, dk, dv
 
 

@@ -208,11 +208,11 @@ int turn_tensors(aig_rope_plan* pl, int dtype, const int32_t* positions, long lo
   DeviceGuard g(ctx->device);
   AIG_REQUIRE(ctx, dtype_known(dtype), "%s: unknown element type %d", who, dtype);
   AIG_REQUIRE(ctx, tokens >= 0, "%s: negative number of tokens", who);
+  if (tokens == 0) return AIG_OK;
   int rc = check_pair(ctx, q, q_out, who);
   if (rc != AIG_OK) return rc;
   AIG_REQUIRE(ctx, (k == nullptr) == (k_out == nullptr), "%s: k and k_out come together", who);
   if (k && (rc = check_pair(ctx, k, k_out, who)) != AIG_OK) return rc;
-  if (tokens == 0) return AIG_OK;
   AIG_REQUIRE(ctx, positions, "%s: null positions", who);
   RopeParams p{};
   p.part[0] = side_of(q, q_out);
@@ -308,17 +308,16 @@ int aig_kv_append(aig_ctx* ctx, const aig_kv_cache* cache, aig_rope_plan* rope, 
   DeviceGuard g(ctx->device);
   int rc = check_cache(ctx, cache, "kv append");
   if (rc != AIG_OK) return rc;
+  AIG_REQUIRE(ctx, tokens >= 0 && batch >= 0 && table_width >= 0, "kv append: bad extents");
+  if (tokens == 0) return AIG_OK;
   AIG_REQUIRE(ctx, heads_sane(k) && heads_sane(v), "kv append: null tensor, negative stride or data off a 2-byte boundary");
   AIG_REQUIRE(ctx, k->heads == cache->kv_heads && v->heads == cache->kv_heads, "kv append: %d and %d heads for a cache of %d", k->heads, v->heads,
               cache->kv_heads);
   AIG_REQUIRE(ctx, (q == nullptr) == (q_out == nullptr), "kv append: q and q_out come together");
   if (q && (rc = check_pair(ctx, q, q_out, "kv append")) != AIG_OK) return rc;
-  AIG_REQUIRE(ctx, tokens >= 0 && batch > 0 && table_width > 0, "kv append: bad extents");
   AIG_REQUIRE(ctx, seqs || tokens <= batch, "kv append: %lld tokens without sequence numbers for a batch of %d", tokens, batch);
   AIG_REQUIRE(ctx, !rope || (rope->ctx->device == ctx->device && rope->desc.head_dim == cache->head_dim),
               "kv append: the rope plan is for another device or head dimension");
-  AIG_REQUIRE(ctx, !rope || rope->desc.head_dim % 2 == 0, "kv append: odd head dimension");
-  if (tokens == 0) return AIG_OK;
   AIG_REQUIRE(ctx, positions && table, "kv append: null positions or table");
   RopeParams p{};
   if (q) p.part[0] = side_of(q, q_out);
