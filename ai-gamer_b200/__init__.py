@@ -707,23 +707,32 @@ def _value_type(t):
     return t.dtype
 
 
-def _check(t, shape, dtype, device, what):
-    """A tensor of this shape and type on the context's device whose last dimension is dense."""
-    if t.shape != shape or t.dtype != dtype or t.get_device() != device or (t.stride(-1) != 1 and shape[-1] > 1):
-        raise ValueError("%s: shape %s and type %s on device %d with a dense last dimension is wanted, got %s, %s, strides %s on %s" % (
-            what, tuple(shape), dtype, device, tuple(t.shape), t.dtype, t.stride(), t.device))
+def _refuse(t, shape, dtype, device, what):
+    raise ValueError("%s: shape %s and type %s on device %d with a dense last dimension is wanted, got %s, %s, strides %s on %s" % (
+        what, tuple(shape), dtype, device, tuple(t.shape), t.dtype, t.stride(), t.device))
 
 
 def _ints(t, shape, device, what):
     """The address of a dense int32 tensor on the context's device."""
-    if t.shape != shape or t.dtype != _types["i32"] or not t.is_contiguous() or t.get_device() != device:
+    if t.shape != shape or t.dtype is not _types["i32"] or not t.is_contiguous() or t.get_device() != device:
         raise ValueError("%s: dense int32 of shape %s on device %d is wanted, got %s of %s on %s" % (what, tuple(shape), device, t.dtype, tuple(t.shape), t.device))
     return t.data_ptr()
 
 
-def _heads(t):
+def _heads(t, shape, dtype, device, what):
+    """aig_heads of a tensor [tokens][heads][head_dim] of this shape and type on the context's device."""
     s = t.stride()
-    return _pack_heads(t.data_ptr(), t.shape[1], s[0], s[1])
+    if t.shape != shape or t.dtype is not dtype or s[2] != 1 or t.get_device() != device:
+        _refuse(t, shape, dtype, device, what)
+    return _pack_heads(t.data_ptr(), shape[1], s[0], s[1])
+
+
+def _seq_heads(t, shape, dtype, device, what):
+    """aig_seq_heads of a tensor [batch][tokens][heads][head_dim]."""
+    s = t.stride()
+    if t.shape != shape or t.dtype is not dtype or s[3] != 1 or t.get_device() != device:
+        _refuse(t, shape, dtype, device, what)
+    return _pack_seq_heads(t.data_ptr(), s[0], s[1], s[2])
 
 
 class RopePlan(_Plan):
@@ -744,19 +753,18 @@ class RopePlan(_Plan):
         return list(out)
 
     def _apply(self, fn, positions, q, q_out, k, k_out):
-        dtype, shape = _value_type(q), q.shape
+        dtype, shape, on = _value_type(q), q.shape, self.ctx.device
         if len(shape) != 3 or shape[2] != self.desc.head_dim:
             raise ValueError("q: [tokens][heads][%d] is wanted, got %s" % (self.desc.head_dim, tuple(shape)))
-        n, on = shape[0], self.ctx.device
-        _check(q, shape, dtype, on, "q")
-        _check(q_out, shape, dtype, on, "q_out")
+        n = shape[0]
         if (k is None) != (k_out is None):
             raise ValueError("k and k_out come together")
+        kh = ko = None
         if k is not None:
-            _check(k, (n, k.shape[1], shape[2]), dtype, on, "k")
-            _check(k_out, k.shape, dtype, on, "k_out")
-        self.check(fn(self.handle, _types[dtype], _ints(positions, (n,), on, "positions"), n, _heads(q), _heads(q_out),
-                      None if k is None else _heads(k), None if k is None else _heads(k_out)))
+            k_shape = (n, k.shape[1], shape[2])
+            kh, ko = _heads(k, k_shape, dtype, on, "k"), _heads(k_out, k_shape, dtype, on, "k_out")
+        self.check(fn(self.handle, _types[dtype], _ints(positions, (n,), on, "positions"), n, _heads(q, shape, dtype, on, "q"),
+                      _heads(q_out, shape, dtype, on, "q_out"), kh, ko))
 
     def forward(self, positions, q, q_out, k=None, k_out=None):
         self._apply(lib().aig_rope_forward, positions, q, q_out, k, k_out)
@@ -774,8 +782,8 @@ class PagedCache:
         if k_pages.dim() != 4 or k_pages.stride() != v_pages.stride():
             raise ValueError("[pages][page_size][kv_heads][head_dim] twice, with the same strides, is wanted")
         on = ctx.device
-        _check(k_pages, k_pages.shape, self.dtype, on, "k_pages")
-        _check(v_pages, k_pages.shape, self.dtype, on, "v_pages")
+        for t in (k_pages, v_pages):
+            _seq_heads(t, k_pages.shape, self.dtype, on, "pages")
         self.ctx, self._keep = ctx, (k_pages, v_pages)
         pages, size, self.heads, self.dim = k_pages.shape
         s = k_pages.stride()
@@ -785,21 +793,18 @@ class PagedCache:
     def append(self, k, v, positions, table, seqs=None, rope=None, q=None, q_out=None):
         """New tokens' k, v [tokens][kv_heads][head_dim] to positions[i] of sequence seqs[i] (None: i); with a rope plan turned on
         the way, q [tokens][heads][head_dim] into q_out too."""
-        n, dtype, on = k.shape[0], self.dtype, self.ctx.device
-        shape = (n, self.heads, self.dim)
-        _check(k, shape, dtype, on, "k")
-        _check(v, shape, dtype, on, "v")
+        ctx, dtype, n = self.ctx, self.dtype, k.shape[0]
+        on, shape = ctx.device, (n, self.heads, self.dim)
         if (q is None) != (q_out is None):
             raise ValueError("q and q_out come together")
+        qh = qo = None
         if q is not None:
-            _check(q, (n, q.shape[1], self.dim), dtype, on, "q")
-            _check(q_out, q.shape, dtype, on, "q_out")
+            q_shape = (n, q.shape[1], self.dim)
+            qh, qo = _heads(q, q_shape, dtype, on, "q"), _heads(q_out, q_shape, dtype, on, "q_out")
         batch, width = table.shape
-        ctx = self.ctx
-        ctx.check(lib().aig_kv_append(ctx.handle, self._ref, None if rope is None else rope.handle, _heads(k), _heads(v),
-                                      None if q is None else _heads(q), None if q is None else _heads(q_out),
-                                      None if seqs is None else _ints(seqs, (n,), on, "seqs"), _ints(positions, (n,), on, "positions"), n,
-                                      _ints(table, (batch, width), on, "table"), batch, width))
+        ctx.check(lib().aig_kv_append(ctx.handle, self._ref, None if rope is None else rope.handle, _heads(k, shape, dtype, on, "k"),
+                                      _heads(v, shape, dtype, on, "v"), qh, qo, None if seqs is None else _ints(seqs, (n,), on, "seqs"),
+                                      _ints(positions, (n,), on, "positions"), n, _ints(table, (batch, width), on, "table"), batch, width))
 
     def copy_pages(self, src, dst):
         """Pages src[i] -> dst[i], host numbers."""
@@ -811,16 +816,13 @@ class PagedCache:
 
     def attend(self, q, out, table, lengths, max_length, scale=None, window=0, sinks=0):
         """One new token of each sequence, q and out [batch][heads][head_dim], over lengths[b] cached positions (its own the last)."""
-        batch, heads, dim = shape = q.shape
-        if dim != self.dim:
-            raise ValueError("q: heads of %d are wanted, got %d" % (self.dim, dim))
-        on = self.ctx.device
-        _check(q, shape, self.dtype, on, "q")
-        _check(out, shape, self.dtype, on, "out")
-        width = table.shape[1]
-        ctx = self.ctx
-        ctx.check(lib().aig_paged_attention(ctx.handle, self._ref, _heads(q), _heads(out), _ints(table, (batch, width), on, "table"), width,
-                                            _ints(lengths, (batch,), on, "lengths"), batch, max_length, dim ** -0.5 if scale is None else scale, window, sinks))
+        ctx, dtype, shape = self.ctx, self.dtype, q.shape
+        if len(shape) != 3 or shape[2] != self.dim:
+            raise ValueError("q: [batch][heads][%d] is wanted, got %s" % (self.dim, tuple(shape)))
+        on, batch, width = ctx.device, shape[0], table.shape[1]
+        ctx.check(lib().aig_paged_attention(ctx.handle, self._ref, _heads(q, shape, dtype, on, "q"), _heads(out, shape, dtype, on, "out"),
+                                            _ints(table, (batch, width), on, "table"), width, _ints(lengths, (batch,), on, "lengths"), batch, max_length,
+                                            self.dim ** -0.5 if scale is None else scale, window, sinks))
         return out
 
 
@@ -886,10 +888,6 @@ class PagePool:
             self.handle = c_void_p()
 
 
-def _seq_heads(t):
-    return _pack_seq_heads(t.data_ptr(), *t.stride()[:3])
-
-
 class WindowAttention:
     """aig_window_attention_*: causal attention over whole sequences with a sliding window and sinks, and its gradients.
     q, out [batch][q_len][heads][head_dim], k, v [batch][kv_len][kv_heads][head_dim], lse fp32 [batch][heads][q_len]."""
@@ -897,38 +895,36 @@ class WindowAttention:
     def __init__(self, ctx, window=0, sinks=0, scale=None):
         self.ctx, self.window, self.sinks, self.scale = ctx, window, sinks, scale
 
-    def _desc(self, q, k, stats, like_q, like_k):
+    def _shapes(self, q, k, *stats):
+        """The call's description, the tensors' shapes, type and device; checks what has the statistics' shape."""
         dtype, on = _value_type(q), self.ctx.device
         if q.dim() != 4 or k.dim() != 4:
             raise ValueError("[batch][tokens][heads][head_dim] is wanted, got %s and %s" % (tuple(q.shape), tuple(k.shape)))
         batch, q_len, heads, dim = q.shape
         kv_len, kv_heads = k.shape[1], k.shape[2]
-        for t in like_q:
-            _check(t, q.shape, dtype, on, "a tensor of the queries' shape")
-        _check(k, (batch, kv_len, kv_heads, dim), dtype, on, "k")
-        for t in like_k:
-            _check(t, k.shape, dtype, on, "a tensor of the keys' shape")
         for t in stats:
-            if t.shape != (batch, heads, q_len) or t.dtype != _types["f32"] or not t.is_contiguous() or t.get_device() != on:
+            if t.shape != (batch, heads, q_len) or t.dtype is not _types["f32"] or not t.is_contiguous() or t.get_device() != on:
                 raise ValueError("lse, delta: dense fp32 tensors of shape %s on device %d are wanted" % ((batch, heads, q_len), on))
-        return _pack_window(_types[dtype], batch, q_len, kv_len, heads, kv_heads, dim, self.window, self.sinks, dim ** -0.5 if self.scale is None else self.scale)
+        desc = _pack_window(_types[dtype], batch, q_len, kv_len, heads, kv_heads, dim, self.window, self.sinks, dim ** -0.5 if self.scale is None else self.scale)
+        return desc, q.shape, (batch, kv_len, kv_heads, dim), dtype, on
 
     def forward(self, q, k, v, out, lse, lengths=None):
-        desc = self._desc(q, k, (lse,), (q, out), (v,))
+        desc, qs, ks, dtype, on = self._shapes(q, k, lse)
         ctx = self.ctx
-        on = ctx.device
-        ctx.check(lib().aig_window_attention_forward(ctx.handle, desc, _seq_heads(q), _seq_heads(k), _seq_heads(v), _seq_heads(out), lse.data_ptr(),
-                                                     None if lengths is None else _ints(lengths, (q.shape[0],), on, "lengths")))
+        ctx.check(lib().aig_window_attention_forward(ctx.handle, desc, _seq_heads(q, qs, dtype, on, "q"), _seq_heads(k, ks, dtype, on, "k"),
+                                                     _seq_heads(v, ks, dtype, on, "v"), _seq_heads(out, qs, dtype, on, "out"), lse.data_ptr(),
+                                                     None if lengths is None else _ints(lengths, (qs[0],), on, "lengths")))
         return out
 
     def backward(self, q, k, v, out, lse, dout, dq, dk, dv, delta, lengths=None):
         """`delta`: scratch of lse's shape."""
-        desc = self._desc(q, k, (lse, delta), (q, out, dout, dq), (v, dk, dv))
+        desc, qs, ks, dtype, on = self._shapes(q, k, lse, delta)
         ctx = self.ctx
-        on = ctx.device
-        ctx.check(lib().aig_window_attention_backward(ctx.handle, desc, _seq_heads(q), _seq_heads(k), _seq_heads(v), _seq_heads(out), lse.data_ptr(),
-                                                      _seq_heads(dout), _seq_heads(dq), _seq_heads(dk), _seq_heads(dv), delta.data_ptr(),
-                                                      None if lengths is None else _ints(lengths, (q.shape[0],), on, "lengths")))
+        ctx.check(lib().aig_window_attention_backward(ctx.handle, desc, _seq_heads(q, qs, dtype, on, "q"), _seq_heads(k, ks, dtype, on, "k"),
+                                                      _seq_heads(v, ks, dtype, on, "v"), _seq_heads(out, qs, dtype, on, "out"), lse.data_ptr(),
+                                                      _seq_heads(dout, qs, dtype, on, "dout"), _seq_heads(dq, qs, dtype, on, "dq"),
+                                                      _seq_heads(dk, ks, dtype, on, "dk"), _seq_heads(dv, ks, dtype, on, "dv"), delta.data_ptr(),
+                                                      None if lengths is None else _ints(lengths, (qs[0],), on, "lengths")))
         return dq, dk, dv
 
 

@@ -30,20 +30,32 @@ struct Side {
   long long in_token, in_head, out_token, out_head;  // strides in elements
 };
 
+// Division of numbers below 2^31 by a constant of the launch: one multiplication
+struct Divisor {
+  uint32_t magic, shift, by;
+  static Divisor of(uint32_t d) {
+    uint32_t l = 1;
+    while (l < 31 && (1u << l) < d) ++l;
+    return Divisor{d == 1 ? 0u : (uint32_t)(((uint64_t)1 << (31 + l)) / d + 1), l - 1, d};
+  }
+  __device__ __forceinline__ uint32_t divide(uint32_t n) const { return magic == 0 ? n : __umulhi(n, magic) >> shift; }
+};
+
 struct RopeParams {
   Side part[3];            // queries, keys, values
   int end[3];              // heads up to and with each part, counted over the parts
   int turned_heads;        // heads below it are turned, the others copied
-  int groups;              // items of a head: rot items that turn V pairs, then items that copy 2 V values
-  int rot_items, half;     // half = rot_dim / 2
-  int chunks, per_chunk;   // a token's heads in chunks of heads that one thread takes
-  long long items;
+  int rot_items, half;     // an item of a head: rot_items that turn V pairs, then those that copy 2 V values; half = rot_dim / 2
+  Divisor groups;          // items of a head
+  Divisor chunks;          // a token's heads in chunks of HP that one thread takes
+  uint32_t items;
   const int32_t* positions;
   const uint64_t* turns;
   float magnitude, sign;
-  // keys and values into pages (page_size > 0)
+  // keys and values into pages (page.by > 0)
   const int32_t *seqs, *table;
-  int batch, table_width, page_size, num_pages;
+  int batch, table_width, num_pages;
+  Divisor page;
   long long page_stride, place_stride;
   int* gerr;
 };
@@ -66,36 +78,52 @@ struct Row {
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<typename Vec<V>::type*>(p) = *reinterpret_cast<const typename Vec<V>::type*>(v); }
 };
 
-// One item: V pairs (or 2 V values to copy) of up to per_chunk heads of a token.
-template <class T, int V, bool INTERLEAVED>
+// One item: V pairs (or 2 V values to copy) of HP heads of a token.  All of them are read before the first is written: the
+// reads of several heads are under way together (an output may be its input, so the compiler cannot move reads ahead itself).
+template <class T, int V, int HP, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeParams p) {
-  const long long item = (long long)blockIdx.x * kThreads + threadIdx.x;
+  const uint32_t item = blockIdx.x * kThreads + threadIdx.x;
   if (item >= p.items) return;
-  const long long row = item / p.groups;
-  const int g = (int)(item - row * p.groups);
-  const long long token = row / p.chunks;
-  const int first = (int)(row - token * p.chunks) * p.per_chunk;
-  const int position = p.positions ? p.positions[token] : 0;
+  const uint32_t row = p.groups.divide(item);
+  const int g = item - row * p.groups.by;
+  const uint32_t token = p.chunks.divide(row);
+  const int first = (row - token * p.chunks.by) * HP;
+  const int position = p.positions[token];
   long long place = 0;  // where the token's keys and values go
-  if (p.page_size > 0) {
+  if (p.page.by > 0) {
     if (position < 0) return;
-    const long long seq = p.seqs ? (long long)p.seqs[token] : token;
-    const int slot = position / p.page_size;
+    const int seq = p.seqs ? p.seqs[token] : (int)token;
+    const int slot = p.page.divide(position);
     if (seq < 0 || seq >= p.batch || slot >= p.table_width) {
       note_error(p.gerr, kErrBadPlace);
       return;
     }
-    const int page = p.table[seq * p.table_width + slot];
+    const int page = p.table[(long long)seq * p.table_width + slot];
     if (page < 0 || page >= p.num_pages) {
       note_error(p.gerr, kErrBadPage);
       return;
     }
-    place = page * p.page_stride + (long long)(position - slot * p.page_size) * p.place_stride;
+    place = page * p.page_stride + (long long)(position - slot * (int)p.page.by) * p.place_stride;
   }
   const bool turn = g < p.rot_items;
   // elements of the item's two vectors within a head
   const int a0 = turn ? (INTERLEAVED ? 2 * V * g : V * g) : 2 * p.half + 2 * V * (g - p.rot_items);
   const int b0 = turn && !INTERLEAVED ? a0 + p.half : a0 + V;
+  Row<T, V> a[HP], b[HP];
+  T* out[HP];
+#pragma unroll
+  for (int i = 0; i < HP; ++i) {
+    const int h = first + i;
+    if (h < p.end[2]) {
+      const int w = h < p.end[0] ? 0 : h < p.end[1] ? 1 : 2;
+      const Side& s = p.part[w];
+      const int head = w == 0 ? h : h - p.end[w - 1];
+      const T* in = reinterpret_cast<const T*>(s.in) + token * s.in_token + head * s.in_head;
+      out[i] = reinterpret_cast<T*>(s.out) + (w > 0 && p.page.by > 0 ? place : token * s.out_token) + head * s.out_head;
+      a[i].load(in + a0);
+      b[i].load(in + b0);
+    }
+  }
   float cs[V], sn[V];
   if (turn) {
 #pragma unroll
@@ -108,23 +136,16 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
       sn[e] = s * p.magnitude * p.sign;
     }
   }
-  const int last = min(first + p.per_chunk, p.end[2]);
-#pragma unroll 4
-  for (int h = first; h < last; ++h) {
-    const int w = h < p.end[0] ? 0 : h < p.end[1] ? 1 : 2;
-    const Side& s = p.part[w];
-    const int head = w == 0 ? h : h - p.end[w - 1];
-    const T* in = reinterpret_cast<const T*>(s.in) + token * s.in_token + head * s.in_head;
-    T* out = reinterpret_cast<T*>(s.out) + (w > 0 && p.page_size > 0 ? place : token * s.out_token) + head * s.out_head;
-    Row<T, V> a, b;
-    a.load(in + a0);
-    b.load(in + b0);
+#pragma unroll
+  for (int i = 0; i < HP; ++i) {
+    const int h = first + i;
+    if (h >= p.end[2]) break;
     if (turn && h < p.turned_heads) {
       if (INTERLEAVED) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {  // pairs lie side by side: the first half of them in a, the second in b
-          T* x = 2 * e < V ? &a.v[2 * e % V] : &b.v[2 * e % V];
-          T* y = 2 * e + 1 < V ? &a.v[(2 * e + 1) % V] : &b.v[(2 * e + 1) % V];
+          T* x = 2 * e < V ? &a[i].v[2 * e % V] : &b[i].v[2 * e % V];
+          T* y = 2 * e + 1 < V ? &a[i].v[(2 * e + 1) % V] : &b[i].v[(2 * e + 1) % V];
           const float u = to_f32(*x), v = to_f32(*y);
           *x = from_f32<T>(u * cs[e] - v * sn[e]);
           *y = from_f32<T>(v * cs[e] + u * sn[e]);
@@ -132,25 +153,29 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
       } else {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float u = to_f32(a.v[e]), v = to_f32(b.v[e]);
-          a.v[e] = from_f32<T>(u * cs[e] - v * sn[e]);
-          b.v[e] = from_f32<T>(v * cs[e] + u * sn[e]);
+          const float u = to_f32(a[i].v[e]), v = to_f32(b[i].v[e]);
+          a[i].v[e] = from_f32<T>(u * cs[e] - v * sn[e]);
+          b[i].v[e] = from_f32<T>(v * cs[e] + u * sn[e]);
         }
       }
     }
-    a.store(out + a0);
-    b.store(out + b0);
+    a[i].store(out[i] + a0);
+    b[i].store(out[i] + b0);
   }
 }
 
-template <class T>
+template <class T, int HP>
 void (*pick_kernel(int v, bool interleaved))(const RopeParams) {
   switch (v) {
-    case 8: return interleaved ? rope_kernel<T, 8, true> : rope_kernel<T, 8, false>;
-    case 4: return interleaved ? rope_kernel<T, 4, true> : rope_kernel<T, 4, false>;
-    case 2: return interleaved ? rope_kernel<T, 2, true> : rope_kernel<T, 2, false>;
-    default: return interleaved ? rope_kernel<T, 1, true> : rope_kernel<T, 1, false>;
+    case 8: return interleaved ? rope_kernel<T, 8, HP, true> : rope_kernel<T, 8, HP, false>;
+    case 4: return interleaved ? rope_kernel<T, 4, HP, true> : rope_kernel<T, 4, HP, false>;
+    case 2: return interleaved ? rope_kernel<T, 2, HP, true> : rope_kernel<T, 2, HP, false>;
+    default: return interleaved ? rope_kernel<T, 1, HP, true> : rope_kernel<T, 1, HP, false>;
   }
+}
+template <class T>
+void (*pick_kernel(int v, int hp, bool interleaved))(const RopeParams) {
+  return hp == 4 ? pick_kernel<T, 4>(v, interleaved) : pick_kernel<T, 1>(v, interleaved);
 }
 
 // The widest vectors that head_dim, rot_dim and all tensors' addresses and strides are multiples of.
@@ -158,7 +183,7 @@ int vector_width(int head_dim, int rot, const RopeParams& p) {
   long long all = (head_dim / 2) | (rot / 2);
   for (const Side& s : p.part)
     if (s.in) all |= (long long)((uintptr_t)s.in / 2) | (long long)((uintptr_t)s.out / 2) | s.in_token | s.in_head | s.out_token | s.out_head;
-  if (p.page_size > 0) all |= p.page_stride | p.place_stride;
+  if (p.page.by > 0) all |= p.page_stride | p.place_stride;
   return all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
 }
 
@@ -166,18 +191,19 @@ int launch(aig_ctx* ctx, int dtype, int head_dim, int rot, bool interleaved, lon
   const int v = vector_width(head_dim, rot, p);
   p.half = rot / 2;
   p.rot_items = rot / 2 / v;
-  p.groups = head_dim / 2 / v;
-  // Heads per thread: sines are shared by more of them, but few tokens need every head as a thread of its own to fill the
-  // device.
-  const int heads = p.end[2];
-  p.per_chunk = tokens * p.groups * heads >= 4ll * 1024 * ctx->sm_count ? 4 : 1;
-  p.chunks = ceil_div(heads, p.per_chunk);
-  p.items = tokens * p.chunks * p.groups;
-  const long long blocks = ceil_div_ll(p.items, kThreads);
-  if (blocks > 0x7fffffffll) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "rotary positions: too many values for one call");
-  void (*kernel)(const RopeParams) = dtype == AIG_F16 ? pick_kernel<__half>(v, interleaved) : pick_kernel<__nv_bfloat16>(v, interleaved);
+  const int groups = head_dim / 2 / v, heads = p.end[2];
+  // Heads per thread: sines are shared by more of them and more reads are under way, but few tokens need every head as a
+  // thread of its own to fill the device.
+  const int hp = (double)tokens * groups * heads >= 4.0 * 1024 * ctx->sm_count ? 4 : 1;
+  const long long per_token = (long long)ceil_div(heads, hp) * groups;
+  if (tokens * (double)per_token > 2147483647.0 - kThreads)
+    return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "rotary positions: too many values for one call");
+  p.groups = Divisor::of(groups);
+  p.chunks = Divisor::of(ceil_div(heads, hp));
+  p.items = (uint32_t)(tokens * per_token);
   p.gerr = ctx->d_err;
-  kernel<<<(unsigned)blocks, kThreads, 0, ctx->stream>>>(p);
+  void (*kernel)(const RopeParams) = dtype == AIG_F16 ? pick_kernel<__half>(v, hp, interleaved) : pick_kernel<__nv_bfloat16>(v, hp, interleaved);
+  kernel<<<(p.items + kThreads - 1) / kThreads, kThreads, 0, ctx->stream>>>(p);
   AIG_LAUNCH_OK(ctx);
   return AIG_OK;
 }
@@ -335,7 +361,7 @@ int aig_kv_append(aig_ctx* ctx, const aig_kv_cache* cache, aig_rope_plan* rope, 
   p.table = table;
   p.batch = batch;
   p.table_width = table_width;
-  p.page_size = cache->page_size;
+  p.page = Divisor::of(cache->page_size);
   p.num_pages = cache->num_pages;
   p.page_stride = cache->page_stride;
   p.place_stride = cache->token_stride;

@@ -183,7 +183,7 @@ def test_refusals(env):
         with pytest.raises(ValueError):
             plan.forward(*args)
     lib = pk.lib()
-    heads = pk._heads(q)
+    heads = pk._pack_heads(q.data_ptr(), 2, 128, 64)
     bad_stride = pk._pack_heads(q.data_ptr(), 2, -128, 64)
     null = pk._pack_heads(0, 2, 128, 64)
     assert lib.aig_rope_forward(plan.handle, 2, pos.data_ptr(), 4, heads, heads, None, None) == -1
