@@ -25,6 +25,19 @@ inline int check_cache(aig_ctx* ctx, const aig_kv_cache* c, const char* who) {
   return AIG_OK;
 }
 
+// Division of numbers below 2^31 by a constant of the launch: one multiplication
+struct Divisor {
+  uint32_t magic, shift, by;
+  static Divisor of(uint32_t d) {
+    uint32_t l = 1;
+    while (l < 31 && (1u << l) < d) ++l;
+    return Divisor{d == 1 ? 0u : (uint32_t)(((uint64_t)1 << (31 + l)) / d + 1), l - 1, d};
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ uint32_t divide(uint32_t n) const { return magic == 0 ? n : __umulhi(n, magic) >> shift; }
+#endif
+};
+
 #ifdef __CUDACC__
 template <class T>
 __device__ __forceinline__ float to_f32(T v);
@@ -58,6 +71,13 @@ template <>
 __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
 template <>
 __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v)); }
+
+// 2^x on the special-function unit (relative error 2^-22; -inf gives 0)
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 __device__ __forceinline__ void note_error(int* gerr, int code) { atomicCAS(gerr, 0, code); }
 #endif

@@ -27,6 +27,8 @@ struct CopyParams {
 };
 
 __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyParams p) {
+  griddep_launch_dependents();
+  griddep_wait();
   const int pair = blockIdx.x / p.blocks;
   const int first = (blockIdx.x - pair * p.blocks) * kCopyThreads * kCopyUnroll + threadIdx.x;
   uint4* const base = blockIdx.y ? p.v : p.k;
@@ -48,15 +50,16 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_c
 
 // ---------------------------------------------------------------------------------------------
 // Attention of one new token.  For each (sequence, cached head) the visible positions are split over the CTAs of a cluster
-// and over their warps; a warp takes tiles of 16 positions through a ring of shared memory filled by cp.async, and holds the
-// query heads of the group as the 16 rows of mma.sync products (the tensor cores' only use here is that 16 query heads
-// cost no more instructions than one: the kernel is bound by reading the cache).  Softmax with a running maximum and sum
-// in fp32; the weights enter the second product as a sum of two 16-bit values each, so that their rounding does not add to
-// the result's.  Warps are joined in shared memory, CTAs over the cluster's distributed shared memory, in a fixed order: one
-// launch, no scratch in global memory, nothing that two calls or captured graphs could share.
+// and over their warps; a warp takes tiles of 16 or 32 positions through a ring of shared memory filled by cp.async.  Products
+// are mma.sync with the positions as rows and the group's query heads as the 8 columns, S^T = K Q^T and O^T = V^T P^T: K and
+// V come from shared memory as they lie there, P turns from result to operand by movmatrix, and eight query heads cost no more
+// than one.  (The kernel is bound by reading the cache, then by issuing instructions: with the heads as 16 rows
+// it took 430 instructions for 16 positions of 64, and 33 us where it takes XXB now, 128 sequences of up to 516 visible.)
+// Softmax with a running maximum and sum in fp32; the weights enter the second product as a sum of two 16-bit values each, so
+// that their rounding does not add to the result's.  Warps are joined in shared memory, CTAs over the cluster's distributed
+// shared memory, in a fixed order: one launch, no scratch in global memory, nothing that two calls or captured
+// graphs could share.
 constexpr int kWarps = 4;
-constexpr int kTile = 16;      // positions
-constexpr int kRows = 16;      // query heads per CTA
 constexpr int kMaxCluster = 16;
 
 struct AttendParams {
@@ -65,27 +68,30 @@ struct AttendParams {
   long long page, place, head;                 // cache strides in bytes
   long long q_seq, q_head, out_seq, out_head;  // in bytes
   const int32_t *table, *lengths;
-  int table_width, page_size, num_pages;
-  int kv_heads, group, row_blocks;             // query heads per cached one, in blocks of kRows
+  int table_width, num_pages;
+  Divisor page_size;
+  int kv_heads, group, row_blocks;             // query heads per cached one, in blocks of 8 or 16
   int splits;
   int window, sinks;
   float scale_log2;                            // scale * log2(e)
   int* gerr;
 };
 
-template <int D>
+template <int D, int HT>
 struct AttendShape {
-  static constexpr int kStages = D == 64 ? 4 : 3;
+  static constexpr int kTile = D == 64 ? 32 : 16;                   // positions
+  static constexpr int kRows = 8 * HT;                              // query heads per CTA
+  static constexpr int kStages = 3;
   static constexpr int kRowBytes = D * 2;
-  static constexpr int kTileBytes = kTile * kRowBytes;              // of keys, and of values
-  static constexpr int kRing = kWarps * kStages * 2 * kTileBytes;   // 64 KB, 96 KB
-  static constexpr int kJoin = kWarps * kRows * (D + 2) * 4;        // the warps' sums take the ring's place
+  static constexpr int kTileBytes = kTile * kRowBytes;              // of keys, and of values: 4 KB
+  static constexpr int kRing = kWarps * kStages * 2 * kTileBytes;   // 96 KB
+  static constexpr int kPitch = D + 4;                              // of a row of sums: lanes' stores fall into different banks
+  static constexpr int kJoin = kWarps * kRows * (kPitch + 2) * 4;   // the warps' sums take the ring's place
   static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
-  static constexpr int kCtasPerSm = D == 64 ? 3 : 2;
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
-  const int bytes = there ? 16 : 0;  // 0: the destination is filled with zeros, nothing is read
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  // (bytes = 0: the destination is filled with zeros, nothing is read)
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -96,6 +102,11 @@ __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
 }
 __device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 template <class T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -114,14 +125,17 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   lo = pack2<T>(x - h.x, y - h.y);
 }
 
-template <class T, int D>
-__global__ void __launch_bounds__(kWarps * 32, AttendShape<D>::kCtasPerSm) paged_attention_kernel(const __grid_constant__ AttendParams p) {
-  using S = AttendShape<D>;
-  constexpr int kChunks = D / 8;             // 16-byte pieces of a row
-  constexpr int kLoads = kTile * kChunks / 32;
+template <class T, int D, int HT>
+__global__ void __launch_bounds__(kWarps * 32, 2) paged_attention_kernel(const __grid_constant__ AttendParams p) {
+  using S = AttendShape<D, HT>;
+  constexpr int kChunks = D / 8;                // 16-byte pieces of a row
+  constexpr int kLoads = S::kTile * kChunks / 32;
+  constexpr int kTile = S::kTile, kRows = S::kRows;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_scale[kMaxCluster][kRows];
   cg::cluster_group cluster = cg::this_cluster();
+  griddep_launch_dependents();
+  griddep_wait();
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = blockIdx.x % p.splits;
@@ -134,7 +148,7 @@ __global__ void __launch_bounds__(kWarps * 32, AttendShape<D>::kCtasPerSm) paged
 
   // visible positions: `front` of them from 0 on, the others from `back` on
   int len = p.lengths[b];
-  const long long most = (long long)p.table_width * p.page_size;
+  const long long most = (long long)p.table_width * p.page_size.by;
   if (len > most) {
     if (threadIdx.x == 0) note_error(p.gerr, kErrBadPlace);
     len = (int)most;
@@ -146,42 +160,43 @@ __global__ void __launch_bounds__(kWarps * 32, AttendShape<D>::kCtasPerSm) paged
     visible = front + p.window;
   }
   // this CTA's share, in whole tiles; its warps take the tiles in turn
-  const int tiles = (visible + kTile - 1) / kTile;
+  const int tiles = (int)(((unsigned)visible + kTile - 1) / kTile);
   const int share = (tiles + p.splits - 1) / p.splits;
   const int tile_end = min((split + 1) * share, tiles);
   const int tile0 = split * share + warp;
 
-  // ---- queries as the A operand: rows are query heads
-  uint32_t qa[D / 16][4];
+  // ---- queries as the B operand: columns are query heads
+  uint32_t qb[HT][D / 16][2];
   {
-    const int r0 = lane >> 2, c = (lane & 3) * 2;
-    const uint8_t* q = p.q + b * p.q_seq + c * 2;
+    const int c = (lane & 3) * 2;
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks)
+    for (int ht = 0; ht < HT; ++ht) {
+      const int r = ht * 8 + (lane >> 2);
+      const uint8_t* q = p.q + b * p.q_seq + (q_head0 + r) * p.q_head + c * 2;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = r0 + (e & 1) * 8, col = ks * 16 + (e >> 1) * 8;
-        qa[ks][e] = r < rows ? *reinterpret_cast<const uint32_t*>(q + (q_head0 + r) * p.q_head + col * 2) : 0u;
-      }
+      for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) qb[ht][ks][e] = r < rows ? *reinterpret_cast<const uint32_t*>(q + (ks * 16 + e * 8) * 2) : 0u;
+    }
   }
 
   const uint32_t ring = smem_u32(smem) + warp * S::kStages * 2 * S::kTileBytes;
-  const uint8_t* const kbase = p.k + kvh * p.head;
-  const uint8_t* const vbase = p.v + kvh * p.head;
+  const uint8_t* const kbase = p.k + kvh * p.head + (lane % kChunks) * 16;
+  const uint8_t* const vbase = p.v + kvh * p.head + (lane % kChunks) * 16;
   const int32_t* const pages = p.table + (long long)b * p.table_width;
 
-  // Row `lane` of a tile (lanes 0..15): its page (-1: none) and its place there, looked up one tile before it is loaded so
-  // that the table's latency is not in the way.
+  // Row `lane` of a tile: its page (-1: none) and its place there, looked up one tile before it is loaded so that the table's
+  // latency is not in the way.
   int row_page = -1, row_place = 0;
   auto look_up = [&](int tile) {
-    const int i = tile * kTile + (lane & 15);
+    const int i = tile * kTile + (lane & (kTile - 1));
     row_page = -1;
     if (tile < tile_end && i < visible) {
       const int t = i < front ? i : back + (i - front);
-      const int slot = t / p.page_size;
-      row_place = t - slot * p.page_size;
+      const int slot = p.page_size.divide(t);
+      row_place = t - slot * (int)p.page_size.by;
       row_page = pages[slot];
-      if (row_page < 0 || row_page >= p.num_pages) {
+      if ((unsigned)row_page >= (unsigned)p.num_pages) {
         note_error(p.gerr, kErrBadPage);
         row_page = -1;
       }
@@ -193,22 +208,29 @@ __global__ void __launch_bounds__(kWarps * 32, AttendShape<D>::kCtasPerSm) paged
       const uint32_t kd = ring + stage * 2 * S::kTileBytes, vd = kd + S::kTileBytes;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int piece = i * 32 + lane, r = piece / kChunks, c = piece % kChunks;
-        const long long at = __shfl_sync(0xffffffffu, mine, r);
+        const int r = i * (32 / kChunks) + lane / kChunks, c = lane % kChunks;
+        long long at = __shfl_sync(0xffffffffu, mine, r);
         const uint32_t to = r * S::kRowBytes + ((c ^ (r & 7)) << 4);  // pieces of 8 rows fall into different banks
-        cp_async16(kd + to, kbase + (at < 0 ? 0 : at) + c * 16, at >= 0);
-        cp_async16(vd + to, vbase + (at < 0 ? 0 : at) + c * 16, at >= 0);
+        const int bytes = at < 0 ? 0 : 16;
+        at = at < 0 ? 0 : at;
+        cp_async16(kd + to, kbase + at, bytes);
+        cp_async16(vd + to, vbase + at, bytes);
       }
     }
     cp_async_commit();  // (an empty group where there is no tile: groups are counted)
   };
 
-  float o[D / 8][4];
+  // sums O^T: rows d, columns heads 2 (lane % 4) and the next; maxima and sums of these two heads
+  float o[HT][D / 16][4], top[HT][2], sum[HT][2];
 #pragma unroll
-  for (int n = 0; n < D / 8; ++n)
+  for (int ht = 0; ht < HT; ++ht) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
-  float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};  // of rows lane/4 and lane/4 + 8, sums of this lane's columns
+    for (int n = 0; n < D / 16; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[ht][n][e] = 0.f;
+    top[ht][0] = top[ht][1] = -INFINITY;
+    sum[ht][0] = sum[ht][1] = 0.f;
+  }
 
   look_up(tile0);
 #pragma unroll
@@ -226,69 +248,87 @@ __global__ void __launch_bounds__(kWarps * 32, AttendShape<D>::kCtasPerSm) paged
       look_up(next + kWarps);
     }
     const uint32_t kd = ring + stage * 2 * S::kTileBytes, vd = kd + S::kTileBytes;
-    // ---- scores of 16 positions
-    float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    {
-      const int r = (lane & 7) + ((lane >> 4) << 3), c0 = (lane >> 3) & 1;
+    // ---- scores: 16 positions a block
+    float sc[HT][kTile / 16][4];
+#pragma unroll
+    for (int kb = 0; kb < kTile / 16; ++kb) {
+#pragma unroll
+      for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[ht][kb][e] = 0.f;
+      const int r = kb * 16 + (lane & 15), c0 = lane >> 4;
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
-        uint32_t kb[4];
-        ldmatrix4(kd + r * S::kRowBytes + (((ks * 2 + c0) ^ (r & 7)) << 4), kb);
-        mma16816<T>(sc[0], qa[ks], kb[0], kb[1]);
-        mma16816<T>(sc[1], qa[ks], kb[2], kb[3]);
+        uint32_t ka[4];
+        ldmatrix4(kd + r * S::kRowBytes + (((ks * 2 + c0) ^ (r & 7)) << 4), ka);
+#pragma unroll
+        for (int ht = 0; ht < HT; ++ht) mma16816<T>(sc[ht][kb], ka, qb[ht][ks][0], qb[ht][ks][1]);
       }
     }
     const int left = visible - tile * kTile;  // positions from here on
+    if (left < kTile) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+      for (int kb = 0; kb < kTile / 16; ++kb)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int col = n * 8 + (lane & 3) * 2 + (e & 1);
-        sc[n][e] = col < left ? sc[n][e] * p.scale_log2 : -INFINITY;
-      }
-    float mx[2];
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float m = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      mx[h] = fmaxf(m, top[h]);
+          for (int ht = 0; ht < HT; ++ht)
+            if (kb * 16 + (lane >> 2) + (e >> 1) * 8 >= left) sc[ht][kb][e] = -INFINITY;
     }
-    if (__any_sync(0xffffffffu, mx[0] > top[0] || mx[1] > top[1])) {
+#pragma unroll
+    for (int ht = 0; ht < HT; ++ht) {
+      float mx[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float f = exp2f(top[h] - mx[h]);  // (a tile has a visible position, so mx is finite if the scores are)
-        top[h] = mx[h];
-        sum[h] *= f;
+        float m = sc[ht][0][h];
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-          o[n][2 * h] *= f;
-          o[n][2 * h + 1] *= f;
+        for (int kb = 0; kb < kTile / 16; ++kb) m = fmaxf(fmaxf(m, sc[ht][kb][h]), sc[ht][kb][h + 2]);
+        mx[h] = m * p.scale_log2;
+      }
+#pragma unroll
+      for (int s = 4; s < 32; s <<= 1)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], s));
+      if (__any_sync(0xffffffffu, mx[0] > top[ht][0] || mx[1] > top[ht][1])) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float m = fmaxf(mx[h], top[ht][h]);
+          const float f = ex2(top[ht][h] - m);  // (a tile has a visible position, so m is finite if the scores are)
+          top[ht][h] = m;
+          sum[ht][h] *= f;
+#pragma unroll
+          for (int n = 0; n < D / 16; ++n) {
+            o[ht][n][h] *= f;
+            o[ht][n][h + 2] *= f;
+          }
         }
       }
     }
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int kb = 0; kb < kTile / 16; ++kb) {
+      uint32_t hi[HT][2], lo[HT][2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        sc[n][e] = exp2f(sc[n][e] - top[e >> 1]);
-        sum[e >> 1] += sc[n][e];
-      }
-    uint32_t hi[4], lo[4];
-    split2<T>(sc[0][0], sc[0][1], hi[0], lo[0]);
-    split2<T>(sc[0][2], sc[0][3], hi[1], lo[1]);
-    split2<T>(sc[1][0], sc[1][1], hi[2], lo[2]);
-    split2<T>(sc[1][2], sc[1][3], hi[3], lo[3]);
-    {
-      const int r = lane & 15, c0 = lane >> 4;
+      for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float x = ex2(fmaf(sc[ht][kb][2 * e], p.scale_log2, -top[ht][0])), y = ex2(fmaf(sc[ht][kb][2 * e + 1], p.scale_log2, -top[ht][1]));
+          sum[ht][0] += x;
+          sum[ht][1] += y;
+          split2<T>(x, y, hi[ht][e], lo[ht][e]);
+          hi[ht][e] = movmatrix_trans(hi[ht][e]);
+          lo[ht][e] = movmatrix_trans(lo[ht][e]);
+        }
+      // matrices of 8 positions x 8 elements, turned: elements are rows
+      const int r = kb * 16 + (lane & 7) + ((lane >> 4) << 3), c0 = (lane >> 3) & 1;
 #pragma unroll
       for (int n = 0; n < D / 16; ++n) {
-        uint32_t vb[4];
-        ldmatrix4_trans(vd + r * S::kRowBytes + (((n * 2 + c0) ^ (r & 7)) << 4), vb);
-        mma16816<T>(o[2 * n], hi, vb[0], vb[1]);
-        mma16816<T>(o[2 * n + 1], hi, vb[2], vb[3]);
-        mma16816<T>(o[2 * n], lo, vb[0], vb[1]);
-        mma16816<T>(o[2 * n + 1], lo, vb[2], vb[3]);
+        uint32_t va[4];
+        ldmatrix4_trans(vd + r * S::kRowBytes + (((n * 2 + c0) ^ (r & 7)) << 4), va);
+#pragma unroll
+        for (int ht = 0; ht < HT; ++ht) {
+          mma16816<T>(o[ht][n], va, hi[ht][0], hi[ht][1]);
+          mma16816<T>(o[ht][n], va, lo[ht][0], lo[ht][1]);
+        }
       }
     }
     __syncwarp();  // the stage is free for the load after next
@@ -296,29 +336,36 @@ __global__ void __launch_bounds__(kWarps * 32, AttendShape<D>::kCtasPerSm) paged
   }
   cp_async_wait<0>();
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-    sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-  }
+  for (int ht = 0; ht < HT; ++ht)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int s = 4; s < 32; s <<= 1) sum[ht][h] += __shfl_xor_sync(0xffffffffu, sum[ht][h], s);
 
   // ---- join the warps: [warp][row][D] weighted sums, then [warp][row] maxima and sums, in the ring's place
   __syncthreads();
+  constexpr int kPitch = S::kPitch;
   float* const acc = reinterpret_cast<float*>(smem);
-  float* const tops = acc + kWarps * kRows * D;
+  float* const tops = acc + kWarps * kRows * kPitch;
   float* const sums = tops + kWarps * kRows;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = (lane >> 2) + 8 * h;
-    if (r < rows) {
+  for (int ht = 0; ht < HT; ++ht)
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n)
-        *reinterpret_cast<float2*>(acc + (warp * kRows + r) * D + n * 8 + (lane & 3) * 2) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+    for (int h = 0; h < 2; ++h) {
+      const int r = ht * 8 + (lane & 3) * 2 + h;
+      if (r < rows) {
+        float* const to = acc + (warp * kRows + r) * kPitch + (lane >> 2);
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {
+          to[n * 16] = o[ht][n][h];
+          to[n * 16 + 8] = o[ht][n][h + 2];
+        }
+      }
+      if (lane < 4) {
+        tops[warp * kRows + r] = top[ht][h];
+        sums[warp * kRows + r] = sum[ht][h];
+      }
     }
-    if ((lane & 3) == 0) {
-      tops[warp * kRows + r] = top[h];
-      sums[warp * kRows + r] = sum[h];
-    }
-  }
   __syncthreads();
   // each warp's factor, and the CTA's maximum and sum in the first warp's place
   if (threadIdx.x < kRows) {
@@ -329,7 +376,7 @@ __global__ void __launch_bounds__(kWarps * 32, AttendShape<D>::kCtasPerSm) paged
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float mw = tops[w * kRows + r];
-      f[w] = mw == -INFINITY ? 0.f : exp2f(mw - m);  // a warp without a position has the weight 0
+      f[w] = mw == -INFINITY ? 0.f : ex2(mw - m);  // a warp without a position has the weight 0
       total += f[w] * sums[w * kRows + r];
     }
 #pragma unroll
@@ -339,11 +386,11 @@ __global__ void __launch_bounds__(kWarps * 32, AttendShape<D>::kCtasPerSm) paged
   }
   __syncthreads();
   for (int i = threadIdx.x; i < rows * D; i += kWarps * 32) {
-    const int r = i / D;
+    const int r = i / D, at = r * kPitch + (i - r * D);
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) v = fmaf(s_scale[w][r], acc[w * kRows * D + i], v);
-    acc[i] = v;
+    for (int w = 0; w < kWarps; ++w) v = fmaf(s_scale[w][r], acc[w * kRows * kPitch + at], v);
+    acc[at] = v;
   }
   // ---- join the CTAs: each takes a share of the outputs
   if (p.splits > 1) cluster.sync();
@@ -354,7 +401,7 @@ __global__ void __launch_bounds__(kWarps * 32, AttendShape<D>::kCtasPerSm) paged
     for (int s = 0; s < p.splits; ++s) m = fmaxf(m, *cluster.map_shared_rank(tops + r, s));
     for (int s = 0; s < p.splits; ++s) {
       const float ms = *cluster.map_shared_rank(tops + r, s);
-      const float f = ms == -INFINITY ? 0.f : exp2f(ms - m);
+      const float f = ms == -INFINITY ? 0.f : ex2(ms - m);
       s_scale[s][r] = f;
       total += f * *cluster.map_shared_rank(sums + r, s);
     }
@@ -364,24 +411,30 @@ __global__ void __launch_bounds__(kWarps * 32, AttendShape<D>::kCtasPerSm) paged
   __syncthreads();
   const int pairs = rows * (D / 2);
   for (int i = split * kWarps * 32 + threadIdx.x; i < pairs; i += p.splits * kWarps * 32) {
-    const int r = i / (D / 2);
+    const int r = i / (D / 2), c = (i - r * (D / 2)) * 2;
     float2 v = make_float2(0.f, 0.f);
     for (int s = 0; s < p.splits; ++s) {
-      const float2 x = *cluster.map_shared_rank(reinterpret_cast<float2*>(acc) + i, s);
+      const float2 x = *reinterpret_cast<const float2*>(cluster.map_shared_rank(acc + r * kPitch + c, s));
       const float f = s_scale[s][r];
       v.x = fmaf(f, x.x, v.x);
       v.y = fmaf(f, x.y, v.y);
     }
     uint8_t* out = p.out + b * p.out_seq + (q_head0 + r) * p.out_head;
-    *reinterpret_cast<uint32_t*>(out + (i - r * (D / 2)) * 4) = pack2<T>(v.x, v.y);
+    *reinterpret_cast<uint32_t*>(out + c * 2) = pack2<T>(v.x, v.y);
   }
   if (p.splits > 1) cluster.sync();  // nobody leaves while its shared memory is read
 }
 
-template <class T, int D>
-int launch_attend(aig_ctx* ctx, const AttendParams& p, int items) {
-  using S = AttendShape<D>;
-  auto kernel = paged_attention_kernel<T, D>;
+template <class T, int D, int HT>
+int launch_attend(aig_ctx* ctx, AttendParams& p, int batch, long long max_visible) {
+  using S = AttendShape<D, HT>;
+  p.row_blocks = ceil_div(p.group, S::kRows);
+  const long long items = (long long)batch * p.kv_heads * p.row_blocks;
+  if (items * kMaxCluster > 0x7fffffffll) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "paged attention: too many sequences and heads for one call");
+  // Splits: enough CTAs for every SM twice, each with a tile per warp at least.
+  p.splits = 1;
+  while (p.splits < kMaxCluster && items * p.splits < 4ll * ctx->sm_count && max_visible > (long long)p.splits * kWarps * S::kTile) p.splits *= 2;
+  auto kernel = paged_attention_kernel<T, D, HT>;
   AIG_CUDA_OK(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
   if (p.splits > 8) AIG_CUDA_OK(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg{};
@@ -389,14 +442,19 @@ int launch_attend(aig_ctx* ctx, const AttendParams& p, int items) {
   cfg.blockDim = dim3(kWarps * 32);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = ctx->stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = p.splits;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1] = pdl_attribute(ctx);
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   AIG_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, kernel, p));
   return AIG_OK;
+}
+template <class T, int D>
+int launch_attend(aig_ctx* ctx, AttendParams& p, int batch, long long max_visible) {
+  return p.group <= 8 ? launch_attend<T, D, 1>(ctx, p, batch, max_visible) : launch_attend<T, D, 2>(ctx, p, batch, max_visible);
 }
 
 }  // namespace
@@ -442,8 +500,7 @@ int aig_kv_copy_pages(aig_ctx* ctx, const aig_kv_cache* cache, const int32_t* sr
     memcpy(p.src, src + done, n * sizeof(int32_t));
     memcpy(p.dst, dst + done, n * sizeof(int32_t));
     if ((long long)n * p.blocks > 0x7fffffffll) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "kv copy pages: too much for one call");
-    copy_pages_kernel<<<dim3((unsigned)(n * p.blocks), 2), kCopyThreads, 0, ctx->stream>>>(p);
-    AIG_LAUNCH_OK(ctx);
+    AIG_CUDA_OK(ctx, launch_pdl(ctx, copy_pages_kernel, dim3((unsigned)(n * p.blocks), 2), dim3(kCopyThreads), 0, p));
   }
   return AIG_OK;
 }
@@ -478,25 +535,19 @@ int aig_paged_attention(aig_ctx* ctx, const aig_kv_cache* cache, const aig_heads
   p.table = table;
   p.lengths = lengths;
   p.table_width = table_width;
-  p.page_size = cache->page_size;
+  p.page_size = Divisor::of(cache->page_size);
   p.num_pages = cache->num_pages;
   p.kv_heads = cache->kv_heads;
   p.group = q->heads / cache->kv_heads;
-  p.row_blocks = ceil_div(p.group, kRows);
   p.window = window;
   p.sinks = sinks;
   p.scale_log2 = (float)((double)scale * 1.4426950408889634);
   p.gerr = ctx->d_err;
-  const long long items = (long long)batch * cache->kv_heads * p.row_blocks;
-  if (items * kMaxCluster > 0x7fffffffll) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "paged attention: too many sequences and heads for one call");
-  // Splits: enough CTAs for every SM twice, each with a tile per warp at least.
   long long visible = max_length;
   if (window > 0 && visible > (long long)window + sinks) visible = (long long)window + sinks;
-  p.splits = 1;
-  while (p.splits < kMaxCluster && items * p.splits < 4ll * ctx->sm_count && visible > (long long)p.splits * kWarps * kTile) p.splits *= 2;
   if (cache->dtype == AIG_F16)
-    return cache->head_dim == 64 ? launch_attend<__half, 64>(ctx, p, (int)items) : launch_attend<__half, 128>(ctx, p, (int)items);
-  return cache->head_dim == 64 ? launch_attend<__nv_bfloat16, 64>(ctx, p, (int)items) : launch_attend<__nv_bfloat16, 128>(ctx, p, (int)items);
+    return cache->head_dim == 64 ? launch_attend<__half, 64>(ctx, p, batch, visible) : launch_attend<__half, 128>(ctx, p, batch, visible);
+  return cache->head_dim == 64 ? launch_attend<__nv_bfloat16, 64>(ctx, p, batch, visible) : launch_attend<__nv_bfloat16, 128>(ctx, p, batch, visible);
 }
 
 }  // extern "C"

@@ -30,17 +30,6 @@ struct Side {
   long long in_token, in_head, out_token, out_head;  // strides in elements
 };
 
-// Division of numbers below 2^31 by a constant of the launch: one multiplication
-struct Divisor {
-  uint32_t magic, shift, by;
-  static Divisor of(uint32_t d) {
-    uint32_t l = 1;
-    while (l < 31 && (1u << l) < d) ++l;
-    return Divisor{d == 1 ? 0u : (uint32_t)(((uint64_t)1 << (31 + l)) / d + 1), l - 1, d};
-  }
-  __device__ __forceinline__ uint32_t divide(uint32_t n) const { return magic == 0 ? n : __umulhi(n, magic) >> shift; }
-};
-
 struct RopeParams {
   Side part[3];            // queries, keys, values
   int end[3];              // heads up to and with each part, counted over the parts
@@ -82,6 +71,8 @@ struct Row {
 // reads of several heads are under way together (an output may be its input, so the compiler cannot move reads ahead itself).
 template <class T, int V, int HP, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ RopeParams p) {
+  griddep_launch_dependents();
+  griddep_wait();
   const uint32_t item = blockIdx.x * kThreads + threadIdx.x;
   if (item >= p.items) return;
   const uint32_t row = p.groups.divide(item);
@@ -203,8 +194,7 @@ int launch(aig_ctx* ctx, int dtype, int head_dim, int rot, bool interleaved, lon
   p.items = (uint32_t)(tokens * per_token);
   p.gerr = ctx->d_err;
   void (*kernel)(const RopeParams) = dtype == AIG_F16 ? pick_kernel<__half>(v, hp, interleaved) : pick_kernel<__nv_bfloat16>(v, hp, interleaved);
-  kernel<<<(p.items + kThreads - 1) / kThreads, kThreads, 0, ctx->stream>>>(p);
-  AIG_LAUNCH_OK(ctx);
+  AIG_CUDA_OK(ctx, launch_pdl(ctx, kernel, dim3((p.items + kThreads - 1) / kThreads), dim3(kThreads), 0, p));
   return AIG_OK;
 }
 
