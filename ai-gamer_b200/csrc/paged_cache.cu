@@ -59,7 +59,6 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_c
 // that their rounding does not add to the result's.  Warps are joined in shared memory, CTAs over the cluster's distributed
 // shared memory, in a fixed order: one launch, no scratch in global memory, nothing that two calls or captured
 // graphs could share.
-constexpr int kWarps = 4;
 constexpr int kMaxCluster = 16;
 
 struct AttendParams {
@@ -77,17 +76,21 @@ struct AttendParams {
   int* gerr;
 };
 
-template <int D, int HT>
+// W warps.  Where there are more sequences and heads than the device holds CTAs, small CTAs of two warps, seven to an SM, hide one
+// another's beginnings and ends; few long sequences need the reads of four warps per CTA (128 sequences, 8 heads of 64: 22.9 us
+// with two, 25.5 with four; 8 sequences of up to 65536, 8 heads of 128: 214 with two, 177 with four).
+template <int D, int HT, int W>
 struct AttendShape {
-  static constexpr int kTile = D == 64 ? 32 : 16;                   // positions
+  static constexpr int kTile = 16;                                  // positions (32 need more shared memory: fewer CTAs, 26 us)
   static constexpr int kRows = 8 * HT;                              // query heads per CTA
   static constexpr int kStages = 3;
   static constexpr int kRowBytes = D * 2;
-  static constexpr int kTileBytes = kTile * kRowBytes;              // of keys, and of values: 4 KB
-  static constexpr int kRing = kWarps * kStages * 2 * kTileBytes;   // 96 KB
+  static constexpr int kTileBytes = kTile * kRowBytes;              // of keys, and of values: 2 KB or 4 KB
+  static constexpr int kRing = W * kStages * 2 * kTileBytes;        // 24 to 96 KB
   static constexpr int kPitch = D + 4;                              // of a row of sums: lanes' stores fall into different banks
-  static constexpr int kJoin = kWarps * kRows * (kPitch + 2) * 4;   // the warps' sums take the ring's place
+  static constexpr int kJoin = W * kRows * (kPitch + 2) * 4;        // the warps' sums take the ring's place
   static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
+  static constexpr int kCtasPerSm = W == 2 ? (D == 64 ? (HT == 1 ? 7 : 5) : 4) : (D == 64 ? (HT == 1 ? 4 : 3) : 2);
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
@@ -125,9 +128,9 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   lo = pack2<T>(x - h.x, y - h.y);
 }
 
-template <class T, int D, int HT>
-__global__ void __launch_bounds__(kWarps * 32, 2) paged_attention_kernel(const __grid_constant__ AttendParams p) {
-  using S = AttendShape<D, HT>;
+template <class T, int D, int HT, int W>
+__global__ void __launch_bounds__(W * 32, AttendShape<D, HT, W>::kCtasPerSm) paged_attention_kernel(const __grid_constant__ AttendParams p) {
+  using S = AttendShape<D, HT, W>;
   constexpr int kChunks = D / 8;                // 16-byte pieces of a row
   constexpr int kLoads = S::kTile * kChunks / 32;
   constexpr int kTile = S::kTile, kRows = S::kRows;
@@ -235,17 +238,17 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_attention_kernel(const _
   look_up(tile0);
 #pragma unroll
   for (int s = 0; s < S::kStages - 1; ++s) {
-    load(tile0 + s * kWarps, s);
-    look_up(tile0 + (s + 1) * kWarps);
+    load(tile0 + s * W, s);
+    look_up(tile0 + (s + 1) * W);
   }
   int stage = 0;
-  for (int tile = tile0; tile < tile_end; tile += kWarps) {
+  for (int tile = tile0; tile < tile_end; tile += W) {
     cp_async_wait<S::kStages - 2>();
     __syncwarp();
     {
-      const int next = tile + (S::kStages - 1) * kWarps;
+      const int next = tile + (S::kStages - 1) * W;
       load(next, stage == 0 ? S::kStages - 1 : stage - 1);
-      look_up(next + kWarps);
+      look_up(next + W);
     }
     const uint32_t kd = ring + stage * 2 * S::kTileBytes, vd = kd + S::kTileBytes;
     // ---- scores: 16 positions a block
@@ -346,8 +349,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_attention_kernel(const _
   __syncthreads();
   constexpr int kPitch = S::kPitch;
   float* const acc = reinterpret_cast<float*>(smem);
-  float* const tops = acc + kWarps * kRows * kPitch;
-  float* const sums = tops + kWarps * kRows;
+  float* const tops = acc + W * kRows * kPitch;
+  float* const sums = tops + W * kRows;
 #pragma unroll
   for (int ht = 0; ht < HT; ++ht)
 #pragma unroll
@@ -370,26 +373,26 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_attention_kernel(const _
   // each warp's factor, and the CTA's maximum and sum in the first warp's place
   if (threadIdx.x < kRows) {
     const int r = threadIdx.x;
-    float m = tops[r], f[kWarps], total = 0.f;
+    float m = tops[r], f[W], total = 0.f;
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) m = fmaxf(m, tops[w * kRows + r]);
+    for (int w = 1; w < W; ++w) m = fmaxf(m, tops[w * kRows + r]);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float mw = tops[w * kRows + r];
       f[w] = mw == -INFINITY ? 0.f : ex2(mw - m);  // a warp without a position has the weight 0
       total += f[w] * sums[w * kRows + r];
     }
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) s_scale[w][r] = f[w];
+    for (int w = 0; w < W; ++w) s_scale[w][r] = f[w];
     tops[r] = m;
     sums[r] = total;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < rows * D; i += kWarps * 32) {
+  for (int i = threadIdx.x; i < rows * D; i += W * 32) {
     const int r = i / D, at = r * kPitch + (i - r * D);
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) v = fmaf(s_scale[w][r], acc[w * kRows * kPitch + at], v);
+    for (int w = 0; w < W; ++w) v = fmaf(s_scale[w][r], acc[w * kRows * kPitch + at], v);
     acc[at] = v;
   }
   // ---- join the CTAs: each takes a share of the outputs
@@ -410,7 +413,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_attention_kernel(const _
   }
   __syncthreads();
   const int pairs = rows * (D / 2);
-  for (int i = split * kWarps * 32 + threadIdx.x; i < pairs; i += p.splits * kWarps * 32) {
+  for (int i = split * W * 32 + threadIdx.x; i < pairs; i += p.splits * W * 32) {
     const int r = i / (D / 2), c = (i - r * (D / 2)) * 2;
     float2 v = make_float2(0.f, 0.f);
     for (int s = 0; s < p.splits; ++s) {
@@ -425,21 +428,20 @@ __global__ void __launch_bounds__(kWarps * 32, 2) paged_attention_kernel(const _
   if (p.splits > 1) cluster.sync();  // nobody leaves while its shared memory is read
 }
 
-template <class T, int D, int HT>
-int launch_attend(aig_ctx* ctx, AttendParams& p, int batch, long long max_visible) {
-  using S = AttendShape<D, HT>;
-  p.row_blocks = ceil_div(p.group, S::kRows);
-  const long long items = (long long)batch * p.kv_heads * p.row_blocks;
-  if (items * kMaxCluster > 0x7fffffffll) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "paged attention: too many sequences and heads for one call");
-  // Splits: enough CTAs for every SM twice, each with a tile per warp at least.
+template <class T, int D, int HT, int W>
+int launch_attend(aig_ctx* ctx, AttendParams& p, int items, long long max_visible) {
+  using S = AttendShape<D, HT, W>;
+  // Splits: enough CTAs for every SM four times, each with a tile per warp at least.  Clusters of 16 leave SMs idle that
+  // a group of 16 does not fit on (177 us with 8, 183 with 16 for 8 sequences): only where 8 would leave more.
+  const int most = items * 8 < ctx->sm_count ? kMaxCluster : 8;
   p.splits = 1;
-  while (p.splits < kMaxCluster && items * p.splits < 4ll * ctx->sm_count && max_visible > (long long)p.splits * kWarps * S::kTile) p.splits *= 2;
-  auto kernel = paged_attention_kernel<T, D, HT>;
+  while (p.splits < most && items * p.splits < 4 * ctx->sm_count && max_visible > (long long)p.splits * W * S::kTile) p.splits *= 2;
+  auto kernel = paged_attention_kernel<T, D, HT, W>;
   AIG_CUDA_OK(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
   if (p.splits > 8) AIG_CUDA_OK(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)items * p.splits);
-  cfg.blockDim = dim3(kWarps * 32);
+  cfg.blockDim = dim3(W * 32);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = ctx->stream;
   cudaLaunchAttribute attr[2];
@@ -451,6 +453,13 @@ int launch_attend(aig_ctx* ctx, AttendParams& p, int batch, long long max_visibl
   cfg.numAttrs = 2;
   AIG_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, kernel, p));
   return AIG_OK;
+}
+template <class T, int D, int HT>
+int launch_attend(aig_ctx* ctx, AttendParams& p, int batch, long long max_visible) {
+  p.row_blocks = ceil_div(p.group, 8 * HT);
+  const long long items = (long long)batch * p.kv_heads * p.row_blocks;
+  if (items * kMaxCluster > 0x7fffffffll) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "paged attention: too many sequences and heads for one call");
+  return items >= 4 * ctx->sm_count ? launch_attend<T, D, HT, 2>(ctx, p, (int)items, max_visible) : launch_attend<T, D, HT, 4>(ctx, p, (int)items, max_visible);
 }
 template <class T, int D>
 int launch_attend(aig_ctx* ctx, AttendParams& p, int batch, long long max_visible) {
