@@ -449,6 +449,183 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
 }
 
 // ---------------------------------------------------------------------------------------------
+// Forward, short sequences: 64 queries of a head per CTA of four warps, products by mma.sync.  A sequence of 64 is half a tile of
+// the tcgen05 kernel, whose CTA owns an SM and spends its time on the way there and back; of these CTAs four to an
+// SM hide one another's (1024 heads of 64 x 64: 11.6 us against 31.5).
+constexpr int kShort = 64;
+
+template <int D>
+struct ShortShape {
+  static constexpr uint32_t kTileB = kShort * D * 2;
+  static constexpr size_t kSmem = 5 * kTileB;  // queries, two stages of keys and values
+};
+
+// 64 rows of D elements, 16-byte pieces of a row exchanged so that those of eight rows fall into different banks
+template <int D>
+__device__ __forceinline__ uint32_t short_at(int r, int c) {
+  return (uint32_t)(r * D * 2 + ((c ^ (r & 7)) << 4));
+}
+template <class T, int D>
+__device__ __forceinline__ void short_load(uint32_t to, const View& v, int b, int h, int first, int end, int tid) {
+  constexpr int kPieces = D / 8, kStep = 128 / kPieces;  // rows that the CTA's threads fetch at once
+  const int r = tid / kPieces, c = tid % kPieces;
+  const T* from = reinterpret_cast<const T*>(v.data) + b * v.batch + h * v.head + (first + r) * v.token + c * 8;
+  const T* const some = reinterpret_cast<const T*>(v.data);  // (an address for copies of no bytes)
+#pragma unroll
+  for (int i = 0; i < kShort / kStep; ++i, from += kStep * v.token) {
+    const bool there = first + r + i * kStep < end;
+    cp_async16(to + short_at<D>(r + i * kStep, c), there ? from : some, there ? 16 : 0);
+  }
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(128, D == 64 ? 4 : 3) window_short_kernel(const __grid_constant__ WinParams p) {
+  using S = ShortShape<D>;
+  extern __shared__ __align__(128) uint8_t sm[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int item = blockIdx.x;
+  const int b = item % p.batch;
+  item /= p.batch;
+  const int h = item % p.heads, r0 = (p.blocks - 1 - item / p.heads) * kShort;
+  const int kvh = h / (p.heads / p.kv_heads);
+  const int len = p.lengths ? min(max(p.lengths[b], 0), p.kv_len) : p.kv_len;
+  const int off = p.kv_len - p.q_len;
+  const int rows_end = min(p.q_len, len - off);
+  if (r0 >= rows_end) return;
+  const KeyTiles kt = key_tiles<kShort>(off + r0, off + min(r0 + kShort, rows_end) - 1, p.window, p.sinks);
+  const int tiles = kt.sink_end + kt.end - kt.begin;
+  auto first_key = [&](int u) { return (u < kt.sink_end ? u : kt.begin + (u - kt.sink_end)) * kShort; };
+  const uint32_t sQ = smem_u32(sm);
+  auto stage = [&](int u) { return sQ + S::kTileB * (1 + 2 * (u & 1)); };  // keys, then values
+  auto fetch = [&](int u) {
+    if (u < tiles) {
+      short_load<T, D>(stage(u), p.k, b, kvh, first_key(u), len, threadIdx.x);
+      short_load<T, D>(stage(u) + S::kTileB, p.v, b, kvh, first_key(u), len, threadIdx.x);
+    }
+    cp_async_commit();
+  };
+  short_load<T, D>(sQ, p.q, b, h, r0, rows_end, threadIdx.x);
+  fetch(0);
+  fetch(1);
+  cp_async_wait<1>();
+  __syncthreads();
+  float o[D / 8][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};  // of rows lane/4 and lane/4 + 8 of the warp's 16
+#pragma unroll
+  for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+  const float c = p.scale * kLog2e;
+  const int first = off + r0 + warp * 16;  // position of the warp's first row
+  for (int u = 0; u < tiles; ++u) {
+    if (u > 0) {
+      cp_async_wait<1>();
+      __syncthreads();
+    }
+    const uint32_t sK = stage(u), sV = sK + S::kTileB;
+    const int j0 = first_key(u);
+    const int keys = first + 16 - j0;  // of the tile, up to the warp's last row's own
+    float sc[8][4];
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[n][e] = (n & ~1) * 8 < keys ? 0.f : -INFINITY;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      uint32_t qa[4];  // (read again for every tile: held, they would cost an SM one of five CTAs)
+      ldmatrix4(sQ + short_at<D>(warp * 16 + (lane & 15), ks * 2 + (lane >> 4)), qa);
+#pragma unroll
+      for (int n = 0; n < 8; n += 2) {
+        if (n * 8 >= keys) continue;
+        uint32_t kb[4];
+        ldmatrix4(sK + short_at<D>(n * 8 + (lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)), kb);
+        mma16816<T>(sc[n], qa, kb[0], kb[1]);
+        mma16816<T>(sc[n + 1], qa, kb[2], kb[3]);
+      }
+    }
+    const bool cut = j0 + kShort - 1 > first || (p.window > 0 && j0 <= first + 15 - p.window && j0 + kShort > p.sinks);
+    if (cut) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int pos = first + (lane >> 2) + 8 * x - j0, lo = p.window > 0 ? pos - p.window + 1 : 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {  // 32 keys, this thread's from bit 0 on
+          const uint32_t shown = (bits_below(pos + 1 - 32 * i) & (~bits_below(lo - 32 * i) | bits_below(p.sinks - j0 - 32 * i))) >> ((lane & 3) * 2);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            if (!(shown >> (8 * n) & 1)) sc[4 * i + n][2 * x] = -INFINITY;
+            if (!(shown >> (8 * n + 1) & 1)) sc[4 * i + n][2 * x + 1] = -INFINITY;
+          }
+        }
+      }
+    }
+    float ref[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      float m = fmaxf(sc[0][2 * x], sc[0][2 * x + 1]);
+#pragma unroll
+      for (int n = 1; n < 8; ++n) m = fmaxf(fmaxf(m, sc[n][2 * x]), sc[n][2 * x + 1]);
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = fmaxf(fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2)) * c, top[x]);
+      if (u == 0) {
+        top[x] = m;
+      } else if (__any_sync(0xffffffffu, m > top[x])) {
+        const float f = m > top[x] ? ex2(top[x] - m) : 1.f;
+        top[x] = m;
+        sum[x] *= f;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+          o[n][2 * x] *= f;
+          o[n][2 * x + 1] *= f;
+        }
+      }
+      ref[x] = top[x] == -INFINITY ? 0.f : top[x];  // a row that has seen no key yet
+    }
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      if (ks * 16 >= keys) continue;
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {  // rows lane/4 and + 8 of 8 keys, then of the next 8
+        const float x = ex2(fmaf(sc[2 * ks + (e >> 1)][2 * (e & 1)], c, -ref[e & 1])), y = ex2(fmaf(sc[2 * ks + (e >> 1)][2 * (e & 1) + 1], c, -ref[e & 1]));
+        sum[e & 1] += x + y;
+        w[e] = pack2<T>(x, y);
+      }
+      const int r = ks * 16 + (lane & 15), c0 = lane >> 4;
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) {
+        uint32_t vb[4];
+        ldmatrix4_trans(sV + short_at<D>(r, n * 2 + c0), vb);
+        mma16816<T>(o[2 * n], w, vb[0], vb[1]);
+        mma16816<T>(o[2 * n + 1], w, vb[2], vb[3]);
+      }
+    }
+    if (u + 1 < tiles) {
+      __syncthreads();
+      fetch(u + 2);
+    }
+  }
+  // ---- results through the warp's own rows of the queries' place, so that they leave in 16-byte pieces
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 1);
+    sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 2);
+    const float inv = 1.f / sum[x];
+    const int r = warp * 16 + (lane >> 2) + 8 * x, row = r0 + r;
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+      *reinterpret_cast<uint32_t*>(sm + short_at<D>(r, n) + (lane & 3) * 4) = pack2<T>(o[n][2 * x] * inv, o[n][2 * x + 1] * inv);
+    if ((lane & 3) == 0 && row < rows_end) p.lse[((long long)b * p.heads + h) * p.q_len + row] = fmaf(top[x], kLn2, logf(sum[x]));
+  }
+  __syncwarp();
+  T* const out = reinterpret_cast<T*>(p.o.data) + b * p.o.batch + h * p.o.head;
+#pragma unroll
+  for (int i = 0; i < 16 * (D / 8) / 32; ++i) {
+    const int r = warp * 16 + (i * 32 + lane) / (D / 8), piece = (i * 32 + lane) % (D / 8);
+    if (r0 + r < rows_end) *reinterpret_cast<uint4*>(out + (r0 + r) * p.o.token + piece * 8) = *reinterpret_cast<const uint4*>(sm + short_at<D>(r, piece));
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
 // Backward: one kernel for dQ (a tile of 128 queries stays, keys pass by), one for dK and dV (a tile of 128 keys stays, the
 // queries of the group's heads pass by).  Each computes the weights again from lse: two more products than one kernel that
 // adds dQ into memory with atomics would need, but every sum has a fixed order.  What passes by comes in tiles of 64 rows
@@ -1164,8 +1341,23 @@ int launch_forward(aig_ctx* ctx, WinParams& p, const CUtensorMap& mq, const CUte
 }
 
 template <class T, int D>
+int launch_short(aig_ctx* ctx, WinParams& p) {
+  using S = ShortShape<D>;
+  p.blocks = ceil_div(p.q_len, kShort);
+  const long long grid = (long long)p.blocks * p.heads * p.batch;
+  if (grid > 0x7fffffffll) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "window attention: too many rows for one call");
+  AIG_CUDA_OK(ctx, cudaFuncSetAttribute(window_short_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
+  window_short_kernel<T, D><<<(unsigned)grid, 128, S::kSmem, ctx->stream>>>(p);
+  AIG_LAUNCH_OK(ctx);
+  return AIG_OK;
+}
+
+template <class T, int D>
 int forward(aig_ctx* ctx, WinParams& p) {
   p.gerr = ctx->d_err;
+  // 128 keys of 64 or 64 of 128: at twice that the two kernels are level (1024 heads: 64 x 64 x 64 11.6 us against 31.5, 128 x 128 x 64
+  // 23 against 34, 256 x 256 x 64 in 512 heads 31 against 32; 64 x 64 x 128 21 against 36, 128 x 128 x 128 50 against 50)
+  if (p.kv_len * D <= 8192) return launch_short<T, D>(ctx, p);
   CUtensorMap mq, mk, mv;
   int rc = encode<T, D, kTile>(ctx, &mq, p.q, p.batch, p.q_len, p.heads);
   if (rc == AIG_OK) rc = encode<T, D, kTile>(ctx, &mk, p.k, p.batch, p.kv_len, p.kv_heads);
