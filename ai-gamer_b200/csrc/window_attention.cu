@@ -670,6 +670,19 @@ constexpr int kFirstPower = 100;
 
 // Shared memory is handed out to the last kilobytes at D = 128 (a tile has to be fetched two before it is needed): dynamic
 // shared memory starts on a 1024-byte boundary, which the tiles' swizzling needs.
+// A place in a ring of N stages, and the parity of its barriers' phases
+template <int N>
+struct Ring {
+  int s = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void next() {
+    if (++s == N) {
+      s = 0;
+      ph ^= 1u;
+    }
+  }
+};
+
 template <int D>
 struct DqShape {
   static constexpr int kKeys = D == 64 ? 8 : 6, kValues = D == 64 ? 6 : 4;  // stages: keys are needed for longer
@@ -702,11 +715,11 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   float* const s_sum = reinterpret_cast<float*>(sm + S::kTiles);  // [2][128]
   uint64_t* const bars = reinterpret_cast<uint64_t*>(s_sum + 256);
   const uint32_t bar0 = smem_u32(bars);
-  // of each group: scores and dP are there, they have been read; of each of four buffers: dS is there, it has been used
-  const uint32_t q_full = bar0, dq_full = bar0 + 8, sd_full = bar0 + 16, sd_free = sd_full + 16, ds_full = sd_free + 16, ds_free = ds_full + 32,
-                 k_full = ds_free + 32, k_free = k_full + 8 * NK, v_full = k_free + 8 * NK, v_free = v_full + 8 * NV, st_full = v_free + 8 * NV;
-  int* const s_power = reinterpret_cast<int*>(bars + 14 + 3 * NK + 2 * NV);  // [NK]
-  int* const s_step = s_power + NK;                                          // [NK]: its change against the tile before
+  // of each group: scores and dP are there, they have been read; of each of four buffers: dS is there
+  const uint32_t q_full = bar0, dq_full = bar0 + 8, sd_full = bar0 + 16, sd_free = sd_full + 16, ds_full = sd_free + 16, kv_full = ds_full + 32,
+                 k_free = kv_full + 8 * NK, v_free = k_free + 8 * NK, st_full = v_free + 8 * NV;
+  int* const s_power = reinterpret_cast<int*>(bars + 10 + 3 * NK + NV);  // [NK]
+  int* const s_step = s_power + NK;                                       // [NK]: its change against the tile before
   uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(s_step + NK);
   volatile int* const s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -731,19 +744,14 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
       mbar_init(sd_full + 8 * w, 1);
       mbar_init(sd_free + 8 * w, 128);
     }
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(ds_full + 8 * i, 128);
-      mbar_init(ds_free + 8 * i, 1);
-    }
+    for (int i = 0; i < 4; ++i) mbar_init(ds_full + 8 * i, 128);
     for (int s = 0; s < NK; ++s) {
-      mbar_init(k_full + 8 * s, 1);
+      mbar_init(kv_full + 8 * s, 1);
       mbar_init(k_free + 8 * s, 1);
       mbar_init(st_full + 8 * s, 1);
     }
-    for (int s = 0; s < NV; ++s) {
-      mbar_init(v_full + 8 * s, 1);
-      mbar_init(v_free + 8 * s, kScaled ? 2 : 1);  // the products are done with it, and so is the search for its largest value
-    }
+    // the products are done with it, and so is the search for its largest value
+    for (int s = 0; s < NV; ++s) mbar_init(v_free + 8 * s, kScaled ? 2 : 1);
     *s_abort = 0;
     fence_mbar_init();
   }
@@ -762,68 +770,73 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
       mbar_expect_tx(q_full, S::kFixed);
       load_tile<D, kTile, kSub>(sQ, &mapQ, q_full, h, r0, b);
       load_tile<D, kTile, kSub>(sG, &mapG, q_full, h, r0, b);
-      for (int u = 0; u < tiles; ++u) {
-        const int sk = u % NK, sv = u % NV;
-        if (u >= NK && !mbar_wait_bounded(k_free + 8 * sk, (uint32_t)(u / NK + 1) & 1u, s_abort, p.gerr, 1121)) break;
-        mbar_expect_tx(k_full + 8 * sk, S::kStage);
-        load_tile<D, kSub, kSub>(sK + sk * S::kStage, &mapK, k_full + 8 * sk, kvh, first_key(u), b);
-        if (u >= NV && !mbar_wait_bounded(v_free + 8 * sv, (uint32_t)(u / NV + 1) & 1u, s_abort, p.gerr, 1133)) break;
-        mbar_expect_tx(v_full + 8 * sv, S::kStage);
-        load_tile<D, kSub, kSub>(sV + sv * S::kStage, &mapV, v_full + 8 * sv, kvh, first_key(u), b);
+      Ring<NK> kr;
+      Ring<NV> vr;
+      for (int u = 0; u < tiles; ++u, kr.next(), vr.next()) {
+        if (u >= NK && !mbar_wait_bounded(k_free + 8 * kr.s, kr.ph ^ 1u, s_abort, p.gerr, 1121)) break;
+        mbar_expect_tx(kv_full + 8 * kr.s, 2 * S::kStage);
+        load_tile<D, kSub, kSub>(sK + kr.s * S::kStage, &mapK, kv_full + 8 * kr.s, kvh, first_key(u), b);
+        if (u >= NV && !mbar_wait_bounded(v_free + 8 * vr.s, vr.ph ^ 1u, s_abort, p.gerr, 1133)) break;
+        load_tile<D, kSub, kSub>(sV + vr.s * S::kStage, &mapV, kv_full + 8 * kr.s, kvh, first_key(u), b);
       }
     }
   } else if (warp == 1) {
     constexpr uint32_t idesc_s = idesc_for<T>(kTile, kSub, false), idesc_q = idesc_for<T>(kTile, D, true);
     const uint32_t leader = elect_one() ? 1u : 0u;
+    Ring<NK> kr, kd;  // of the next scores, of the next product with dS
+    Ring<NV> vr;
     auto scores = [&](int u) {
-      const uint32_t k = sK + (u % NK) * S::kStage, v = sV + (u % NV) * S::kStage, t = tmem + 128 * (u & 1);
-      if (!warp_wait(k_full + 8 * (u % NK), (uint32_t)(u / NK) & 1u, s_abort, p.gerr, 1122)) return false;
-      if (first_key(u) + kSub > len) clear_rows<D, kSub>(sm + (k - base), len - first_key(u), lane);
-      if (!warp_wait(v_full + 8 * (u % NV), (uint32_t)(u / NV) & 1u, s_abort, p.gerr, 1134)) return false;
+      const uint32_t k = sK + kr.s * S::kStage, v = sV + vr.s * S::kStage, t = tmem + 128 * (u & 1);
+      if (!warp_wait(kv_full + 8 * kr.s, kr.ph, s_abort, p.gerr, 1122)) return false;
+      if (u + 1 == tiles && first_key(u) + kSub > len) clear_rows<D, kSub>(sm + (k - base), len - first_key(u), lane);
       tc_fence_after();
-      {
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, t, desc_k<kTile>(sQ, ks), desc_k<kSub>(k, ks), idesc_s, ks != 0);
+      for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, t, desc_k<kTile>(sQ, ks), desc_k<kSub>(k, ks), idesc_s, ks != 0);
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, t + 64, desc_k<kTile>(sG, ks), desc_k<kSub>(v, ks), idesc_s, ks != 0);
-        commit(leader, sd_full + 8 * (u & 1));
-        commit(leader, v_free + 8 * (u % NV));
-      }
+      for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, t + 64, desc_k<kTile>(sG, ks), desc_k<kSub>(v, ks), idesc_s, ks != 0);
+      commit(leader, sd_full + 8 * (u & 1));
+      commit(leader, v_free + 8 * vr.s);
+      kr.next();
+      vr.next();
       return true;
     };
-    if (warp_wait(q_full, 0, s_abort, p.gerr, 1123) && scores(0) && (tiles < 2 || scores(1))) {
-      for (int u = 0; u < tiles + 2; ++u) {
-        if (u + 2 < tiles) {
-          if (!warp_wait(sd_free + 8 * (u & 1), (uint32_t)(u >> 1) & 1u, s_abort, p.gerr, 1124)) break;
-          if (!scores(u + 2)) break;
-        }
-        if (u < 2 || u - 2 >= tiles) continue;
-        const int x = u - 2;  // the tile that this group had before: its dS is there
-        if (!warp_wait(ds_full + 8 * (x & 3), (uint32_t)(x >> 2) & 1u, s_abort, p.gerr, 1125)) break;
-        tc_fence_after();
-        {
+    auto add = [&](int x) {  // dQ += dS K
 #pragma unroll
-          for (int ks = 0; ks < kSub / 16; ++ks)
-            mma_ts(leader, tdQ, tdS + 32 * (x & 3) + ks * 8, desc_rows<kSub>(sK + (x % NK) * S::kStage, ks), idesc_q, x != 0 || ks != 0);
-          commit(leader, ds_free + 8 * (x & 3));
-          commit(leader, k_free + 8 * (x % NK));
-          if (x + 1 == tiles) commit(leader, dq_full);
-        }
-      }
+      for (int ks = 0; ks < kSub / 16; ++ks)
+        mma_ts(leader, tdQ, tdS + 32 * (x & 3) + ks * 8, desc_rows<kSub>(sK + kd.s * S::kStage, ks), idesc_q, x != 0 || ks != 0);
+      commit(leader, k_free + 8 * kd.s);
+      kd.next();
+    };
+    bool ok = warp_wait(q_full, 0, s_abort, p.gerr, 1123) && scores(0) && (tiles < 2 || scores(1));
+    for (int u = 0; u + 2 < tiles && ok; ++u) {
+      // The group has read tile u: it has written dS of tile u - 2 before.  That product goes ahead of the next scores, so that
+      // whoever finds these knows its buffer free.
+      if (!(ok = warp_wait(sd_free + 8 * (u & 1), (uint32_t)(u >> 1) & 1u, s_abort, p.gerr, 1124))) break;
+      tc_fence_after();
+      if (u >= 2) add(u - 2);
+      ok = scores(u + 2);
     }
+    for (int x = max(tiles - 4, 0); x < tiles && ok; ++x) {
+      if (!(ok = warp_wait(ds_full + 8 * (x & 3), (uint32_t)(x >> 2) & 1u, s_abort, p.gerr, 1125))) break;
+      tc_fence_after();
+      add(x);
+    }
+    if (ok) commit(leader, dq_full);
   } else if (warp == 2) {
     if (kScaled && warp_wait(q_full, 0, s_abort, p.gerr, 1126)) {
       const int eg = tile_exponent<D, kTile>(sm + (sG - base), min(kTile, rows_end - r0), lane) + (D == 64 ? 3 : 4);
       int k = kFirstPower;
-      for (int u = 0; u < tiles; ++u) {
-        if (!warp_wait(v_full + 8 * (u % NV), (uint32_t)(u / NV) & 1u, s_abort, p.gerr, 1127)) break;
-        const int k_new = next_power(k, eg + tile_exponent<D, kSub>(sm + (sV - base) + (u % NV) * S::kStage, min(kSub, len - first_key(u)), lane));
+      Ring<NK> kr;
+      Ring<NV> vr;
+      for (int u = 0; u < tiles; ++u, kr.next(), vr.next()) {
+        if (!warp_wait(kv_full + 8 * kr.s, kr.ph, s_abort, p.gerr, 1127)) break;
+        const int k_new = next_power(k, eg + tile_exponent<D, kSub>(sm + (sV - base) + vr.s * S::kStage, min(kSub, len - first_key(u)), lane));
         __syncwarp();
         if (lane == 0) {
-          s_power[u % NK] = k_new;
-          s_step[u % NK] = u == 0 ? 0 : k_new - k;
-          mbar_arrive(st_full + 8 * (u % NK));
-          mbar_arrive(v_free + 8 * (u % NV));
+          s_power[kr.s] = k_new;
+          s_step[kr.s] = u == 0 ? 0 : k_new - k;
+          mbar_arrive(st_full + 8 * kr.s);
+          mbar_arrive(v_free + 8 * vr.s);
         }
         k = k_new;
       }
@@ -865,14 +878,16 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
       named_bar_sync(2, 256);
     }
     bool ok = true;
-    for (int u = w, n = 0; u < tiles; u += 2, ++n) {
-      const int s = u % NK, j0 = first_key(u);
+    Ring<NK> kr;
+    if (w == 1) kr.next();
+    for (int u = w, n = 0; u < tiles; u += 2, ++n, kr.next(), kr.next()) {
+      const int s = kr.s, j0 = first_key(u);
       const uint32_t t = tmem + 128 * w + lanes;
       float r = 1.f;
       int step = 0;
       ok = warp_wait(sd_full + 8 * w, (uint32_t)n & 1u, s_abort, p.gerr, 1128);
       if (kScaled && ok) {
-        ok = warp_wait(st_full + 8 * s, (uint32_t)(u / NK) & 1u, s_abort, p.gerr, 1129);
+        ok = warp_wait(st_full + 8 * s, kr.ph, s_abort, p.gerr, 1129);
         r = pow2(s_power[s]);
         step = s_step[s];
       }
@@ -919,9 +934,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
         named_bar_sync(2, 256);
         delta = s_sum[in_tile] + s_sum[128 + in_tile];
       }
-      if (u >= 4 && !(ok = warp_wait(ds_free + 8 * (u & 3), (uint32_t)(u / 4 - 1) & 1u, s_abort, p.gerr, 1130))) break;
       if (kScaled && step != 0) {  // what has been summed so far, the other group's last tile included, follows
-        if (!(ok = warp_wait(ds_free + 8 * ((u - 1) & 3), (uint32_t)((u - 1) >> 2) & 1u, s_abort, p.gerr, 1131))) break;
+        if (!(ok = warp_wait(k_free + 8 * ((u - 1) % NK), (uint32_t)((u - 1) / NK) & 1u, s_abort, p.gerr, 1131))) break;
         tc_fence_after();
         scale_row<D>(tdQ + lanes, pow2(max(step, -126)));
       }
@@ -1003,7 +1017,18 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
   const int row_last = p.window > 0 && j0 >= p.sinks ? min(rows_end - 1, j1 + p.window - 1 - off) : rows_end - 1;
   const int t_first = row_first / kSub, per_head = row_last < row_first ? 0 : row_last / kSub - t_first + 1;
   const int tiles = per_head * group;
-  auto first_row = [&](int u) { return (t_first + u % per_head) * kSub; };
+  // the tiles one after the other: those of a head, then the next head's
+  struct Walk {
+    int t, h, per_head;
+    __device__ __forceinline__ void next() {
+      if (++t == per_head) {
+        t = 0;
+        ++h;
+      }
+    }
+  };
+  const Walk start{0, kvh * group, per_head};
+  auto first_row = [&](const Walk& at) { return (t_first + at.t) * kSub; };
 
   if (tiles == 0) {  // no query sees these keys
     for (int i = threadIdx.x; i < (j1 - j0 + 1) * (D / 8); i += kBwdThreads) {
@@ -1046,40 +1071,42 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
       mbar_expect_tx(kv_full, S::kFixed);
       load_tile<D, kTile, kSub>(sK, &mapK, kv_full, kvh, j0, b);
       load_tile<D, kTile, kSub>(sV, &mapV, kv_full, kvh, j0, b);
-      for (int u = 0; u < tiles; ++u) {
-        const int s = u % NS, h = kvh * group + u / per_head;
-        if (u >= NS && !mbar_wait_bounded(q_free + 8 * s, (uint32_t)(u / NS + 1) & 1u, s_abort, p.gerr, 1141)) break;
+      Ring<NS> ring_at;
+      Walk at = start;
+      for (int u = 0; u < tiles; ++u, ring_at.next(), at.next()) {
+        const int s = ring_at.s;
+        if (u >= NS && !mbar_wait_bounded(q_free + 8 * s, ring_at.ph ^ 1u, s_abort, p.gerr, 1141)) break;
         mbar_expect_tx(q_full + 8 * s, S::kStage);
-        load_tile<D, kSub, kSub>(ring + s * S::kStage, &mapQ, q_full + 8 * s, h, first_row(u), b);
-        load_tile<D, kSub, kSub>(ring + s * S::kStage + kTileBytes<D, kSub>, &mapG, q_full + 8 * s, h, first_row(u), b);
+        load_tile<D, kSub, kSub>(ring + s * S::kStage, &mapQ, q_full + 8 * s, at.h, first_row(at), b);
+        load_tile<D, kSub, kSub>(ring + s * S::kStage + kTileBytes<D, kSub>, &mapG, q_full + 8 * s, at.h, first_row(at), b);
       }
     }
   } else if (warp == 1) {
     constexpr uint32_t idesc_s = idesc_for<T>(kTile, kSub, false), idesc_g = idesc_for<T>(kTile, D, true);
     const uint32_t leader = elect_one() ? 1u : 0u;
+    Ring<NS> rs, rp, rv, rk;  // of the next scores, dP, product for dV, product for dK
+    Walk at = start;
     auto scores = [&](int u) {
-      const int s = u % NS, row = first_row(u);
-      const uint32_t at = ring + s * S::kStage;
-      if (!warp_wait(q_full + 8 * s, (uint32_t)(u / NS) & 1u, s_abort, p.gerr, 1142)) return false;
-      if (row + kSub > rows_end) {  // rows behind the sequence's end are summed over too
-        clear_rows<D, kSub>(sm + (at - base), rows_end - row, lane);
-        clear_rows<D, kSub>(sm + (at - base) + kTileBytes<D, kSub>, rows_end - row, lane);
+      const uint32_t q = ring + rs.s * S::kStage;
+      if (!warp_wait(q_full + 8 * rs.s, rs.ph, s_abort, p.gerr, 1142)) return false;
+      if (first_row(at) + kSub > rows_end) {  // rows behind the sequence's end are summed over too
+        clear_rows<D, kSub>(sm + (q - base), rows_end - first_row(at), lane);
+        clear_rows<D, kSub>(sm + (q - base) + kTileBytes<D, kSub>, rows_end - first_row(at), lane);
       }
       tc_fence_after();
-      {
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, tmem + 128 * (u & 1), desc_k<kTile>(sK, ks), desc_k<kSub>(at, ks), idesc_s, ks != 0);
-        commit(leader, s_full + 8 * (u & 1));
-      }
+      for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, tmem + 128 * (u & 1), desc_k<kTile>(sK, ks), desc_k<kSub>(q, ks), idesc_s, ks != 0);
+      commit(leader, s_full + 8 * (u & 1));
+      rs.next();
+      at.next();
       return true;
     };
     auto dps = [&](int u) {
-      {
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
-          mma_ss(leader, tmem + 128 * (u & 1) + 64, desc_k<kTile>(sV, ks), desc_k<kSub>(ring + (u % NS) * S::kStage + kTileBytes<D, kSub>, ks), idesc_s, ks != 0);
-        commit(leader, dp_full + 8 * (u & 1));
-      }
+      for (int ks = 0; ks < D / 16; ++ks)
+        mma_ss(leader, tmem + 128 * (u & 1) + 64, desc_k<kTile>(sV, ks), desc_k<kSub>(ring + rp.s * S::kStage + kTileBytes<D, kSub>, ks), idesc_s, ks != 0);
+      commit(leader, dp_full + 8 * (u & 1));
+      rp.next();
     };
     bool ok = warp_wait(kv_full, 0, s_abort, p.gerr, 1143);
     for (int u = 0; u < 2 && u < tiles && ok; ++u) {
@@ -1090,31 +1117,29 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
       if (u < tiles) {
         if (!warp_wait(p_full + 8 * (u & 1), (uint32_t)(u >> 1) & 1u, s_abort, p.gerr, 1144)) break;
         tc_fence_after();
-        {
 #pragma unroll
-          for (int ks = 0; ks < kSub / 16; ++ks)
-            mma_ts(leader, tdV, tmem + 128 * (u & 1) + ks * 8, desc_rows<kSub>(ring + (u % NS) * S::kStage + kTileBytes<D, kSub>, ks), idesc_g, u != 0 || ks != 0);
-        }
+        for (int ks = 0; ks < kSub / 16; ++ks)
+          mma_ts(leader, tdV, tmem + 128 * (u & 1) + ks * 8, desc_rows<kSub>(ring + rv.s * S::kStage + kTileBytes<D, kSub>, ks), idesc_g, u != 0 || ks != 0);
+        rv.next();
         if (u + 2 < tiles && !scores(u + 2)) break;
       }
       if (u == 0) continue;
       const int x = u - 1;  // the other group's tile
       if (!warp_wait(ds_full + 8 * (x & 1), (uint32_t)(x >> 1) & 1u, s_abort, p.gerr, 1145)) break;
       tc_fence_after();
-      {
 #pragma unroll
-        for (int ks = 0; ks < kSub / 16; ++ks)
-          mma_ts(leader, tdK, tmem + 128 * (x & 1) + 64 + ks * 8, desc_rows<kSub>(ring + (x % NS) * S::kStage, ks), idesc_g, x != 0 || ks != 0);
-        commit(leader, q_free + 8 * (x % NS));
-        if (u == tiles) commit(leader, all_done);
-      }
+      for (int ks = 0; ks < kSub / 16; ++ks)
+        mma_ts(leader, tdK, tmem + 128 * (x & 1) + 64 + ks * 8, desc_rows<kSub>(ring + rk.s * S::kStage, ks), idesc_g, x != 0 || ks != 0);
+      commit(leader, q_free + 8 * rk.s);
+      rk.next();
+      if (u == tiles) commit(leader, all_done);
       if (x + 2 < tiles) dps(x + 2);
     }
   } else if (warp == 2) {
     // statistics of the queries, the next tile's on their way while the stage is awaited
-    auto fetch = [&](int u, float2 (&x)[2]) {
-      const int h = kvh * group + u / per_head, row = first_row(u);
-      const long long stat = ((long long)b * p.heads + h) * p.q_len + row;
+    auto fetch = [&](int u, const Walk& at, float2 (&x)[2]) {
+      const int row = first_row(at);
+      const long long stat = ((long long)b * p.heads + at.h) * p.q_len + row;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int r = lane + 32 * i;
@@ -1124,10 +1149,12 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
       }
     };
     float2 x[2];
-    fetch(0, x);
-    for (int u = 0; u < tiles; ++u) {
-      const int s = u % NS;
-      if (u >= NS && !warp_wait(q_free + 8 * s, (uint32_t)(u / NS + 1) & 1u, s_abort, p.gerr, 1147)) break;
+    Ring<NS> ring_at;
+    Walk at = start;
+    fetch(0, at, x);
+    for (int u = 0; u < tiles; ++u, ring_at.next()) {
+      const int s = ring_at.s;
+      if (u >= NS && !warp_wait(q_free + 8 * s, ring_at.ph ^ 1u, s_abort, p.gerr, 1147)) break;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         s_lse[s * kSub + lane + 32 * i] = fmaf(x[i].x, -kLog2e, (float)kWeightBits<T>);
@@ -1135,17 +1162,20 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(st_full + 8 * s);
-      fetch(u + 1, x);
+      at.next();
+      fetch(u + 1, at, x);
     }
   } else if (warp == 3) {
     // the power for dS
     if (kScaled && warp_wait(kv_full, 0, s_abort, p.gerr, 1146)) {
       const int ev = tile_exponent<D, kTile>(sm + (sV - base), min(kTile, len - j0), lane) + (D == 64 ? 3 : 4);
       int k = kFirstPower;
-      for (int u = 0; u < tiles; ++u) {
-        const int s = u % NS;
-        if (!warp_wait(q_full + 8 * s, (uint32_t)(u / NS) & 1u, s_abort, p.gerr, 1148)) break;
-        const int k_new = next_power(k, ev + tile_exponent<D, kSub>(sm + S::kFixed + s * S::kStage + kTileBytes<D, kSub>, min(kSub, rows_end - first_row(u)), lane));
+      Ring<NS> ring_at;
+      Walk at = start;
+      for (int u = 0; u < tiles; ++u, ring_at.next(), at.next()) {
+        const int s = ring_at.s;
+        if (!warp_wait(q_full + 8 * s, ring_at.ph, s_abort, p.gerr, 1148)) break;
+        const int k_new = next_power(k, ev + tile_exponent<D, kSub>(sm + S::kFixed + s * S::kStage + kTileBytes<D, kSub>, min(kSub, rows_end - first_row(at)), lane));
         if (lane == 0) {
           s_power[s] = k_new;
           s_step[s] = u == 0 ? 0 : k_new - k;
@@ -1161,13 +1191,19 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
     const float c = p.scale * kLog2e;
     const bool sink = key < p.sinks, no_ds = p.window == 1 && p.sinks == 0;
     bool ok = true;
-    for (int u = w, n = 0; u < tiles; u += 2, ++n) {
-      const int s = u % NS, first = off + first_row(u);  // position of the tile's first query
+    Ring<NS> ring_at;
+    Walk at = start;
+    if (w == 1) {
+      ring_at.next();
+      at.next();
+    }
+    for (int u = w, n = 0; u < tiles; u += 2, ++n, ring_at.next(), ring_at.next(), at.next(), at.next()) {
+      const int s = ring_at.s, first = off + first_row(at);  // position of the tile's first query
       const float4 *lse2 = reinterpret_cast<const float4*>(s_lse + s * kSub), *delta = reinterpret_cast<const float4*>(s_delta + s * kSub);
       const bool cut = j0 + kTile - 1 > first || (p.window > 0 && j0 <= first + kSub - 1 - p.window && j0 + kTile > p.sinks);
       // columns whose queries see this thread's key: from `from` on, and before `to` unless it is a sink
       const int from = key - first, to = p.window > 0 && !sink ? from + p.window : 0x7fffffff;
-      if (!(ok = warp_wait(st_full + 8 * s, (uint32_t)(u / NS) & 1u, s_abort, p.gerr, 1149))) break;
+      if (!(ok = warp_wait(st_full + 8 * s, ring_at.ph, s_abort, p.gerr, 1149))) break;
       if (!(ok = warp_wait(s_full + 8 * w, (uint32_t)n & 1u, s_abort, p.gerr, 1150))) break;
       tc_fence_after();
       uint32_t wt[2][32];
