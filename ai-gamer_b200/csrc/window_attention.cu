@@ -939,12 +939,13 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
         tc_fence_after();
         scale_row<D>(tdQ + lanes, pow2(max(step, -126)));
       }
+      const float shift = -delta * r;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         uint32_t o[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          const float2 x = mul2(mul2(pair_of(sc[i][e], sc[i][e + 1]), make_float2(r, r)), add2(pair_of(dp[i][e], dp[i][e + 1]), make_float2(-delta, -delta)));
+          const float2 x = mul2(pair_of(sc[i][e], sc[i][e + 1]), fma2(pair_of(dp[i][e], dp[i][e + 1]), make_float2(r, r), make_float2(shift, shift)));
           o[e / 2] = pack2<T>(x.x, x.y);
         }
         tmem_st_32x16(tdS + 32 * (u & 3) + lanes + 16 * i, o);
