@@ -123,6 +123,11 @@ __device__ __forceinline__ float2 pair_of(uint32_t a, uint32_t b) { return make_
 // bits 0 .. n-1
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
 constexpr uint32_t kMinusInf = 0xff800000u;
+// The roles' shares of a block's registers (by all warps of a group of four)
+template <int R>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
+template <int R>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
 // A bounded wait whose answer all lanes of the warp share
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* gerr, int code) {
   return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, gerr, code));
@@ -215,12 +220,15 @@ __device__ __forceinline__ KeyTiles key_tiles(int first, int last, int window, i
 // Forward
 template <int D, int NT>  // NT tiles of queries
 struct FwdShape {
-  static constexpr int kStages = NT == 2 ? (D == 64 ? 4 : 2) : 2;
+  static constexpr int kStages = D == 64 ? 3 : 2;
   static constexpr int kThreads = 128 + 128 * NT;
-  static constexpr int kCtasPerSm = 1;
+  static constexpr int kCtasPerSm = NT == 1 && D == 64 ? 2 : 1;
+  // registers of the warps that fetch and issue, and of those that hold a row of scores: 128 x 64 + 256 x 216 of a block's 384 x 168,
+  // 128 x 40 + 128 x 208 of its 256 x 128; one tile of heads of 128 has enough
+  static constexpr int kFewer = NT == 2 ? 64 : D == 64 ? 40 : 0, kMore = NT == 2 ? 216 : 208;
   static constexpr int kTmemCols = NT == 2 ? 512 : 256;  // scores 128 columns a tile, then outputs D columns a tile
   static constexpr uint32_t kQ = NT * kTileBytes<D, kTile>;
-  static constexpr size_t kSmem = kQ + 2 * kStages * kTileBytes<D, kTile> + 1024 + 256;
+  static constexpr size_t kSmem = kQ + 2 * kStages * kTileBytes<D, kTile> + 256;
 };
 constexpr float kLazy = 8.f;  // a row's maximum may grow by 2^8 before its sums are rescaled: weights stay below 2^8
 
@@ -230,9 +238,12 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
                       const __grid_constant__ WinParams p) {
   using S = FwdShape<D, NT>;
   constexpr int NS = S::kStages;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
-  uint8_t* const sm = smem_raw + (base - raw);
+  extern __shared__ __align__(1024) uint8_t sm[];
+  const uint32_t base = smem_u32(sm);
+  if (base & 1023u) {  // (never seen; tiles could not be fetched)
+    if (threadIdx.x == 0) note_error(p.gerr, 1100);
+    return;
+  }
   const uint32_t sQ = base, sK = sQ + S::kQ, sV = sK + NS * kTileBytes<D, kTile>;
   uint64_t* const bars = reinterpret_cast<uint64_t*>(sm + S::kQ + 2 * NS * kTileBytes<D, kTile>);
   const uint32_t bar0 = smem_u32(bars);
@@ -294,6 +305,7 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
   const uint32_t tmem = *s_tmem;
   const uint32_t tS = tmem, tO = tmem + 128 * NT;
 
+  if (S::kFewer > 0 && warp < 4) fewer_registers<S::kFewer>();
   if (warp == 0) {
     if (lane == 0) {
       mbar_expect_tx(q_full, S::kQ);
@@ -358,6 +370,7 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
       }
     }
   } else if (warp >= 4) {
+    if (S::kFewer > 0) more_registers<S::kMore>();
     const int w = (warp - 4) >> 2, q = warp & 3;
     const int row = (block * NT + w) * kTile + q * 32 + lane, pos = off + row;
     const int first = off + (block * NT + w) * kTile;  // position of the tile's first row
@@ -637,7 +650,6 @@ __global__ void __launch_bounds__(128, D == 64 ? 4 : 3) window_short_kernel(cons
 // multiples of 2^-24.  So the weights are multiplied by 2^8, and dS by a power of two 2^k that follows the largest
 // |dO| * |V| seen so far: |dS| stays below 2^15.5 whatever the values, and typical ones around 1.  Where a tile asks for a
 // smaller power the sums so far are scaled (rare: it keeps two bits in hand).
-constexpr int kBwdThreads = 384;
 constexpr int kSub = 64;
 template <class T>
 constexpr int kWeightBits = std::is_same<T, __half>::value ? 8 : 0;
@@ -683,26 +695,37 @@ struct Ring {
   }
 };
 
-template <int D>
-struct DqShape {
-  static constexpr int kKeys = D == 64 ? 8 : 6, kValues = D == 64 ? 6 : 4;  // stages: keys are needed for longer
+// G groups of 128 threads, each with a tile of its own in hand.  A CTA of two groups has an SM to itself.  Heads of 64 leave room
+// for two CTAs of one group, which hide each other's beginnings and ends too, but each is slower by itself: they are taken
+// where no CTA has more than its half SM's share of all tiles (see `balanced`).  2 x 4099 with a window of 1024, 16 heads:
+// dQ 95 us with one group, 109 with two; dK and dV, where two sinks make one CTA the longest by far, 190 and 116; 128 x 64, 8 heads:
+// 22 + 25 against 77 for both; 4096 without a window, 4 heads: 57 + 74 against 42 + 46.
+template <int D, int G>
+struct BwdShape {
+  static constexpr int kCtasPerSm = G == 1 ? 2 : 1;
+  static constexpr int kThreads = 128 + 128 * G;
+  static constexpr int kTmemCols = 256 * G;
+};
+template <int D, int G>
+struct DqShape : BwdShape<D, G> {
+  static constexpr int kKeys = D == 128 ? 6 : G == 2 ? 8 : 5, kValues = D == 64 && G == 2 ? 6 : 4;  // stages: keys are needed for longer
   static constexpr uint32_t kFixed = 2 * kTileBytes<D, kTile>, kStage = kTileBytes<D, kSub>;
   static constexpr uint32_t kTiles = kFixed + (kKeys + kValues) * kStage;
   static constexpr size_t kSmem = kTiles + 1024 + 512;
 };
-template <int D>
-struct DkvShape {
-  static constexpr int kStages = D == 64 ? 7 : 5;
+template <int D, int G>
+struct DkvShape : BwdShape<D, G> {
+  static constexpr int kStages = D == 128 ? 5 : G == 2 ? 7 : 4;
   static constexpr uint32_t kFixed = 2 * kTileBytes<D, kTile>, kStage = 2 * kTileBytes<D, kSub>;
   static constexpr uint32_t kTiles = kFixed + kStages * kStage;
   static constexpr size_t kSmem = kTiles + kStages * kSub * 8 + 384;
 };
 
-template <class T, int D>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+template <class T, int D, int G>
+__global__ void __launch_bounds__(DqShape<D, G>::kThreads, DqShape<D, G>::kCtasPerSm)
 window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
                  const __grid_constant__ CUtensorMap mapG, const __grid_constant__ WinParams p) {
-  using S = DqShape<D>;
+  using S = DqShape<D, G>;
   constexpr int NK = S::kKeys, NV = S::kValues;
   constexpr bool kScaled = std::is_same<T, __half>::value;
   extern __shared__ __align__(1024) uint8_t sm[];
@@ -715,7 +738,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   float* const s_sum = reinterpret_cast<float*>(sm + S::kTiles);  // [2][128]
   uint64_t* const bars = reinterpret_cast<uint64_t*>(s_sum + 256);
   const uint32_t bar0 = smem_u32(bars);
-  // of each group: scores and dP are there, they have been read; of each of four buffers: dS is there
+  // of each group: scores and dP are there, they have been read; of each of two buffers of a group: dS is there
   const uint32_t q_full = bar0, dq_full = bar0 + 8, sd_full = bar0 + 16, sd_free = sd_full + 16, ds_full = sd_free + 16, kv_full = ds_full + 32,
                  k_free = kv_full + 8 * NK, v_free = k_free + 8 * NK, st_full = v_free + 8 * NV;
   int* const s_power = reinterpret_cast<int*>(bars + 10 + 3 * NK + NV);  // [NK]
@@ -740,11 +763,11 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(dq_full, 1);
-    for (int w = 0; w < 2; ++w) {
+    for (int w = 0; w < G; ++w) {
       mbar_init(sd_full + 8 * w, 1);
       mbar_init(sd_free + 8 * w, 128);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(ds_full + 8 * i, 128);
+    for (int i = 0; i < 2 * G; ++i) mbar_init(ds_full + 8 * i, 128);
     for (int s = 0; s < NK; ++s) {
       mbar_init(kv_full + 8 * s, 1);
       mbar_init(k_free + 8 * s, 1);
@@ -756,14 +779,15 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(s_tmem), 512);
+    tmem_alloc(smem_u32(s_tmem), S::kTmemCols);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // of each group: 64 columns of scores, 64 of dP; then four buffers of 32 for dS; then dQ
-  const uint32_t tmem = *s_tmem, tdS = tmem + 256, tdQ = tmem + 384;
+  // of each group: 64 columns of scores, 64 of dP; then each group's two buffers of 32 for dS; then dQ
+  const uint32_t tmem = *s_tmem, tdS = tmem + 128 * G, tdQ = tmem + 192 * G;
+  if (S::kCtasPerSm == 2 && warp < 4) fewer_registers<40>();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -786,7 +810,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
     Ring<NK> kr, kd;  // of the next scores, of the next product with dS
     Ring<NV> vr;
     auto scores = [&](int u) {
-      const uint32_t k = sK + kr.s * S::kStage, v = sV + vr.s * S::kStage, t = tmem + 128 * (u & 1);
+      const uint32_t k = sK + kr.s * S::kStage, v = sV + vr.s * S::kStage, t = tmem + 128 * (u % G);
       if (!warp_wait(kv_full + 8 * kr.s, kr.ph, s_abort, p.gerr, 1122)) return false;
       if (u + 1 == tiles && first_key(u) + kSub > len) clear_rows<D, kSub>(sm + (k - base), len - first_key(u), lane);
       tc_fence_after();
@@ -794,7 +818,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
       for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, t, desc_k<kTile>(sQ, ks), desc_k<kSub>(k, ks), idesc_s, ks != 0);
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, t + 64, desc_k<kTile>(sG, ks), desc_k<kSub>(v, ks), idesc_s, ks != 0);
-      commit(leader, sd_full + 8 * (u & 1));
+      commit(leader, sd_full + 8 * (u % G));
       commit(leader, v_free + 8 * vr.s);
       kr.next();
       vr.next();
@@ -803,21 +827,22 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
     auto add = [&](int x) {  // dQ += dS K
 #pragma unroll
       for (int ks = 0; ks < kSub / 16; ++ks)
-        mma_ts(leader, tdQ, tdS + 32 * (x & 3) + ks * 8, desc_rows<kSub>(sK + kd.s * S::kStage, ks), idesc_q, x != 0 || ks != 0);
+        mma_ts(leader, tdQ, tdS + 32 * (x % (2 * G)) + ks * 8, desc_rows<kSub>(sK + kd.s * S::kStage, ks), idesc_q, x != 0 || ks != 0);
       commit(leader, k_free + 8 * kd.s);
       kd.next();
     };
-    bool ok = warp_wait(q_full, 0, s_abort, p.gerr, 1123) && scores(0) && (tiles < 2 || scores(1));
-    for (int u = 0; u + 2 < tiles && ok; ++u) {
-      // The group has read tile u: it has written dS of tile u - 2 before.  That product goes ahead of the next scores, so that
+    bool ok = warp_wait(q_full, 0, s_abort, p.gerr, 1123);
+    for (int u = 0; u < G && u < tiles && ok; ++u) ok = scores(u);
+    for (int u = 0; u + G < tiles && ok; ++u) {
+      // The group has read tile u: it has written dS of its tile before.  That product goes ahead of the next scores, so that
       // whoever finds these knows its buffer free.
-      if (!(ok = warp_wait(sd_free + 8 * (u & 1), (uint32_t)(u >> 1) & 1u, s_abort, p.gerr, 1124))) break;
+      if (!(ok = warp_wait(sd_free + 8 * (u % G), (uint32_t)(u / G) & 1u, s_abort, p.gerr, 1124))) break;
       tc_fence_after();
-      if (u >= 2) add(u - 2);
-      ok = scores(u + 2);
+      if (u >= G) add(u - G);
+      ok = scores(u + G);
     }
-    for (int x = max(tiles - 4, 0); x < tiles && ok; ++x) {
-      if (!(ok = warp_wait(ds_full + 8 * (x & 3), (uint32_t)(x >> 2) & 1u, s_abort, p.gerr, 1125))) break;
+    for (int x = max(tiles - 2 * G, 0); x < tiles && ok; ++x) {
+      if (!(ok = warp_wait(ds_full + 8 * (x % (2 * G)), (uint32_t)(x / (2 * G)) & 1u, s_abort, p.gerr, 1125))) break;
       tc_fence_after();
       add(x);
     }
@@ -842,6 +867,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
       }
     }
   } else if (warp >= 4) {
+    if (S::kCtasPerSm == 2) more_registers<208>();
     const int w = (warp - 4) >> 2, q = warp & 3, in_tile = q * 32 + lane;
     const int row = r0 + in_tile, pos = off + row;
     const bool there = row < rows_end;
@@ -851,36 +877,34 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
     const float lse2 = there ? p.lse[stat] * kLog2e : INFINITY;  // (weights of 0)
     // a query that sees one key has the weight 1 whatever its score: no gradient through it
     const bool single = pos == 0 || (p.window == 1 && p.sinks == 0);
+    // D = dO . O has the output's rounding in it.  Where a row sees a few keys, that is large against dP: a row that sees only the
+    // first tile's takes the sum over its weights instead, below.
+    const bool few = first_key(0) + kSub > off + r0, mine_few = first_key(0) + kSub > pos;
+    constexpr int kShare = D / G;  // a row's dot product and its result are shared by the groups
     float delta = 0.f;
-    if (tiles > 2) {
-      // (dO . O has the output's rounding in it; with two tiles' keys or fewer, where that is large against dP, the sum over
-      // the weights is taken instead, below)
-      float d = 0.f;
-      if (there) {
-        const T* g = reinterpret_cast<const T*>(p.dout.data) + b * p.dout.batch + row * p.dout.token + h * p.dout.head + w * (D / 2);
-        const T* o = reinterpret_cast<const T*>(p.o.data) + b * p.o.batch + row * p.o.token + h * p.o.head + w * (D / 2);
+    if (there) {
+      const T* g = reinterpret_cast<const T*>(p.dout.data) + b * p.dout.batch + row * p.dout.token + h * p.dout.head + w * kShare;
+      const T* o = reinterpret_cast<const T*>(p.o.data) + b * p.o.batch + row * p.o.token + h * p.o.head + w * kShare;
 #pragma unroll
-        for (int i = 0; i < D / 2; i += 8) {
-          const uint4 x = *reinterpret_cast<const uint4*>(g + i), y = *reinterpret_cast<const uint4*>(o + i);
-          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+      for (int i = 0; i < kShare; i += 8) {
+        const uint4 x = *reinterpret_cast<const uint4*>(g + i), y = *reinterpret_cast<const uint4*>(o + i);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 a = unpack2<T>(xs[e]), z = unpack2<T>(ys[e]);
-            d = fmaf(a.x, z.x, fmaf(a.y, z.y, d));
-          }
+        for (int e = 0; e < 4; ++e) {
+          const float2 a = unpack2<T>(xs[e]), z = unpack2<T>(ys[e]);
+          delta = fmaf(a.x, z.x, fmaf(a.y, z.y, delta));
         }
       }
-      s_sum[w * 128 + in_tile] = d;
+    }
+    if (G == 2) {
+      s_sum[w * 128 + in_tile] = delta;
       named_bar_sync(2, 256);
       delta = s_sum[in_tile] + s_sum[128 + in_tile];
-    } else if (w >= tiles) {
-      s_sum[w * 128 + in_tile] = 0.f;
-      named_bar_sync(2, 256);
     }
     bool ok = true;
     Ring<NK> kr;
     if (w == 1) kr.next();
-    for (int u = w, n = 0; u < tiles; u += 2, ++n, kr.next(), kr.next()) {
+    for (int u = w, n = 0; u < tiles; u += G, ++n) {
       const int s = kr.s, j0 = first_key(u);
       const uint32_t t = tmem + 128 * w + lanes;
       float r = 1.f;
@@ -891,10 +915,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
         r = pow2(s_power[s]);
         step = s_step[s];
       }
-      if (!ok) {
-        if (tiles <= 2) named_bar_sync(2, 256);  // (the other group may be waiting below)
-        break;
-      }
+      if (!ok) break;
       tc_fence_after();
       uint32_t sc[2][32], dp[2][32];
       tmem_ld_32x32(t, sc[0]);
@@ -918,7 +939,6 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
           }
         }
       }
-      float2 own = make_float2(0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -927,12 +947,14 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
           const float2 y = make_float2(ex2(x.x), ex2(x.y));
           sc[i][e] = __float_as_uint(y.x);
           sc[i][e + 1] = __float_as_uint(y.y);
-          if (tiles <= 2) own = fma2(y, pair_of(dp[i][e], dp[i][e + 1]), own);
         }
-      if (tiles <= 2) {
-        s_sum[w * 128 + in_tile] = own.x + own.y;
-        named_bar_sync(2, 256);
-        delta = s_sum[in_tile] + s_sum[128 + in_tile];
+      if (few && u == 0) {
+        float2 own = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) own = fma2(pair_of(sc[i][e], sc[i][e + 1]), pair_of(dp[i][e], dp[i][e + 1]), own);
+        if (mine_few) delta = own.x + own.y;
       }
       if (kScaled && step != 0) {  // what has been summed so far, the other group's last tile included, follows
         if (!(ok = warp_wait(k_free + 8 * ((u - 1) % NK), (uint32_t)((u - 1) / NK) & 1u, s_abort, p.gerr, 1131))) break;
@@ -948,19 +970,20 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
           const float2 x = mul2(pair_of(sc[i][e], sc[i][e + 1]), fma2(pair_of(dp[i][e], dp[i][e + 1]), make_float2(r, r), make_float2(shift, shift)));
           o[e / 2] = pack2<T>(x.x, x.y);
         }
-        tmem_st_32x16(tdS + 32 * (u & 3) + lanes + 16 * i, o);
+        tmem_st_32x16(tdS + 32 * (u % (2 * G)) + lanes + 16 * i, o);
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(ds_full + 8 * (u & 3));
+      mbar_arrive(ds_full + 8 * (u % (2 * G)));
+      for (int i = 0; i < G; ++i) kr.next();
     }
     if (ok && warp_wait(dq_full, 0, s_abort, p.gerr, 1132)) {
       tc_fence_after();
       if (there && w == 0) p.delta[stat] = delta;
       float f = p.scale;
       if (kScaled) f *= pow2(-s_power[(tiles - 1) % NK]);
-      T* const out = reinterpret_cast<T*>(p.dq.data) + b * p.dq.batch + row * p.dq.token + h * p.dq.head + w * (D / 2);
-      store_row<T, D / 2>(tdQ + lanes + w * (D / 2), out, f, there);
+      T* const out = reinterpret_cast<T*>(p.dq.data) + b * p.dq.batch + row * p.dq.token + h * p.dq.head + w * kShare;
+      store_row<T, kShare>(tdQ + lanes + w * kShare, out, f, there);
     }
   }
 
@@ -971,15 +994,15 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, S::kTmemCols);
   }
 }
 
-template <class T, int D>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+template <class T, int D, int G>
+__global__ void __launch_bounds__(DkvShape<D, G>::kThreads, DkvShape<D, G>::kCtasPerSm)
 window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
                   const __grid_constant__ CUtensorMap mapG, const __grid_constant__ WinParams p) {
-  using S = DkvShape<D>;
+  using S = DkvShape<D, G>;
   constexpr int NS = S::kStages;
   constexpr bool kScaled = std::is_same<T, __half>::value;
   extern __shared__ __align__(1024) uint8_t sm[];
@@ -1032,7 +1055,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
   auto first_row = [&](const Walk& at) { return (t_first + at.t) * kSub; };
 
   if (tiles == 0) {  // no query sees these keys
-    for (int i = threadIdx.x; i < (j1 - j0 + 1) * (D / 8); i += kBwdThreads) {
+    for (int i = threadIdx.x; i < (j1 - j0 + 1) * (D / 8); i += S::kThreads) {
       const int j = j0 + i / (D / 8), c = i % (D / 8) * 8;
       *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.dk.data) + b * p.dk.batch + j * p.dk.token + kvh * p.dk.head + c) = make_uint4(0, 0, 0, 0);
       *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.dv.data) + b * p.dv.batch + j * p.dv.token + kvh * p.dv.head + c) = make_uint4(0, 0, 0, 0);
@@ -1043,7 +1066,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
     mbar_init(all_done, 1);
-    for (int w = 0; w < 2; ++w) {
+    for (int w = 0; w < G; ++w) {
       mbar_init(s_full + 8 * w, 1);
       mbar_init(p_full + 8 * w, 128);
       mbar_init(dp_full + 8 * w, 1);
@@ -1058,14 +1081,15 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(s_tmem), 512);
+    tmem_alloc(smem_u32(s_tmem), S::kTmemCols);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   // of each group: 64 columns of scores, then weights, 64 of dP, then dS; then dV and dK
-  const uint32_t tmem = *s_tmem, tdV = tmem + 256, tdK = tmem + 256 + D;
+  const uint32_t tmem = *s_tmem, tdV = tmem + 128 * G, tdK = tdV + D;
+  if (S::kCtasPerSm == 2 && warp < 4) fewer_registers<40>();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -1096,8 +1120,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
       }
       tc_fence_after();
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, tmem + 128 * (u & 1), desc_k<kTile>(sK, ks), desc_k<kSub>(q, ks), idesc_s, ks != 0);
-      commit(leader, s_full + 8 * (u & 1));
+      for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, tmem + 128 * (u % G), desc_k<kTile>(sK, ks), desc_k<kSub>(q, ks), idesc_s, ks != 0);
+      commit(leader, s_full + 8 * (u % G));
       rs.next();
       at.next();
       return true;
@@ -1105,36 +1129,37 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
     auto dps = [&](int u) {
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks)
-        mma_ss(leader, tmem + 128 * (u & 1) + 64, desc_k<kTile>(sV, ks), desc_k<kSub>(ring + rp.s * S::kStage + kTileBytes<D, kSub>, ks), idesc_s, ks != 0);
-      commit(leader, dp_full + 8 * (u & 1));
+        mma_ss(leader, tmem + 128 * (u % G) + 64, desc_k<kTile>(sV, ks), desc_k<kSub>(ring + rp.s * S::kStage + kTileBytes<D, kSub>, ks), idesc_s, ks != 0);
+      commit(leader, dp_full + 8 * (u % G));
       rp.next();
     };
     bool ok = warp_wait(kv_full, 0, s_abort, p.gerr, 1143);
-    for (int u = 0; u < 2 && u < tiles && ok; ++u) {
+    for (int u = 0; u < G && u < tiles && ok; ++u) {
       ok = scores(u);
       if (ok) dps(u);
     }
-    for (int u = 0; u <= tiles && ok; ++u) {
+    // a tile's weights, then the dS of the tile before (of the other group, where there are two)
+    for (int u = 0; u < tiles + G - 1 && ok; ++u) {
       if (u < tiles) {
-        if (!warp_wait(p_full + 8 * (u & 1), (uint32_t)(u >> 1) & 1u, s_abort, p.gerr, 1144)) break;
+        if (!warp_wait(p_full + 8 * (u % G), (uint32_t)(u / G) & 1u, s_abort, p.gerr, 1144)) break;
         tc_fence_after();
 #pragma unroll
         for (int ks = 0; ks < kSub / 16; ++ks)
-          mma_ts(leader, tdV, tmem + 128 * (u & 1) + ks * 8, desc_rows<kSub>(ring + rv.s * S::kStage + kTileBytes<D, kSub>, ks), idesc_g, u != 0 || ks != 0);
+          mma_ts(leader, tdV, tmem + 128 * (u % G) + ks * 8, desc_rows<kSub>(ring + rv.s * S::kStage + kTileBytes<D, kSub>, ks), idesc_g, u != 0 || ks != 0);
         rv.next();
-        if (u + 2 < tiles && !scores(u + 2)) break;
+        if (u + G < tiles && !scores(u + G)) break;
       }
-      if (u == 0) continue;
-      const int x = u - 1;  // the other group's tile
-      if (!warp_wait(ds_full + 8 * (x & 1), (uint32_t)(x >> 1) & 1u, s_abort, p.gerr, 1145)) break;
+      const int x = u - (G - 1);
+      if (x < 0) continue;
+      if (!warp_wait(ds_full + 8 * (x % G), (uint32_t)(x / G) & 1u, s_abort, p.gerr, 1145)) break;
       tc_fence_after();
 #pragma unroll
       for (int ks = 0; ks < kSub / 16; ++ks)
-        mma_ts(leader, tdK, tmem + 128 * (x & 1) + 64 + ks * 8, desc_rows<kSub>(ring + rk.s * S::kStage, ks), idesc_g, x != 0 || ks != 0);
+        mma_ts(leader, tdK, tmem + 128 * (x % G) + 64 + ks * 8, desc_rows<kSub>(ring + rk.s * S::kStage, ks), idesc_g, x != 0 || ks != 0);
       commit(leader, q_free + 8 * rk.s);
       rk.next();
-      if (u == tiles) commit(leader, all_done);
-      if (x + 2 < tiles) dps(x + 2);
+      if (x + 1 == tiles) commit(leader, all_done);
+      if (x + G < tiles) dps(x + G);
     }
   } else if (warp == 2) {
     // statistics of the queries, the next tile's on their way while the stage is awaited
@@ -1186,6 +1211,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
       }
     }
   } else {
+    if (S::kCtasPerSm == 2) more_registers<208>();
     const int w = (warp - 4) >> 2, q = warp & 3, in_tile = q * 32 + lane;
     const int key = j0 + in_tile;
     const uint32_t lanes = (uint32_t)(q * 32) << 16, t = tmem + 128 * w + lanes;
@@ -1198,7 +1224,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
       ring_at.next();
       at.next();
     }
-    for (int u = w, n = 0; u < tiles; u += 2, ++n, ring_at.next(), ring_at.next(), at.next(), at.next()) {
+    for (int u = w, n = 0; u < tiles; u += G, ++n) {
       const int s = ring_at.s, first = off + first_row(at);  // position of the tile's first query
       const float4 *lse2 = reinterpret_cast<const float4*>(s_lse + s * kSub), *delta = reinterpret_cast<const float4*>(s_delta + s * kSub);
       const bool cut = j0 + kTile - 1 > first || (p.window > 0 && j0 <= first + kSub - 1 - p.window && j0 + kTile > p.sinks);
@@ -1285,15 +1311,20 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(ds_full + 8 * w);
+      for (int i = 0; i < G; ++i) {
+        ring_at.next();
+        at.next();
+      }
     }
     if (ok && warp_wait(all_done, 0, s_abort, p.gerr, 1153)) {
       tc_fence_after();
       float f = p.scale;
       if (kScaled) f *= pow2(-s_power[(tiles - 1) % NS]);
-      T* const dk = reinterpret_cast<T*>(p.dk.data) + b * p.dk.batch + key * p.dk.token + kvh * p.dk.head + w * (D / 2);
-      T* const dv = reinterpret_cast<T*>(p.dv.data) + b * p.dv.batch + key * p.dv.token + kvh * p.dv.head + w * (D / 2);
-      store_row<T, D / 2>(tdV + lanes + w * (D / 2), dv, pow2(-kWeightBits<T>), key < len);
-      store_row<T, D / 2>(tdK + lanes + w * (D / 2), dk, f, key < len);
+      constexpr int kShare = D / G;
+      T* const dk = reinterpret_cast<T*>(p.dk.data) + b * p.dk.batch + key * p.dk.token + kvh * p.dk.head + w * kShare;
+      T* const dv = reinterpret_cast<T*>(p.dv.data) + b * p.dv.batch + key * p.dv.token + kvh * p.dv.head + w * kShare;
+      store_row<T, kShare>(tdV + lanes + w * kShare, dv, pow2(-kWeightBits<T>), key < len);
+      store_row<T, kShare>(tdK + lanes + w * kShare, dk, f, key < len);
     }
   }
 
@@ -1304,7 +1335,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, S::kTmemCols);
   }
 }
 
@@ -1400,8 +1431,28 @@ int forward(aig_ctx* ctx, WinParams& p) {
   if (rc == AIG_OK) rc = encode<T, D, kTile>(ctx, &mk, p.k, p.batch, p.kv_len, p.kv_heads);
   if (rc == AIG_OK) rc = encode<T, D, kTile>(ctx, &mv, p.v, p.batch, p.kv_len, p.kv_heads);
   if (rc != AIG_OK) return rc;
-  return p.q_len <= kTile ? launch_forward<T, D, 1>(ctx, p, mq, mk, mv) : launch_forward<T, D, 2>(ctx, p, mq, mk, mv);
+  // Heads of 64 leave room for two CTAs with a tile of queries each on an SM, which hide each other's beginnings and ends (2 x 4099,
+  // 16 heads: 71 us; one CTA with two tiles 77); heads of 128 for one, whose two tiles share the keys they fetch.
+  if (D == 64 || p.q_len <= kTile) return launch_forward<T, D, 1>(ctx, p, mq, mk, mv);
+  if constexpr (D == 128) return launch_forward<T, D, 2>(ctx, p, mq, mk, mv);
 }
+template <class T, int D, int G>
+int launch_dq(aig_ctx* ctx, const WinParams& p, unsigned grid, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mg) {
+  using S = DqShape<D, G>;
+  AIG_CUDA_OK(ctx, cudaFuncSetAttribute(window_dq_kernel<T, D, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
+  window_dq_kernel<T, D, G><<<grid, S::kThreads, S::kSmem, ctx->stream>>>(mq, mk, mv, mg, p);
+  AIG_LAUNCH_OK(ctx);
+  return AIG_OK;
+}
+template <class T, int D, int G>
+int launch_dkv(aig_ctx* ctx, const WinParams& p, unsigned grid, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mg) {
+  using S = DkvShape<D, G>;
+  AIG_CUDA_OK(ctx, cudaFuncSetAttribute(window_dkv_kernel<T, D, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
+  window_dkv_kernel<T, D, G><<<grid, S::kThreads, S::kSmem, ctx->stream>>>(mq, mk, mv, mg, p);
+  AIG_LAUNCH_OK(ctx);
+  return AIG_OK;
+}
+
 template <class T, int D>
 int backward(aig_ctx* ctx, WinParams& p) {
   p.gerr = ctx->d_err;
@@ -1412,15 +1463,23 @@ int backward(aig_ctx* ctx, WinParams& p) {
   if (rc == AIG_OK) rc = encode<T, D, kSub>(ctx, &mg, p.dout, p.batch, p.q_len, p.heads);
   if (rc != AIG_OK) return rc;
   p.blocks = ceil_div(p.q_len, kTile);
-  const long long grid = (long long)p.blocks * p.heads * p.batch, grid_kv = (long long)ceil_div(p.kv_len, kTile) * p.kv_heads * p.batch;
+  const int blocks_kv = ceil_div(p.kv_len, kTile);
+  const long long grid = (long long)p.blocks * p.heads * p.batch, grid_kv = (long long)blocks_kv * p.kv_heads * p.batch;
   if (grid > 0x7fffffffll || grid_kv > 0x7fffffffll) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "window attention backward: too many rows for one call");
-  AIG_CUDA_OK(ctx, cudaFuncSetAttribute(window_dq_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DqShape<D>::kSmem));
-  AIG_CUDA_OK(ctx, cudaFuncSetAttribute(window_dkv_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DkvShape<D>::kSmem));
-  window_dq_kernel<T, D><<<(unsigned)grid, kBwdThreads, DqShape<D>::kSmem, ctx->stream>>>(mq, mk, mv, mg, p);
-  AIG_LAUNCH_OK(ctx);
-  window_dkv_kernel<T, D><<<(unsigned)grid_kv, kBwdThreads, DkvShape<D>::kSmem, ctx->stream>>>(mq, mk, mv, mg, p);
-  AIG_LAUNCH_OK(ctx);
-  return AIG_OK;
+  if constexpr (D == 64) {
+    // tiles of 64 that pass by: of all CTAs together, of the longest for dQ and for dK and dV (a sink is seen by every query)
+    const double seen = p.window > 0 ? p.window + kTile : p.kv_len - 0.5 * p.q_len;
+    const double all = seen / kSub * grid;
+    const double longest = (p.window > 0 ? p.window + p.sinks + kTile : p.kv_len) / (double)kSub;
+    const double longest_kv = (p.window > 0 && p.sinks == 0 && p.window + kTile < p.q_len ? p.window + kTile : p.q_len) / (double)kSub * (p.heads / p.kv_heads);
+    auto balanced = [&](double most) { return most * 2 * ctx->sm_count <= all; };
+    rc = balanced(longest) ? launch_dq<T, D, 1>(ctx, p, (unsigned)grid, mq, mk, mv, mg) : launch_dq<T, D, 2>(ctx, p, (unsigned)grid, mq, mk, mv, mg);
+    if (rc != AIG_OK) return rc;
+    return balanced(longest_kv) ? launch_dkv<T, D, 1>(ctx, p, (unsigned)grid_kv, mq, mk, mv, mg) : launch_dkv<T, D, 2>(ctx, p, (unsigned)grid_kv, mq, mk, mv, mg);
+  } else {
+    rc = launch_dq<T, D, 2>(ctx, p, (unsigned)grid, mq, mk, mv, mg);
+    return rc != AIG_OK ? rc : launch_dkv<T, D, 2>(ctx, p, (unsigned)grid_kv, mq, mk, mv, mg);
+  }
 }
 
 }  // namespace
