@@ -1339,8 +1339,9 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
   }
 }
 
-bool tensor_ok(const aig_seq_heads* t) {
-  return t && t->data && aligned_to(t->data, 16) && t->batch_stride >= 0 && t->token_stride >= 0 && t->head_stride >= 0 && t->batch_stride % 8 == 0 &&
+// (a stride of 0 over a dimension above 1 is refused: TMA has none)
+bool tensor_ok(const aig_seq_heads* t, int batch, int tokens, int heads) {
+  return t && t->data && (t->batch_stride > 0 || batch == 1) && (t->token_stride > 0 || tokens == 1) && (t->head_stride > 0 || heads == 1) && aligned_to(t->data, 16) && t->batch_stride >= 0 && t->token_stride >= 0 && t->head_stride >= 0 && t->batch_stride % 8 == 0 &&
          t->token_stride % 8 == 0 && t->head_stride % 8 == 0;
 }
 View view_of(const aig_seq_heads* t) { return View{(uint8_t*)t->data, t->batch_stride, t->token_stride, t->head_stride}; }
@@ -1493,8 +1494,9 @@ int aig_window_attention_forward(aig_ctx* ctx, const aig_window_desc* d, const a
   const int rc = check_desc(ctx, d, "window attention");
   if (rc != AIG_OK) return rc;
   if (d->batch == 0 || d->q_len == 0) return AIG_OK;
-  AIG_REQUIRE(ctx, tensor_ok(q) && tensor_ok(k) && tensor_ok(v) && tensor_ok(out) && lse,
-              "window attention: null tensor, data off a 16-byte boundary, or strides that are negative or no multiples of 8");
+  const int b = d->batch, tq = d->q_len, tk = d->kv_len, h = d->heads, hk = d->kv_heads;
+  AIG_REQUIRE(ctx, tensor_ok(q, b, tq, h) && tensor_ok(k, b, tk, hk) && tensor_ok(v, b, tk, hk) && tensor_ok(out, b, tq, h) && lse && aligned_to(lse, 4),
+              "window attention: null tensor, data off a 16-byte boundary, or strides that are not positive multiples of 8");
   WinParams p = params_of(d);
   p.q = view_of(q);
   p.k = view_of(k);
@@ -1514,10 +1516,11 @@ int aig_window_attention_backward(aig_ctx* ctx, const aig_window_desc* d, const 
   const int rc = check_desc(ctx, d, "window attention backward");
   if (rc != AIG_OK) return rc;
   if (d->batch == 0 || d->kv_len == 0) return AIG_OK;
-  AIG_REQUIRE(ctx, tensor_ok(q) && tensor_ok(k) && tensor_ok(v) && tensor_ok(out) && tensor_ok(dout) && tensor_ok(dq) && tensor_ok(dk) && tensor_ok(dv) &&
-                       lse && delta,
-              "window attention backward: null tensor, data off a 16-byte boundary, or strides that are negative or no multiples of 8");
-  AIG_REQUIRE(ctx, d->q_len > 0, "window attention backward: no queries");
+  const int b = d->batch, tq = d->q_len, tk = d->kv_len, h = d->heads, hk = d->kv_heads;
+  AIG_REQUIRE(ctx, tq > 0, "window attention backward: no queries");
+  AIG_REQUIRE(ctx, tensor_ok(q, b, tq, h) && tensor_ok(k, b, tk, hk) && tensor_ok(v, b, tk, hk) && tensor_ok(out, b, tq, h) && tensor_ok(dout, b, tq, h) &&
+                       tensor_ok(dq, b, tq, h) && tensor_ok(dk, b, tk, hk) && tensor_ok(dv, b, tk, hk) && lse && delta && aligned_to(lse, 4) && aligned_to(delta, 4),
+              "window attention backward: null tensor, data off a 16-byte boundary, or strides that are not positive multiples of 8");
   WinParams p = params_of(d);
   p.q = view_of(q);
   p.k = view_of(k);

@@ -92,3 +92,244 @@ def test_forward_and_gradients(env, kind, d, B, Tq, Tk, H, KV, window, sinks, le
     check((out, lse), want, bound, ("out", "lse"))
     grads = run_backward(env, q, k, v, out, lse, g, window, sinks, lengths)
     check(grads, want, bound, ("dq", "dk", "dv"))
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_rows_behind_the_end_may_hold_anything(env, kind, d):
+    """Padding of q, k, v, out's gradient and the statistics: NaN and infinities there reach no row that is there."""
+    import math
+
+    import torch
+
+    dtype = {"f16": torch.float16, "bf16": torch.bfloat16}[kind]
+    for Tq, Tk, lengths, window, sinks in ((64, 64, [64, 1, 33], 0, 0), (300, 300, [300, 65, 200], 70, 2), (150, 400, [400, 251, 390], 0, 0)):
+        q, k, v, g = tensors(3, dtype, 3, Tq, Tk, 4, 2, d)
+        want, bound = R.window_attention(q, k, v, window, sinks, lengths, d ** -0.5, g)
+        for b, n in enumerate(lengths):
+            rows = max(0, n - (Tk - Tq))
+            q[b, rows:], g[b, rows:], k[b, n:], v[b, n:] = math.nan, math.inf, math.nan, -math.inf
+        out, lse = run_forward(env, q, k, v, window, sinks, lengths)
+        check((out, lse), want, bound, ("out", "lse"))
+        lse[lse == MARK] = math.nan
+        out[out == MARK] = math.nan
+        grads = run_backward(env, q, k, v, out, lse, g, window, sinks, lengths)
+        check(grads, want, bound, ("dq", "dk", "dv"))
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_layouts(env, d):
+    """Columns of a fused projection, heads outside of tokens, a batch with gaps; results into strided tensors too."""
+    import torch
+
+    B, T, H, KV = 2, 150, 4, 2
+    q, k, v, g = tensors(5, torch.bfloat16, B, T, T, H, KV, d)
+    want, bound = R.window_attention(q, k, v, 40, 1, None, d ** -0.5, g)
+
+    def fused(*parts):
+        row = torch.cat(parts, 2).contiguous()
+        out, at = [], 0
+        for x in parts:
+            out.append(row[:, :, at:at + x.shape[2]])
+            at += x.shape[2]
+        return out
+
+    heads_first = lambda *parts: [x.transpose(1, 2).contiguous().transpose(1, 2) for x in parts]  # noqa: E731
+    gaps = lambda *parts: [torch.stack((x, x), 1)[:, 0] for x in parts]  # noqa: E731
+    wa = env.pkg().WindowAttention(env.ctx(), 40, 1)
+    for arrange in (fused, heads_first, gaps):
+        a, b, c = arrange(q, k, v)
+        o, da, e = arrange(torch.full_like(q, MARK), torch.full_like(q, MARK), g)
+        dk, dv = arrange(torch.full_like(k, MARK), torch.full_like(k, MARK))
+        lse, delta = torch.empty((B, H, T), device="cuda"), torch.empty((B, H, T), device="cuda")
+        wa.forward(a, b, c, o, lse)
+        wa.backward(a, b, c, o, lse, e, da, dk, dv, delta)
+        env.ctx().sync()
+        check((o, lse, da, dk, dv), want, bound, ("out", "lse", "dq", "dk", "dv"))
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("T", [1, 60, 300, 700])
+def test_one_visible_key_has_no_gradient(env, T, d):
+    """A window of one key: the weight is 1 whatever the score, dq and dk are zero exactly, dv is the gradient of the output."""
+    import torch
+
+    q, k, v, g = tensors(6, torch.float16, 1, T, T, 2, 2, d)
+    out, lse = run_forward(env, q, k, v, window=1)
+    assert torch.equal(out, v)
+    dq, dk, dv = run_backward(env, q, k, v, out, lse, g, window=1)
+    assert not dq.any() and not dk.any() and torch.equal(dv, g)
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("grow", [False, True])
+@pytest.mark.parametrize("scale", [2.0 ** -18, 2.0 ** -9, 1.0, 2.0 ** 7])
+def test_fp16_gradients_of_any_size(env, scale, grow, d):
+    """Gradients from 4e-6 to 500, even or growing (and shrinking) a thousandfold along the sequence, values likewise: what a plain
+    16-bit dS would lose to its smallest steps or its largest value.  The bound leaves out both."""
+    import torch
+
+    T = 900
+    q, k, v, g = tensors(7, torch.float16, 1, T, T, 2, 1, d)
+    slope = torch.logspace(-1.5, 1.5, T, device="cuda")[None, :, None, None] if grow else 1.0
+    g = (g.float() * slope * scale).half()
+    v = (v.float() * (slope.flip(1) if grow else 1.0)).half()
+    want, bound = R.window_attention(q, k, v, 0, 0, None, d ** -0.5, g)
+    out, lse = run_forward(env, q, k, v)
+    dq, dk, dv = run_backward(env, q, k, v, out, lse, g)
+    u = 2.0 ** -11
+    for name, x, other in (("dq", dq, k), ("dk", dk, q), ("dv", dv, g)):
+        # in the 2-norm: each weight or dS off by a rounding of its own, D by that of the output; the result by its own and by fp16's smallest step
+        off, size = (x.double() - want[name]).norm(), want[name].norm()
+        assert off <= 4 * u * size + 2.0 ** -25 * x.numel() ** 0.5, (name, float(off / size))
+
+
+@gpu
+def test_gradients_against_differences(env):
+    """The derivative of sum(w * out) along a direction, by central differences of the 64-bit form, is what the gradients say."""
+    import torch
+
+    B, T, H, KV, d = 1, 90, 4, 2, 64
+    q, k, v, w = tensors(8, torch.float16, B, T, T, H, KV, d)
+    out, lse = run_forward(env, q, k, v, 30, 2)
+    grads = run_backward(env, q, k, v, out, lse, w, 30, 2)
+    g = torch.Generator("cuda").manual_seed(9)
+    for x, dx in zip((q, k, v), grads):
+        way = torch.randn(x.shape, device="cuda", generator=g, dtype=torch.float64)
+
+        def value(step):
+            moved = [t.double() + (step * way if t is x else 0) for t in (q, k, v)]
+            s = torch.einsum("bqkgd,btkd->bkgqt", moved[0].view(B, T, KV, H // KV, d), moved[1]) * d ** -0.5
+            seen = R.visible(T, T, 30, 2, T, "cuda")
+            p = torch.softmax(s.masked_fill(~seen, -float("inf")), -1)
+            return (torch.einsum("bkgqt,btkd->bqkgd", p, moved[2]).reshape(B, T, H, d) * w.double()).sum()
+
+        h = 1e-4
+        slope = (value(h) - value(-h)) / (2 * h)  # off by h^2 times a third derivative of order 1 a term
+        said = (dx.double() * way).sum()
+        size = (dx.double().abs() * way.abs()).sum()
+        assert abs(slope - said) <= 4 * 2.0 ** -11 * size
+
+
+@gpu
+@pytest.mark.parametrize("T,d", [(64, 64), (700, 64), (700, 128)])
+def test_same_bits_every_time(env, T, d):
+    import torch
+
+    q, k, v, g = tensors(10, torch.float16, 3, T, T, 4, 2, d)
+    first = None
+    for _ in range(3):
+        out, lse = run_forward(env, q, k, v, 100, 1)
+        got = (out, lse) + run_backward(env, q, k, v, out, lse, g, 100, 1)
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(first, got))
+
+
+@gpu
+def test_every_kernel_of_heads_of_64(env):
+    """Sizes on both sides of the choices between kernels: many short sequences and few long ones, with and without sinks."""
+    import torch
+
+    for B, T, H, KV, window, sinks in ((40, 130, 8, 8, 0, 0), (24, 500, 8, 8, 64, 0), (24, 500, 8, 4, 64, 3), (1, 1500, 2, 1, 0, 0), (80, 128, 8, 8, 0, 0), (80, 129, 8, 8, 0, 0)):
+        q, k, v, g = tensors(T, torch.float16, B, T, T, H, KV, 64)
+        some = [0, B // 2, B - 1] if B > 1 else [0]
+        want, bound = R.window_attention(q[some], k[some], v[some], window, sinks, None, 0.125, g[some])
+        out, lse = run_forward(env, q, k, v, window, sinks)
+        grads = run_backward(env, q, k, v, out, lse, g, window, sinks)
+        check([x[some] for x in (out, lse) + grads], want, bound, ("out", "lse", "dq", "dk", "dv"))
+
+
+@gpu
+def test_captured_training_step_and_other_streams(env):
+    """Forward and backward captured twice and replayed in turn on changing inputs; a context with a stream of its own."""
+    import torch
+
+    U, pk = env, env.pkg()
+    main = U.ctx()
+    for ctx in (main, pk.Context(0, use_torch_stream=False)):
+        q, k, v, g = tensors(11, torch.bfloat16, 2, 200, 200, 4, 2, 64)
+        out, dq, dk, dv = (torch.empty_like(x) for x in (q, q, k, v))
+        lse, delta = torch.empty((2, 4, 200), device="cuda"), torch.empty((2, 4, 200), device="cuda")
+        wa = pk.WindowAttention(ctx, 50, 2)
+        torch.cuda.synchronize()
+
+        def step():
+            wa.forward(q, k, v, out, lse)
+            wa.backward(q, k, v, out, lse, g, dq, dk, dv, delta)
+
+        step()
+        ctx.sync()
+        graphs = []
+        for _ in range(2):
+            ctx.graph_begin()
+            step()
+            graphs.append(ctx.graph_end())
+        for i in range(4):
+            for x in (q, k, v, g):
+                x.normal_()
+            torch.cuda.synchronize()
+            ctx.graph_launch(graphs[i % 2])
+            ctx.sync()
+            want, bound = R.window_attention(q, k, v, 50, 2, None, 0.125, g)
+            check((out, lse, dq, dk, dv), want, bound, ("out", "lse", "dq", "dk", "dv"))
+        for x in graphs:
+            pk.lib().aig_graph_destroy(x)
+        if ctx is not main:
+            ctx.close()
+
+
+@gpu
+def test_refusals(env):
+    import torch
+
+    U, pk = env, env.pkg()
+    ctx = U.ctx()
+    q, k, v, g = tensors(12, torch.float16, 2, 8, 8, 4, 2, 64)
+    out, lse = torch.empty_like(q), torch.empty((2, 4, 8), device="cuda")
+    n = torch.tensor([8, 8], device="cuda").int()
+    wa = pk.WindowAttention(ctx)
+    for args in ((q.float(), k.float(), v.float(), out.float(), lse), (q, k.bfloat16(), v, out, lse), (q, k, v[:, :7], out, lse), (q, k, v, out[:, :7], lse),
+                 (q, k, v, out, lse.double()), (q, k, v, out, lse[:, :3]), (q, k, v, out, lse, n[:1]), (q, k, v, out, lse, n.long()), (q[0], k[0], v[0], out[0], lse),
+                 (q, k.cpu(), v, out, lse), (q.transpose(2, 3), k, v, out, lse)):
+        with pytest.raises(ValueError):
+            wa.forward(*args)
+    for change in (dict(scale=0.0), dict(scale=-0.1), dict(scale=float("nan")), dict(sinks=-1)):
+        with pytest.raises(pk.AigError) as e:
+            pk.WindowAttention(ctx, **change).forward(q, k, v, out, lse)
+        assert e.value.code == -1
+    with pytest.raises(pk.AigError):  # more queries than keys
+        wa.forward(q, k[:, :7], v[:, :7], out, lse)
+    with pytest.raises(pk.AigError):  # three heads over two
+        wa.forward(q[:, :, :3], k, v, out[:, :, :3], torch.empty((2, 3, 8), device="cuda"))
+    with pytest.raises(pk.AigError) as e:  # heads of 32
+        wa.forward(q[..., :32], k[..., :32], v[..., :32], out[..., :32], lse)
+    assert e.value.code == -4
+    flat = torch.empty(q.numel() + 8, dtype=torch.float16, device="cuda")
+    with pytest.raises(pk.AigError):  # off a 16-byte boundary
+        wa.forward(flat[1:q.numel() + 1].view(q.shape), k, v, out, lse)
+    wide = torch.empty((2, 8, 4, 68), dtype=torch.float16, device="cuda")[..., :64]
+    with pytest.raises(pk.AigError):  # strides that are no multiples of 8
+        wa.forward(wide, k, v, out, lse)
+    with pytest.raises(pk.AigError):  # one head's keys for all: a stride of 0
+        wa.forward(q, k[:, :, :1].expand(2, 8, 2, 64), v, out, lse)
+    empty = q[:0]
+    wa.forward(empty, k[:0], v[:0], out[:0], lse[:0])
+    wa.forward(q[:, :0], k, v, out[:, :0], lse[:, :, :0].contiguous())
+    ctx.sync()
+
+
+@gpu
+def test_no_queries_leave_keys_without_gradient(env):
+    """A chunk whose window no longer reaches the first keys: their gradients are zeros."""
+    import torch
+
+    q, k, v, g = tensors(13, torch.bfloat16, 1, 100, 600, 2, 1, 64)
+    want, bound = R.window_attention(q, k, v, 50, 0, None, 0.125, g)
+    out, lse = run_forward(env, q, k, v, 50)
+    grads = run_backward(env, q, k, v, out, lse, g, 50)
+    check((out, lse) + grads, want, bound, ("out", "lse", "dq", "dk", "dv"))
+    assert not grads[1][:, :400].any() and not grads[2][:, :400].any()
