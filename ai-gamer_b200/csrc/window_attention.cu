@@ -757,8 +757,15 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   const int rows_end = min(p.q_len, len - off);
   if (r0 >= rows_end) return;
   const KeyTiles kt = key_tiles<kSub>(off + r0, off + min(r0 + kTile, rows_end) - 1, p.window, p.sinks);
-  const int tiles = kt.sink_end + kt.end - kt.begin;
-  auto first_key = [&](int u) { return (u < kt.sink_end ? u : kt.begin + (u - kt.sink_end)) * kSub; };
+  // D = dO . O has the output's rounding in it, which is large against dP where a row sees a few keys.  Rows that see only the
+  // first tile's keys take the sum of P o dP over them instead; with a window of few keys all rows do, in a pass of its own over
+  // the tiles ahead of the one that adds up dQ.
+  const int seen = kt.sink_end + kt.end - kt.begin;
+  const int ahead = p.window > 0 && p.window + p.sinks <= kSub ? seen : 0, tiles = ahead + seen;
+  auto first_key = [&](int u) {
+    const int t = u < ahead ? u : u - ahead;
+    return (t < kt.sink_end ? t : kt.begin + (t - kt.sink_end)) * kSub;
+  };
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -812,7 +819,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
     auto scores = [&](int u) {
       const uint32_t k = sK + kr.s * S::kStage, v = sV + vr.s * S::kStage, t = tmem + 128 * (u % G);
       if (!warp_wait(kv_full + 8 * kr.s, kr.ph, s_abort, p.gerr, 1122)) return false;
-      if (u + 1 == tiles && first_key(u) + kSub > len) clear_rows<D, kSub>(sm + (k - base), len - first_key(u), lane);
+      if (first_key(u) + kSub > len) clear_rows<D, kSub>(sm + (k - base), len - first_key(u), lane);
       tc_fence_after();
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, t, desc_k<kTile>(sQ, ks), desc_k<kSub>(k, ks), idesc_s, ks != 0);
@@ -825,9 +832,11 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
       return true;
     };
     auto add = [&](int x) {  // dQ += dS K
+      if (x >= ahead) {
 #pragma unroll
-      for (int ks = 0; ks < kSub / 16; ++ks)
-        mma_ts(leader, tdQ, tdS + 32 * (x % (2 * G)) + ks * 8, desc_rows<kSub>(sK + kd.s * S::kStage, ks), idesc_q, x != 0 || ks != 0);
+        for (int ks = 0; ks < kSub / 16; ++ks)
+          mma_ts(leader, tdQ, tdS + 32 * (x % (2 * G)) + ks * 8, desc_rows<kSub>(sK + kd.s * S::kStage, ks), idesc_q, x != ahead || ks != 0);
+      }
       commit(leader, k_free + 8 * kd.s);
       kd.next();
     };
@@ -877,12 +886,10 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
     const float lse2 = there ? p.lse[stat] * kLog2e : INFINITY;  // (weights of 0)
     // a query that sees one key has the weight 1 whatever its score: no gradient through it
     const bool single = pos == 0 || (p.window == 1 && p.sinks == 0);
-    // D = dO . O has the output's rounding in it.  Where a row sees a few keys, that is large against dP: a row that sees only the
-    // first tile's takes the sum over its weights instead, below.
-    const bool few = first_key(0) + kSub > off + r0, mine_few = first_key(0) + kSub > pos;
+    const bool few = ahead == 0 && first_key(0) + kSub > off + r0, mine_few = first_key(0) + kSub > pos;
     constexpr int kShare = D / G;  // a row's dot product and its result are shared by the groups
     float delta = 0.f;
-    if (there) {
+    if (there && ahead == 0) {
       const T* g = reinterpret_cast<const T*>(p.dout.data) + b * p.dout.batch + row * p.dout.token + h * p.dout.head + w * kShare;
       const T* o = reinterpret_cast<const T*>(p.o.data) + b * p.o.batch + row * p.o.token + h * p.o.head + w * kShare;
 #pragma unroll
@@ -896,16 +903,24 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
         }
       }
     }
-    if (G == 2) {
-      s_sum[w * 128 + in_tile] = delta;
-      named_bar_sync(2, 256);
-      delta = s_sum[in_tile] + s_sum[128 + in_tile];
-    }
+    auto join = [&] {  // the groups' parts of it
+      if (G == 2) {
+        s_sum[w * 128 + in_tile] = delta;
+        named_bar_sync(2, 256);
+        delta = s_sum[in_tile] + s_sum[128 + in_tile];
+      }
+    };
+    bool joined = ahead == 0;
+    if (joined) join();
     bool ok = true;
     Ring<NK> kr;
     if (w == 1) kr.next();
     for (int u = w, n = 0; u < tiles; u += G, ++n) {
       const int s = kr.s, j0 = first_key(u);
+      if (!joined && u >= ahead) {
+        join();
+        joined = true;
+      }
       const uint32_t t = tmem + 128 * w + lanes;
       float r = 1.f;
       int step = 0;
@@ -948,35 +963,39 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
           sc[i][e] = __float_as_uint(y.x);
           sc[i][e + 1] = __float_as_uint(y.y);
         }
-      if (few && u == 0) {
+      if (u < ahead || (few && u == 0)) {
         float2 own = make_float2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int e = 0; e < 32; e += 2) own = fma2(pair_of(sc[i][e], sc[i][e + 1]), pair_of(dp[i][e], dp[i][e + 1]), own);
-        if (mine_few) delta = own.x + own.y;
+        if (u < ahead) delta += own.x + own.y;
+        else if (mine_few) delta = own.x + own.y;
       }
-      if (kScaled && step != 0) {  // what has been summed so far, the other group's last tile included, follows
+      if (kScaled && step != 0 && u > ahead) {  // what has been summed so far, the other group's last tile included, follows
         if (!(ok = warp_wait(k_free + 8 * ((u - 1) % NK), (uint32_t)((u - 1) / NK) & 1u, s_abort, p.gerr, 1131))) break;
         tc_fence_after();
         scale_row<D>(tdQ + lanes, pow2(max(step, -126)));
       }
-      const float shift = -delta * r;
+      if (u >= ahead) {
+        const float shift = -delta * r;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t o[16];
+        for (int i = 0; i < 2; ++i) {
+          uint32_t o[16];
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          const float2 x = mul2(pair_of(sc[i][e], sc[i][e + 1]), fma2(pair_of(dp[i][e], dp[i][e + 1]), make_float2(r, r), make_float2(shift, shift)));
-          o[e / 2] = pack2<T>(x.x, x.y);
+          for (int e = 0; e < 32; e += 2) {
+            const float2 x = mul2(pair_of(sc[i][e], sc[i][e + 1]), fma2(pair_of(dp[i][e], dp[i][e + 1]), make_float2(r, r), make_float2(shift, shift)));
+            o[e / 2] = pack2<T>(x.x, x.y);
+          }
+          tmem_st_32x16(tdS + 32 * (u % (2 * G)) + lanes + 16 * i, o);
         }
-        tmem_st_32x16(tdS + 32 * (u % (2 * G)) + lanes + 16 * i, o);
       }
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(ds_full + 8 * (u % (2 * G)));
       for (int i = 0; i < G; ++i) kr.next();
     }
+    if (!joined) join();
     if (ok && warp_wait(dq_full, 0, s_abort, p.gerr, 1132)) {
       tc_fence_after();
       if (there && w == 0) p.delta[stat] = delta;
