@@ -784,7 +784,7 @@ class PagedCache:
         on = ctx.device
         for t in (k_pages, v_pages):
             _seq_heads(t, k_pages.shape, self.dtype, on, "pages")
-        self.ctx, self._keep = ctx, (k_pages, v_pages)
+        self.ctx, self._lib, self._keep = ctx, lib(), (k_pages, v_pages)
         pages, size, self.heads, self.dim = k_pages.shape
         s = k_pages.stride()
         self.desc = KvCacheDesc(k_pages.data_ptr(), v_pages.data_ptr(), _types[self.dtype], self.heads, self.dim, size, pages, s[0], s[1], s[2])
@@ -802,7 +802,7 @@ class PagedCache:
             q_shape = (n, q.shape[1], self.dim)
             qh, qo = _heads(q, q_shape, dtype, on, "q"), _heads(q_out, q_shape, dtype, on, "q_out")
         batch, width = table.shape
-        ctx.check(lib().aig_kv_append(ctx.handle, self._ref, None if rope is None else rope.handle, _heads(k, shape, dtype, on, "k"),
+        ctx.check(self._lib.aig_kv_append(ctx.handle, self._ref, None if rope is None else rope.handle, _heads(k, shape, dtype, on, "k"),
                                       _heads(v, shape, dtype, on, "v"), qh, qo, None if seqs is None else _ints(seqs, (n,), on, "seqs"),
                                       _ints(positions, (n,), on, "positions"), n, _ints(table, (batch, width), on, "table"), batch, width))
 
@@ -812,7 +812,7 @@ class PagedCache:
         if len(dst) != n:
             raise ValueError("as many sources as destinations")
         src, dst = array.array("i", src), array.array("i", dst)
-        self.ctx.check(lib().aig_kv_copy_pages(self.ctx.handle, self._ref, src.buffer_info()[0], dst.buffer_info()[0], n))
+        self.ctx.check(self._lib.aig_kv_copy_pages(self.ctx.handle, self._ref, src.buffer_info()[0], dst.buffer_info()[0], n))
 
     def attend(self, q, out, table, lengths, max_length, scale=None, window=0, sinks=0):
         """One new token of each sequence, q and out [batch][heads][head_dim], over lengths[b] cached positions (its own the last)."""
@@ -820,7 +820,7 @@ class PagedCache:
         if len(shape) != 3 or shape[2] != self.dim:
             raise ValueError("q: [batch][heads][%d] is wanted, got %s" % (self.dim, tuple(shape)))
         on, batch, width = ctx.device, shape[0], table.shape[1]
-        ctx.check(lib().aig_paged_attention(ctx.handle, self._ref, _heads(q, shape, dtype, on, "q"), _heads(out, shape, dtype, on, "out"),
+        ctx.check(self._lib.aig_paged_attention(ctx.handle, self._ref, _heads(q, shape, dtype, on, "q"), _heads(out, shape, dtype, on, "out"),
                                             _ints(table, (batch, width), on, "table"), width, _ints(lengths, (batch,), on, "lengths"), batch, max_length,
                                             self.dim ** -0.5 if scale is None else scale, window, sinks))
         return out
@@ -893,7 +893,7 @@ class WindowAttention:
     q, out [batch][q_len][heads][head_dim], k, v [batch][kv_len][kv_heads][head_dim], lse fp32 [batch][heads][q_len]."""
 
     def __init__(self, ctx, window=0, sinks=0, scale=None):
-        self.ctx, self.window, self.sinks, self.scale = ctx, window, sinks, scale
+        self.ctx, self._lib, self.window, self.sinks, self.scale = ctx, lib(), window, sinks, scale
 
     def _shapes(self, q, k, *stats):
         """The call's description, the tensors' shapes, type and device; checks what has the statistics' shape."""
@@ -911,7 +911,7 @@ class WindowAttention:
     def forward(self, q, k, v, out, lse, lengths=None):
         desc, qs, ks, dtype, on = self._shapes(q, k, lse)
         ctx = self.ctx
-        ctx.check(lib().aig_window_attention_forward(ctx.handle, desc, _seq_heads(q, qs, dtype, on, "q"), _seq_heads(k, ks, dtype, on, "k"),
+        ctx.check(self._lib.aig_window_attention_forward(ctx.handle, desc, _seq_heads(q, qs, dtype, on, "q"), _seq_heads(k, ks, dtype, on, "k"),
                                                      _seq_heads(v, ks, dtype, on, "v"), _seq_heads(out, qs, dtype, on, "out"), lse.data_ptr(),
                                                      None if lengths is None else _ints(lengths, (qs[0],), on, "lengths")))
         return out
@@ -920,7 +920,7 @@ class WindowAttention:
         """`delta`: scratch of lse's shape."""
         desc, qs, ks, dtype, on = self._shapes(q, k, lse, delta)
         ctx = self.ctx
-        ctx.check(lib().aig_window_attention_backward(ctx.handle, desc, _seq_heads(q, qs, dtype, on, "q"), _seq_heads(k, ks, dtype, on, "k"),
+        ctx.check(self._lib.aig_window_attention_backward(ctx.handle, desc, _seq_heads(q, qs, dtype, on, "q"), _seq_heads(k, ks, dtype, on, "k"),
                                                       _seq_heads(v, ks, dtype, on, "v"), _seq_heads(out, qs, dtype, on, "out"), lse.data_ptr(),
                                                       _seq_heads(dout, qs, dtype, on, "dout"), _seq_heads(dq, qs, dtype, on, "dq"),
                                                       _seq_heads(dk, ks, dtype, on, "dk"), _seq_heads(dv, ks, dtype, on, "dv"), delta.data_ptr(),

@@ -706,12 +706,16 @@ struct BwdShape {
   static constexpr int kThreads = 128 + 128 * G;
   static constexpr int kTmemCols = 256 * G;
 };
+// dQ, heads of 128: both groups share tiles of 128 keys, half of the columns each.  A product of 128 x 128 takes 67 clocks, two of
+// 128 x 64 100 (both operands come from shared memory), and the products are what heads of 128 wait for.
 template <int D, int G>
 struct DqShape : BwdShape<D, G> {
-  static constexpr int kKeys = D == 128 ? 6 : G == 2 ? 8 : 5, kValues = D == 64 && G == 2 ? 6 : 4;  // stages: keys are needed for longer
-  static constexpr uint32_t kFixed = 2 * kTileBytes<D, kTile>, kStage = kTileBytes<D, kSub>;
+  static constexpr int kKeyRows = D == 128 ? 128 : kSub;              // of a tile
+  static constexpr int kStreams = D == 128 ? 1 : G, kHalves = G / kStreams;
+  static constexpr int kKeys = D == 128 ? 3 : G == 2 ? 8 : 5, kValues = D == 128 ? 2 : G == 2 ? 6 : 4;  // stages: keys are needed for longer
+  static constexpr uint32_t kFixed = 2 * kTileBytes<D, kTile>, kStage = kTileBytes<D, kKeyRows>;
   static constexpr uint32_t kTiles = kFixed + (kKeys + kValues) * kStage;
-  static constexpr size_t kSmem = kTiles + 1024 + 512;
+  static constexpr size_t kSmem = kTiles + 2048 + 512;
 };
 template <int D, int G>
 struct DkvShape : BwdShape<D, G> {
@@ -726,7 +730,7 @@ __global__ void __launch_bounds__(DqShape<D, G>::kThreads, DqShape<D, G>::kCtasP
 window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
                  const __grid_constant__ CUtensorMap mapG, const __grid_constant__ WinParams p) {
   using S = DqShape<D, G>;
-  constexpr int NK = S::kKeys, NV = S::kValues;
+  constexpr int NK = S::kKeys, NV = S::kValues, KR = S::kKeyRows, ST = S::kStreams, H = S::kHalves;
   constexpr bool kScaled = std::is_same<T, __half>::value;
   extern __shared__ __align__(1024) uint8_t sm[];
   const uint32_t base = smem_u32(sm);
@@ -736,9 +740,10 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   }
   const uint32_t sQ = base, sG = sQ + kTileBytes<D, kTile>, sK = base + S::kFixed, sV = sK + NK * S::kStage;
   float* const s_sum = reinterpret_cast<float*>(sm + S::kTiles);  // [2][128]
-  uint64_t* const bars = reinterpret_cast<uint64_t*>(s_sum + 256);
+  float* const s_own = s_sum + 256;                                // [2][128]
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(s_own + 256);
   const uint32_t bar0 = smem_u32(bars);
-  // of each group: scores and dP are there, they have been read; of each of two buffers of a group: dS is there
+  // of each stream of tiles: scores and dP are there, they have been read; of each of its two buffers: dS is there
   const uint32_t q_full = bar0, dq_full = bar0 + 8, sd_full = bar0 + 16, sd_free = sd_full + 16, ds_full = sd_free + 16, kv_full = ds_full + 32,
                  k_free = kv_full + 8 * NK, v_free = k_free + 8 * NK, st_full = v_free + 8 * NV;
   int* const s_power = reinterpret_cast<int*>(bars + 10 + 3 * NK + NV);  // [NK]
@@ -756,7 +761,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   const int off = p.kv_len - p.q_len, r0 = block * kTile;
   const int rows_end = min(p.q_len, len - off);
   if (r0 >= rows_end) return;
-  const KeyTiles kt = key_tiles<kSub>(off + r0, off + min(r0 + kTile, rows_end) - 1, p.window, p.sinks);
+  const KeyTiles kt = key_tiles<KR>(off + r0, off + min(r0 + kTile, rows_end) - 1, p.window, p.sinks);
   // D = dO . O has the output's rounding in it, which is large against dP where a row sees a few keys.  Rows that see only the
   // first tile's keys take the sum of P o dP over them instead; with a window of few keys all rows do, in a pass of its own over
   // the tiles ahead of the one that adds up dQ.
@@ -764,17 +769,17 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   const int ahead = p.window > 0 && p.window + p.sinks <= kSub ? seen : 0, tiles = ahead + seen;
   auto first_key = [&](int u) {
     const int t = u < ahead ? u : u - ahead;
-    return (t < kt.sink_end ? t : kt.begin + (t - kt.sink_end)) * kSub;
+    return (t < kt.sink_end ? t : kt.begin + (t - kt.sink_end)) * KR;
   };
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(dq_full, 1);
-    for (int w = 0; w < G; ++w) {
-      mbar_init(sd_full + 8 * w, 1);
-      mbar_init(sd_free + 8 * w, 128);
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(sd_full + 8 * i, 1);
+      mbar_init(sd_free + 8 * i, 128 * H);
     }
-    for (int i = 0; i < 2 * G; ++i) mbar_init(ds_full + 8 * i, 128);
+    for (int i = 0; i < 2 * ST; ++i) mbar_init(ds_full + 8 * i, 128 * H);
     for (int s = 0; s < NK; ++s) {
       mbar_init(kv_full + 8 * s, 1);
       mbar_init(k_free + 8 * s, 1);
@@ -792,8 +797,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // of each group: 64 columns of scores, 64 of dP; then each group's two buffers of 32 for dS; then dQ
-  const uint32_t tmem = *s_tmem, tdS = tmem + 128 * G, tdQ = tmem + 192 * G;
+  // of each stream: scores, dP; then each stream's two buffers for dS; then dQ
+  const uint32_t tmem = *s_tmem, tdS = tmem + 2 * KR * ST, tdQ = tmem + 3 * KR * ST;
   if (S::kCtasPerSm == 2 && warp < 4) fewer_registers<40>();
 
   if (warp == 0) {
@@ -806,26 +811,26 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
       for (int u = 0; u < tiles; ++u, kr.next(), vr.next()) {
         if (u >= NK && !mbar_wait_bounded(k_free + 8 * kr.s, kr.ph ^ 1u, s_abort, p.gerr, 1121)) break;
         mbar_expect_tx(kv_full + 8 * kr.s, 2 * S::kStage);
-        load_tile<D, kSub, kSub>(sK + kr.s * S::kStage, &mapK, kv_full + 8 * kr.s, kvh, first_key(u), b);
+        load_tile<D, KR, kSub>(sK + kr.s * S::kStage, &mapK, kv_full + 8 * kr.s, kvh, first_key(u), b);
         if (u >= NV && !mbar_wait_bounded(v_free + 8 * vr.s, vr.ph ^ 1u, s_abort, p.gerr, 1133)) break;
-        load_tile<D, kSub, kSub>(sV + vr.s * S::kStage, &mapV, kv_full + 8 * kr.s, kvh, first_key(u), b);
+        load_tile<D, KR, kSub>(sV + vr.s * S::kStage, &mapV, kv_full + 8 * kr.s, kvh, first_key(u), b);
       }
     }
   } else if (warp == 1) {
-    constexpr uint32_t idesc_s = idesc_for<T>(kTile, kSub, false), idesc_q = idesc_for<T>(kTile, D, true);
+    constexpr uint32_t idesc_s = idesc_for<T>(kTile, KR, false), idesc_q = idesc_for<T>(kTile, D, true);
     const uint32_t leader = elect_one() ? 1u : 0u;
     Ring<NK> kr, kd;  // of the next scores, of the next product with dS
     Ring<NV> vr;
     auto scores = [&](int u) {
-      const uint32_t k = sK + kr.s * S::kStage, v = sV + vr.s * S::kStage, t = tmem + 128 * (u % G);
+      const uint32_t k = sK + kr.s * S::kStage, v = sV + vr.s * S::kStage, t = tmem + 2 * KR * (u % ST);
       if (!warp_wait(kv_full + 8 * kr.s, kr.ph, s_abort, p.gerr, 1122)) return false;
-      if (first_key(u) + kSub > len) clear_rows<D, kSub>(sm + (k - base), len - first_key(u), lane);
+      if (first_key(u) + KR > len) clear_rows<D, KR>(sm + (k - base), len - first_key(u), lane);
       tc_fence_after();
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, t, desc_k<kTile>(sQ, ks), desc_k<kSub>(k, ks), idesc_s, ks != 0);
+      for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, t, desc_k<kTile>(sQ, ks), desc_k<KR>(k, ks), idesc_s, ks != 0);
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, t + 64, desc_k<kTile>(sG, ks), desc_k<kSub>(v, ks), idesc_s, ks != 0);
-      commit(leader, sd_full + 8 * (u % G));
+      for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, t + KR, desc_k<kTile>(sG, ks), desc_k<KR>(v, ks), idesc_s, ks != 0);
+      commit(leader, sd_full + 8 * (u % ST));
       commit(leader, v_free + 8 * vr.s);
       kr.next();
       vr.next();
@@ -834,24 +839,24 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
     auto add = [&](int x) {  // dQ += dS K
       if (x >= ahead) {
 #pragma unroll
-        for (int ks = 0; ks < kSub / 16; ++ks)
-          mma_ts(leader, tdQ, tdS + 32 * (x % (2 * G)) + ks * 8, desc_rows<kSub>(sK + kd.s * S::kStage, ks), idesc_q, x != ahead || ks != 0);
+        for (int ks = 0; ks < KR / 16; ++ks)
+          mma_ts(leader, tdQ, tdS + KR / 2 * (x % (2 * ST)) + ks * 8, desc_rows<KR>(sK + kd.s * S::kStage, ks), idesc_q, x != ahead || ks != 0);
       }
       commit(leader, k_free + 8 * kd.s);
       kd.next();
     };
     bool ok = warp_wait(q_full, 0, s_abort, p.gerr, 1123);
-    for (int u = 0; u < G && u < tiles && ok; ++u) ok = scores(u);
-    for (int u = 0; u + G < tiles && ok; ++u) {
-      // The group has read tile u: it has written dS of its tile before.  That product goes ahead of the next scores, so that
+    for (int u = 0; u < ST && u < tiles && ok; ++u) ok = scores(u);
+    for (int u = 0; u + ST < tiles && ok; ++u) {
+      // The stream's threads have read tile u: they have written dS of their tile before.  That product goes ahead of the next scores, so that
       // whoever finds these knows its buffer free.
-      if (!(ok = warp_wait(sd_free + 8 * (u % G), (uint32_t)(u / G) & 1u, s_abort, p.gerr, 1124))) break;
+      if (!(ok = warp_wait(sd_free + 8 * (u % ST), (uint32_t)(u / ST) & 1u, s_abort, p.gerr, 1124))) break;
       tc_fence_after();
-      if (u >= G) add(u - G);
-      ok = scores(u + G);
+      if (u >= ST) add(u - ST);
+      ok = scores(u + ST);
     }
-    for (int x = max(tiles - 2 * G, 0); x < tiles && ok; ++x) {
-      if (!(ok = warp_wait(ds_full + 8 * (x % (2 * G)), (uint32_t)(x / (2 * G)) & 1u, s_abort, p.gerr, 1125))) break;
+    for (int x = max(tiles - 2 * ST, 0); x < tiles && ok; ++x) {
+      if (!(ok = warp_wait(ds_full + 8 * (x % (2 * ST)), (uint32_t)(x / (2 * ST)) & 1u, s_abort, p.gerr, 1125))) break;
       tc_fence_after();
       add(x);
     }
@@ -864,7 +869,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
       Ring<NV> vr;
       for (int u = 0; u < tiles; ++u, kr.next(), vr.next()) {
         if (!warp_wait(kv_full + 8 * kr.s, kr.ph, s_abort, p.gerr, 1127)) break;
-        const int k_new = next_power(k, eg + tile_exponent<D, kSub>(sm + (sV - base) + vr.s * S::kStage, min(kSub, len - first_key(u)), lane));
+        const int k_new = next_power(k, eg + tile_exponent<D, KR>(sm + (sV - base) + vr.s * S::kStage, min(KR, len - first_key(u)), lane));
         __syncwarp();
         if (lane == 0) {
           s_power[kr.s] = k_new;
@@ -878,6 +883,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   } else if (warp >= 4) {
     if (S::kCtasPerSm == 2) more_registers<208>();
     const int w = (warp - 4) >> 2, q = warp & 3, in_tile = q * 32 + lane;
+    const int stream = w % ST, half = H == 2 ? w : 0;
     const int row = r0 + in_tile, pos = off + row;
     const bool there = row < rows_end;
     const uint32_t lanes = (uint32_t)(q * 32) << 16;
@@ -886,7 +892,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
     const float lse2 = there ? p.lse[stat] * kLog2e : INFINITY;  // (weights of 0)
     // a query that sees one key has the weight 1 whatever its score: no gradient through it
     const bool single = pos == 0 || (p.window == 1 && p.sinks == 0);
-    const bool few = ahead == 0 && first_key(0) + kSub > off + r0, mine_few = first_key(0) + kSub > pos;
+    const bool few = ahead == 0 && first_key(0) + KR > off + r0, mine_few = first_key(0) + KR > pos;
     constexpr int kShare = D / G;  // a row's dot product and its result are shared by the groups
     float delta = 0.f;
     if (there && ahead == 0) {
@@ -914,36 +920,39 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
     if (joined) join();
     bool ok = true;
     Ring<NK> kr;
-    if (w == 1) kr.next();
-    for (int u = w, n = 0; u < tiles; u += G, ++n) {
+    if (stream == 1) kr.next();
+    for (int u = stream, n = 0; u < tiles; u += ST, ++n) {
       const int s = kr.s, j0 = first_key(u);
       if (!joined && u >= ahead) {
         join();
         joined = true;
       }
-      const uint32_t t = tmem + 128 * w + lanes;
+      const uint32_t t = tmem + 2 * KR * stream + 64 * half + lanes;
       float r = 1.f;
       int step = 0;
-      ok = warp_wait(sd_full + 8 * w, (uint32_t)n & 1u, s_abort, p.gerr, 1128);
+      ok = warp_wait(sd_full + 8 * stream, (uint32_t)n & 1u, s_abort, p.gerr, 1128);
       if (kScaled && ok) {
         ok = warp_wait(st_full + 8 * s, kr.ph, s_abort, p.gerr, 1129);
         r = pow2(s_power[s]);
         step = s_step[s];
       }
-      if (!ok) break;
+      if (!ok) {
+        if (H == 2 && few && u == 0) named_bar_sync(2, 256);  // (the other half may be waiting below)
+        break;
+      }
       tc_fence_after();
       uint32_t sc[2][32], dp[2][32];
       tmem_ld_32x32(t, sc[0]);
       tmem_ld_32x32(t + 32, sc[1]);
-      tmem_ld_32x32(t + 64, dp[0]);
-      tmem_ld_32x32(t + 96, dp[1]);
+      tmem_ld_32x32(t + KR, dp[0]);
+      tmem_ld_32x32(t + KR + 32, dp[1]);
       tmem_ld_wait();
       tc_fence_before();
-      mbar_arrive(sd_free + 8 * w);
+      mbar_arrive(sd_free + 8 * stream);
       if (single) r = 0.f;
-      const bool cut = j0 + kSub - 1 > off + r0 || (p.window > 0 && j0 <= off + r0 + kTile - 1 - p.window && j0 + kSub > p.sinks);
+      const bool cut = j0 + KR - 1 > off + r0 || (p.window > 0 && j0 <= off + r0 + kTile - 1 - p.window && j0 + KR > p.sinks);
       if (cut) {
-        const int lo = p.window > 0 ? pos - p.window + 1 - j0 : -1, hi = pos - j0, sinks = p.sinks - j0;
+        const int c0 = j0 + 64 * half, lo = p.window > 0 ? pos - p.window + 1 - c0 : -1, hi = pos - c0, sinks = p.sinks - c0;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint32_t shown = bits_below(hi + 1 - 32 * i) & (~bits_below(lo - 32 * i) | bits_below(sinks - 32 * i));
@@ -969,13 +978,22 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int e = 0; e < 32; e += 2) own = fma2(pair_of(sc[i][e], sc[i][e + 1]), pair_of(dp[i][e], dp[i][e + 1]), own);
-        if (u < ahead) delta += own.x + own.y;
-        else if (mine_few) delta = own.x + own.y;
+        float sum = own.x + own.y;
+        if (u < ahead) {
+          delta += sum;
+        } else {
+          if (H == 2) {
+            s_own[w * 128 + in_tile] = sum;
+            named_bar_sync(2, 256);
+            sum = s_own[in_tile] + s_own[128 + in_tile];
+          }
+          if (mine_few) delta = sum;
+        }
       }
       if (kScaled && step != 0 && u > ahead) {  // what has been summed so far, the other group's last tile included, follows
         if (!(ok = warp_wait(k_free + 8 * ((u - 1) % NK), (uint32_t)((u - 1) / NK) & 1u, s_abort, p.gerr, 1131))) break;
         tc_fence_after();
-        scale_row<D>(tdQ + lanes, pow2(max(step, -126)));
+        scale_row<D / H>(tdQ + lanes + half * (D / H), pow2(max(step, -126)));
       }
       if (u >= ahead) {
         const float shift = -delta * r;
@@ -987,13 +1005,13 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
             const float2 x = mul2(pair_of(sc[i][e], sc[i][e + 1]), fma2(pair_of(dp[i][e], dp[i][e + 1]), make_float2(r, r), make_float2(shift, shift)));
             o[e / 2] = pack2<T>(x.x, x.y);
           }
-          tmem_st_32x16(tdS + 32 * (u % (2 * G)) + lanes + 16 * i, o);
+          tmem_st_32x16(tdS + KR / 2 * (u % (2 * ST)) + 32 * half + lanes + 16 * i, o);
         }
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(ds_full + 8 * (u % (2 * G)));
-      for (int i = 0; i < G; ++i) kr.next();
+      mbar_arrive(ds_full + 8 * (u % (2 * ST)));
+      for (int i = 0; i < ST; ++i) kr.next();
     }
     if (!joined) join();
     if (ok && warp_wait(dq_full, 0, s_abort, p.gerr, 1132)) {
