@@ -14,19 +14,23 @@ namespace {
 
 // ---------------------------------------------------------------------------------------------
 // Page copies.  The pairs travel as kernel parameters: nothing to upload, nothing that a later call could overwrite while
-// an earlier one (or a captured graph) still reads it.
-constexpr int kPairs = 1000;  // per launch
+// an earlier one (or a captured graph) still reads it.  Bound by memory: 1021 pages of 128 KB in 43 us, 6.2 TB/s.
+constexpr int kFewPairs = 32, kManyPairs = 2000;  // per launch: a fork's few parameters are not carried in 16 KB
 constexpr int kCopyThreads = 256, kCopyUnroll = 4;
 
-struct CopyParams {
+struct CopyShape {
   uint4 *k, *v;
   long long page, place, head;  // strides in 16-byte units
   int run, heads;               // consecutive 16-byte units of a run; runs: places x heads (1 x 1 where a page is one run)
   int units, blocks;            // of a page, and blocks that copy it
-  int32_t src[kPairs], dst[kPairs];
+};
+template <int N>
+struct CopyParams : CopyShape {
+  int32_t src[N], dst[N];
 };
 
-__global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyParams p) {
+template <int N>
+__global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_constant__ CopyParams<N> p) {
   griddep_launch_dependents();
   griddep_wait();
   const int pair = blockIdx.x / p.blocks;
@@ -48,13 +52,27 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_c
     if (first + i * kCopyThreads < p.units) dst[at[i]] = got[i];
 }
 
+template <int N>
+int launch_copies(aig_ctx* ctx, const CopyShape& shape, const int32_t* src, const int32_t* dst, int pairs) {
+  CopyParams<N> p;
+  static_cast<CopyShape&>(p) = shape;
+  for (int done = 0; done < pairs; done += N) {
+    const int n = pairs - done < N ? pairs - done : N;
+    memcpy(p.src, src + done, n * sizeof(int32_t));
+    memcpy(p.dst, dst + done, n * sizeof(int32_t));
+    if ((long long)n * p.blocks > 0x7fffffffll) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "kv copy pages: too much for one call");
+    AIG_CUDA_OK(ctx, launch_pdl(ctx, copy_pages_kernel<N>, dim3((unsigned)(n * p.blocks), 2), dim3(kCopyThreads), 0, p));
+  }
+  return AIG_OK;
+}
+
 // ---------------------------------------------------------------------------------------------
 // Attention of one new token.  For each (sequence, cached head) the visible positions are split over the CTAs of a cluster
 // and over their warps; a warp takes tiles of 16 or 32 positions through a ring of shared memory filled by cp.async.  Products
 // are mma.sync with the positions as rows and the group's query heads as the 8 columns, S^T = K Q^T and O^T = V^T P^T: K and
 // V come from shared memory as they lie there, P turns from result to operand by movmatrix, and eight query heads cost no more
 // than one.  (The kernel is bound by reading the cache, then by issuing instructions: with the heads as 16 rows
-// it took 430 instructions for 16 positions of 64, and 33 us where it takes XXB now, 128 sequences of up to 516 visible.)
+// it took 430 instructions for 16 positions of 64, and 33 us where it takes 23, 128 sequences of up to 516 visible.)
 // Softmax with a running maximum and sum in fp32; the weights enter the second product as a sum of two 16-bit values each, so
 // that their rounding does not add to the result's.  Warps are joined in shared memory, CTAs over the cluster's distributed
 // shared memory, in a fixed order: one launch, no scratch in global memory, nothing that two calls or captured
@@ -454,7 +472,7 @@ int aig_kv_copy_pages(aig_ctx* ctx, const aig_kv_cache* cache, const int32_t* sr
   } catch (const std::bad_alloc&) {
     return aig_fail(ctx, AIG_ERR_CUDA, "kv copy pages: out of host memory");
   }
-  CopyParams p;
+  CopyShape p;
   p.k = (uint4*)cache->k;
   p.v = (uint4*)cache->v;
   p.page = cache->page_stride / 8;
@@ -469,14 +487,7 @@ int aig_kv_copy_pages(aig_ctx* ctx, const aig_kv_cache* cache, const int32_t* sr
   p.run = places_outside || heads_outside ? p.units : row;
   p.heads = places_outside || heads_outside ? 1 : cache->kv_heads;
   p.blocks = (int)ceil_div_ll(units, kCopyThreads * kCopyUnroll);
-  for (int done = 0; done < pairs; done += kPairs) {
-    const int n = pairs - done < kPairs ? pairs - done : kPairs;
-    memcpy(p.src, src + done, n * sizeof(int32_t));
-    memcpy(p.dst, dst + done, n * sizeof(int32_t));
-    if ((long long)n * p.blocks > 0x7fffffffll) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "kv copy pages: too much for one call");
-    AIG_CUDA_OK(ctx, launch_pdl(ctx, copy_pages_kernel, dim3((unsigned)(n * p.blocks), 2), dim3(kCopyThreads), 0, p));
-  }
-  return AIG_OK;
+  return pairs <= kFewPairs ? launch_copies<kFewPairs>(ctx, p, src, dst, pairs) : launch_copies<kManyPairs>(ctx, p, src, dst, pairs);
 }
 
 int aig_paged_attention(aig_ctx* ctx, const aig_kv_cache* cache, const aig_heads* q, const aig_heads* out, const int32_t* table, int table_width,

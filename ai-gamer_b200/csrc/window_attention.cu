@@ -641,10 +641,9 @@ __global__ void __launch_bounds__(128, D == 64 ? 4 : 3) window_short_kernel(cons
 // ---------------------------------------------------------------------------------------------
 // Backward: one kernel for dQ (a tile of 128 queries stays, keys pass by), one for dK and dV (a tile of 128 keys stays, the
 // queries of the group's heads pass by).  Each computes the weights again from lse: two more products than one kernel that
-// adds dQ into memory with atomics would need, but every sum has a fixed order.  What passes by comes in tiles of 64 rows
-// for two groups of 128 threads in turn, so that one group's exponentials (the special-function unit's share is the
-// longest) run beside the other's waits, loads and products; a thread owns a row of scores.  (One tile of 128 at a
-// time for both groups, whose products are faster by a third per row, took 257 us where this takes XXX: 2 x 4099, 16 heads of 64.)
+// adds dQ into memory with atomics would need, but every sum has a fixed order.  A thread owns a row of scores, 64 columns of it
+// at a time.  Bound by the chain from products to exponentials to products: so two tiles are under way on an SM, in two groups of
+// 128 threads of one CTA or in two CTAs.  (2 x 4099, 16 heads of 64: 212 us; one tile of 128 at a time for both groups 257.)
 //
 // fp16 has few small numbers: weights of a row over thousands of keys, and dS of small gradients, would be rounded to
 // multiples of 2^-24.  So the weights are multiplied by 2^8, and dS by a power of two 2^k that follows the largest
@@ -695,11 +694,11 @@ struct Ring {
   }
 };
 
-// G groups of 128 threads, each with a tile of its own in hand.  A CTA of two groups has an SM to itself.  Heads of 64 leave room
-// for two CTAs of one group, which hide each other's beginnings and ends too, but each is slower by itself: they are taken
-// where no CTA has more than its half SM's share of all tiles (see `balanced`).  2 x 4099 with a window of 1024, 16 heads:
-// dQ 95 us with one group, 109 with two; dK and dV, where two sinks make one CTA the longest by far, 190 and 116; 128 x 64, 8 heads:
-// 22 + 25 against 77 for both; 4096 without a window, 4 heads: 57 + 74 against 42 + 46.
+// G groups of 128 threads, each with a tile of 64 rows of its own in hand.  A CTA of two groups has an SM to itself.  Heads of 64
+// leave room for two CTAs of one group, which hide each other's beginnings and ends too, but each is slower by itself: they are
+// taken where no CTA has more than its half SM's share of all tiles (`balanced` below).  2 x 4099 with a window of 1024, 16
+// heads: dQ 94 us with one group, 109 with two; dK and dV, where two sinks make one CTA the longest by far, 190 and 118; 128 x 64,
+// 8 heads: 22 + 25 against 77 for both; 4096 without a window, 4 heads: 57 + 74 against 39 + 46.
 template <int D, int G>
 struct BwdShape {
   static constexpr int kCtasPerSm = G == 1 ? 2 : 1;

@@ -117,7 +117,7 @@ def test_append_leaves_out_what_has_no_place(env):
 # ------------------------------------------------------------------------------------------------ copies
 @gpu
 @pytest.mark.parametrize("order", ["pshd", "phsd"])
-@pytest.mark.parametrize("pages,size,kv,dim,n", [(8, 1, 1, 8, 3), (64, 16, 8, 64, 20), (40, 100, 3, 128, 11), (2600, 2, 1, 64, 1203), (16, 16, 8, 64, 0)])
+@pytest.mark.parametrize("pages,size,kv,dim,n", [(8, 1, 1, 8, 3), (64, 16, 8, 64, 20), (40, 100, 3, 128, 11), (2600, 2, 1, 64, 1203), (16, 16, 8, 64, 0), (5000, 1, 1, 8, 2101)])
 def test_copy_pages(env, order, pages, size, kv, dim, n):
     import torch
 
