@@ -459,18 +459,24 @@ int aig_kv_copy_pages(aig_ctx* ctx, const aig_kv_cache* cache, const int32_t* sr
   const int rc = check_cache(ctx, cache, "kv copy pages");
   if (rc != AIG_OK) return rc;
   AIG_REQUIRE(ctx, pairs >= 0 && (pairs == 0 || (src && dst)), "kv copy pages: null list or negative number");
-  try {
-    std::vector<uint8_t> role(cache->num_pages, 0);  // 1: a source, 2: a destination
-    for (int i = 0; i < pairs; ++i) {
-      AIG_REQUIRE(ctx, src[i] >= 0 && src[i] < cache->num_pages && dst[i] >= 0 && dst[i] < cache->num_pages,
-                  "kv copy pages: pair %d (%d -> %d) names no page of the pool", i, src[i], dst[i]);
-      AIG_REQUIRE(ctx, role[dst[i]] == 0 && !(role[src[i]] & 2) && src[i] != dst[i],
-                  "kv copy pages: pair %d (%d -> %d): a page is a destination twice, or a source and a destination", i, src[i], dst[i]);
-      role[src[i]] |= 1;
-      role[dst[i]] |= 2;
+  for (int i = 0; i < pairs; ++i)
+    AIG_REQUIRE(ctx, src[i] >= 0 && src[i] < cache->num_pages && dst[i] >= 0 && dst[i] < cache->num_pages,
+                "kv copy pages: pair %d (%d -> %d) names no page of the pool", i, src[i], dst[i]);
+  const char* const twice = "kv copy pages: pair %d (%d -> %d): a page is a destination twice, or a source and a destination";
+  if (pairs <= kFewPairs) {  // (a fork's copy does not pay for a large pool)
+    for (int i = 0; i < pairs; ++i)
+      for (int j = 0; j < pairs; ++j) AIG_REQUIRE(ctx, dst[i] != src[j] && (i == j || dst[i] != dst[j]), twice, i, src[i], dst[i]);
+  } else {
+    try {
+      std::vector<uint8_t> role(cache->num_pages, 0);  // 1: a source, 2: a destination
+      for (int i = 0; i < pairs; ++i) {
+        AIG_REQUIRE(ctx, role[dst[i]] == 0 && !(role[src[i]] & 2) && src[i] != dst[i], twice, i, src[i], dst[i]);
+        role[src[i]] |= 1;
+        role[dst[i]] |= 2;
+      }
+    } catch (const std::bad_alloc&) {
+      return aig_fail(ctx, AIG_ERR_CUDA, "kv copy pages: out of host memory");
     }
-  } catch (const std::bad_alloc&) {
-    return aig_fail(ctx, AIG_ERR_CUDA, "kv copy pages: out of host memory");
   }
   CopyShape p;
   p.k = (uint4*)cache->k;
@@ -501,7 +507,8 @@ int aig_paged_attention(aig_ctx* ctx, const aig_kv_cache* cache, const aig_heads
   AIG_REQUIRE(ctx, batch >= 0 && table_width > 0 && max_length >= 0 && sinks >= 0, "paged attention: bad extents");
   AIG_REQUIRE(ctx, scale > 0.f && scale - scale == 0.f, "paged attention: the scale has to be positive and finite");
   if (batch == 0) return AIG_OK;
-  AIG_REQUIRE(ctx, heads_sane(q) && heads_sane(out) && table && lengths, "paged attention: null tensor or negative stride");
+  AIG_REQUIRE(ctx, heads_sane(q) && heads_sane(out) && table && lengths && aligned_to(table, 4) && aligned_to(lengths, 4),
+              "paged attention: null tensor, negative stride, or integers off a 4-byte boundary");
   AIG_REQUIRE(ctx, heads_vectorised(*q) && heads_vectorised(*out), "paged attention: q and out on 16-byte boundaries, strides multiples of 8");
   AIG_REQUIRE(ctx, q->heads == out->heads && q->heads % cache->kv_heads == 0, "paged attention: %d query heads, %d in the output, %d cached", q->heads,
               out->heads, cache->kv_heads);

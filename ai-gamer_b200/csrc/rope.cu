@@ -229,7 +229,7 @@ int turn_tensors(aig_rope_plan* pl, int dtype, const int32_t* positions, long lo
   if (rc != AIG_OK) return rc;
   AIG_REQUIRE(ctx, (k == nullptr) == (k_out == nullptr), "%s: k and k_out come together", who);
   if (k && (rc = check_pair(ctx, k, k_out, who)) != AIG_OK) return rc;
-  AIG_REQUIRE(ctx, positions, "%s: null positions", who);
+  AIG_REQUIRE(ctx, positions && aligned_to(positions, 4), "%s: null positions, or off a 4-byte boundary", who);
   RopeParams p{};
   p.part[0] = side_of(q, q_out);
   p.end[0] = p.end[1] = p.end[2] = q->heads;
@@ -334,7 +334,8 @@ int aig_kv_append(aig_ctx* ctx, const aig_kv_cache* cache, aig_rope_plan* rope, 
   AIG_REQUIRE(ctx, seqs || tokens <= batch, "kv append: %lld tokens without sequence numbers for a batch of %d", tokens, batch);
   AIG_REQUIRE(ctx, !rope || (rope->ctx->device == ctx->device && rope->desc.head_dim == cache->head_dim),
               "kv append: the rope plan is for another device or head dimension");
-  AIG_REQUIRE(ctx, positions && table, "kv append: null positions or table");
+  AIG_REQUIRE(ctx, positions && table && aligned_to(positions, 4) && aligned_to(table, 4) && aligned_to(seqs, 4),
+              "kv append: null positions or table, or integers off a 4-byte boundary");
   RopeParams p{};
   if (q) p.part[0] = side_of(q, q_out);
   p.end[0] = q ? q->heads : 0;

@@ -1389,7 +1389,7 @@ int check_desc(aig_ctx* ctx, const aig_window_desc* d, const char* who) {
   AIG_REQUIRE(ctx, d->scale > 0.f && d->scale - d->scale == 0.f, "%s: the scale has to be positive and finite", who);
   if (d->head_dim != 64 && d->head_dim != 128)
     return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "%s: head dimension must be 64 or 128 (got %d)", who, d->head_dim);
-  if (d->batch > 65535 || d->heads > 65535) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "%s: more than 65535 sequences or heads", who);
+  if (d->kv_len > 1 << 30) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "%s: more than 2^30 keys", who);
   return AIG_OK;
 }
 WinParams params_of(const aig_window_desc* d) {
@@ -1531,7 +1531,8 @@ int aig_window_attention_forward(aig_ctx* ctx, const aig_window_desc* d, const a
   if (rc != AIG_OK) return rc;
   if (d->batch == 0 || d->q_len == 0) return AIG_OK;
   const int b = d->batch, tq = d->q_len, tk = d->kv_len, h = d->heads, hk = d->kv_heads;
-  AIG_REQUIRE(ctx, tensor_ok(q, b, tq, h) && tensor_ok(k, b, tk, hk) && tensor_ok(v, b, tk, hk) && tensor_ok(out, b, tq, h) && lse && aligned_to(lse, 4),
+  AIG_REQUIRE(ctx, tensor_ok(q, b, tq, h) && tensor_ok(k, b, tk, hk) && tensor_ok(v, b, tk, hk) && tensor_ok(out, b, tq, h) && lse && aligned_to(lse, 4) &&
+                       aligned_to(lengths, 4),
               "window attention: null tensor, data off a 16-byte boundary, or strides that are not positive multiples of 8");
   WinParams p = params_of(d);
   p.q = view_of(q);
@@ -1555,7 +1556,8 @@ int aig_window_attention_backward(aig_ctx* ctx, const aig_window_desc* d, const 
   const int b = d->batch, tq = d->q_len, tk = d->kv_len, h = d->heads, hk = d->kv_heads;
   AIG_REQUIRE(ctx, tq > 0, "window attention backward: no queries");
   AIG_REQUIRE(ctx, tensor_ok(q, b, tq, h) && tensor_ok(k, b, tk, hk) && tensor_ok(v, b, tk, hk) && tensor_ok(out, b, tq, h) && tensor_ok(dout, b, tq, h) &&
-                       tensor_ok(dq, b, tq, h) && tensor_ok(dk, b, tk, hk) && tensor_ok(dv, b, tk, hk) && lse && delta && aligned_to(lse, 4) && aligned_to(delta, 4),
+                       tensor_ok(dq, b, tq, h) && tensor_ok(dk, b, tk, hk) && tensor_ok(dv, b, tk, hk) && lse && delta && aligned_to(lse, 4) && aligned_to(delta, 4) &&
+                       aligned_to(lengths, 4),
               "window attention backward: null tensor, data off a 16-byte boundary, or strides that are not positive multiples of 8");
   WinParams p = params_of(d);
   p.q = view_of(q);

@@ -485,7 +485,8 @@ int aig_kv_copy_pages(aig_ctx* ctx, const aig_kv_cache* cache, const int32_t* sr
  * is the last of them.  Query head h reads cached head h / (q_heads / kv_heads); out = softmax(scale * q.k) v over the
  * visible positions: the last `window` (<= 0: all) and the first `sinks` (with a window).  Pages without a visible position are
  * not read and their table entries may be anything; a length of 0 or less gives zeros.  max_length is the host's bound of
- * the lengths: work is split by it, and lengths above it are as right, only slower.  head_dim 64 or 128. */
+ * the lengths: work is split by it, and lengths above it are as right, only slower.  scale positive; head_dim 64 or 128; q and
+ * out on 16-byte boundaries with strides that are multiples of 8, out may be q. */
 int aig_paged_attention(aig_ctx* ctx, const aig_kv_cache* cache, const aig_heads* q, const aig_heads* out, const int32_t* table, int table_width,
                         const int32_t* lengths, int batch, int max_length, float scale, int window, int sinks);
 
@@ -525,7 +526,8 @@ int aig_page_pool_shared(const aig_page_pool* pool, int page);
  * backward: from the forward's inputs, out, lse and the gradient dout, writes dq, dk, dv (each rounded once; dk and dv
  * summed over the query heads that read them, in a fixed order); rows at or behind a sequence's length are left as they
  * were.  delta: fp32 scratch of lse's shape, the caller's.
- * head_dim 64 or 128; data on 16-byte boundaries, strides multiples of 8. */
+ * scale positive; head_dim 64 or 128; data on 16-byte boundaries, strides positive multiples of 8 (of a dimension of one any
+ * multiple).  Outputs overlap no inputs.  A backward call has one query at least. */
 typedef struct aig_seq_heads {
   void* data;
   long long batch_stride, token_stride, head_stride;
