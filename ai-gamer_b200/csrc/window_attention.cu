@@ -224,8 +224,8 @@ struct FwdShape {
   static constexpr int kThreads = 128 + 128 * NT;
   static constexpr int kCtasPerSm = NT == 1 && D == 64 ? 2 : 1;
   // registers of the warps that fetch and issue, and of those that hold a row of scores: 128 x 64 + 256 x 216 of a block's 384 x 168,
-  // 128 x 40 + 128 x 208 of its 256 x 128; one tile of heads of 128 has enough
-  static constexpr int kFewer = NT == 2 ? 64 : D == 64 ? 40 : 0, kMore = NT == 2 ? 216 : 208;
+  // 128 x 64 + 128 x 192 of its 256 x 128 (with 40 the issuing warp spills: 72 us where it takes 69); one tile of heads of 128 has enough
+  static constexpr int kFewer = NT == 2 || D == 64 ? 64 : 0, kMore = NT == 2 ? 216 : 192;
   static constexpr int kTmemCols = NT == 2 ? 512 : 256;  // scores 128 columns a tile, then outputs D columns a tile
   static constexpr uint32_t kQ = NT * kTileBytes<D, kTile>;
   static constexpr size_t kSmem = kQ + 2 * kStages * kTileBytes<D, kTile> + 256;
@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(128, D == 64 ? 4 : 3) window_short_kernel(cons
 // queries of the group's heads pass by).  Each computes the weights again from lse: two more products than one kernel that
 // adds dQ into memory with atomics would need, but every sum has a fixed order.  A thread owns a row of scores, 64 columns of it
 // at a time.  Bound by the chain from products to exponentials to products: so two tiles are under way on an SM, in two groups of
-// 128 threads of one CTA or in two CTAs.  (2 x 4099, 16 heads of 64: 212 us; one tile of 128 at a time for both groups 257.)
+// 128 threads of one CTA or in two CTAs.  (2 x 4099, 16 heads of 64: 208 us; one tile of 128 at a time for both groups 257.)
 //
 // fp16 has few small numbers: weights of a row over thousands of keys, and dS of small gradients, would be rounded to
 // multiples of 2^-24.  So the weights are multiplied by 2^8, and dS by a power of two 2^k that follows the largest
@@ -697,7 +697,7 @@ struct Ring {
 // G groups of 128 threads, each with a tile of 64 rows of its own in hand.  A CTA of two groups has an SM to itself.  Heads of 64
 // leave room for two CTAs of one group, which hide each other's beginnings and ends too, but each is slower by itself: they are
 // taken where no CTA has more than its half SM's share of all tiles (`balanced` below).  2 x 4099 with a window of 1024, 16
-// heads: dQ 94 us with one group, 109 with two; dK and dV, where two sinks make one CTA the longest by far, 190 and 118; 128 x 64,
+// heads: dQ 92 us with one group, 109 with two; dK and dV, where two sinks make one CTA the longest by far, 190 and 116; 128 x 64,
 // 8 heads: 22 + 25 against 77 for both; 4096 without a window, 4 heads: 57 + 74 against 39 + 46.
 template <int D, int G>
 struct BwdShape {
@@ -798,7 +798,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   tc_fence_after();
   // of each stream: scores, dP; then each stream's two buffers for dS; then dQ
   const uint32_t tmem = *s_tmem, tdS = tmem + 2 * KR * ST, tdQ = tmem + 3 * KR * ST;
-  if (S::kCtasPerSm == 2 && warp < 4) fewer_registers<40>();
+  if (S::kCtasPerSm == 2 && warp < 4) fewer_registers<64>();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -829,6 +829,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
       for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, t, desc_k<kTile>(sQ, ks), desc_k<KR>(k, ks), idesc_s, ks != 0);
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) mma_ss(leader, t + KR, desc_k<kTile>(sG, ks), desc_k<KR>(v, ks), idesc_s, ks != 0);
+      // (whoever finds the scores finds their power too: awaited by each thread that scales, dQ of 2 x 4099 took 95 us, not 92)
+      if (kScaled && !warp_wait(st_full + 8 * kr.s, kr.ph, s_abort, p.gerr, 1129)) return false;
       commit(leader, sd_full + 8 * (u % ST));
       commit(leader, v_free + 8 * vr.s);
       kr.next();
@@ -880,7 +882,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
       }
     }
   } else if (warp >= 4) {
-    if (S::kCtasPerSm == 2) more_registers<208>();
+    if (S::kCtasPerSm == 2) more_registers<192>();
     const int w = (warp - 4) >> 2, q = warp & 3, in_tile = q * 32 + lane;
     const int stream = w % ST, half = H == 2 ? w : 0;
     const int row = r0 + in_tile, pos = off + row;
@@ -930,8 +932,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
       float r = 1.f;
       int step = 0;
       ok = warp_wait(sd_full + 8 * stream, (uint32_t)n & 1u, s_abort, p.gerr, 1128);
-      if (kScaled && ok) {
-        ok = warp_wait(st_full + 8 * s, kr.ph, s_abort, p.gerr, 1129);
+      if (kScaled) {
         r = pow2(s_power[s]);
         step = s_step[s];
       }
@@ -1125,7 +1126,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
   tc_fence_after();
   // of each group: 64 columns of scores, then weights, 64 of dP, then dS; then dV and dK
   const uint32_t tmem = *s_tmem, tdV = tmem + 128 * G, tdK = tdV + D;
-  if (S::kCtasPerSm == 2 && warp < 4) fewer_registers<40>();
+  if (S::kCtasPerSm == 2 && warp < 4) fewer_registers<64>();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -1247,7 +1248,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
       }
     }
   } else {
-    if (S::kCtasPerSm == 2) more_registers<208>();
+    if (S::kCtasPerSm == 2) more_registers<192>();
     const int w = (warp - 4) >> 2, q = warp & 3, in_tile = q * 32 + lane;
     const int key = j0 + in_tile;
     const uint32_t lanes = (uint32_t)(q * 32) << 16, t = tmem + 128 * w + lanes;
@@ -1469,7 +1470,7 @@ int forward(aig_ctx* ctx, WinParams& p) {
   if (rc == AIG_OK) rc = encode<T, D, kTile>(ctx, &mv, p.v, p.batch, p.kv_len, p.kv_heads);
   if (rc != AIG_OK) return rc;
   // Heads of 64 leave room for two CTAs with a tile of queries each on an SM, which hide each other's beginnings and ends (2 x 4099,
-  // 16 heads: 71 us; one CTA with two tiles 77); heads of 128 for one, whose two tiles share the keys they fetch.
+  // 16 heads: 69 us; one CTA with two tiles 77); heads of 128 for one, whose two tiles share the keys they fetch.
   if (D == 64 || p.q_len <= kTile) return launch_forward<T, D, 1>(ctx, p, mq, mk, mv);
   if constexpr (D == 128) return launch_forward<T, D, 2>(ctx, p, mq, mk, mv);
 }
