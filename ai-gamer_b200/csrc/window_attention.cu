@@ -463,14 +463,15 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
 
 // ---------------------------------------------------------------------------------------------
 // Forward, short sequences: 64 queries of a head per CTA of four warps, products by mma.sync.  A sequence of 64 is half a tile of
-// the tcgen05 kernel, whose CTA owns an SM and spends its time on the way there and back; of these CTAs four to an
-// SM hide one another's (1024 heads of 64 x 64: 11.6 us against 31.5).
+// the tcgen05 kernel, whose CTA owns an SM and spends its time on the way there and back; of these CTAs four or seven to an
+// SM hide one another's (1024 heads of 64 x 64: 8.7 us against 31.5; four to an SM 10.8).  One or two tiles of keys, fetched at once.
 constexpr int kShort = 64;
 
-template <int D>
+template <int D, int Tiles>
 struct ShortShape {
   static constexpr uint32_t kTileB = kShort * D * 2;
-  static constexpr size_t kSmem = 5 * kTileB;  // queries, two stages of keys and values
+  static constexpr size_t kSmem = (1 + 2 * Tiles) * kTileB;  // queries, keys and values
+  static constexpr int kCtasPerSm = Tiles == 1 && D == 64 ? 7 : 4;
 };
 
 // 64 rows of D elements, 16-byte pieces of a row exchanged so that those of eight rows fall into different banks
@@ -491,9 +492,9 @@ __device__ __forceinline__ void short_load(uint32_t to, const View& v, int b, in
   }
 }
 
-template <class T, int D>
-__global__ void __launch_bounds__(128, D == 64 ? 4 : 3) window_short_kernel(const __grid_constant__ WinParams p) {
-  using S = ShortShape<D>;
+template <class T, int D, int Tiles>
+__global__ void __launch_bounds__(128, (ShortShape<D, Tiles>::kCtasPerSm)) window_short_kernel(const __grid_constant__ WinParams p) {
+  using S = ShortShape<D, Tiles>;
   extern __shared__ __align__(128) uint8_t sm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int item = blockIdx.x;
@@ -506,10 +507,10 @@ __global__ void __launch_bounds__(128, D == 64 ? 4 : 3) window_short_kernel(cons
   const int rows_end = min(p.q_len, len - off);
   if (r0 >= rows_end) return;
   const KeyTiles kt = key_tiles<kShort>(off + r0, off + min(r0 + kShort, rows_end) - 1, p.window, p.sinks);
-  const int tiles = kt.sink_end + kt.end - kt.begin;
-  auto first_key = [&](int u) { return (u < kt.sink_end ? u : kt.begin + (u - kt.sink_end)) * kShort; };
+  const int tiles = Tiles == 1 ? 1 : kt.sink_end + kt.end - kt.begin;
+  auto first_key = [&](int u) { return Tiles == 1 ? 0 : (u < kt.sink_end ? u : kt.begin + (u - kt.sink_end)) * kShort; };
   const uint32_t sQ = smem_u32(sm);
-  auto stage = [&](int u) { return sQ + S::kTileB * (1 + 2 * (u & 1)); };  // keys, then values
+  auto stage = [&](int u) { return sQ + S::kTileB * (1 + 2 * u); };  // keys, then values
   auto fetch = [&](int u) {
     if (u < tiles) {
       short_load<T, D>(stage(u), p.k, b, kvh, first_key(u), len, threadIdx.x);
@@ -518,9 +519,9 @@ __global__ void __launch_bounds__(128, D == 64 ? 4 : 3) window_short_kernel(cons
     cp_async_commit();
   };
   short_load<T, D>(sQ, p.q, b, h, r0, rows_end, threadIdx.x);
-  fetch(0);
-  fetch(1);
-  cp_async_wait<1>();
+#pragma unroll
+  for (int u = 0; u < Tiles; ++u) fetch(u);
+  cp_async_wait<Tiles - 1>();
   __syncthreads();
   float o[D / 8][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};  // of rows lane/4 and lane/4 + 8 of the warp's 16
 #pragma unroll
@@ -531,7 +532,7 @@ __global__ void __launch_bounds__(128, D == 64 ? 4 : 3) window_short_kernel(cons
   const int first = off + r0 + warp * 16;  // position of the warp's first row
   for (int u = 0; u < tiles; ++u) {
     if (u > 0) {
-      cp_async_wait<1>();
+      cp_async_wait<0>();
       __syncthreads();
     }
     const uint32_t sK = stage(u), sV = sK + S::kTileB;
@@ -544,7 +545,7 @@ __global__ void __launch_bounds__(128, D == 64 ? 4 : 3) window_short_kernel(cons
       for (int e = 0; e < 4; ++e) sc[n][e] = (n & ~1) * 8 < keys ? 0.f : -INFINITY;
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
-      uint32_t qa[4];  // (read again for every tile: held, they would cost an SM one of five CTAs)
+      uint32_t qa[4];  // (read again for every tile: held, they would cost an SM some of its CTAs)
       ldmatrix4(sQ + short_at<D>(warp * 16 + (lane & 15), ks * 2 + (lane >> 4)), qa);
 #pragma unroll
       for (int n = 0; n < 8; n += 2) {
@@ -593,28 +594,26 @@ __global__ void __launch_bounds__(128, D == 64 ? 4 : 3) window_short_kernel(cons
       }
       ref[x] = top[x] == -INFINITY ? 0.f : top[x];  // a row that has seen no key yet
     }
+    uint32_t w[4][4];
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      if (ks * 16 >= keys) continue;
-      uint32_t w[4];
+    for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {  // rows lane/4 and + 8 of 8 keys, then of the next 8
         const float x = ex2(fmaf(sc[2 * ks + (e >> 1)][2 * (e & 1)], c, -ref[e & 1])), y = ex2(fmaf(sc[2 * ks + (e >> 1)][2 * (e & 1) + 1], c, -ref[e & 1]));
         sum[e & 1] += x + y;
-        w[e] = pack2<T>(x, y);
+        w[ks][e] = pack2<T>(x, y);
       }
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      if (ks * 16 >= keys) continue;
       const int r = ks * 16 + (lane & 15), c0 = lane >> 4;
 #pragma unroll
       for (int n = 0; n < D / 16; ++n) {
         uint32_t vb[4];
         ldmatrix4_trans(sV + short_at<D>(r, n * 2 + c0), vb);
-        mma16816<T>(o[2 * n], w, vb[0], vb[1]);
-        mma16816<T>(o[2 * n + 1], w, vb[2], vb[3]);
+        mma16816<T>(o[2 * n], w[ks], vb[0], vb[1]);
+        mma16816<T>(o[2 * n + 1], w[ks], vb[2], vb[3]);
       }
-    }
-    if (u + 1 < tiles) {
-      __syncthreads();
-      fetch(u + 2);
     }
   }
   // ---- results through the warp's own rows of the queries' place, so that they leave in 16-byte pieces
@@ -1446,14 +1445,14 @@ int launch_forward(aig_ctx* ctx, WinParams& p, const CUtensorMap& mq, const CUte
   return AIG_OK;
 }
 
-template <class T, int D>
+template <class T, int D, int Tiles>
 int launch_short(aig_ctx* ctx, WinParams& p) {
-  using S = ShortShape<D>;
+  using S = ShortShape<D, Tiles>;
   p.blocks = ceil_div(p.q_len, kShort);
   const long long grid = (long long)p.blocks * p.heads * p.batch;
   if (grid > 0x7fffffffll) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "window attention: too many rows for one call");
-  AIG_CUDA_OK(ctx, cudaFuncSetAttribute(window_short_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
-  window_short_kernel<T, D><<<(unsigned)grid, 128, S::kSmem, ctx->stream>>>(p);
+  if (S::kSmem > (48u << 10)) AIG_CUDA_OK(ctx, cudaFuncSetAttribute(window_short_kernel<T, D, Tiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
+  window_short_kernel<T, D, Tiles><<<(unsigned)grid, 128, S::kSmem, ctx->stream>>>(p);
   AIG_LAUNCH_OK(ctx);
   return AIG_OK;
 }
@@ -1461,9 +1460,12 @@ int launch_short(aig_ctx* ctx, WinParams& p) {
 template <class T, int D>
 int forward(aig_ctx* ctx, WinParams& p) {
   p.gerr = ctx->d_err;
-  // 128 keys of 64 or 64 of 128: at twice that the two kernels are level (1024 heads: 64 x 64 x 64 11.6 us against 31.5, 128 x 128 x 64
-  // 23 against 34, 256 x 256 x 64 in 512 heads 31 against 32; 64 x 64 x 128 21 against 36, 128 x 128 x 128 50 against 50)
-  if (p.kv_len * D <= 8192) return launch_short<T, D>(ctx, p);
+  // 128 keys of 64 or 64 of 128: at twice that the two kernels are level (1024 heads: 64 x 64 x 64 8.7 us against 31.5, 128 x 128 x 64
+  // 22 against 34, 256 x 256 x 64 in 512 heads 31 against 27; 64 x 64 x 128 17 against 36, 128 x 128 x 128 50 against 46)
+  if (p.kv_len <= kShort) return launch_short<T, D, 1>(ctx, p);
+  if constexpr (D == 64) {
+    if (p.kv_len <= 2 * kShort) return launch_short<T, D, 2>(ctx, p);
+  }
   CUtensorMap mq, mk, mv;
   int rc = encode<T, D, kTile>(ctx, &mq, p.q, p.batch, p.q_len, p.heads);
   if (rc == AIG_OK) rc = encode<T, D, kTile>(ctx, &mk, p.k, p.batch, p.kv_len, p.kv_heads);
