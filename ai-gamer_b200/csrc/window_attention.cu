@@ -9,6 +9,8 @@
 // weights go back to TMEM as 16-bit values over the scores and are the second product's A operand from there, V its B
 // operand as it lies in memory (MN-major).  Tiles that the window, the sinks and the causal order leave empty are not
 // visited; only tiles that they cut are masked.
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "long_context.h"
@@ -31,6 +33,8 @@ struct WinParams {
   int window, sinks;
   float scale;
   int blocks;  // of query rows per head
+  int first_block, split;  // of a launch of the dK and dV kernel: its first block of keys, log2 of CTAs per block
+  bool after;               // it overlaps the launch before it
   int* gerr;
 };
 
@@ -695,9 +699,15 @@ struct Ring {
 
 // G groups of 128 threads, each with a tile of 64 rows of its own in hand.  A CTA of two groups has an SM to itself.  Heads of 64
 // leave room for two CTAs of one group, which hide each other's beginnings and ends too, but each is slower by itself: they are
-// taken where no CTA has more than its half SM's share of all tiles (`balanced` below).  2 x 4099 with a window of 1024, 16
+// taken where no CTA has more than its half SM's share of all tiles.  2 x 4099 with a window of 1024, 16
 // heads: dQ 92 us with one group, 109 with two; dK and dV, where two sinks make one CTA the longest by far, 190 and 116; 128 x 64,
 // 8 heads: 22 + 25 against 77 for both; 4096 without a window, 4 heads: 57 + 74 against 39 + 46.
+//
+// A block of keys that many queries see (all heads of its group; all of a sequence where it holds a sink) is one long walk, and few
+// blocks leave SMs idle.  It is then shared by the CTAs of a cluster, a part of the queries each, joined through their shared memory
+// in a fixed order.  Blocks that only sinks make long get a launch of their own, beside that of the other blocks.  dK and dV of one
+// sequence, 8 query heads on one of 64: 4096 tokens 305 -> 75 us, with a window of 512 and 4 sinks 444 -> 69; 8 on 2 heads, 32768 tokens,
+// window 1024, 4 sinks 1817 -> 260 (heads of 128 1947 -> 300); 2 x 1000, 4 on 2 heads 26 -> 15.
 template <int D, int G>
 struct BwdShape {
   static constexpr int kCtasPerSm = G == 1 ? 2 : 1;
@@ -1034,7 +1044,34 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   }
 }
 
-template <class T, int D, int G>
+// A CTA's part of a key's dV and dK, kept in its shared memory: 128 rows of 2 D floats, 16-byte pieces exchanged so that eight threads'
+// own rows fall into different banks
+template <int D>
+__device__ __forceinline__ uint32_t kept_at(int r, int column) {
+  return (uint32_t)(r * 8 * D + ((column / 4 ^ (r & 7)) << 4));
+}
+template <int D, int N>
+__device__ __forceinline__ void keep_row(uint32_t taddr, uint32_t to, int r, int column, float f) {
+#pragma unroll
+  for (int c0 = 0; c0 < N; c0 += 32) {
+    uint32_t v[32];
+    tmem_ld_32x32(taddr + c0, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 32; e += 4)
+      asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + kept_at<D>(r, column + c0 + e)), "f"(__uint_as_float(v[e]) * f),
+                   "f"(__uint_as_float(v[e + 1]) * f), "f"(__uint_as_float(v[e + 2]) * f), "f"(__uint_as_float(v[e + 3]) * f)
+                   : "memory");
+  }
+}
+__device__ __forceinline__ float4 peer_load(uint32_t cluster_addr) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(cluster_addr) : "memory");
+  return x;
+}
+
+// Split: a block of keys is a cluster's, each of whose CTAs has a part of the queries.
+template <class T, int D, int G, bool Split>
 __global__ void __launch_bounds__(DkvShape<D, G>::kThreads, DkvShape<D, G>::kCtasPerSm)
 window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
                   const __grid_constant__ CUtensorMap mapG, const __grid_constant__ WinParams p) {
@@ -1043,9 +1080,14 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
   constexpr bool kScaled = std::is_same<T, __half>::value;
   extern __shared__ __align__(1024) uint8_t sm[];
   const uint32_t base = smem_u32(sm);
+  asm volatile("griddepcontrol.launch_dependents;");
+  // Where two launches overlap, the second ends after the first: its last CTA to start waits.
+  auto leave = [&] {
+    if (p.after && threadIdx.x == 0 && blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
+  };
   if (base & 1023u) {  // (never seen; tiles could not be fetched)
     if (threadIdx.x == 0) note_error(p.gerr, 1100);
-    return;
+    return leave();
   }
   const uint32_t sK = base, sV = sK + kTileBytes<D, kTile>, ring = base + S::kFixed;  // a stage: queries, gradients of outputs
   float* const s_lse = reinterpret_cast<float*>(sm + S::kTiles);  // [NS][64]: -lse in log2, plus the weights' power
@@ -1061,22 +1103,25 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
   volatile int* const s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
-  int item = blockIdx.x;
+  const int split = Split ? p.split : 0, parts = 1 << split, part = blockIdx.x & (parts - 1);
+  int item = blockIdx.x >> split;
   const int b = item % p.batch;
   item /= p.batch;
-  const int kvh = item % p.kv_heads, j0 = item / p.kv_heads * kTile;
+  const int kvh = item % p.kv_heads, j0 = (p.first_block + item / p.kv_heads) * kTile;
   const int group = p.heads / p.kv_heads;
-  const int len = p.lengths ? min(max(p.lengths[b], 0), p.kv_len) : p.kv_len;
+  const int len = p.lengths ? min(max(__ldcg(p.lengths + b), 0), p.kv_len) : p.kv_len;
   const int off = p.kv_len - p.q_len;
   const int rows_end = min(p.q_len, len - off);
-  if (j0 >= len) return;
+  if (j0 >= len) return leave();
   // tiles of queries that see a key of this one: rows from the first key's position on, as far as the window of the last key
   // reaches, or all where a key is a sink
   const int j1 = min(j0 + kTile, len) - 1;
   const int row_first = max(0, j0 - off);
   const int row_last = p.window > 0 && j0 >= p.sinks ? min(rows_end - 1, j1 + p.window - 1 - off) : rows_end - 1;
   const int t_first = row_first / kSub, per_head = row_last < row_first ? 0 : row_last / kSub - t_first + 1;
-  const int tiles = per_head * group;
+  const int all_tiles = per_head * group;
+  auto part_begin = [&](int r) { return (all_tiles >> split) * r + min(r, all_tiles & (parts - 1)); };
+  const int begin = part_begin(part), tiles = part_begin(part + 1) - begin;
   // the tiles one after the other: those of a head, then the next head's
   struct Walk {
     int t, h, per_head;
@@ -1087,16 +1132,18 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
       }
     }
   };
-  const Walk start{0, kvh * group, per_head};
+  // (the same for all threads, which the compiler has to know: products are issued from uniform registers)
+  const int skipped = !Split || per_head == 0 ? 0 : __shfl_sync(0xffffffffu, begin / per_head, 0);
+  const Walk start{begin - skipped * per_head, kvh * group + skipped, per_head};
   auto first_row = [&](const Walk& at) { return (t_first + at.t) * kSub; };
 
-  if (tiles == 0) {  // no query sees these keys
-    for (int i = threadIdx.x; i < (j1 - j0 + 1) * (D / 8); i += S::kThreads) {
+  if (all_tiles == 0) {  // no query sees these keys
+    for (int i = threadIdx.x; part == 0 && i < (j1 - j0 + 1) * (D / 8); i += S::kThreads) {
       const int j = j0 + i / (D / 8), c = i % (D / 8) * 8;
       *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.dk.data) + b * p.dk.batch + j * p.dk.token + kvh * p.dk.head + c) = make_uint4(0, 0, 0, 0);
       *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.dv.data) + b * p.dv.batch + j * p.dv.token + kvh * p.dv.head + c) = make_uint4(0, 0, 0, 0);
     }
-    return;
+    return leave();
   }
 
   if (threadIdx.x == 0) {
@@ -1128,7 +1175,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
   if (S::kCtasPerSm == 2 && warp < 4) fewer_registers<64>();
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (lane == 0 && (!Split || tiles > 0)) {
       mbar_expect_tx(kv_full, S::kFixed);
       load_tile<D, kTile, kSub>(sK, &mapK, kv_full, kvh, j0, b);
       load_tile<D, kTile, kSub>(sV, &mapV, kv_full, kvh, j0, b);
@@ -1169,7 +1216,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
       commit(leader, dp_full + 8 * (u % G));
       rp.next();
     };
-    bool ok = warp_wait(kv_full, 0, s_abort, p.gerr, 1143);
+    bool ok = (!Split || tiles > 0) && warp_wait(kv_full, 0, s_abort, p.gerr, 1143);
     for (int u = 0; u < G && u < tiles && ok; ++u) {
       ok = scores(u);
       if (ok) dps(u);
@@ -1206,8 +1253,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
       for (int i = 0; i < 2; ++i) {
         const int r = lane + 32 * i;
         const bool there = u < tiles && row + r < rows_end;
-        x[i].x = there ? p.lse[stat + r] : INFINITY;  // (a weight of 0)
-        x[i].y = there ? p.delta[stat + r] : 0.f;
+        x[i].x = there ? __ldcg(p.lse + stat + r) : INFINITY;  // (a weight of 0)
+        x[i].y = there ? __ldcg(p.delta + stat + r) : 0.f;
       }
     };
     float2 x[2];
@@ -1229,7 +1276,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
     }
   } else if (warp == 3) {
     // the power for dS
-    if (kScaled && warp_wait(kv_full, 0, s_abort, p.gerr, 1146)) {
+    if (kScaled && (!Split || tiles > 0) && warp_wait(kv_full, 0, s_abort, p.gerr, 1146)) {
       const int ev = tile_exponent<D, kTile>(sm + (sV - base), min(kTile, len - j0), lane) + (D == 64 ? 3 : 4);
       int k = kFirstPower;
       Ring<NS> ring_at;
@@ -1352,15 +1399,20 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
         at.next();
       }
     }
-    if (ok && warp_wait(all_done, 0, s_abort, p.gerr, 1153)) {
+    if (ok && (!Split || tiles > 0) && warp_wait(all_done, 0, s_abort, p.gerr, 1153)) {
       tc_fence_after();
       float f = p.scale;
       if (kScaled) f *= pow2(-s_power[(tiles - 1) % NS]);
       constexpr int kShare = D / G;
-      T* const dk = reinterpret_cast<T*>(p.dk.data) + b * p.dk.batch + key * p.dk.token + kvh * p.dk.head + w * kShare;
-      T* const dv = reinterpret_cast<T*>(p.dv.data) + b * p.dv.batch + key * p.dv.token + kvh * p.dv.head + w * kShare;
-      store_row<T, kShare>(tdV + lanes + w * kShare, dv, pow2(-kWeightBits<T>), key < len);
-      store_row<T, kShare>(tdK + lanes + w * kShare, dk, f, key < len);
+      if constexpr (!Split) {
+        T* const dk = reinterpret_cast<T*>(p.dk.data) + b * p.dk.batch + key * p.dk.token + kvh * p.dk.head + w * kShare;
+        T* const dv = reinterpret_cast<T*>(p.dv.data) + b * p.dv.batch + key * p.dv.token + kvh * p.dv.head + w * kShare;
+        store_row<T, kShare>(tdV + lanes + w * kShare, dv, pow2(-kWeightBits<T>), key < len);
+        store_row<T, kShare>(tdK + lanes + w * kShare, dk, f, key < len);
+      } else {  // (the tiles' places are free: every product is done)
+        keep_row<D, kShare>(tdV + lanes + w * kShare, base, in_tile, w * kShare, pow2(-kWeightBits<T>));
+        keep_row<D, kShare>(tdK + lanes + w * kShare, base, in_tile, D + w * kShare, f);
+      }
     }
   }
 
@@ -1373,6 +1425,35 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
     tc_fence_after();
     tmem_dealloc(tmem, S::kTmemCols);
   }
+  if constexpr (Split) {  // the parts' sums, in a fixed order: a share of the keys for each CTA, eight reads under way per thread
+    cluster_sync_all();
+    const int rows = kTile >> split, units = rows * (D / 2);  // of four columns of dV, then of dK
+    for (int i = threadIdx.x; i < units; i += S::kThreads << (3 - split)) {
+      float4 x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int n = k & (parts - 1), at = i + (k >> split) * S::kThreads;
+        x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (at < units && part_begin(n + 1) > part_begin(n))  // (a part may have had no queries)
+          x[k] = peer_load(mapa_shared(base + kept_at<D>(part * rows + at / (D / 2), at % (D / 2) * 4), (uint32_t)n));
+      }
+#pragma unroll
+      for (int step = 1; step < 8; step *= 2)
+#pragma unroll
+        for (int k = 0; k < 8; k += 2 * step)
+          if (step < parts) x[k] = make_float4(x[k].x + x[k + step].x, x[k].y + x[k + step].y, x[k].z + x[k + step].z, x[k].w + x[k + step].w);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int at = i + (k >> split) * S::kThreads, j = j0 + part * rows + at / (D / 2), c = at % (D / 2) * 4;
+        if ((k & (parts - 1)) != 0 || at >= units || j >= len) continue;
+        T* const to = c < D ? reinterpret_cast<T*>(p.dv.data) + b * p.dv.batch + j * p.dv.token + kvh * p.dv.head + c
+                            : reinterpret_cast<T*>(p.dk.data) + b * p.dk.batch + j * p.dk.token + kvh * p.dk.head + c - D;
+        *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(x[k].x, x[k].y), pack2<T>(x[k].z, x[k].w));
+      }
+    }
+    cluster_sync_all();  // nobody leaves while its shared memory is read
+  }
+  leave();
 }
 
 // (a stride of 0 over a dimension above 1 is refused: TMA has none)
@@ -1472,8 +1553,11 @@ int forward(aig_ctx* ctx, WinParams& p) {
   if (rc == AIG_OK) rc = encode<T, D, kTile>(ctx, &mv, p.v, p.batch, p.kv_len, p.kv_heads);
   if (rc != AIG_OK) return rc;
   // Heads of 64 leave room for two CTAs with a tile of queries each on an SM, which hide each other's beginnings and ends (2 x 4099,
-  // 16 heads: 69 us; one CTA with two tiles 77); heads of 128 for one, whose two tiles share the keys they fetch.
-  if (D == 64 || p.q_len <= kTile) return launch_forward<T, D, 1>(ctx, p, mq, mk, mv);
+  // 16 heads: 69 us; one CTA with two tiles 77); heads of 128 for one, whose two tiles share the keys they fetch, or
+  // with one tile where every tile finds an SM of its own (4096 without a window, 4 heads: 54 us against 59; 8 heads with a window of
+  // 256, twice as many tiles as SMs: 20 against 14).
+  const bool few = (long long)ceil_div(p.q_len, kTile) * p.heads * p.batch <= ctx->sm_count;
+  if (D == 64 || few || p.q_len <= kTile) return launch_forward<T, D, 1>(ctx, p, mq, mk, mv);
   if constexpr (D == 128) return launch_forward<T, D, 2>(ctx, p, mq, mk, mv);
 }
 template <class T, int D, int G>
@@ -1484,11 +1568,37 @@ int launch_dq(aig_ctx* ctx, const WinParams& p, unsigned grid, const CUtensorMap
   AIG_LAUNCH_OK(ctx);
   return AIG_OK;
 }
-template <class T, int D, int G>
-int launch_dkv(aig_ctx* ctx, const WinParams& p, unsigned grid, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mg) {
+// dK and dV of `blocks` blocks of 128 keys from the first on, each in `parts` CTAs of a cluster; `after`: beside the launch before it
+template <class T, int D, int G, bool Split>
+int launch_dkv(aig_ctx* ctx, WinParams p, int first, int blocks, int parts, bool after, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+               const CUtensorMap& mg) {
   using S = DkvShape<D, G>;
-  AIG_CUDA_OK(ctx, cudaFuncSetAttribute(window_dkv_kernel<T, D, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
-  window_dkv_kernel<T, D, G><<<grid, S::kThreads, S::kSmem, ctx->stream>>>(mq, mk, mv, mg, p);
+  static_assert(kTile * 2 * D * 4 <= S::kTiles, "a part's sums take the tiles' place");
+  p.first_block = first;
+  p.after = after;
+  p.split = parts == 8 ? 3 : parts >> 1;
+  const long long grid = (long long)blocks * p.kv_heads * p.batch * parts;
+  if (grid > 0x7fffffffll) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "window attention backward: too many rows for one call");
+  AIG_CUDA_OK(ctx, cudaFuncSetAttribute(window_dkv_kernel<T, D, G, Split>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(S::kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr;
+  if (Split) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = parts;
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (after) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  AIG_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, window_dkv_kernel<T, D, G, Split>, mq, mk, mv, mg, (const WinParams&)p));
   AIG_LAUNCH_OK(ctx);
   return AIG_OK;
 }
@@ -1506,20 +1616,37 @@ int backward(aig_ctx* ctx, WinParams& p) {
   const int blocks_kv = ceil_div(p.kv_len, kTile);
   const long long grid = (long long)p.blocks * p.heads * p.batch, grid_kv = (long long)blocks_kv * p.kv_heads * p.batch;
   if (grid > 0x7fffffffll || grid_kv > 0x7fffffffll) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "window attention backward: too many rows for one call");
-  if constexpr (D == 64) {
-    // tiles of 64 that pass by: of all CTAs together, of the longest for dQ and for dK and dV (a sink is seen by every query)
-    const double seen = p.window > 0 ? p.window + kTile : p.kv_len - 0.5 * p.q_len;
-    const double all = seen / kSub * grid;
-    const double longest = (p.window > 0 ? p.window + p.sinks + kTile : p.kv_len) / (double)kSub;
-    const double longest_kv = (p.window > 0 && p.sinks == 0 && p.window + kTile < p.q_len ? p.window + kTile : p.q_len) / (double)kSub * (p.heads / p.kv_heads);
-    auto balanced = [&](double most) { return most * 2 * ctx->sm_count <= all; };
-    rc = balanced(longest) ? launch_dq<T, D, 1>(ctx, p, (unsigned)grid, mq, mk, mv, mg) : launch_dq<T, D, 2>(ctx, p, (unsigned)grid, mq, mk, mv, mg);
-    if (rc != AIG_OK) return rc;
-    return balanced(longest_kv) ? launch_dkv<T, D, 1>(ctx, p, (unsigned)grid_kv, mq, mk, mv, mg) : launch_dkv<T, D, 2>(ctx, p, (unsigned)grid_kv, mq, mk, mv, mg);
-  } else {
-    rc = launch_dq<T, D, 2>(ctx, p, (unsigned)grid, mq, mk, mv, mg);
-    return rc != AIG_OK ? rc : launch_dkv<T, D, 2>(ctx, p, (unsigned)grid_kv, mq, mk, mv, mg);
-  }
+  // tiles of 64 that pass by: of all CTAs together, of the longest
+  const double sms = ctx->sm_count, reach = p.window > 0 ? (double)p.window + kTile : p.kv_len;
+  const double all = std::min(reach, p.kv_len - 0.5 * p.q_len) * p.blocks * p.batch * p.heads / kSub;
+  const bool two = D == 64 && (p.window > 0 ? reach + p.sinks : reach) / kSub * 2 * sms <= all;
+  if constexpr (D == 64) rc = two ? launch_dq<T, D, 1>(ctx, p, (unsigned)grid, mq, mk, mv, mg) : launch_dq<T, D, 2>(ctx, p, (unsigned)grid, mq, mk, mv, mg);
+  else rc = launch_dq<T, D, 2>(ctx, p, (unsigned)grid, mq, mk, mv, mg);
+  if (rc != AIG_OK) return rc;
+  const double group = (double)(p.heads / p.kv_heads) / kSub, heads = (double)p.kv_heads * p.batch;  // tiles per query that sees a block
+  auto keys = [&](int first, int blocks, bool after, double most, double all) {  // most: tiles of the longest block
+    if (blocks == 0) return (int)AIG_OK;
+    if constexpr (D == 64) {
+      if (most * 2 * sms <= all) return launch_dkv<T, D, 1, false>(ctx, p, first, blocks, 1, after, mq, mk, mv, mg);
+    }
+    int parts = 1;
+    double least = 1e300;
+    for (int n = 1; n <= 8; n *= 2) {
+      // a card of 148 SMs holds 74 clusters of two, 33 of four, 15 of eight; a CTA's beginning and end cost as much as three tiles, with
+      // the join as seven
+      const double waves = std::ceil(blocks * heads / (sms * (n == 1 ? 1. : n == 2 ? 0.5 : n == 4 ? 0.223 : 0.102)));
+      const double t = std::max(most, all / (blocks * heads) * waves) / n + (n == 1 ? 3 : 7) * waves;
+      if (t < least) least = t, parts = n;
+    }
+    return parts == 1 ? launch_dkv<T, D, 2, false>(ctx, p, first, blocks, 1, after, mq, mk, mv, mg)
+                      : launch_dkv<T, D, 2, true>(ctx, p, first, blocks, parts, after, mq, mk, mv, mg);
+  };
+  // one launch where the longest block holds nothing up, else two
+  const int sinks = p.window > 0 && reach < p.q_len ? std::min((int)(((long long)p.sinks + kTile - 1) / kTile), blocks_kv) : 0;  // blocks that every query sees
+  const double most = std::min(reach, (double)p.q_len) * group, of_sinks = p.q_len * group * sinks * heads;
+  if (sinks == 0 || p.q_len * group * sms <= 1.25 * (all + of_sinks)) return keys(0, blocks_kv, false, sinks ? p.q_len * group : most, all + of_sinks);
+  rc = keys(0, sinks, false, p.q_len * group, of_sinks);
+  return rc != AIG_OK ? rc : keys(sinks, blocks_kv - sinks, true, most, all);
 }
 
 }  // namespace

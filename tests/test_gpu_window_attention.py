@@ -333,3 +333,92 @@ def test_no_queries_leave_keys_without_gradient(env):
     grads = run_backward(env, q, k, v, out, lse, g, 50)
     check((out, lse) + grads, want, bound, ("out", "lse", "dq", "dk", "dv"))
     assert not grads[1][:, :400].any() and not grads[2][:, :400].any()
+
+
+SHARED = [
+    # few blocks of keys, each of which many queries see: several thread blocks share one; short sequences leave some of them nothing
+    (1, 700, 700, 8, 1, 0, 0, None),
+    (1, 700, 700, 3, 1, 0, 0, [70]),
+    (2, 1000, 1000, 4, 2, 0, 0, [1000, 130]),
+    (1, 90, 2000, 8, 1, 0, 0, None),
+    # the sinks' blocks in a launch of their own, next to the others'
+    (1, 1500, 1500, 8, 1, 100, 3, None),
+    (2, 1500, 1500, 8, 2, 100, 130, [1500, 200]),
+    (1, 900, 1200, 8, 1, 64, 1, [1100]),
+    (2, 600, 600, 8, 1, 1, 2, [600, 0]),
+    (1, 400, 1500, 6, 2, 30, 1600, None),
+    (24, 1000, 1000, 8, 2, 30, 1, None),
+]
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("B,Tq,Tk,H,KV,window,sinks,lengths", SHARED)
+def test_blocks_of_keys_that_many_queries_see(env, kind, d, B, Tq, Tk, H, KV, window, sinks, lengths):
+    test_forward_and_gradients(env, kind, d, B, Tq, Tk, H, KV, window, sinks, lengths)
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 2)])
+def test_fp16_gradients_that_grow_over_shared_blocks(env, d, window, sinks):
+    """Thread blocks that share a block of keys meet gradients of sizes that differ a thousandfold: each has its own power of two."""
+    import torch
+
+    T = 1200
+    q, k, v, g = tensors(41, torch.float32, 1, T, T, 8, 1, d)
+    size = torch.logspace(-3, 3, T, base=2 ** 3.3, device="cuda")[None, :, None, None]
+    q, k, v, g = q.half(), k.half(), v.half(), (g * size).half()
+    want, bound = R.window_attention(q, k, v, window, sinks, None, d ** -0.5, g)
+    out, lse = run_forward(env, q, k, v, window, sinks)
+    check(run_backward(env, q, k, v, out, lse, g, window, sinks), want, bound, ("dq", "dk", "dv"))
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lengths", [None, [2000, 150]])
+def test_what_follows_finds_all_gradients(env, lengths, d):
+    """The backward's last two launches overlap: a call right behind it, eager or in a graph, reads complete gradients, with the
+    same bits every time."""
+    import torch
+
+    U, pk = env, env.pkg()
+    ctx = U.ctx()
+    B, T, H = 2, 2000, 8
+    q, k, v, g = tensors(42, torch.bfloat16, B, T, T, H, 1, d)
+    n = None if lengths is None else torch.tensor(lengths, device="cuda").int()
+    out, dq = torch.zeros_like(q), torch.zeros_like(q)
+    lse, delta = torch.empty((B, H, T), device="cuda"), torch.empty((B, H, T), device="cuda")
+    dk, dv, seen = torch.zeros_like(k), torch.zeros_like(v), torch.zeros_like(q)
+    statistics = torch.zeros_like(lse)
+    wa, next_op = pk.WindowAttention(ctx, 64, 1), pk.WindowAttention(ctx)
+    torch.cuda.synchronize()
+
+    def step():
+        wa.forward(q, k, v, out, lse, n)
+        wa.backward(q, k, v, out, lse, g, dq, dk, dv, delta, n)
+        next_op.forward(q, dk, dv, seen, statistics, n)
+
+    step()
+    ctx.sync()
+    first = [x.clone() for x in (dk, dv, seen, statistics)]
+    again = torch.zeros_like(q)
+    next_op.forward(q, dk, dv, again, torch.empty_like(lse), n)
+    ctx.sync()
+    assert torch.equal(again, seen)
+    ctx.graph_begin()
+    step()
+    graph = ctx.graph_end()
+    for i in range(20):
+        for x in (dk, dv):
+            x.fill_(float("nan"))
+            if lengths is not None:
+                x[1, lengths[1]:] = 0
+        torch.cuda.synchronize()
+        ctx.graph_launch(graph) if i % 2 else step()
+        ctx.sync()
+        valid = slice(None) if lengths is None else slice(0, lengths[1])
+        for x, y in zip((dk, dv, seen), first):
+            assert torch.equal(x[0], y[0]) and torch.equal(x[1, valid], y[1, valid])
+    pk.lib().aig_graph_destroy(graph)
