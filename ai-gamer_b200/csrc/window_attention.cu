@@ -34,7 +34,7 @@ struct WinParams {
   float scale;
   int blocks;  // of query rows per head
   int first_block, split;  // of a launch of the dK and dV kernel: its first block of keys, log2 of CTAs per block
-  bool after;               // it overlaps the launch before it
+  bool leads, after;        // it overlaps the launch behind it, before it
   int* gerr;
 };
 
@@ -220,27 +220,63 @@ __device__ __forceinline__ KeyTiles key_tiles(int first, int last, int window, i
   return k;
 }
 
+// ---- CTAs of a cluster that share a sum: each keeps its part in its shared memory, rows of N floats, 16-byte pieces exchanged so that
+// eight threads' own rows fall into different banks
+template <int N>
+__device__ __forceinline__ uint32_t kept_at(int r, int column) {
+  return (uint32_t)(r * 4 * N + ((column / 4 ^ (r & 7)) << 4));
+}
+template <int N, int Columns>
+__device__ __forceinline__ void keep_row(uint32_t taddr, uint32_t to, int r, int column, float f) {
+#pragma unroll
+  for (int c0 = 0; c0 < Columns; c0 += 32) {
+    uint32_t v[32];
+    tmem_ld_32x32(taddr + c0, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 32; e += 4)
+      asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + kept_at<N>(r, column + c0 + e)), "f"(__uint_as_float(v[e]) * f),
+                   "f"(__uint_as_float(v[e + 1]) * f), "f"(__uint_as_float(v[e + 2]) * f), "f"(__uint_as_float(v[e + 3]) * f)
+                   : "memory");
+  }
+}
+__device__ __forceinline__ float2 peer_load2(uint32_t cluster_addr) {
+  float2 x;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(cluster_addr) : "memory");
+  return x;
+}
+__device__ __forceinline__ float4 peer_load(uint32_t cluster_addr) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(cluster_addr) : "memory");
+  return x;
+}
+
+// first of n units of work of part r of 2^split
+__device__ __forceinline__ int part_begin(int n, int split, int r) { return (n >> split) * r + min(r, n & ((1 << split) - 1)); }
+
 // ---------------------------------------------------------------------------------------------
 // Forward
-template <int D, int NT>  // NT tiles of queries
+template <int D, int NT, bool Split>  // NT tiles of queries
 struct FwdShape {
   static constexpr int kStages = D == 64 ? 3 : 2;
   static constexpr int kThreads = 128 + 128 * NT;
-  static constexpr int kCtasPerSm = NT == 1 && D == 64 ? 2 : 1;
+  static constexpr int kCtasPerSm = NT == 1 && D == 64 && !Split ? 2 : 1;
   // registers of the warps that fetch and issue, and of those that hold a row of scores: 128 x 64 + 256 x 216 of a block's 384 x 168,
-  // 128 x 64 + 128 x 192 of its 256 x 128 (with 40 the issuing warp spills: 72 us where it takes 69); one tile of heads of 128 has enough
-  static constexpr int kFewer = NT == 2 || D == 64 ? 64 : 0, kMore = NT == 2 ? 216 : 192;
+  // 128 x 64 + 128 x 192 of its 256 x 128 (with 40 the issuing warp spills: 72 us where it takes 69); one CTA of one tile to an SM has enough
+  static constexpr int kFewer = NT == 2 || kCtasPerSm == 2 ? 64 : 0, kMore = NT == 2 ? 216 : 192;
   static constexpr int kTmemCols = NT == 2 ? 512 : 256;  // scores 128 columns a tile, then outputs D columns a tile
   static constexpr uint32_t kQ = NT * kTileBytes<D, kTile>;
   static constexpr size_t kSmem = kQ + 2 * kStages * kTileBytes<D, kTile> + 256;
 };
 constexpr float kLazy = 8.f;  // a row's maximum may grow by 2^8 before its sums are rescaled: weights stay below 2^8
 
-template <class T, int D, int NT>
-__global__ void __launch_bounds__(FwdShape<D, NT>::kThreads, FwdShape<D, NT>::kCtasPerSm)
+// Split: a tile of queries is a cluster's, each of whose CTAs has a part of the keys.
+template <class T, int D, int NT, bool Split>
+__global__ void __launch_bounds__((FwdShape<D, NT, Split>::kThreads), (FwdShape<D, NT, Split>::kCtasPerSm))
 window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
                       const __grid_constant__ WinParams p) {
-  using S = FwdShape<D, NT>;
+  static_assert(!Split || NT == 1, "one tile of queries is shared");
+  using S = FwdShape<D, NT, Split>;
   constexpr int NS = S::kStages;
   extern __shared__ __align__(1024) uint8_t sm[];
   const uint32_t base = smem_u32(sm);
@@ -255,10 +291,12 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
                  k_free = k_full + 8 * NS, v_full = k_free + 8 * NS, v_free = v_full + 8 * NS;
   uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bars + 1 + 3 * NT + 4 * NS);
   volatile int* const s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
+  float2* const s_stat = reinterpret_cast<float2*>(sm + kTile * D * 4);  // [128], behind a part's rows
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
   // the blocks of the last queries, which see the most keys, come first
-  int item = blockIdx.x;
+  const int split = Split ? p.split : 0, parts = 1 << split, part = blockIdx.x & (parts - 1);
+  int item = blockIdx.x >> split;
   const int b = item % p.batch;
   item /= p.batch;
   const int h = item % p.heads, block = p.blocks - 1 - item / p.heads;
@@ -280,8 +318,9 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
   }
   if (end == 0) return;  // no query row within the sequence
   begin = max(begin, sink_end);
-  const int tiles = sink_end + end - begin;
-  auto tile_at = [&](int it) { return it < sink_end ? it : begin + (it - sink_end); };
+  const int all_tiles = sink_end + end - begin;
+  const int skipped = part_begin(all_tiles, split, part), tiles = part_begin(all_tiles, split, part + 1) - skipped;
+  auto tile_at = [&](int it) { return (Split ? it + skipped : it) < sink_end ? (Split ? it + skipped : it) : begin + ((Split ? it + skipped : it) - sink_end); };
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -311,7 +350,7 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
 
   if (S::kFewer > 0 && warp < 4) fewer_registers<S::kFewer>();
   if (warp == 0) {
-    if (lane == 0) {
+    if (lane == 0 && (!Split || tiles > 0)) {
       mbar_expect_tx(q_full, S::kQ);
 #pragma unroll
       for (int w = 0; w < NT; ++w) load_tile<D, kTile, kTile>(sQ + w * kTileBytes<D, kTile>, &mapQ, q_full, h, (block * NT + w) * kTile, b);
@@ -340,7 +379,7 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
         commit(leader, s_full + 8 * w);
       }
     };
-    bool ok = warp_wait(q_full, 0, s_abort, p.gerr, 1103) && warp_wait(k_full, 0, s_abort, p.gerr, 1104);
+    bool ok = (!Split || tiles > 0) && warp_wait(q_full, 0, s_abort, p.gerr, 1103) && warp_wait(k_full, 0, s_abort, p.gerr, 1104);
     if (ok) {
       tc_fence_after();
 #pragma unroll
@@ -363,7 +402,7 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
                 mma_ts(leader, tO + D * w, tS + 128 * w + ks * 8, desc_rows<kTile>(sV + s * kTileBytes<D, kTile>, ks), idesc_o, done[w] != 0 || ks != 0);
             }
             ++done[w];
-            if (t + 1 == kt[w].end) commit(leader, o_full + 8 * w);
+            if (Split ? next == tiles : t + 1 == kt[w].end) commit(leader, o_full + 8 * w);
           }
           if (next < tiles && kt[w].has(tile_at(next))) scores(w, next);
         }
@@ -447,10 +486,15 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
     }
     if (ok && n > 0 && warp_wait(o_full + 8 * w, 0, s_abort, p.gerr, 1109)) {
       tc_fence_after();
-      const float inv = 1.f / sum;
-      T* const out = reinterpret_cast<T*>(p.o.data) + b * p.o.batch + row * p.o.token + h * p.o.head;
-      store_row<T, D>(tOw, out, inv, row < rows_end);
-      if (row < rows_end) p.lse[((long long)b * p.heads + h) * p.q_len + row] = fmaf(top, kLn2, logf(sum));
+      if constexpr (Split) {  // (the tiles' places are free: every product is done)
+        keep_row<D, D>(tOw, base, q * 32 + lane, 0, 1.f);
+        s_stat[q * 32 + lane] = make_float2(top, sum);
+      } else {
+        const float inv = 1.f / sum;
+        T* const out = reinterpret_cast<T*>(p.o.data) + b * p.o.batch + row * p.o.token + h * p.o.head;
+        store_row<T, D>(tOw, out, inv, row < rows_end);
+        if (row < rows_end) p.lse[((long long)b * p.heads + h) * p.q_len + row] = fmaf(top, kLn2, logf(sum));
+      }
     }
   }
 
@@ -462,6 +506,44 @@ window_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_con
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, S::kTmemCols);
+  }
+  if constexpr (Split) {  // the parts' sums, in a fixed order: a share of the rows for each CTA, eight reads under way per thread
+    cluster_sync_all();
+    const int rows = kTile >> split, units = rows * (D / 4);  // of four columns
+    for (int i = threadIdx.x; i < units; i += S::kThreads << (3 - split)) {
+      float4 x[8];
+      float2 stat[8];  // what the weights are relative to, their sum
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int n = k & (parts - 1), at = i + (k >> split) * S::kThreads, r = part * rows + at / (D / 4);
+        x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        stat[k] = make_float2(-INFINITY, 0.f);
+        if (at < units && part_begin(all_tiles, split, n + 1) > part_begin(all_tiles, split, n)) {  // (a part may have had no keys)
+          x[k] = peer_load(mapa_shared(base + kept_at<D>(r, at % (D / 4) * 4), (uint32_t)n));
+          stat[k] = peer_load2(mapa_shared(smem_u32(s_stat + r), (uint32_t)n));
+        }
+      }
+#pragma unroll
+      for (int step = 1; step < 8; step *= 2)
+#pragma unroll
+        for (int k = 0; k < 8; k += 2 * step)
+          if (step < parts) {
+            const float top = fmaxf(stat[k].x, stat[k + step].x), ref = top == -INFINITY ? 0.f : top;
+            const float f = ex2(stat[k].x - ref), g = ex2(stat[k + step].x - ref);
+            x[k] = make_float4(f * x[k].x + g * x[k + step].x, f * x[k].y + g * x[k + step].y, f * x[k].z + g * x[k + step].z, f * x[k].w + g * x[k + step].w);
+            stat[k] = make_float2(top, f * stat[k].y + g * stat[k + step].y);
+          }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int at = i + (k >> split) * S::kThreads, row = block * kTile + part * rows + at / (D / 4), c = at % (D / 4) * 4;
+        if ((k & (parts - 1)) != 0 || at >= units || row >= rows_end) continue;
+        const float inv = 1.f / stat[k].y;
+        T* const to = reinterpret_cast<T*>(p.o.data) + b * p.o.batch + row * p.o.token + h * p.o.head + c;
+        *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(x[k].x * inv, x[k].y * inv), pack2<T>(x[k].z * inv, x[k].w * inv));
+        if (c == 0) p.lse[((long long)b * p.heads + h) * p.q_len + row] = fmaf(stat[k].x, kLn2, logf(stat[k].y));
+      }
+    }
+    cluster_sync_all();  // nobody leaves while its shared memory is read
   }
 }
 
@@ -1044,32 +1126,6 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   }
 }
 
-// A CTA's part of a key's dV and dK, kept in its shared memory: 128 rows of 2 D floats, 16-byte pieces exchanged so that eight threads'
-// own rows fall into different banks
-template <int D>
-__device__ __forceinline__ uint32_t kept_at(int r, int column) {
-  return (uint32_t)(r * 8 * D + ((column / 4 ^ (r & 7)) << 4));
-}
-template <int D, int N>
-__device__ __forceinline__ void keep_row(uint32_t taddr, uint32_t to, int r, int column, float f) {
-#pragma unroll
-  for (int c0 = 0; c0 < N; c0 += 32) {
-    uint32_t v[32];
-    tmem_ld_32x32(taddr + c0, v);
-    tmem_ld_wait();
-#pragma unroll
-    for (int e = 0; e < 32; e += 4)
-      asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + kept_at<D>(r, column + c0 + e)), "f"(__uint_as_float(v[e]) * f),
-                   "f"(__uint_as_float(v[e + 1]) * f), "f"(__uint_as_float(v[e + 2]) * f), "f"(__uint_as_float(v[e + 3]) * f)
-                   : "memory");
-  }
-}
-__device__ __forceinline__ float4 peer_load(uint32_t cluster_addr) {
-  float4 x;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(cluster_addr) : "memory");
-  return x;
-}
-
 // Split: a block of keys is a cluster's, each of whose CTAs has a part of the queries.
 template <class T, int D, int G, bool Split>
 __global__ void __launch_bounds__(DkvShape<D, G>::kThreads, DkvShape<D, G>::kCtasPerSm)
@@ -1080,10 +1136,11 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
   constexpr bool kScaled = std::is_same<T, __half>::value;
   extern __shared__ __align__(1024) uint8_t sm[];
   const uint32_t base = smem_u32(sm);
-  asm volatile("griddepcontrol.launch_dependents;");
-  // Where two launches overlap, the second ends after the first: its last CTA to start waits.
+  // Where two launches overlap, the second ends after the first, so that what follows finds both complete: its last CTA waits.  (It
+  // starts once every CTA of the first has, and reads nothing that the first writes.)
+  if (p.leads) griddep_launch_dependents();
   auto leave = [&] {
-    if (p.after && threadIdx.x == 0 && blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (p.after && threadIdx.x == 0 && blockIdx.x == gridDim.x - 1) griddep_wait();
   };
   if (base & 1023u) {  // (never seen; tiles could not be fetched)
     if (threadIdx.x == 0) note_error(p.gerr, 1100);
@@ -1120,8 +1177,7 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
   const int row_last = p.window > 0 && j0 >= p.sinks ? min(rows_end - 1, j1 + p.window - 1 - off) : rows_end - 1;
   const int t_first = row_first / kSub, per_head = row_last < row_first ? 0 : row_last / kSub - t_first + 1;
   const int all_tiles = per_head * group;
-  auto part_begin = [&](int r) { return (all_tiles >> split) * r + min(r, all_tiles & (parts - 1)); };
-  const int begin = part_begin(part), tiles = part_begin(part + 1) - begin;
+  const int begin = part_begin(all_tiles, split, part), tiles = part_begin(all_tiles, split, part + 1) - begin;
   // the tiles one after the other: those of a head, then the next head's
   struct Walk {
     int t, h, per_head;
@@ -1410,8 +1466,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
         store_row<T, kShare>(tdV + lanes + w * kShare, dv, pow2(-kWeightBits<T>), key < len);
         store_row<T, kShare>(tdK + lanes + w * kShare, dk, f, key < len);
       } else {  // (the tiles' places are free: every product is done)
-        keep_row<D, kShare>(tdV + lanes + w * kShare, base, in_tile, w * kShare, pow2(-kWeightBits<T>));
-        keep_row<D, kShare>(tdK + lanes + w * kShare, base, in_tile, D + w * kShare, f);
+        keep_row<2 * D, kShare>(tdV + lanes + w * kShare, base, in_tile, w * kShare, pow2(-kWeightBits<T>));
+        keep_row<2 * D, kShare>(tdK + lanes + w * kShare, base, in_tile, D + w * kShare, f);
       }
     }
   }
@@ -1434,8 +1490,8 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
       for (int k = 0; k < 8; ++k) {
         const int n = k & (parts - 1), at = i + (k >> split) * S::kThreads;
         x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (at < units && part_begin(n + 1) > part_begin(n))  // (a part may have had no queries)
-          x[k] = peer_load(mapa_shared(base + kept_at<D>(part * rows + at / (D / 2), at % (D / 2) * 4), (uint32_t)n));
+        if (at < units && part_begin(all_tiles, split, n + 1) > part_begin(all_tiles, split, n))  // (a part may have had no queries)
+          x[k] = peer_load(mapa_shared(base + kept_at<2 * D>(part * rows + at / (D / 2), at % (D / 2) * 4), (uint32_t)n));
       }
 #pragma unroll
       for (int step = 1; step < 8; step *= 2)
@@ -1514,14 +1570,45 @@ int encode(aig_ctx* ctx, CUtensorMap* m, const View& v, int batch, int tokens, i
   return AIG_OK;
 }
 
-template <class T, int D, int NT>
-int launch_forward(aig_ctx* ctx, WinParams& p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv) {
-  using S = FwdShape<D, NT>;
+cudaLaunchAttribute cluster_attribute(int ctas) {
+  cudaLaunchAttribute a{};
+  a.id = cudaLaunchAttributeClusterDimension;
+  a.val.clusterDim.x = ctas;
+  a.val.clusterDim.y = a.val.clusterDim.z = 1;
+  return a;
+}
+// CTAs of a cluster that share a long walk over tiles: `blocks` of them, the longest of `most` tiles, `all` together, one CTA to an SM.
+// A card of 148 SMs holds 74 clusters of two, 33 of four, 15 of eight; a CTA's beginning and end cost as much as `alone` tiles, with the
+// join as `joined`.
+int cluster_size(double sms, double blocks, double most, double all, double alone, double joined) {
+  int size = 1;
+  double least = 1e300;
+  for (int n = 1; n <= 8; n *= 2) {
+    const double waves = std::ceil(blocks / (sms * (n == 1 ? 1. : n == 2 ? 0.5 : n == 4 ? 0.223 : 0.102)));
+    const double t = std::max(most, all / blocks * waves) / n + (n == 1 ? alone : joined) * waves;
+    if (t < least) least = t, size = n;
+  }
+  return size;
+}
+
+template <class T, int D, int NT, bool Split>
+int launch_forward(aig_ctx* ctx, WinParams& p, int parts, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv) {
+  using S = FwdShape<D, NT, Split>;
+  static_assert(!Split || kTile * (D + 2) * 4 <= S::kSmem - 256, "a part's sums take the tiles' place");
   p.blocks = ceil_div(p.q_len, kTile * NT);
-  const long long grid = (long long)p.blocks * p.heads * p.batch;
+  p.split = parts == 8 ? 3 : parts >> 1;
+  const long long grid = (long long)p.blocks * p.heads * p.batch * parts;
   if (grid > 0x7fffffffll) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "window attention: too many rows for one call");
-  AIG_CUDA_OK(ctx, cudaFuncSetAttribute(window_forward_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
-  window_forward_kernel<T, D, NT><<<(unsigned)grid, S::kThreads, S::kSmem, ctx->stream>>>(mq, mk, mv, p);
+  AIG_CUDA_OK(ctx, cudaFuncSetAttribute(window_forward_kernel<T, D, NT, Split>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(S::kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[1];
+  cfg.attrs = attr;
+  if (Split) attr[cfg.numAttrs++] = cluster_attribute(parts);
+  AIG_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, window_forward_kernel<T, D, NT, Split>, mq, mk, mv, (const WinParams&)p));
   AIG_LAUNCH_OK(ctx);
   return AIG_OK;
 }
@@ -1552,13 +1639,18 @@ int forward(aig_ctx* ctx, WinParams& p) {
   if (rc == AIG_OK) rc = encode<T, D, kTile>(ctx, &mk, p.k, p.batch, p.kv_len, p.kv_heads);
   if (rc == AIG_OK) rc = encode<T, D, kTile>(ctx, &mv, p.v, p.batch, p.kv_len, p.kv_heads);
   if (rc != AIG_OK) return rc;
+  // Where every tile of queries finds an SM of its own, or more, clusters share tiles that see many keys: 64 rows over 8192 keys, 8 heads
+  // of 128 on 2, 101 -> 21 us; 4096 rows of one head of 64 44 -> 16; 512 rows over 8192, 8 heads of 64 84 -> 27.
+  const double n = (double)ceil_div(p.q_len, kTile) * p.heads * p.batch, reach = p.window > 0 ? std::min(p.window + p.sinks + 2. * kTile, (double)p.kv_len) : p.kv_len;
+  if (n <= ctx->sm_count) {
+    const int parts = cluster_size(ctx->sm_count, n, reach / kTile, std::min(reach, p.kv_len - 0.5 * p.q_len) / kTile * n, 6, 9);
+    return parts == 1 ? launch_forward<T, D, 1, false>(ctx, p, 1, mq, mk, mv) : launch_forward<T, D, 1, true>(ctx, p, parts, mq, mk, mv);
+  }
   // Heads of 64 leave room for two CTAs with a tile of queries each on an SM, which hide each other's beginnings and ends (2 x 4099,
-  // 16 heads: 69 us; one CTA with two tiles 77); heads of 128 for one, whose two tiles share the keys they fetch, or
-  // with one tile where every tile finds an SM of its own (4096 without a window, 4 heads: 54 us against 59; 8 heads with a window of
-  // 256, twice as many tiles as SMs: 20 against 14).
-  const bool few = (long long)ceil_div(p.q_len, kTile) * p.heads * p.batch <= ctx->sm_count;
-  if (D == 64 || few || p.q_len <= kTile) return launch_forward<T, D, 1>(ctx, p, mq, mk, mv);
-  if constexpr (D == 128) return launch_forward<T, D, 2>(ctx, p, mq, mk, mv);
+  // 16 heads: 69 us; one CTA with two tiles 77); heads of 128 for one, whose two tiles share the keys they fetch (4096 without a window, 4
+  // heads, a tile for each SM: 59 us against 54; 8 heads with a window of 256, twice as many: 14 against 20).
+  if (D == 64 || p.q_len <= kTile) return launch_forward<T, D, 1, false>(ctx, p, 1, mq, mk, mv);
+  if constexpr (D == 128) return launch_forward<T, D, 2, false>(ctx, p, 1, mq, mk, mv);
 }
 template <class T, int D, int G>
 int launch_dq(aig_ctx* ctx, const WinParams& p, unsigned grid, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mg) {
@@ -1568,13 +1660,15 @@ int launch_dq(aig_ctx* ctx, const WinParams& p, unsigned grid, const CUtensorMap
   AIG_LAUNCH_OK(ctx);
   return AIG_OK;
 }
-// dK and dV of `blocks` blocks of 128 keys from the first on, each in `parts` CTAs of a cluster; `after`: beside the launch before it
+// dK and dV of `blocks` blocks of 128 keys from the first on, each in `parts` CTAs of a cluster; `leads`, `after`: beside the launch behind it,
+// before it
 template <class T, int D, int G, bool Split>
-int launch_dkv(aig_ctx* ctx, WinParams p, int first, int blocks, int parts, bool after, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+int launch_dkv(aig_ctx* ctx, WinParams p, int first, int blocks, int parts, bool leads, bool after, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                const CUtensorMap& mg) {
   using S = DkvShape<D, G>;
   static_assert(kTile * 2 * D * 4 <= S::kTiles, "a part's sums take the tiles' place");
   p.first_block = first;
+  p.leads = leads;
   p.after = after;
   p.split = parts == 8 ? 3 : parts >> 1;
   const long long grid = (long long)blocks * p.kv_heads * p.batch * parts;
@@ -1587,17 +1681,8 @@ int launch_dkv(aig_ctx* ctx, WinParams p, int first, int blocks, int parts, bool
   cfg.stream = ctx->stream;
   cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
-  if (Split) {
-    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    attr[cfg.numAttrs].val.clusterDim.x = parts;
-    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
-    ++cfg.numAttrs;
-  }
-  if (after) {
-    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
-    ++cfg.numAttrs;
-  }
+  if (Split) attr[cfg.numAttrs++] = cluster_attribute(parts);
+  if (after) attr[cfg.numAttrs++] = pdl_attribute(ctx);
   AIG_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, window_dkv_kernel<T, D, G, Split>, mq, mk, mv, mg, (const WinParams&)p));
   AIG_LAUNCH_OK(ctx);
   return AIG_OK;
@@ -1624,29 +1709,21 @@ int backward(aig_ctx* ctx, WinParams& p) {
   else rc = launch_dq<T, D, 2>(ctx, p, (unsigned)grid, mq, mk, mv, mg);
   if (rc != AIG_OK) return rc;
   const double group = (double)(p.heads / p.kv_heads) / kSub, heads = (double)p.kv_heads * p.batch;  // tiles per query that sees a block
-  auto keys = [&](int first, int blocks, bool after, double most, double all) {  // most: tiles of the longest block
+  auto keys = [&](int first, int blocks, bool leads, bool after, double most, double all) {  // most: tiles of the longest block
     if (blocks == 0) return (int)AIG_OK;
     if constexpr (D == 64) {
-      if (most * 2 * sms <= all) return launch_dkv<T, D, 1, false>(ctx, p, first, blocks, 1, after, mq, mk, mv, mg);
+      if (most * 2 * sms <= all) return launch_dkv<T, D, 1, false>(ctx, p, first, blocks, 1, leads, after, mq, mk, mv, mg);
     }
-    int parts = 1;
-    double least = 1e300;
-    for (int n = 1; n <= 8; n *= 2) {
-      // a card of 148 SMs holds 74 clusters of two, 33 of four, 15 of eight; a CTA's beginning and end cost as much as three tiles, with
-      // the join as seven
-      const double waves = std::ceil(blocks * heads / (sms * (n == 1 ? 1. : n == 2 ? 0.5 : n == 4 ? 0.223 : 0.102)));
-      const double t = std::max(most, all / (blocks * heads) * waves) / n + (n == 1 ? 3 : 7) * waves;
-      if (t < least) least = t, parts = n;
-    }
-    return parts == 1 ? launch_dkv<T, D, 2, false>(ctx, p, first, blocks, 1, after, mq, mk, mv, mg)
-                      : launch_dkv<T, D, 2, true>(ctx, p, first, blocks, parts, after, mq, mk, mv, mg);
+    const int parts = cluster_size(sms, blocks * heads, most, all, 3, 7);
+    return parts == 1 ? launch_dkv<T, D, 2, false>(ctx, p, first, blocks, 1, leads, after, mq, mk, mv, mg)
+                      : launch_dkv<T, D, 2, true>(ctx, p, first, blocks, parts, leads, after, mq, mk, mv, mg);
   };
   // one launch where the longest block holds nothing up, else two
   const int sinks = p.window > 0 && reach < p.q_len ? std::min((int)(((long long)p.sinks + kTile - 1) / kTile), blocks_kv) : 0;  // blocks that every query sees
   const double most = std::min(reach, (double)p.q_len) * group, of_sinks = p.q_len * group * sinks * heads;
-  if (sinks == 0 || p.q_len * group * sms <= 1.25 * (all + of_sinks)) return keys(0, blocks_kv, false, sinks ? p.q_len * group : most, all + of_sinks);
-  rc = keys(0, sinks, false, p.q_len * group, of_sinks);
-  return rc != AIG_OK ? rc : keys(sinks, blocks_kv - sinks, true, most, all);
+  if (sinks == 0 || p.q_len * group * sms <= 1.25 * (all + of_sinks)) return keys(0, blocks_kv, false, false, sinks ? p.q_len * group : most, all + of_sinks);
+  rc = keys(0, sinks, sinks < blocks_kv, false, p.q_len * group, of_sinks);
+  return rc != AIG_OK ? rc : keys(sinks, blocks_kv - sinks, false, true, most, all);
 }
 
 }  // namespace

@@ -422,3 +422,40 @@ def test_what_follows_finds_all_gradients(env, lengths, d):
         for x, y in zip((dk, dv, seen), first):
             assert torch.equal(x[0], y[0]) and torch.equal(x[1, valid], y[1, valid])
     pk.lib().aig_graph_destroy(graph)
+
+
+FEW = [
+    # few tiles of queries that see many keys: the keys are shared by several thread blocks, some of which may see none
+    (1, 70, 4000, 2, 1, 0, 0, None),
+    (1, 4000, 4000, 1, 1, 0, 0, [3900]),
+    (2, 300, 3000, 2, 1, 0, 0, [3000, 2701]),
+    (1, 128, 3000, 3, 3, 1500, 130, None),
+    (2, 200, 2500, 2, 2, 1000, 3, [2500, 2301]),
+    (1, 1, 5000, 1, 1, 0, 0, None),
+    (1, 257, 2000, 1, 1, 700, 1100, [1999]),
+    (2, 1030, 1030, 4, 2, 0, 0, None),
+]
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("B,Tq,Tk,H,KV,window,sinks,lengths", FEW)
+def test_few_queries_that_see_many_keys(env, kind, d, B, Tq, Tk, H, KV, window, sinks, lengths):
+    test_forward_and_gradients(env, kind, d, B, Tq, Tk, H, KV, window, sinks, lengths)
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_shared_keys_of_very_different_scores(env, d):
+    """Scores that grow along the keys by hundreds: the parts' maxima differ by more than fp32's exponents reach."""
+    import torch
+
+    q, k, v, g = tensors(43, torch.float32, 1, 130, 3000, 2, 1, d)
+    k = k + q[:, :1, :1] * torch.linspace(-3, 3, 3000, device="cuda")[None, :, None, None] * (q * q)[:, :1, :1].sum(-1, keepdim=True) ** -0.5 * 8
+    q = q + q[:, :1, :1] * 4
+    q, k, v, g = (x.bfloat16() for x in (q, k, v, g))
+    want, bound = R.window_attention(q, k, v, 0, 0, None, d ** -0.5, g)
+    out, lse = run_forward(env, q, k, v)
+    check((out, lse), want, bound, ("out", "lse"))
+    check(run_backward(env, q, k, v, out, lse, g), want, bound, ("dq", "dk", "dv"))
