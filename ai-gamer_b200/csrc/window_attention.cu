@@ -253,6 +253,32 @@ __device__ __forceinline__ float4 peer_load(uint32_t cluster_addr) {
 
 // first of n units of work of part r of 2^split
 __device__ __forceinline__ int part_begin(int n, int split, int r) { return (n >> split) * r + min(r, n & ((1 << split) - 1)); }
+// The parts' sums of a share of the 128 rows for each CTA, in a fixed order, eight reads under way per thread; `work`: units that were
+// shared (a part may have had none).  store(row, column, four sums).
+template <int N, int Threads, class Store>
+__device__ __forceinline__ void join_rows(uint32_t base, int work, int split, int part, Store store) {
+  const int parts = 1 << split, rows = kTile >> split, units = rows * (N / 4);  // of four columns
+  for (int i = threadIdx.x; i < units; i += Threads << (3 - split)) {
+    float4 x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int n = k & (parts - 1), at = i + (k >> split) * Threads;
+      x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (at < units && part_begin(work, split, n + 1) > part_begin(work, split, n))
+        x[k] = peer_load(mapa_shared(base + kept_at<N>(part * rows + at / (N / 4), at % (N / 4) * 4), (uint32_t)n));
+    }
+#pragma unroll
+    for (int step = 1; step < 8; step *= 2)
+#pragma unroll
+      for (int k = 0; k < 8; k += 2 * step)
+        if (step < parts) x[k] = make_float4(x[k].x + x[k + step].x, x[k].y + x[k + step].y, x[k].z + x[k + step].z, x[k].w + x[k + step].w);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int at = i + (k >> split) * Threads;
+      if ((k & (parts - 1)) == 0 && at < units) store(part * rows + at / (N / 4), at % (N / 4) * 4, x[k]);
+    }
+  }
+}
 
 // ---------------------------------------------------------------------------------------------
 // Forward
@@ -789,7 +815,8 @@ struct Ring {
 // blocks leave SMs idle.  It is then shared by the CTAs of a cluster, a part of the queries each, joined through their shared memory
 // in a fixed order.  Blocks that only sinks make long get a launch of their own, beside that of the other blocks.  dK and dV of one
 // sequence, 8 query heads on one of 64: 4096 tokens 305 -> 75 us, with a window of 512 and 4 sinks 444 -> 69; 8 on 2 heads, 32768 tokens,
-// window 1024, 4 sinks 1817 -> 260 (heads of 128 1947 -> 300); 2 x 1000, 4 on 2 heads 26 -> 15.
+// window 1024, 4 sinks 1817 -> 260 (heads of 128 1947 -> 300); 2 x 1000, 4 on 2 heads 26 -> 15.  So are dQ's tiles of queries where they
+// are no more than the SMs: 4096 tokens, one head of 64 38 -> 18, of 128 50 -> 23; 2048, 4 heads 23 -> 18, 30 -> 23.
 template <int D, int G>
 struct BwdShape {
   static constexpr int kCtasPerSm = G == 1 ? 2 : 1;
@@ -815,7 +842,8 @@ struct DkvShape : BwdShape<D, G> {
   static constexpr size_t kSmem = kTiles + kStages * kSub * 8 + 384;
 };
 
-template <class T, int D, int G>
+// Split: a tile of queries is a cluster's, each of whose CTAs has a part of the keys.
+template <class T, int D, int G, bool Split>
 __global__ void __launch_bounds__(DqShape<D, G>::kThreads, DqShape<D, G>::kCtasPerSm)
 window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
                  const __grid_constant__ CUtensorMap mapG, const __grid_constant__ WinParams p) {
@@ -842,7 +870,8 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   volatile int* const s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
-  int item = blockIdx.x;
+  const int split = Split ? p.split : 0, parts = 1 << split, part = blockIdx.x & (parts - 1);
+  int item = blockIdx.x >> split;
   const int b = item % p.batch;
   item /= p.batch;
   const int h = item % p.heads, block = p.blocks - 1 - item / p.heads;
@@ -856,9 +885,12 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   // first tile's keys take the sum of P o dP over them instead; with a window of few keys all rows do, in a pass of its own over
   // the tiles ahead of the one that adds up dQ.
   const int seen = kt.sink_end + kt.end - kt.begin;
-  const int ahead = p.window > 0 && p.window + p.sinks <= kSub ? seen : 0, tiles = ahead + seen;
+  const int ahead = !Split && p.window > 0 && p.window + p.sinks <= kSub ? seen : 0;
+  // (where rows see only the first tile's keys, there are few tiles: the first part has them all)
+  const bool shared = Split && (kt.sink_end > 0 ? 0 : kt.begin) * KR + KR <= off + r0;
+  const int skipped = shared ? part_begin(seen, split, part) : part == 0 ? 0 : seen, tiles = ahead + (shared ? part_begin(seen, split, part + 1) : seen) - skipped;
   auto first_key = [&](int u) {
-    const int t = u < ahead ? u : u - ahead;
+    const int t = (u < ahead ? u : u - ahead) + (Split ? skipped : 0);
     return (t < kt.sink_end ? t : kt.begin + (t - kt.sink_end)) * KR;
   };
 
@@ -892,7 +924,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   if (S::kCtasPerSm == 2 && warp < 4) fewer_registers<64>();
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (lane == 0 && (!Split || tiles > 0)) {
       mbar_expect_tx(q_full, S::kFixed);
       load_tile<D, kTile, kSub>(sQ, &mapQ, q_full, h, r0, b);
       load_tile<D, kTile, kSub>(sG, &mapG, q_full, h, r0, b);
@@ -937,7 +969,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
       commit(leader, k_free + 8 * kd.s);
       kd.next();
     };
-    bool ok = warp_wait(q_full, 0, s_abort, p.gerr, 1123);
+    bool ok = (!Split || tiles > 0) && warp_wait(q_full, 0, s_abort, p.gerr, 1123);
     for (int u = 0; u < ST && u < tiles && ok; ++u) ok = scores(u);
     for (int u = 0; u + ST < tiles && ok; ++u) {
       // The stream's threads have read tile u: they have written dS of their tile before.  That product goes ahead of the next scores, so that
@@ -954,7 +986,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
     }
     if (ok) commit(leader, dq_full);
   } else if (warp == 2) {
-    if (kScaled && warp_wait(q_full, 0, s_abort, p.gerr, 1126)) {
+    if (kScaled && (!Split || tiles > 0) && warp_wait(q_full, 0, s_abort, p.gerr, 1126)) {
       const int eg = tile_exponent<D, kTile>(sm + (sG - base), min(kTile, rows_end - r0), lane) + (D == 64 ? 3 : 4);
       int k = kFirstPower;
       Ring<NK> kr;
@@ -984,7 +1016,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
     const float lse2 = there ? p.lse[stat] * kLog2e : INFINITY;  // (weights of 0)
     // a query that sees one key has the weight 1 whatever its score: no gradient through it
     const bool single = pos == 0 || (p.window == 1 && p.sinks == 0);
-    const bool few = ahead == 0 && first_key(0) + KR > off + r0, mine_few = first_key(0) + KR > pos;
+    const bool few = ahead == 0 && !shared && first_key(0) + KR > off + r0, mine_few = first_key(0) + KR > pos;
     constexpr int kShare = D / G;  // a row's dot product and its result are shared by the groups
     float delta = 0.f;
     if (there && ahead == 0) {
@@ -1105,13 +1137,17 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
       for (int i = 0; i < ST; ++i) kr.next();
     }
     if (!joined) join();
-    if (ok && warp_wait(dq_full, 0, s_abort, p.gerr, 1132)) {
+    if (ok && (!Split || tiles > 0) && warp_wait(dq_full, 0, s_abort, p.gerr, 1132)) {
       tc_fence_after();
-      if (there && w == 0) p.delta[stat] = delta;
+      if (there && w == 0 && part == 0) p.delta[stat] = delta;
       float f = p.scale;
       if (kScaled) f *= pow2(-s_power[(tiles - 1) % NK]);
-      T* const out = reinterpret_cast<T*>(p.dq.data) + b * p.dq.batch + row * p.dq.token + h * p.dq.head + w * kShare;
-      store_row<T, kShare>(tdQ + lanes + w * kShare, out, f, there);
+      if constexpr (Split) {  // (the tiles' places are free: every product is done)
+        keep_row<D, kShare>(tdQ + lanes + w * kShare, base, in_tile, w * kShare, f);
+      } else {
+        T* const out = reinterpret_cast<T*>(p.dq.data) + b * p.dq.batch + row * p.dq.token + h * p.dq.head + w * kShare;
+        store_row<T, kShare>(tdQ + lanes + w * kShare, out, f, there);
+      }
     }
   }
 
@@ -1123,6 +1159,15 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, S::kTmemCols);
+  }
+  if constexpr (Split) {
+    cluster_sync_all();
+    join_rows<D, S::kThreads>(base, shared ? seen : 1, split, part, [&](int r, int c, float4 x) {
+      const int row = r0 + r;
+      if (row < rows_end)
+        *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.dq.data) + b * p.dq.batch + row * p.dq.token + h * p.dq.head + c) = make_uint2(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w));
+    });
+    cluster_sync_all();  // nobody leaves while its shared memory is read
   }
 }
 
@@ -1481,32 +1526,15 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
     tc_fence_after();
     tmem_dealloc(tmem, S::kTmemCols);
   }
-  if constexpr (Split) {  // the parts' sums, in a fixed order: a share of the keys for each CTA, eight reads under way per thread
+  if constexpr (Split) {
     cluster_sync_all();
-    const int rows = kTile >> split, units = rows * (D / 2);  // of four columns of dV, then of dK
-    for (int i = threadIdx.x; i < units; i += S::kThreads << (3 - split)) {
-      float4 x[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int n = k & (parts - 1), at = i + (k >> split) * S::kThreads;
-        x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (at < units && part_begin(all_tiles, split, n + 1) > part_begin(all_tiles, split, n))  // (a part may have had no queries)
-          x[k] = peer_load(mapa_shared(base + kept_at<2 * D>(part * rows + at / (D / 2), at % (D / 2) * 4), (uint32_t)n));
-      }
-#pragma unroll
-      for (int step = 1; step < 8; step *= 2)
-#pragma unroll
-        for (int k = 0; k < 8; k += 2 * step)
-          if (step < parts) x[k] = make_float4(x[k].x + x[k + step].x, x[k].y + x[k + step].y, x[k].z + x[k + step].z, x[k].w + x[k + step].w);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int at = i + (k >> split) * S::kThreads, j = j0 + part * rows + at / (D / 2), c = at % (D / 2) * 4;
-        if ((k & (parts - 1)) != 0 || at >= units || j >= len) continue;
-        T* const to = c < D ? reinterpret_cast<T*>(p.dv.data) + b * p.dv.batch + j * p.dv.token + kvh * p.dv.head + c
-                            : reinterpret_cast<T*>(p.dk.data) + b * p.dk.batch + j * p.dk.token + kvh * p.dk.head + c - D;
-        *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(x[k].x, x[k].y), pack2<T>(x[k].z, x[k].w));
-      }
-    }
+    join_rows<2 * D, S::kThreads>(base, all_tiles, split, part, [&](int r, int c, float4 x) {  // columns of dV, then of dK
+      const int j = j0 + r;
+      if (j >= len) return;
+      T* const to = c < D ? reinterpret_cast<T*>(p.dv.data) + b * p.dv.batch + j * p.dv.token + kvh * p.dv.head + c
+                          : reinterpret_cast<T*>(p.dk.data) + b * p.dk.batch + j * p.dk.token + kvh * p.dk.head + c - D;
+      *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w));
+    });
     cluster_sync_all();  // nobody leaves while its shared memory is read
   }
   leave();
@@ -1652,11 +1680,21 @@ int forward(aig_ctx* ctx, WinParams& p) {
   if (D == 64 || p.q_len <= kTile) return launch_forward<T, D, 1, false>(ctx, p, 1, mq, mk, mv);
   if constexpr (D == 128) return launch_forward<T, D, 2, false>(ctx, p, 1, mq, mk, mv);
 }
-template <class T, int D, int G>
-int launch_dq(aig_ctx* ctx, const WinParams& p, unsigned grid, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mg) {
+template <class T, int D, int G, bool Split>
+int launch_dq(aig_ctx* ctx, WinParams p, int parts, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mg) {
   using S = DqShape<D, G>;
-  AIG_CUDA_OK(ctx, cudaFuncSetAttribute(window_dq_kernel<T, D, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
-  window_dq_kernel<T, D, G><<<grid, S::kThreads, S::kSmem, ctx->stream>>>(mq, mk, mv, mg, p);
+  static_assert(kTile * D * 4 <= S::kTiles, "a part's sums take the tiles' place");
+  p.split = parts == 8 ? 3 : parts >> 1;
+  AIG_CUDA_OK(ctx, cudaFuncSetAttribute(window_dq_kernel<T, D, G, Split>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)p.blocks * p.heads * p.batch * parts);
+  cfg.blockDim = dim3(S::kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[1];
+  cfg.attrs = attr;
+  if (Split) attr[cfg.numAttrs++] = cluster_attribute(parts);
+  AIG_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, window_dq_kernel<T, D, G, Split>, mq, mk, mv, mg, (const WinParams&)p));
   AIG_LAUNCH_OK(ctx);
   return AIG_OK;
 }
@@ -1704,9 +1742,13 @@ int backward(aig_ctx* ctx, WinParams& p) {
   // tiles of 64 that pass by: of all CTAs together, of the longest
   const double sms = ctx->sm_count, reach = p.window > 0 ? (double)p.window + kTile : p.kv_len;
   const double all = std::min(reach, p.kv_len - 0.5 * p.q_len) * p.blocks * p.batch * p.heads / kSub;
-  const bool two = D == 64 && (p.window > 0 ? reach + p.sinks : reach) / kSub * 2 * sms <= all;
-  if constexpr (D == 64) rc = two ? launch_dq<T, D, 1>(ctx, p, (unsigned)grid, mq, mk, mv, mg) : launch_dq<T, D, 2>(ctx, p, (unsigned)grid, mq, mk, mv, mg);
-  else rc = launch_dq<T, D, 2>(ctx, p, (unsigned)grid, mq, mk, mv, mg);
+  const double most_dq = p.window > 0 ? std::min(reach + p.sinks, (double)p.kv_len) : p.kv_len;
+  const bool two = D == 64 && most_dq / kSub * 2 * sms <= all, again = p.window > 0 && p.window + p.sinks <= kSub;  // (again: two passes over the keys, few)
+  constexpr int kr = DqShape<D, 2>::kKeyRows;
+  const int parts = two || again || grid > ctx->sm_count ? 1 : cluster_size(sms, (double)grid, most_dq / kr, all * kSub / kr, 512. / kr, 900. / kr);
+  if (parts > 1) rc = launch_dq<T, D, 2, true>(ctx, p, parts, mq, mk, mv, mg);
+  else if (D == 64 && two) rc = launch_dq<T, D, D == 64 ? 1 : 2, false>(ctx, p, 1, mq, mk, mv, mg);
+  else rc = launch_dq<T, D, 2, false>(ctx, p, 1, mq, mk, mv, mg);
   if (rc != AIG_OK) return rc;
   const double group = (double)(p.heads / p.kv_heads) / kSub, heads = (double)p.kv_heads * p.batch;  // tiles per query that sees a block
   auto keys = [&](int first, int blocks, bool leads, bool after, double most, double all) {  // most: tiles of the longest block

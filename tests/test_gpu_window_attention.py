@@ -459,3 +459,20 @@ def test_shared_keys_of_very_different_scores(env, d):
     out, lse = run_forward(env, q, k, v)
     check((out, lse), want, bound, ("out", "lse"))
     check(run_backward(env, q, k, v, out, lse, g), want, bound, ("dq", "dk", "dv"))
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window,sinks,Tq", [(0, 0, 2500), (0, 0, 100), (900, 2, 400)])
+def test_fp16_gradients_over_shared_keys_of_growing_values(env, d, window, sinks, Tq):
+    """Thread blocks that share a tile of queries meet values that differ a thousandfold: each has its own power of two."""
+    import torch
+
+    T = 2500
+    q, k, v, g = tensors(44, torch.float32, 1, Tq, T, 1, 1, d)
+    v = v * torch.logspace(-3, 3, T, base=2 ** 3.3, device="cuda")[None, :, None, None]
+    q, k, v, g = q.half(), k.half(), v.half(), (g * 2.0 ** -6).half()
+    want, bound = R.window_attention(q, k, v, window, sinks, None, d ** -0.5, g)
+    out, lse = run_forward(env, q, k, v, window, sinks)
+    check((out, lse), want, bound, ("out", "lse"))
+    check(run_backward(env, q, k, v, out, lse, g, window, sinks), want, bound, ("dq", "dk", "dv"))
