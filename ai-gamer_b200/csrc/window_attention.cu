@@ -790,6 +790,198 @@ __device__ __forceinline__ int next_power(int k, int e) {
 }
 constexpr int kFirstPower = 100;
 
+// ---------------------------------------------------------------------------------------------
+// Backward, sequences of one tile of 64 keys: a cached head of a sequence per CTA of four warps, products by mma.sync, all three
+// gradients at once.  A warp has 16 queries for scores, weights, dS and dQ, then 16 keys for dV = P^T dO and dK = dS^T Q, whose
+// operands come through shared memory; the heads of the group follow one another, 4 us each.  D = sum of P o dP, in fp32: every visible key is at
+// hand.  Bound, like the forward, by the way there and back, which several CTAs to an SM hide.
+template <int D>
+struct ShortGradShape {
+  static constexpr uint32_t kTileB = kShort * D * 2, kWeights = kShort * kShort * 2;
+  static constexpr size_t kSmem = 4 * kTileB + 2 * kWeights + 64;  // keys, values, queries, gradients of outputs; weights, dS; largest |dS| of each warp
+  static constexpr int kCtasPerSm = D == 64 ? 3 : 2;
+};
+// acc += A^T B over `rows` rows: 16 columns of A (64 wide) from `column` on, B of D columns
+template <class T, int D>
+__device__ __forceinline__ void short_product(float (&acc)[D / 8][4], uint32_t a, uint32_t b, int column, int rows, int lane) {
+#pragma unroll
+  for (int ks = 0; ks < kShort / 16; ++ks) {
+    if (ks * 16 >= rows) break;
+    uint32_t w[4];
+    ldmatrix4_trans(a + short_at<kShort>(ks * 16 + (lane & 7) + ((lane >> 4) << 3), column / 8 + ((lane >> 3) & 1)), w);
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) {
+      uint32_t vb[4];
+      ldmatrix4_trans(b + short_at<D>(ks * 16 + (lane & 15), n * 2 + (lane >> 4)), vb);
+      mma16816<T>(acc[2 * n], w, vb[0], vb[1]);
+      mma16816<T>(acc[2 * n + 1], w, vb[2], vb[3]);
+    }
+  }
+}
+// 16 rows that a warp holds, times f, through its rows of `tile`, to memory in 16-byte pieces; rows before `end`
+template <class T, int D>
+__device__ __forceinline__ void short_store(const float (&acc)[D / 8][4], float f, uint8_t* tile, const View& v, int b, int h, int first, int end, int lane) {
+  __syncwarp();
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+      *reinterpret_cast<uint32_t*>(tile + short_at<D>(first + (lane >> 2) + 8 * x, n) + (lane & 3) * 4) = pack2<T>(acc[n][2 * x] * f, acc[n][2 * x + 1] * f);
+  __syncwarp();
+  T* const out = reinterpret_cast<T*>(v.data) + b * v.batch + h * v.head;
+#pragma unroll
+  for (int i = 0; i < 16 * (D / 8) / 32; ++i) {
+    const int r = first + (i * 32 + lane) / (D / 8), piece = (i * 32 + lane) % (D / 8);
+    if (r < end) *reinterpret_cast<uint4*>(out + r * v.token + piece * 8) = *reinterpret_cast<const uint4*>(tile + short_at<D>(r, piece));
+  }
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(128, ShortGradShape<D>::kCtasPerSm) window_short_backward_kernel(const __grid_constant__ WinParams p) {
+  using S = ShortGradShape<D>;
+  constexpr bool kScaled = std::is_same<T, __half>::value;
+  extern __shared__ __align__(128) uint8_t sm[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.x % p.batch, kvh = blockIdx.x / p.batch, group = p.heads / p.kv_heads;
+  const int len = p.lengths ? min(max(p.lengths[b], 0), p.kv_len) : p.kv_len;
+  const int off = p.kv_len - p.q_len;
+  const int rows_end = min(p.q_len, len - off);
+  if (len == 0) return;
+  uint8_t* const tQ = sm + 2 * S::kTileB;
+  const uint32_t sK = smem_u32(sm), sV = sK + S::kTileB, sQ = sV + S::kTileB, sG = sQ + S::kTileB, sP = sG + S::kTileB, sD = sP + S::kWeights;
+  uint8_t* const tP = sm + 4 * S::kTileB;
+  float* const s_most = reinterpret_cast<float*>(tP + 2 * S::kWeights);  // [4]
+  float dk[D / 8][4], dv[D / 8][4];
+#pragma unroll
+  for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) dk[n][e] = dv[n][e] = 0.f;
+  if (rows_end > 0) {
+    short_load<T, D>(sK, p.k, b, kvh, 0, len, threadIdx.x);
+    short_load<T, D>(sV, p.v, b, kvh, 0, len, threadIdx.x);
+  }
+  const float c = p.scale * kLog2e;
+  const int first = off + warp * 16, keys = warp * 16 < rows_end ? min(first + 16, len) : 0;  // of the warp's rows: position, keys up to the last one's own
+  int power = kFirstPower;  // of dS in the sums for dK
+  for (int i = 0; i < group && rows_end > 0; ++i) {
+    const int h = kvh * group + i;
+    short_load<T, D>(sQ, p.q, b, h, 0, rows_end, threadIdx.x);
+    short_load<T, D>(sG, p.dout, b, h, 0, rows_end, threadIdx.x);
+    cp_async_commit();
+    cp_async_wait<0>();
+    __syncthreads();
+    float sc[8][4], dp[8][4];
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[n][e] = dp[n][e] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      uint32_t qa[4], ga[4];
+      ldmatrix4(sQ + short_at<D>(warp * 16 + (lane & 15), ks * 2 + (lane >> 4)), qa);
+      ldmatrix4(sG + short_at<D>(warp * 16 + (lane & 15), ks * 2 + (lane >> 4)), ga);
+#pragma unroll
+      for (int n = 0; n < 8; n += 2) {
+        if (n * 8 >= keys) continue;
+        uint32_t kb[4];
+        ldmatrix4(sK + short_at<D>(n * 8 + (lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)), kb);
+        mma16816<T>(sc[n], qa, kb[0], kb[1]);
+        mma16816<T>(sc[n + 1], qa, kb[2], kb[3]);
+        ldmatrix4(sV + short_at<D>(n * 8 + (lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)), kb);
+        mma16816<T>(dp[n], ga, kb[0], kb[1]);
+        mma16816<T>(dp[n + 1], ga, kb[2], kb[3]);
+      }
+    }
+    float most = 0.f;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int row = warp * 16 + (lane >> 2) + 8 * x, pos = off + row, lo = p.window > 0 ? pos - p.window + 1 : 0;
+      const bool there = row < rows_end, single = pos == 0 || (p.window == 1 && p.sinks == 0);  // (one visible key: no gradient through its weight)
+      const float lse2 = there ? p.lse[((long long)b * p.heads + h) * p.q_len + row] * kLog2e : 0.f;
+      float own = 0.f;
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int e = 2 * x; e < 2 * x + 2; ++e) {
+          const int j = n * 8 + (lane & 3) * 2 + (e & 1);
+          const bool shown = there && j <= pos && (j >= lo || j < p.sinks);
+          sc[n][e] = shown ? ex2(fmaf(sc[n][e], c, -lse2)) : 0.f;
+          if (shown) own = fmaf(sc[n][e], dp[n][e], own);
+        }
+      own += __shfl_xor_sync(0xffffffffu, own, 1);
+      own += __shfl_xor_sync(0xffffffffu, own, 2);
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int e = 2 * x; e < 2 * x + 2; ++e) {
+          dp[n][e] = single || sc[n][e] == 0.f ? 0.f : sc[n][e] * (dp[n][e] - own);
+          most = fmaxf(most, fabsf(dp[n][e]));
+        }
+    }
+    // powers of two of dS, as its largest value asks: this head's for dQ, the smallest so far for dK
+    int k_dq = 0, k_dk = 0;
+    if (kScaled) {
+      most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));  // (not negative: as integers)
+      if (lane == 0) s_most[warp] = most;
+      __syncthreads();
+      most = fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3]));
+      k_dq = max(min(13 + 127 - (int)(__float_as_uint(most) >> 23), kFirstPower), -kFirstPower);
+      k_dk = min(power, k_dq);
+      if (k_dk != power) {
+        const float f = pow2(max(k_dk - power, -126));
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dk[n][e] *= f;
+        power = k_dk;
+      }
+    }
+    const float f_dq = kScaled ? pow2(k_dq) : 1.f, f_dk = kScaled ? pow2(k_dk) : 1.f, f_p = pow2(kWeightBits<T>);
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const uint32_t at = short_at<kShort>(warp * 16 + (lane >> 2) + 8 * x, n) + (lane & 3) * 4;
+        *reinterpret_cast<uint32_t*>(tP + at) = pack2<T>(sc[n][2 * x] * f_p, sc[n][2 * x + 1] * f_p);
+        *reinterpret_cast<uint32_t*>(tP + S::kWeights + at) = pack2<T>(dp[n][2 * x] * f_dk, dp[n][2 * x + 1] * f_dk);
+      }
+    uint32_t w[4][4];
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[ks][e] = pack2<T>(dp[2 * ks + (e >> 1)][2 * (e & 1)] * f_dq, dp[2 * ks + (e >> 1)][2 * (e & 1) + 1] * f_dq);
+    float dq[D / 8][4];
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dq[n][e] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      if (ks * 16 >= keys) continue;
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) {
+        uint32_t kb[4];
+        ldmatrix4_trans(sK + short_at<D>(ks * 16 + (lane & 15), n * 2 + (lane >> 4)), kb);
+        mma16816<T>(dq[2 * n], w[ks], kb[0], kb[1]);
+        mma16816<T>(dq[2 * n + 1], w[ks], kb[2], kb[3]);
+      }
+    }
+    __syncthreads();
+    if (warp * 16 < len) {
+      short_product<T, D>(dv, sP, sG, warp * 16, rows_end, lane);
+      short_product<T, D>(dk, sD, sQ, warp * 16, rows_end, lane);
+    }
+    __syncthreads();  // everyone is done with the head's tiles
+    if (keys > 0) short_store<T, D>(dq, p.scale * (kScaled ? pow2(-k_dq) : 1.f), tQ, p.dq, b, h, warp * 16, rows_end, lane);
+    if (i + 1 < group) __syncthreads();
+  }
+  __syncthreads();
+  if (warp * 16 < len) {
+    short_store<T, D>(dk, p.scale * (kScaled ? pow2(-power) : 1.f), sm, p.dk, b, kvh, warp * 16, len, lane);
+    short_store<T, D>(dv, pow2(-kWeightBits<T>), sm + S::kTileB, p.dv, b, kvh, warp * 16, len, lane);
+  }
+}
+
 // Shared memory is handed out to the last kilobytes at D = 128 (a tile has to be fetched two before it is needed): dynamic
 // shared memory starts on a 1024-byte boundary, which the tiles' swizzling needs.
 // A place in a ring of N stages, and the parity of its barriers' phases
@@ -808,8 +1000,8 @@ struct Ring {
 // G groups of 128 threads, each with a tile of 64 rows of its own in hand.  A CTA of two groups has an SM to itself.  Heads of 64
 // leave room for two CTAs of one group, which hide each other's beginnings and ends too, but each is slower by itself: they are
 // taken where no CTA has more than its half SM's share of all tiles.  2 x 4099 with a window of 1024, 16
-// heads: dQ 92 us with one group, 109 with two; dK and dV, where two sinks make one CTA the longest by far, 190 and 116; 128 x 64,
-// 8 heads: 22 + 25 against 77 for both; 4096 without a window, 4 heads: 57 + 74 against 39 + 46.
+// heads: dQ 92 us with one group, 109 with two; dK and dV, where two sinks make one CTA the longest by far, 190 and 116;
+// 4096 without a window, 4 heads: 57 + 74 against 39 + 46.
 //
 // A block of keys that many queries see (all heads of its group; all of a sequence where it holds a sink) is one long walk, and few
 // blocks leave SMs idle.  It is then shared by the CTAs of a cluster, a part of the queries each, joined through their shared memory
@@ -1727,8 +1919,22 @@ int launch_dkv(aig_ctx* ctx, WinParams p, int first, int blocks, int parts, bool
 }
 
 template <class T, int D>
+int launch_short_backward(aig_ctx* ctx, const WinParams& p) {
+  using S = ShortGradShape<D>;
+  const long long grid = (long long)p.kv_heads * p.batch;
+  if (grid > 0x7fffffffll) return aig_fail(ctx, AIG_ERR_UNSUPPORTED, "window attention backward: too many rows for one call");
+  AIG_CUDA_OK(ctx, cudaFuncSetAttribute(window_short_backward_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
+  window_short_backward_kernel<T, D><<<(unsigned)grid, 128, S::kSmem, ctx->stream>>>(p);
+  AIG_LAUNCH_OK(ctx);
+  return AIG_OK;
+}
+
+template <class T, int D>
 int backward(aig_ctx* ctx, WinParams& p) {
   p.gerr = ctx->d_err;
+  // Sequences of one tile, unless a few CTAs would take the heads of large groups one after the other (1024 heads of 64 x 64 x 64 23 us, the
+  // two kernels 47; of 64 x 64 x 128 45 and 115; 64 x 64 x 64, 16 heads on 2: of 128 sequences 46 and 61, of one 37 and 17).
+  if (p.kv_len <= kShort && (p.heads <= 2 * p.kv_heads || (long long)p.kv_heads * p.batch >= ctx->sm_count)) return launch_short_backward<T, D>(ctx, p);
   CUtensorMap mq{}, mk, mv, mg{};
   int rc = encode<T, D, kSub>(ctx, &mk, p.k, p.batch, p.kv_len, p.kv_heads);
   if (rc == AIG_OK) rc = encode<T, D, kSub>(ctx, &mv, p.v, p.batch, p.kv_len, p.kv_heads);

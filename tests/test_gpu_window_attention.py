@@ -476,3 +476,41 @@ def test_fp16_gradients_over_shared_keys_of_growing_values(env, d, window, sinks
     out, lse = run_forward(env, q, k, v, window, sinks)
     check((out, lse), want, bound, ("out", "lse"))
     check(run_backward(env, q, k, v, out, lse, g, window, sinks), want, bound, ("dq", "dk", "dv"))
+
+
+SHORT = [
+    # sequences of one tile: many of them with heads on their own or in groups, and a few with large groups
+    (80, 33, 33, 6, 2, 0, 0, [33, 1, 0, 17] * 20),
+    (160, 64, 64, 3, 1, 5, 2, None),
+    (150, 7, 60, 8, 1, 30, 1, [60, 59, 53, 40, 0] * 30),
+    (3, 64, 64, 16, 1, 0, 0, [64, 20, 3]),
+    (2, 50, 61, 8, 1, 16, 20, None),
+    (5, 1, 64, 2, 2, 0, 0, [64, 63, 0, 1, 64]),
+    (1, 16, 16, 2, 1, 1, 0, None),
+    (1, 49, 49, 1, 1, 48, 0, None),
+]
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("B,Tq,Tk,H,KV,window,sinks,lengths", SHORT)
+def test_sequences_of_one_tile(env, kind, d, B, Tq, Tk, H, KV, window, sinks, lengths):
+    test_forward_and_gradients(env, kind, d, B, Tq, Tk, H, KV, window, sinks, lengths)
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("B,H,KV", [(1, 2, 1), (160, 5, 1)])
+@pytest.mark.parametrize("scale", [2.0 ** -18, 1.0, 2.0 ** 7])
+def test_fp16_gradients_of_short_sequences(env, scale, B, H, KV, d):
+    """Heads of a group whose gradients differ two hundredfold, rising and falling, and sequences likewise."""
+    import torch
+
+    q, k, v, g = tensors(45, torch.float32, B, 61, 61, H, KV, d)
+    size = torch.tensor([1.0, 2.0 ** -7.5, 2.0 ** -3, 0.0, 2.0 ** -5], device="cuda")
+    heads = size[(torch.arange(H, device="cuda")[None] + torch.arange(B, device="cuda")[:, None]) % 5]
+    q, k, v, g = q.half(), k.half(), v.half(), (g * heads[:, None, :, None] * scale).half()
+    want, bound = R.window_attention(q, k, v, 20, 1, None, d ** -0.5, g)
+    out, lse = run_forward(env, q, k, v, 20, 1)
+    check(run_backward(env, q, k, v, out, lse, g, 20, 1), want, bound, ("dq", "dk", "dv"))
