@@ -758,8 +758,10 @@ __global__ void __launch_bounds__(128, (ShortShape<D, Tiles>::kCtasPerSm)) windo
 //
 // fp16 has few small numbers: weights of a row over thousands of keys, and dS of small gradients, would be rounded to
 // multiples of 2^-24.  So the weights are multiplied by 2^8, and dS by a power of two 2^k that follows the largest
-// |dO| * |V| seen so far: |dS| stays below 2^15.5 whatever the values, and typical ones around 1.  Where a tile asks for a
-// smaller power the sums so far are scaled (rare: it keeps two bits in hand).
+// |dO| * |V| seen so far: typical ones lie around 1.  dS = P (dP - D), and D comes from the values of all keys that a query sees, other
+// tiles' too (this one's may be zero): dK's power follows the queries' |D| as well.  Then 2^k |dP| < 2^14 (|dO| |V| times 2^3, 2^4
+// for heads of 128, is held below 2^11, and a sum of 64 or 128 products is at most 2^3 times that) and 2^k |D| < 2^11: no dS passes fp16's
+// largest value.  Where a tile asks for a smaller power the sums so far are scaled (rare: it keeps two bits in hand).
 constexpr int kSub = 64;
 template <class T>
 constexpr int kWeightBits = std::is_same<T, __half>::value ? 8 : 0;
@@ -767,7 +769,9 @@ constexpr int kMostBits = 11, kAimBits = 9;  // of 2^k * |dO| * |V| * sqrt(D)
 
 __device__ __forceinline__ float pow2(int k) { return __int_as_float((k + 127) << 23); }  // -126 .. 127
 
-// Exponent e with max |x| < 2^e over rows [0, rows) of a tile in shared memory, by one warp (x finite; -126 at least)
+// Exponent e with x < 2^e (x finite and not negative, as bits; -126 at least)
+__device__ __forceinline__ int exponent_of(uint32_t x) { return (int)(x >> 23) - 126; }
+// ... with max |x| < 2^e over rows [0, rows) of a tile in shared memory, by one warp
 template <int D, int R>
 __device__ __forceinline__ int tile_exponent(const uint8_t* tile, int rows, int lane) {
   __half2 m[2] = {__half2half2(__ushort_as_half(0)), __half2half2(__ushort_as_half(0))};
@@ -782,7 +786,7 @@ __device__ __forceinline__ int tile_exponent(const uint8_t* tile, int rows, int 
     }
   const __half2 both = __hmax2(m[0], m[1]);
   const uint32_t x = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(__low2float(both), __high2float(both))));  // (not negative: as integers)
-  return min((int)(x >> 23) - 126, 20);
+  return min(exponent_of(x), 20);
 }
 // the power for a tile whose bound has the exponent e, given the one so far
 __device__ __forceinline__ int next_power(int k, int e) {
@@ -1568,16 +1572,26 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
       fetch(u + 1, at, x);
     }
   } else if (warp == 3) {
-    // the power for dS
+    // the power for dS, as this block's values and the queries' D ask; D of the next tile on its way while the stage is awaited
     if (kScaled && (!Split || tiles > 0) && warp_wait(kv_full, 0, s_abort, p.gerr, 1146)) {
       const int ev = tile_exponent<D, kTile>(sm + (sV - base), min(kTile, len - j0), lane) + (D == 64 ? 3 : 4);
+      Walk at = start;
+      auto largest = [&](int u) {  // of this lane's two
+        const int row = first_row(at) + lane;
+        const float* const delta = p.delta + ((long long)b * p.heads + at.h) * p.q_len + row;
+        const float x = u < tiles && row < rows_end ? fabsf(__ldcg(delta)) : 0.f, y = u < tiles && row + 32 < rows_end ? fabsf(__ldcg(delta + 32)) : 0.f;
+        return __float_as_uint(fmaxf(x, y));
+      };
+      uint32_t most = largest(0);
       int k = kFirstPower;
       Ring<NS> ring_at;
-      Walk at = start;
-      for (int u = 0; u < tiles; ++u, ring_at.next(), at.next()) {
+      for (int u = 0; u < tiles; ++u, ring_at.next()) {
         const int s = ring_at.s;
         if (!warp_wait(q_full + 8 * s, ring_at.ph, s_abort, p.gerr, 1148)) break;
-        const int k_new = next_power(k, ev + tile_exponent<D, kSub>(sm + S::kFixed + s * S::kStage + kTileBytes<D, kSub>, min(kSub, rows_end - first_row(at)), lane));
+        const int eg = tile_exponent<D, kSub>(sm + S::kFixed + s * S::kStage + kTileBytes<D, kSub>, min(kSub, rows_end - first_row(at)), lane);
+        const int k_new = next_power(k, max(ev + eg, exponent_of(__reduce_max_sync(0xffffffffu, most))));
+        at.next();
+        most = largest(u + 1);
         if (lane == 0) {
           s_power[s] = k_new;
           s_step[s] = u == 0 ? 0 : k_new - k;

@@ -514,3 +514,72 @@ def test_fp16_gradients_of_short_sequences(env, scale, B, H, KV, d):
     want, bound = R.window_attention(q, k, v, 20, 1, None, d ** -0.5, g)
     out, lse = run_forward(env, q, k, v, 20, 1)
     check(run_backward(env, q, k, v, out, lse, g, 20, 1), want, bound, ("dq", "dk", "dv"))
+
+
+def put(v, pattern):
+    """Values with blocks of keys whose sizes have nothing to do with the others'."""
+    import torch
+
+    T = v.shape[1]
+    if pattern == "first 64 zero":
+        v[:, :64] = 0
+    elif pattern == "first 128 zero":
+        v[:, :128] = 0
+    elif pattern == "middle zero":
+        v[:, T // 2 // 128 * 128:T // 2 // 128 * 128 + 128] = 0
+    elif pattern == "zero but the last":
+        v[:, :T - 1] = 0
+    elif pattern == "small":
+        v[:, T // 2 // 128 * 128 - 128:T // 2 // 128 * 128] *= 2.0 ** -16
+    elif pattern == "step":
+        v[:, :T // 2] *= 2.0 ** -10
+        v[:, T // 2:] *= 2.0 ** 9
+    elif pattern == "zero but a part":  # of the keys that thread blocks share
+        v[:, :T * 3 // 8] = 0
+        v[:, T * 5 // 8:] = 0
+    return v
+
+
+UNEVEN = [
+    (1, 512, 512, 2, 1, 0, 0, None),
+    (2, 515, 515, 3, 1, 200, 1, [515, 290]),
+    (1, 700, 700, 4, 2, 30, 70, None),
+    (1, 400, 400, 1, 1, 40, 0, None),
+    # shared tiles of queries, shared blocks of keys, the sinks' blocks in a launch of their own
+    (1, 100, 2500, 2, 1, 0, 0, None),
+    (1, 300, 2500, 1, 1, 900, 2, [2400]),
+    (1, 1100, 1100, 8, 1, 0, 0, None),
+    (1, 1500, 1500, 8, 1, 300, 3, None),
+    # many sequences
+    (40, 260, 260, 8, 4, 0, 0, None),
+]
+
+
+def uneven_gradients(env, d, pattern, B, Tq, Tk, H, KV, window, sinks, lengths):
+    import torch
+
+    q, k, v, g = tensors(46, torch.float32, B, Tq, Tk, H, KV, d)
+    v = put(v, pattern)
+    # (max |g| max |v| stays near 20, so that dS's smallest step after its power of two, 2^-28 of that product times the scale,
+    # lies below the 2^-24 that the bound has for it)
+    g = g * (2.0 ** -9 if pattern == "step" else 1.0)
+    q = q * (8.0 if pattern == "small" else 1.0)
+    q, k, v, g = (x.half() for x in (q, k, v, g))
+    some = slice(None) if B < 10 else [0, B // 2, B - 1]
+    want, bound = R.window_attention(q[some], k[some], v[some], window, sinks, lengths, d ** -0.5, g[some])
+    out, lse = run_forward(env, q, k, v, window, sinks, lengths)
+    check((out[some], lse[some]), want, bound, ("out", "lse"))
+    return [x[some] for x in run_backward(env, q, k, v, out, lse, g, window, sinks, lengths)], want, bound
+
+
+PATTERNS = ["first 64 zero", "first 128 zero", "middle zero", "zero but the last", "small", "step", "zero but a part"]
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("pattern", PATTERNS)
+@pytest.mark.parametrize("B,Tq,Tk,H,KV,window,sinks,lengths", UNEVEN)
+def test_fp16_gradients_of_keys_with_uneven_values(env, d, pattern, B, Tq, Tk, H, KV, window, sinks, lengths):
+    """dK of a block of keys whose values are zero or small: rowsum(dO o O) comes from other blocks' values and is not."""
+    grads, want, bound = uneven_gradients(env, d, pattern, B, Tq, Tk, H, KV, window, sinks, lengths)
+    check(grads[1:], want, bound, ("dk", "dv"))
