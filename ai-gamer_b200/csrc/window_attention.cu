@@ -759,7 +759,7 @@ __global__ void __launch_bounds__(128, (ShortShape<D, Tiles>::kCtasPerSm)) windo
 // fp16 has few small numbers: weights of a row over thousands of keys, and dS of small gradients, would be rounded to
 // multiples of 2^-24.  So the weights are multiplied by 2^8, and dS by a power of two 2^k that follows the largest
 // |dO| * |V| seen so far: typical ones lie around 1.  dS = P (dP - D), and D comes from the values of all keys that a query sees, other
-// tiles' too (this one's may be zero): dK's power follows the queries' |D| as well.  Then 2^k |dP| < 2^14 (|dO| |V| times 2^3, 2^4
+// tiles' too (this one's may be zero): the power follows the queries' |D| as well.  Then 2^k |dP| < 2^14 (|dO| |V| times 2^3, 2^4
 // for heads of 128, is held below 2^11, and a sum of 64 or 128 products is at most 2^3 times that) and 2^k |D| < 2^11: no dS passes fp16's
 // largest value.  Where a tile asks for a smaller power the sums so far are scaled (rare: it keeps two bits in hand).
 constexpr int kSub = 64;
@@ -1029,6 +1029,7 @@ struct DqShape : BwdShape<D, G> {
   static constexpr uint32_t kFixed = 2 * kTileBytes<D, kTile>, kStage = kTileBytes<D, kKeyRows>;
   static constexpr uint32_t kTiles = kFixed + (kKeys + kValues) * kStage;
   static constexpr size_t kSmem = kTiles + 2048 + 512;
+  static_assert((11 + 3 * kKeys + kValues) * 8 + 2 * kKeys * 4 + 8 + 16 <= 512, "barriers, powers and flags behind the sums");
 };
 template <int D, int G>
 struct DkvShape : BwdShape<D, G> {
@@ -1059,11 +1060,12 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
   const uint32_t bar0 = smem_u32(bars);
   // of each stream of tiles: scores and dP are there, they have been read; of each of its two buffers: dS is there
   const uint32_t q_full = bar0, dq_full = bar0 + 8, sd_full = bar0 + 16, sd_free = sd_full + 16, ds_full = sd_free + 16, kv_full = ds_full + 32,
-                 k_free = kv_full + 8 * NK, v_free = k_free + 8 * NK, st_full = v_free + 8 * NV;
-  int* const s_power = reinterpret_cast<int*>(bars + 10 + 3 * NK + NV);  // [NK]
+                 k_free = kv_full + 8 * NK, v_free = k_free + 8 * NK, st_full = v_free + 8 * NV, d_full = st_full + 8 * NK;
+  int* const s_power = reinterpret_cast<int*>(bars + 11 + 3 * NK + NV);  // [NK]
   int* const s_step = s_power + NK;                                       // [NK]: its change against the tile before
   uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(s_step + NK);
   volatile int* const s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
+  uint32_t* const s_most = s_tmem + 2;  // [4]: each warp's largest |D|, as bits
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
   const int split = Split ? p.split : 0, parts = 1 << split, part = blockIdx.x & (parts - 1);
@@ -1103,6 +1105,7 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
       mbar_init(k_free + 8 * s, 1);
       mbar_init(st_full + 8 * s, 1);
     }
+    mbar_init(d_full, 4);
     // the products are done with it, and so is the search for its largest value
     for (int s = 0; s < NV; ++s) mbar_init(v_free + 8 * s, kScaled ? 2 : 1);
     *s_abort = 0;
@@ -1182,14 +1185,16 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
     }
     if (ok) commit(leader, dq_full);
   } else if (warp == 2) {
-    if (kScaled && (!Split || tiles > 0) && warp_wait(q_full, 0, s_abort, p.gerr, 1126)) {
+    // (with two passes the first, over all keys, has seen what D is made of)
+    if (kScaled && (!Split || tiles > 0) && warp_wait(q_full, 0, s_abort, p.gerr, 1126) && (ahead > 0 || warp_wait(d_full, 0, s_abort, p.gerr, 1134))) {
+      const int ed = ahead > 0 ? -126 : exponent_of(max(max(s_most[0], s_most[1]), max(s_most[2], s_most[3])));
       const int eg = tile_exponent<D, kTile>(sm + (sG - base), min(kTile, rows_end - r0), lane) + (D == 64 ? 3 : 4);
       int k = kFirstPower;
       Ring<NK> kr;
       Ring<NV> vr;
       for (int u = 0; u < tiles; ++u, kr.next(), vr.next()) {
         if (!warp_wait(kv_full + 8 * kr.s, kr.ph, s_abort, p.gerr, 1127)) break;
-        const int k_new = next_power(k, eg + tile_exponent<D, KR>(sm + (sV - base) + vr.s * S::kStage, min(KR, len - first_key(u)), lane));
+        const int k_new = next_power(k, max(ed, eg + tile_exponent<D, KR>(sm + (sV - base) + vr.s * S::kStage, min(KR, len - first_key(u)), lane)));
         __syncwarp();
         if (lane == 0) {
           s_power[kr.s] = k_new;
@@ -1238,6 +1243,13 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
     };
     bool joined = ahead == 0;
     if (joined) join();
+    if (kScaled && w == 0) {
+      const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(delta)));
+      if (lane == 0) {
+        s_most[q] = most;
+        mbar_arrive(d_full);
+      }
+    }
     bool ok = true;
     Ring<NK> kr;
     if (stream == 1) kr.next();

@@ -583,3 +583,13 @@ def test_fp16_gradients_of_keys_with_uneven_values(env, d, pattern, B, Tq, Tk, H
     """dK of a block of keys whose values are zero or small: rowsum(dO o O) comes from other blocks' values and is not."""
     grads, want, bound = uneven_gradients(env, d, pattern, B, Tq, Tk, H, KV, window, sinks, lengths)
     check(grads[1:], want, bound, ("dk", "dv"))
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("pattern", PATTERNS)
+@pytest.mark.parametrize("B,Tq,Tk,H,KV,window,sinks,lengths", UNEVEN)
+def test_fp16_gradients_of_queries_with_uneven_values(env, d, pattern, B, Tq, Tk, H, KV, window, sinks, lengths):
+    """dQ where the first tiles of keys, or those of a thread block that shares the keys, have values of zero or small ones."""
+    grads, want, bound = uneven_gradients(env, d, pattern, B, Tq, Tk, H, KV, window, sinks, lengths)
+    check(grads[:1], want, bound, ("dq",))
