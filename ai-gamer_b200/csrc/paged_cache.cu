@@ -1,5 +1,6 @@
 // paged_cache.cu -- copies of a cache's pages, and attention of one new token of each sequence over its pages.
 #include <cooperative_groups.h>
+#include <float.h>
 #include <string.h>
 
 #include <new>
@@ -269,7 +270,9 @@ __global__ void __launch_bounds__(W * 32, AttendShape<D, HT, W>::kCtasPerSm) pag
         float m = sc[ht][0][h];
 #pragma unroll
         for (int kb = 0; kb < kTile / 16; ++kb) m = fmaxf(fmaxf(m, sc[ht][kb][h]), sc[ht][kb][h + 2]);
-        mx[h] = m * p.scale_log2;
+        // (scores of minus infinity are held against a finite value, which gives them the weight 0; top = -inf says that there was no
+        // position at all)
+        mx[h] = fmaxf(m * p.scale_log2, -FLT_MAX);
       }
 #pragma unroll
       for (int s = 4; s < 32; s <<= 1)
@@ -279,7 +282,7 @@ __global__ void __launch_bounds__(W * 32, AttendShape<D, HT, W>::kCtasPerSm) pag
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float m = fmaxf(mx[h], top[ht][h]);
-          const float f = ex2(top[ht][h] - m);  // (a tile has a visible position, so m is finite if the scores are)
+          const float f = ex2(top[ht][h] - m);  // (a tile has a visible position, so m is above -inf)
           top[ht][h] = m;
           sum[ht][h] *= f;
 #pragma unroll
@@ -391,7 +394,7 @@ __global__ void __launch_bounds__(W * 32, AttendShape<D, HT, W>::kCtasPerSm) pag
       s_scale[s][r] = f;
       total += f * *cluster.map_shared_rank(sums + r, s);
     }
-    const float inv = total == 0.f ? 0.f : 1.f / total;  // nothing visible: zeros
+    const float inv = m == -INFINITY ? 0.f : 1.f / total;  // nothing visible: zeros (every score minus infinity: 0 / 0)
     for (int s = 0; s < p.splits; ++s) s_scale[s][r] *= inv;
   }
   __syncthreads();

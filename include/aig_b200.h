@@ -484,7 +484,8 @@ int aig_kv_copy_pages(aig_ctx* ctx, const aig_kv_cache* cache, const int32_t* sr
  * sequence to sequence), lengths int32 [batch] on the device: positions 0 .. lengths[b]-1 are in the cache, the new token
  * is the last of them.  Query head h reads cached head h / (q_heads / kv_heads); out = softmax(scale * q.k) v over the
  * visible positions: the last `window` (<= 0: all) and the first `sinks` (with a window).  Pages without a visible position are
- * not read and their table entries may be anything; a length of 0 or less gives zeros.  max_length is the host's bound of
+ * not read and their table entries may be anything; a length of 0 or less gives zeros.  Keys and values that no position shows may be
+ * anything; a visible score of minus infinity has the weight 0, and where all of them are, the result is NaN.  max_length is the host's bound of
  * the lengths: work is split by it, and lengths above it are as right, only slower.  scale positive; head_dim 64 or 128; q and
  * out on 16-byte boundaries with strides that are multiples of 8, out may be q. */
 int aig_paged_attention(aig_ctx* ctx, const aig_kv_cache* cache, const aig_heads* q, const aig_heads* out, const int32_t* table, int table_width,

@@ -447,3 +447,46 @@ def test_captured_steps_and_other_streams(env):
         rope.close()
         if ctx is not main:
             ctx.close()
+
+
+def kept_ref(q, kp, vp, where, scale):
+    """attend_ref of one sequence over these (page, place) pairs alone."""
+    import torch
+
+    n = len(where)
+    page, place = (torch.tensor(x, device="cuda") for x in zip(*where))
+    return attend_ref(q, kp[page, place][:, None], vp[page, place][:, None], torch.arange(n, device="cuda")[None], [n], 0, 0, scale)
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("finite", [False, True])
+@pytest.mark.parametrize("heads,kv", [(2, 2), (12, 1)])
+@pytest.mark.parametrize("hidden", ["first", "last", "all but one", "between"])
+def test_attend_scores_of_minus_infinity(env, hidden, heads, kv, finite, d):
+    """Keys of minus infinity, or finite ones whose product passes 32 bits: weights of 0, wherever they lie; where no other key
+    is visible the formula has no value."""
+    import torch
+
+    U, pk = env, env.pkg()
+    size, n = 16, 700
+    kp, vp = pages_of((60, size, kv, d), torch.bfloat16, 17)
+    table = table_for([n, 40], size, 60, 18)
+    q = torch.randn((2, heads, d), device="cuda", generator=torch.Generator("cuda").manual_seed(19)).bfloat16()
+    q[:, :, 0] = 1e20 if finite else 1.0
+    kp[..., 0] = 0
+    gone = {"first": lambda t: t < 400, "last": lambda t: t >= 300, "all but one": lambda t: t != 555, "between": lambda t: t % 64 >= 16}[hidden]
+    place = lambda t: (int(table[0, t // size]), t % size)  # noqa: E731
+    for t in filter(gone, range(n)):
+        kp[place(t)][:, 0] = -1e30 if finite else -math.inf
+    for t in range(40):  # the other sequence has no other keys
+        kp[int(table[1, t // size]), t % size][:, 0] = -1e30 if finite else -math.inf
+    out = torch.empty_like(q)
+    lengths = torch.tensor([n, 40], device="cuda").int()
+    want, bound = kept_ref(q[:1], kp, vp, [place(t) for t in range(n) if not gone(t)], d ** -0.5)
+    cache = pk.PagedCache(U.ctx(), kp, vp)
+    for most in (1, n):
+        cache.attend(q, out, table, lengths, most)
+        U.ctx().sync()
+        assert R.worst(out[:1], want, bound) <= 1.0
+        assert out[1].isnan().all()
