@@ -189,9 +189,12 @@ __global__ void __launch_bounds__(W * 32, AttendShape<D, HT, W>::kCtasPerSm) pag
       }
     }
   };
+  // (returns which of the tile's positions take part, as bits)
   auto load = [&](int tile, int stage) {
+    uint32_t there = 0;
     if (tile < tile_end) {
       const long long mine = row_page < 0 ? -1 : row_page * p.page + row_place * p.place;
+      there = __ballot_sync(0xffffffffu, row_page >= 0);
       const uint32_t kd = ring + stage * 2 * S::kTileBytes, vd = kd + S::kTileBytes;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
@@ -205,6 +208,7 @@ __global__ void __launch_bounds__(W * 32, AttendShape<D, HT, W>::kCtasPerSm) pag
       }
     }
     cp_async_commit();  // (an empty group where there is no tile: groups are counted)
+    return there;
   };
 
   // sums O^T: rows d, columns heads 2 (lane % 4) and the next; maxima and sums of these two heads
@@ -220,20 +224,25 @@ __global__ void __launch_bounds__(W * 32, AttendShape<D, HT, W>::kCtasPerSm) pag
   }
 
   look_up(tile0);
+  uint32_t there[S::kStages];  // of the tiles on their way, the next to be taken first
 #pragma unroll
   for (int s = 0; s < S::kStages - 1; ++s) {
-    load(tile0 + s * W, s);
+    there[s] = load(tile0 + s * W, s);
     look_up(tile0 + (s + 1) * W);
   }
   int stage = 0;
-  for (int tile = tile0; tile < tile_end; tile += W) {
+  for (int tile = tile0; tile < tile_end; tile += W, stage = stage + 1 == S::kStages ? 0 : stage + 1) {
     cp_async_wait<S::kStages - 2>();
     __syncwarp();
     {
       const int next = tile + (S::kStages - 1) * W;
-      load(next, stage == 0 ? S::kStages - 1 : stage - 1);
+      there[S::kStages - 1] = load(next, stage == 0 ? S::kStages - 1 : stage - 1);
       look_up(next + W);
     }
+    const uint32_t shown = there[0];
+#pragma unroll
+    for (int s = 0; s + 1 < S::kStages; ++s) there[s] = there[s + 1];
+    if (shown == 0) continue;  // none of them has a page
     const uint32_t kd = ring + stage * 2 * S::kTileBytes, vd = kd + S::kTileBytes;
     // ---- scores: 16 positions a block
     float sc[HT][kTile / 16][4];
@@ -252,15 +261,15 @@ __global__ void __launch_bounds__(W * 32, AttendShape<D, HT, W>::kCtasPerSm) pag
         for (int ht = 0; ht < HT; ++ht) mma16816<T>(sc[ht][kb], ka, qb[ht][ks][0], qb[ht][ks][1]);
       }
     }
-    const int left = visible - tile * kTile;  // positions from here on
-    if (left < kTile) {
+    if (shown != 0xffffffffu) {  // behind the last position, or without a page
+      static_assert(kTile <= 32, "a bit for each position");
 #pragma unroll
       for (int kb = 0; kb < kTile / 16; ++kb)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
           for (int ht = 0; ht < HT; ++ht)
-            if (kb * 16 + (lane >> 2) + (e >> 1) * 8 >= left) sc[ht][kb][e] = -INFINITY;
+            if (!(shown >> (kb * 16 + (lane >> 2) + (e >> 1) * 8) & 1)) sc[ht][kb][e] = -INFINITY;
     }
 #pragma unroll
     for (int ht = 0; ht < HT; ++ht) {
@@ -321,7 +330,6 @@ __global__ void __launch_bounds__(W * 32, AttendShape<D, HT, W>::kCtasPerSm) pag
       }
     }
     __syncwarp();  // the stage is free for the load after next
-    stage = stage + 1 == S::kStages ? 0 : stage + 1;
   }
   cp_async_wait<0>();
 #pragma unroll

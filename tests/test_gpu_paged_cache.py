@@ -490,3 +490,33 @@ def test_attend_scores_of_minus_infinity(env, hidden, heads, kv, finite, d):
         U.ctx().sync()
         assert R.worst(out[:1], want, bound) <= 1.0
         assert out[1].isnan().all()
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size,bad", [(16, [0]), (16, [3, 40]), (7, [1, 2, 50]), (100, [2]), (16, list(range(43))), (16, list(range(44)))])
+def test_attend_leaves_out_pages_that_are_none(env, size, bad, d):
+    """Positions whose table entry names no page have no share in the softmax; with no other position the result is zeros."""
+    import torch
+
+    U, pk = env, env.pkg()
+    ctx = U.ctx()
+    n, pages = 700, 110
+    kp, vp = pages_of((pages, size, 2, d), torch.float16, 21)
+    kp *= 3  # (a score of 0 would take a visible share)
+    table = table_for([n], size, pages, 22)
+    where = [(int(table[0, t // size]), t % size) for t in range(n) if t // size not in bad]
+    for i, p in enumerate(bad):
+        table[0, p] = [-1, pages, 1 << 30][i % 3]
+    q = torch.randn((1, 8, d), device="cuda", generator=torch.Generator("cuda").manual_seed(23)).half()
+    out = torch.full_like(q, 7.0)
+    for most in (1, n):
+        pk.PagedCache(ctx, kp, vp).attend(q, out, table, torch.tensor([n], device="cuda").int(), most)
+        with pytest.raises(pk.AigError) as e:
+            ctx.sync()
+        assert e.value.code == -1
+        if where:
+            want, bound = kept_ref(q, kp, vp, where, d ** -0.5)
+            assert R.worst(out, want, bound) <= 1.0
+        else:
+            assert not out.any()
