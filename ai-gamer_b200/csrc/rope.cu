@@ -80,20 +80,23 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
   const uint32_t token = p.chunks.divide(row);
   const int first = (row - token * p.chunks.by) * HP;
   const int position = p.positions[token];
-  long long place = 0;  // where the token's keys and values go
+  long long place = 0;   // where the token's keys and values go
+  int heads = p.end[2];  // without a place for them only queries are turned
   if (p.page.by > 0) {
     if (position < 0) return;
     const int seq = p.seqs ? p.seqs[token] : (int)token;
     const int slot = p.page.divide(position);
+    int page = -1;
     if (seq < 0 || seq >= p.batch || slot >= p.table_width) {
       note_error(p.gerr, kErrBadPlace);
-      return;
+    } else {
+      page = p.table[(long long)seq * p.table_width + slot];
+      if (page < 0 || page >= p.num_pages) {
+        note_error(p.gerr, kErrBadPage);
+        page = -1;
+      }
     }
-    const int page = p.table[(long long)seq * p.table_width + slot];
-    if (page < 0 || page >= p.num_pages) {
-      note_error(p.gerr, kErrBadPage);
-      return;
-    }
+    if (page < 0) heads = p.end[0];
     place = page * p.page_stride + (long long)(position - slot * (int)p.page.by) * p.place_stride;
   }
   const bool turn = g < p.rot_items;
@@ -105,7 +108,7 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
 #pragma unroll
   for (int i = 0; i < HP; ++i) {
     const int h = first + i;
-    if (h < p.end[2]) {
+    if (h < heads) {
       const int w = h < p.end[0] ? 0 : h < p.end[1] ? 1 : 2;
       const Side& s = p.part[w];
       const int head = w == 0 ? h : h - p.end[w - 1];
@@ -130,7 +133,7 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
 #pragma unroll
   for (int i = 0; i < HP; ++i) {
     const int h = first + i;
-    if (h >= p.end[2]) break;
+    if (h >= heads) break;
     if (turn && h < p.turned_heads) {
       if (INTERLEAVED) {
 #pragma unroll

@@ -464,8 +464,8 @@ int aig_rope_backward(aig_rope_plan* plan, int dtype, const int32_t* positions, 
  * token_stride + head * head_stride + i.  A sequence's position p lies at place p % page_size of the page that its row of
  * the page table (int32, device) names at p / page_size.  head_dim and the strides are multiples of 8, data on 16-byte
  * boundaries.  A table entry that a call needs and that names no page of the pool, or a position beyond the table's
- * width, faults nothing: nothing is written there, the attention goes over the other positions (none: zeros), and the next
- * aig_ctx_sync returns AIG_ERR_INVALID. */
+ * width, faults nothing: no keys and values are written there (queries are turned all the same), the attention goes
+ * over the other positions (none: zeros), and the next aig_ctx_sync returns AIG_ERR_INVALID. */
 typedef struct aig_kv_cache {
   void *k, *v;
   int dtype, kv_heads, head_dim, page_size, num_pages;

@@ -520,3 +520,39 @@ def test_attend_leaves_out_pages_that_are_none(env, size, bad, d):
             assert R.worst(out, want, bound) <= 1.0
         else:
             assert not out.any()
+
+
+@gpu
+@pytest.mark.parametrize("heads", [2, 64])
+def test_append_turns_queries_of_tokens_without_a_place(env, heads):
+    """A place that is none leaves out the token's keys and values; its queries are turned like the others'."""
+    import torch
+
+    U, pk = env, env.pkg()
+    ctx = U.ctx()
+    n = 3000 if heads > 2 else 5  # (enough for several heads a thread, and few)
+    kp, vp = pages_of((n, 1, 1, 64), torch.float16, 25)
+    table = torch.arange(n, device="cuda").int()[None].contiguous()
+    table[0, 1], table[0, 3] = -1, n
+    positions = torch.arange(n, device="cuda").int()
+    positions[4] = n  # beyond the table
+    positions[2] = -1
+    seqs = torch.zeros(n, dtype=torch.int32, device="cuda")
+    seqs[0] = 1
+    row = torch.randn((n, heads + 2, 64), device="cuda", generator=torch.Generator("cuda").manual_seed(26)).half()
+    q, k, v = row[:, :heads], row[:, heads:heads + 1], row[:, heads + 1:]
+    q_out = torch.full(q.shape, 7.0, dtype=q.dtype, device="cuda")
+    before_k, before_v = kp.clone(), vp.clone()
+    rope = pk.RopePlan(ctx, 64)
+    pk.PagedCache(ctx, kp, vp).append(k, v, positions, table, seqs=seqs, rope=rope, q=q, q_out=q_out)
+    with pytest.raises(pk.AigError) as e:
+        ctx.sync()
+    assert e.value.code == -1
+    there = positions >= 0
+    want, bound = turned(q[there], positions[there], rope.frequencies(), 64, False, 1.0, 1)
+    assert R.worst(q_out[there], want, bound) <= 1.0
+    assert (q_out[2] == 7.0).all()
+    want, bound = turned(k, positions, rope.frequencies(), 64, False, 1.0, 1)
+    assert R.worst(kp[5:, 0], want[5:], bound[5:]) <= 1.0 and torch.equal(vp[5:, 0], v[5:])
+    assert torch.equal(kp[:5], before_k[:5]) and torch.equal(vp[:5], before_v[:5])
+    rope.close()
