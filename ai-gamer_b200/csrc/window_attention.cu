@@ -597,7 +597,7 @@ __device__ __forceinline__ void short_load(uint32_t to, const View& v, int b, in
 template <class T, int D, int Tiles>
 __global__ void __launch_bounds__(128, (ShortShape<D, Tiles>::kCtasPerSm)) window_short_kernel(const __grid_constant__ WinParams p) {
   using S = ShortShape<D, Tiles>;
-  extern __shared__ __align__(128) uint8_t sm[];
+  extern __shared__ __align__(1024) uint8_t sm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int item = blockIdx.x;
   const int b = item % p.batch;
@@ -834,7 +834,7 @@ template <class T, int D>
 __global__ void __launch_bounds__(128, ShortGradShape<D>::kCtasPerSm) window_short_backward_kernel(const __grid_constant__ WinParams p) {
   using S = ShortGradShape<D>;
   constexpr bool kScaled = std::is_same<T, __half>::value;
-  extern __shared__ __align__(128) uint8_t sm[];
+  extern __shared__ __align__(1024) uint8_t sm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x % p.batch, kvh = blockIdx.x / p.batch, group = p.heads / p.kv_heads;
   const int len = p.lengths ? min(max(p.lengths[b], 0), p.kv_len) : p.kv_len;
