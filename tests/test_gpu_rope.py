@@ -196,3 +196,24 @@ def test_refusals(env):
     plan.forward(pos[:0], empty, empty)
     ctx.sync()
     plan.close()
+
+
+@gpu
+def test_offsets_beyond_32_bits(env):
+    """Tokens so far apart that they pass 2^32 elements."""
+    import torch
+
+    n, tokens, dim = 5 << 30, 70, 64
+    if torch.cuda.mem_get_info()[0] < 14 << 30:
+        pytest.skip("not enough memory")
+    wide = torch.empty(n, dtype=torch.float16, device="cuda")
+    row = n // tokens // 8 * 8
+    q, q_out = (wide.as_strided((tokens, 3, dim), (row, dim, 1), at) for at in (0, 3 * dim))
+    q.normal_(generator=torch.Generator("cuda").manual_seed(31))
+    positions = torch.arange(tokens, device="cuda").int()
+    plan = env.pkg().RopePlan(env.ctx(), dim)
+    plan.forward(positions, q, q_out)
+    env.ctx().sync()
+    want, bound = turned(q, positions, plan.frequencies(), dim, False, 1.0, 1)
+    assert R.worst(q_out, want, bound) <= 1.0
+    plan.close()

@@ -593,3 +593,37 @@ def test_fp16_gradients_of_queries_with_uneven_values(env, d, pattern, B, Tq, Tk
     """dQ where the first tiles of keys, or those of a thread block that shares the keys, have values of zero or small ones."""
     grads, want, bound = uneven_gradients(env, d, pattern, B, Tq, Tk, H, KV, window, sinks, lengths)
     check(grads[:1], want, bound, ("dq",))
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("T", [60, 300])
+def test_offsets_beyond_32_bits(env, T, d):
+    """Rows so far apart that a sequence passes 2^32 elements: all tensors as columns of one of 10 GB."""
+    import torch
+
+    H, KV, n = 4, 2, 5 << 30
+    if torch.cuda.mem_get_info()[0] < 14 << 30:
+        pytest.skip("not enough memory")
+    row = n // T // 8 * 8
+    wide = torch.empty(n, dtype=torch.float16, device="cuda")
+    at = 0
+
+    def column(x):
+        nonlocal at
+        view = wide.as_strided(x.shape, (T * row, row, d, 1), at)
+        view.copy_(x)
+        at += x.shape[2] * d
+        return view
+
+    made = tensors(47, torch.float16, 1, T, T, H, KV, d)
+    want, bound = R.window_attention(*made[:3], 50, 1, None, d ** -0.5, made[3])
+    q, k, v, g = (column(x) for x in made)
+    out, dq = (column(torch.full_like(made[0], MARK)) for _ in range(2))
+    dk, dv = (column(torch.full_like(made[1], MARK)) for _ in range(2))
+    lse, delta = torch.empty((1, H, T), device="cuda"), torch.empty((1, H, T), device="cuda")
+    wa = env.pkg().WindowAttention(env.ctx(), 50, 1)
+    wa.forward(q, k, v, out, lse)
+    wa.backward(q, k, v, out, lse, g, dq, dk, dv, delta)
+    env.ctx().sync()
+    check((out, lse, dq, dk, dv), want, bound, ("out", "lse", "dq", "dk", "dv"))
