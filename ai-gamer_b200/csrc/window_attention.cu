@@ -761,9 +761,9 @@ __device__ __forceinline__ float pow2(int k) { return __int_as_float((k + 127) <
 
 // Exponent e with x < 2^e (x finite and not negative, as bits; -126 at least)
 __device__ __forceinline__ int exponent_of(uint32_t x) { return (int)(x >> 23) - 126; }
-// ... with max |x| < 2^e over rows [0, rows) of a tile in shared memory, by one warp
+// ... with |x| < 2^e for this lane's values of rows [0, rows) of a tile in shared memory ...
 template <int D, int R>
-__device__ __forceinline__ int tile_exponent(const uint8_t* tile, int rows, int lane) {
+__device__ __forceinline__ int lane_exponent(const uint8_t* tile, int rows, int lane) {
   __half2 m[2] = {__half2half2(__ushort_as_half(0)), __half2half2(__ushort_as_half(0))};
 #pragma unroll
   for (int c = 0; c < D / 64; ++c)
@@ -775,8 +775,12 @@ __device__ __forceinline__ int tile_exponent(const uint8_t* tile, int rows, int 
       m[1] = __hmax2(m[1], __hmax2(__habs2(h[2]), __habs2(h[3])));
     }
   const __half2 both = __hmax2(m[0], m[1]);
-  const uint32_t x = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(__low2float(both), __high2float(both))));  // (not negative: as integers)
-  return min(exponent_of(x), 20);
+  return min(exponent_of(__float_as_uint(fmaxf(__low2float(both), __high2float(both)))), 20);
+}
+// ... and for all of them, by one warp
+template <int D, int R>
+__device__ __forceinline__ int tile_exponent(const uint8_t* tile, int rows, int lane) {
+  return __reduce_max_sync(0xffffffffu, lane_exponent<D, R>(tile, rows, lane));
 }
 // the power for a tile whose bound has the exponent e, given the one so far
 __device__ __forceinline__ int next_power(int k, int e) {
@@ -1175,16 +1179,19 @@ window_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant
     }
     if (ok) commit(leader, dq_full);
   } else if (warp == 2) {
-    // (with two passes the first, over all keys, has seen what D is made of)
-    if (kScaled && (!Split || tiles > 0) && warp_wait(q_full, 0, s_abort, p.gerr, 1126) && (ahead > 0 || warp_wait(d_full, 0, s_abort, p.gerr, 1134))) {
-      const int ed = ahead > 0 ? -126 : exponent_of(max(max(s_most[0], s_most[1]), max(s_most[2], s_most[3])));
+    if (kScaled && (!Split || tiles > 0) && warp_wait(q_full, 0, s_abort, p.gerr, 1126)) {
       const int eg = tile_exponent<D, kTile>(sm + (sG - base), min(kTile, rows_end - r0), lane) + (D == 64 ? 3 : 4);
       int k = kFirstPower;
       Ring<NK> kr;
       Ring<NV> vr;
       for (int u = 0; u < tiles; ++u, kr.next(), vr.next()) {
         if (!warp_wait(kv_full + 8 * kr.s, kr.ph, s_abort, p.gerr, 1127)) break;
-        const int k_new = next_power(k, max(ed, eg + tile_exponent<D, KR>(sm + (sV - base) + vr.s * S::kStage, min(KR, len - first_key(u)), lane)));
+        int e = eg + tile_exponent<D, KR>(sm + (sV - base) + vr.s * S::kStage, min(KR, len - first_key(u)), lane);
+        if (u == 0 && ahead == 0) {  // (with two passes the first, over all keys, meets what D is made of)
+          if (!warp_wait(d_full, 0, s_abort, p.gerr, 1134)) break;
+          e = max(e, exponent_of(max(max(s_most[0], s_most[1]), max(s_most[2], s_most[3]))));
+        }
+        const int k_new = next_power(k, e);
         __syncwarp();
         if (lane == 0) {
           s_power[kr.s] = k_new;
@@ -1575,31 +1582,34 @@ window_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constan
     }
   } else if (warp == 3) {
     // the power for dS, as this block's values and the queries' D ask; D of the next tile on its way while the stage is awaited
-    if (kScaled && (!Split || tiles > 0) && warp_wait(kv_full, 0, s_abort, p.gerr, 1146)) {
-      const int ev = tile_exponent<D, kTile>(sm + (sV - base), min(kTile, len - j0), lane) + (D == 64 ? 3 : 4);
-      Walk at = start;
-      auto largest = [&](int u) {  // of this lane's two
-        const int row = first_row(at) + lane;
-        const float* const delta = p.delta + ((long long)b * p.heads + at.h) * p.q_len + row;
-        const float x = u < tiles && row < rows_end ? fabsf(__ldcg(delta)) : 0.f, y = u < tiles && row + 32 < rows_end ? fabsf(__ldcg(delta + 32)) : 0.f;
-        return __float_as_uint(fmaxf(x, y));
-      };
-      uint32_t most = largest(0);
-      int k = kFirstPower;
-      Ring<NS> ring_at;
-      for (int u = 0; u < tiles; ++u, ring_at.next()) {
-        const int s = ring_at.s;
-        if (!warp_wait(q_full + 8 * s, ring_at.ph, s_abort, p.gerr, 1148)) break;
-        const int eg = tile_exponent<D, kSub>(sm + S::kFixed + s * S::kStage + kTileBytes<D, kSub>, min(kSub, rows_end - first_row(at)), lane);
-        const int k_new = next_power(k, max(ev + eg, exponent_of(__reduce_max_sync(0xffffffffu, most))));
-        at.next();
-        most = largest(u + 1);
-        if (lane == 0) {
-          s_power[s] = k_new;
-          s_step[s] = u == 0 ? 0 : k_new - k;
-          mbar_arrive(st_full + 8 * s);
+    Walk at = start;
+    float d0, d1;
+    auto fetch = [&] {  // of this lane's two queries (the last one's again where there are none)
+      const float* const delta = p.delta + ((long long)b * p.heads + at.h) * p.q_len;
+      const int row = first_row(at) + lane;
+      d0 = __ldcg(delta + min(row, rows_end - 1));
+      d1 = __ldcg(delta + min(row + 32, rows_end - 1));
+    };
+    if (kScaled && (!Split || tiles > 0)) {
+      fetch();
+      if (warp_wait(kv_full, 0, s_abort, p.gerr, 1146)) {
+        const int ev = tile_exponent<D, kTile>(sm + (sV - base), min(kTile, len - j0), lane) + (D == 64 ? 3 : 4);
+        int k = kFirstPower;
+        Ring<NS> ring_at;
+        for (int u = 0; u < tiles; ++u, ring_at.next()) {
+          const int s = ring_at.s;
+          if (!warp_wait(q_full + 8 * s, ring_at.ph, s_abort, p.gerr, 1148)) break;
+          const int eg = lane_exponent<D, kSub>(sm + S::kFixed + s * S::kStage + kTileBytes<D, kSub>, min(kSub, rows_end - first_row(at)), lane);
+          const int k_new = next_power(k, __reduce_max_sync(0xffffffffu, max(ev + eg, exponent_of(__float_as_uint(fmaxf(fabsf(d0), fabsf(d1)))))));
+          if (lane == 0) {
+            s_power[s] = k_new;
+            s_step[s] = u == 0 ? 0 : k_new - k;
+            mbar_arrive(st_full + 8 * s);
+          }
+          k = k_new;
+          at.next();
+          if (u + 1 < tiles) fetch();
         }
-        k = k_new;
       }
     }
   } else {
