@@ -73,7 +73,7 @@ int launch_copies(aig_ctx* ctx, const CopyShape& shape, const int32_t* src, cons
 // are mma.sync with the positions as rows and the group's query heads as the 8 columns, S^T = K Q^T and O^T = V^T P^T: K and
 // V come from shared memory as they lie there, P turns from result to operand by movmatrix, and eight query heads cost no more
 // than one.  (The kernel is bound by reading the cache, then by issuing instructions: with the heads as 16 rows
-// it took 430 instructions for 16 positions of 64, and 33 us where it takes 23, 128 sequences of up to 516 visible.)
+// it took 430 instructions for 16 positions of 64, and 33 us where it takes 24, 128 sequences of up to 516 visible.)
 // Softmax with a running maximum and sum in fp32; the weights enter the second product as a sum of two 16-bit values each, so
 // that their rounding does not add to the result's.  Warps are joined in shared memory, CTAs over the cluster's distributed
 // shared memory, in a fixed order: one launch, no scratch in global memory, nothing that two calls or captured
@@ -97,7 +97,7 @@ struct AttendParams {
 
 // W warps.  Where there are more sequences and heads than the device holds CTAs, small CTAs of two warps, seven to an SM, hide one
 // another's beginnings and ends; few long sequences need the reads of four warps per CTA (128 sequences, 8 heads of 64: 22.9 us
-// with two, 25.5 with four; 8 sequences of up to 65536, 8 heads of 128: 214 with two, 177 with four).
+// with two, 25.5 with four; 8 sequences of up to 65536, 8 heads of 128: 214 with two, 177 to 192 with four).
 template <int D, int HT, int W>
 struct AttendShape {
   static constexpr int kTile = 16;                                  // positions (32 need more shared memory: fewer CTAs, 26 us)
@@ -426,7 +426,8 @@ template <class T, int D, int HT, int W>
 int launch_attend(aig_ctx* ctx, AttendParams& p, int items, long long max_visible) {
   using S = AttendShape<D, HT, W>;
   // Splits: enough CTAs for every SM four times, each with a tile per warp at least.  Clusters of 16 leave SMs idle that
-  // a group of 16 does not fit on (177 us with 8, 183 with 16 for 8 sequences): only where 8 would leave more.
+  // a group of 16 does not fit on (8 sequences of up to 65536: 179 to 191 us with 8, 192 to 200 with 16, five runs of each): only where
+  // 8 would leave more (one sequence of 65536, 8 heads of 128: 104 with 8, 71 with 16).
   const int most = items * 8 < ctx->sm_count ? kMaxCluster : 8;
   p.splits = 1;
   while (p.splits < most && items * p.splits < 4 * ctx->sm_count && max_visible > (long long)p.splits * W * S::kTile) p.splits *= 2;

@@ -744,7 +744,7 @@ __global__ void __launch_bounds__(128, (ShortShape<D, Tiles>::kCtasPerSm)) windo
 // queries of the group's heads pass by).  Each computes the weights again from lse: two more products than one kernel that
 // adds dQ into memory with atomics would need, but every sum has a fixed order.  A thread owns a row of scores, 64 columns of it
 // at a time.  Bound by the chain from products to exponentials to products: so two tiles are under way on an SM, in two groups of
-// 128 threads of one CTA or in two CTAs.  (2 x 4099, 16 heads of 64: 208 us; one tile of 128 at a time for both groups 257.)
+// 128 threads of one CTA or in two CTAs.  (2 x 4099, 16 heads of 64: 208 us; one tile of 128 at a time for both groups 257; now 210.)
 //
 // fp16 has few small numbers: weights of a row over thousands of keys, and dS of small gradients, would be rounded to
 // multiples of 2^-24.  So the weights are multiplied by 2^8, and dS by a power of two 2^k that follows the largest
@@ -1004,8 +1004,8 @@ struct Ring {
 // A block of keys that many queries see (all heads of its group; all of a sequence where it holds a sink) is one long walk, and few
 // blocks leave SMs idle.  It is then shared by the CTAs of a cluster, a part of the queries each, joined through their shared memory
 // in a fixed order.  Blocks that only sinks make long get a launch of their own, beside that of the other blocks.  dK and dV of one
-// sequence, 8 query heads on one of 64: 4096 tokens 305 -> 75 us, with a window of 512 and 4 sinks 444 -> 69; 8 on 2 heads, 32768 tokens,
-// window 1024, 4 sinks 1817 -> 260 (heads of 128 1947 -> 300); 2 x 1000, 4 on 2 heads 26 -> 15.  So are dQ's tiles of queries where they
+// sequence, 8 query heads on one of 64: 4096 tokens 305 -> 77 us, with a window of 512 and 4 sinks 444 -> 68; 8 on 2 heads, 32768 tokens,
+// window 1024, 4 sinks 1817 -> 254 (heads of 128 1947 -> 300); 2 x 1000, 4 on 2 heads 26 -> 15.  So are dQ's tiles of queries where they
 // are no more than the SMs: 4096 tokens, one head of 64 38 -> 18, of 128 50 -> 23; 2048, 4 heads 23 -> 18, 30 -> 23.
 template <int D, int G>
 struct BwdShape {

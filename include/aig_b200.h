@@ -416,7 +416,7 @@ int aig_mha_reset(aig_mha_plan* plan);
  *
  * Tensors hold fp16 or bf16 values (`dtype`), heads are rows of head_dim consecutive elements, all strides count elements
  * and are at least 0.  Sums, softmax statistics and angles are held in 32 bits or more and results are rounded once.
- * Nothing is kept between calls except in the objects that the caller makes, and no call allocates: all of them can be
+ * Nothing is kept between calls except in the objects that the caller makes, and no call allocates device memory: all of them can be
  * captured (aig_graph_begin), and captured graphs share nothing but the tensors they were given. */
 enum { AIG_F16 = 0, AIG_BF16 = 1 };
 
@@ -435,7 +435,8 @@ typedef struct aig_heads {
  *                    floor(j(high)) to ceil(j(low)), where j(t) = rot_dim * ln(L / (2 pi t)) / (2 ln base) is the pair that
  *                    makes t turns over L; the ends are held within 0 .. rot_dim - 1
  *   AIG_ROPE_TURNS   the share falls linearly with the turns L * f / (2 pi) from 1 at `low` to 0 at `high`
- * Angles are exact for every 32-bit position, negative ones too: a frequency is kept as a 64-bit fraction of a turn.
+ * Angles are as good at every 32-bit position, negative ones too: a frequency is kept as a 64-bit fraction of a turn, the angle is
+ * reduced modulo a turn in 64-bit integers and held to 2^-25 of a turn, its sine and cosine to about 2^-21.
  * backward applies the transpose, which takes gradients of turned tensors to gradients of the tensors before.
  * Outputs may be the inputs themselves (same data and strides); other overlaps are not allowed.  k and k_out may both be
  * null.  head_dim even and at most 1024, rot_dim even. */
@@ -479,7 +480,7 @@ int aig_kv_append(aig_ctx* ctx, const aig_kv_cache* cache, aig_rope_plan* rope, 
                   const aig_heads* q_out, const int32_t* seqs, const int32_t* positions, long long tokens, const int32_t* table, int batch,
                   int table_width);
 /* Copies whole pages, keys and values: src[i] -> dst[i], host arrays.  No page may be a destination twice, or a source
- * and a destination. */
+ * and a destination (which the call checks; for more than 32 pairs with a byte of host memory per page of the pool while it lasts). */
 int aig_kv_copy_pages(aig_ctx* ctx, const aig_kv_cache* cache, const int32_t* src, const int32_t* dst, int pairs);
 /* Attention of one new token of each sequence over its pages: q, out [batch][q_heads][head_dim] (token_stride from
  * sequence to sequence), lengths int32 [batch] on the device: positions 0 .. lengths[b]-1 are in the cache, the new token
